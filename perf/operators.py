@@ -392,8 +392,8 @@ def _own(s):
         c_ext.dequantize_kv_blocks(s["back_ids_host"], s["back_ptrs"], back.shape[1] * size, size,
                                    s["ids_host"], mx, mx.stride(0), 0, chunk, *shape, back.dtype)
         return back
-    return c_ext.mx4_attention(s["query"], s["mx"], s["table"], s["lens"], s["starts"],
-                               scale=s["scale"])
+    return c_ext.mx4_attention(s["query"], s["mx"], case["heads"], s["table"], s["lens"],
+                               s["starts"], scale=s["scale"])
 
 
 def run(state):
