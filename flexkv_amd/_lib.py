@@ -23,6 +23,12 @@ FKV_XFER_KERNEL = 0
 FKV_XFER_CE = 1
 FKV_XFER_CE_PER_CHUNK = 2
 
+FKV_DTYPE_BF16 = 0
+FKV_DTYPE_FP16 = 1
+FKV_DTYPE_FP32 = 2
+DTYPES = {torch.bfloat16: FKV_DTYPE_BF16, torch.float16: FKV_DTYPE_FP16,
+          torch.float32: FKV_DTYPE_FP32}
+
 FKV_HOST_DEFAULT = 0
 FKV_HOST_COHERENT = 1
 FKV_HOST_NONCOHERENT = 2
@@ -34,6 +40,10 @@ EXPORTED_SYMBOLS = (
     "fkv_transfer_kv_blocks_noalloc",
     "fkv_gather_kv_blocks",
     "fkv_scatter_kv_blocks",
+    "fkv_quantize_kv_blocks",
+    "fkv_dequantize_kv_blocks",
+    "fkv_quantize_kv_tokens",
+    "fkv_mx4_attention",
     "fkv_transfer_kv_blocks_layerwise",
     "fkv_handle_num_groups",
     "fkv_handle_query",
@@ -100,6 +110,40 @@ class SsdStats(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class Mx4AttentionArgs(ctypes.Structure):
+    """fkv_mx4_attention_args."""
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("query_row_stride_bytes", ctypes.c_int64),
+        ("query_head_stride_bytes", ctypes.c_int64),
+        ("out_row_stride_bytes", ctypes.c_int64),
+        ("out_head_stride_bytes", ctypes.c_int64),
+        ("lse_row_stride", ctypes.c_int64),
+        ("lse_head_stride", ctypes.c_int64),
+        ("mx_ptr", ctypes.c_void_p),
+        ("mx_kv_stride_bytes", ctypes.c_int64),
+        ("mx_block_stride_bytes", ctypes.c_int64),
+        ("num_mx_blocks", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_starts", ctypes.c_void_p),
+        ("table_row_stride", ctypes.c_int64),
+        ("index_is_64bit", ctypes.c_int),
+        ("table_width", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("num_queries", ctypes.c_int),
+        ("tokens_per_block", ctypes.c_int),
+        ("num_heads", ctypes.c_int),
+        ("group_size", ctypes.c_int),
+        ("head_size", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 # Counts finalize() calls: handles and streams made before the latest one
@@ -125,6 +169,18 @@ def _declare(lib: ctypes.CDLL) -> None:
         g = getattr(lib, name)
         g.restype = c_int
         g.argtypes = [c_int, c_int, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_sz, c_vp, c_int]
+    for name in ("fkv_quantize_kv_blocks", "fkv_dequantize_kv_blocks"):
+        g = getattr(lib, name)
+        g.restype = c_int
+        g.argtypes = [c_int, c_int, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64,
+                      c_i64, c_int, c_int, c_int, c_int, c_vp, c_int]
+    f = lib.fkv_quantize_kv_tokens
+    f.restype = c_int
+    f.argtypes = [c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_int, c_vp, c_i64, c_i64,
+                  c_i64, c_int, c_int, c_int, c_int, c_vp]
+    f = lib.fkv_mx4_attention
+    f.restype = c_int
+    f.argtypes = [ctypes.POINTER(Mx4AttentionArgs), c_vp]
     f = lib.fkv_transfer_kv_blocks_layerwise
     f.restype = c_int
     f.argtypes = [c_int, c_int, c_int, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64,

@@ -10,13 +10,15 @@ the HIP C-ABI entry ``fkv_transfer_kv_blocks``.
 from __future__ import annotations
 
 import contextlib
+import operator
 
 import torch
 
 from . import _lib
 
 __all__ = ["transfer_kv_blocks", "transfer_kv_blocks_kv_ptrs", "gather_kv_blocks",
-           "scatter_kv_blocks",
+           "scatter_kv_blocks", "mx4_chunk_bytes", "quantize_kv_blocks", "dequantize_kv_blocks",
+           "quantize_kv_tokens", "mx4_attention",
            "transfer_kv_blocks_layerwise", "LayerwiseTransfer", "transfer_stream",
            "release_transfer_stream", "set_copy_engine_policy", "copy_engine_policy",
            "TPTransferThreadGroup", "SSDIOCTX", "transfer_kv_blocks_ssd"]
@@ -194,6 +196,246 @@ def scatter_kv_blocks(gpu_block_id_tensor: torch.Tensor, gpu_layer_ptrs_tensor: 
     _contiguous("fkv_scatter_kv_blocks", gpu_block_id_tensor, gpu_layer_ptrs_tensor,
                 gpu_kv_stride_in_bytes, gpu_block_stride_in_bytes, chunk_size_in_bytes, buffer,
                 is_mla)
+
+
+def mx4_chunk_bytes(tokens_per_block: int, num_heads: int, head_size: int) -> int:
+    """Bytes of one block of one half of one layer in a 4-bit cache: the codes
+    [head][token][head_size / 2], then the scale bytes [head][head_size / 32][token]."""
+    if tokens_per_block < 16 or tokens_per_block % 16:
+        raise ValueError(f"tokens_per_block must be a multiple of 16, got {tokens_per_block}")
+    if head_size < 32 or head_size % 32:
+        raise ValueError(f"head_size must be a multiple of 32, got {head_size}")
+    if num_heads < 1:
+        raise ValueError(f"num_heads must be positive, got {num_heads}")
+    return tokens_per_block * num_heads * (head_size // 32) * 17
+
+
+def _dtype_code(dtype: torch.dtype, fn_name: str) -> int:
+    code = _lib.DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"{fn_name} takes bfloat16, float16 or float32 elements, got {dtype}")
+    return code
+
+
+def _mx_blocks(fn_name: str, gpu_block_id_tensor, gpu_layer_ptrs_tensor, gpu_kv_stride_in_bytes,
+               gpu_block_stride_in_bytes, mx_block_id_tensor, mx_tensor, mx_kv_stride_in_bytes,
+               mx_layer_stride_in_bytes, mx_block_stride_in_bytes, tokens_per_block, num_heads,
+               head_size, dtype, start_layer_id, is_mla) -> None:
+    _require_int64_host(gpu_block_id_tensor, "gpu_block_id_tensor")
+    _require_int64_host(gpu_layer_ptrs_tensor, "gpu_layer_ptrs_tensor")
+    _require_int64_host(mx_block_id_tensor, "mx_block_id_tensor")
+    if not isinstance(mx_tensor, torch.Tensor):
+        raise TypeError(f"mx_tensor must be a torch.Tensor, got {type(mx_tensor).__name__}")
+    n = gpu_block_id_tensor.numel()
+    if mx_block_id_tensor.numel() != n:
+        raise RuntimeError(f"gpu_block_id_tensor has {n} ids but mx_block_id_tensor has "
+                           f"{mx_block_id_tensor.numel()}")
+    code = _dtype_code(dtype, fn_name)
+    stream = _stream_handle(fn_name)
+    rc = getattr(_lib.load(), "fkv_" + fn_name)(
+        n, int(start_layer_id), int(gpu_layer_ptrs_tensor.numel()),
+        gpu_block_id_tensor.data_ptr(), gpu_layer_ptrs_tensor.data_ptr(),
+        int(gpu_kv_stride_in_bytes), int(gpu_block_stride_in_bytes),
+        mx_block_id_tensor.data_ptr(), mx_tensor.data_ptr(), int(mx_kv_stride_in_bytes),
+        int(mx_layer_stride_in_bytes), int(mx_block_stride_in_bytes), int(tokens_per_block),
+        int(num_heads), int(head_size), code, stream, 1 if is_mla else 0)
+    if rc != 0:
+        raise RuntimeError(_lib.last_error() or f"{fn_name} failed ({rc})")
+
+
+def quantize_kv_blocks(gpu_block_id_tensor: torch.Tensor, gpu_layer_ptrs_tensor: torch.Tensor,
+                       gpu_kv_stride_in_bytes: int, gpu_block_stride_in_bytes: int,
+                       mx_block_id_tensor: torch.Tensor, mx_tensor: torch.Tensor,
+                       mx_kv_stride_in_bytes: int, mx_layer_stride_in_bytes: int,
+                       mx_block_stride_in_bytes: int, tokens_per_block: int, num_heads: int,
+                       head_size: int, dtype: torch.dtype, start_layer_id: int = 0,
+                       is_mla: bool = False) -> None:
+    """Quantise blocks of the per-layer GPU cache (elements of ``dtype``,
+    [token][head][head_size] a chunk) into blocks of a 4-bit cache in device or
+    pinned host memory (extension).  The GPU side is described as in
+    transfer_kv_blocks, the 4-bit side as its host cache is, with chunks of
+    ``mx4_chunk_bytes``; ``KVCacheLayout.mx4()`` gives its strides.  Synchronous,
+    on the current torch stream."""
+    _mx_blocks("quantize_kv_blocks", gpu_block_id_tensor, gpu_layer_ptrs_tensor,
+               gpu_kv_stride_in_bytes, gpu_block_stride_in_bytes, mx_block_id_tensor, mx_tensor,
+               mx_kv_stride_in_bytes, mx_layer_stride_in_bytes, mx_block_stride_in_bytes,
+               tokens_per_block, num_heads, head_size, dtype, start_layer_id, is_mla)
+
+
+def dequantize_kv_blocks(gpu_block_id_tensor: torch.Tensor, gpu_layer_ptrs_tensor: torch.Tensor,
+                         gpu_kv_stride_in_bytes: int, gpu_block_stride_in_bytes: int,
+                         mx_block_id_tensor: torch.Tensor, mx_tensor: torch.Tensor,
+                         mx_kv_stride_in_bytes: int, mx_layer_stride_in_bytes: int,
+                         mx_block_stride_in_bytes: int, tokens_per_block: int, num_heads: int,
+                         head_size: int, dtype: torch.dtype, start_layer_id: int = 0,
+                         is_mla: bool = False) -> None:
+    """Inverse of quantize_kv_blocks: read blocks of the 4-bit cache back into
+    the per-layer GPU cache."""
+    _mx_blocks("dequantize_kv_blocks", gpu_block_id_tensor, gpu_layer_ptrs_tensor,
+               gpu_kv_stride_in_bytes, gpu_block_stride_in_bytes, mx_block_id_tensor, mx_tensor,
+               mx_kv_stride_in_bytes, mx_layer_stride_in_bytes, mx_block_stride_in_bytes,
+               tokens_per_block, num_heads, head_size, dtype, start_layer_id, is_mla)
+
+
+def _require_device(t, name: str, fn_name: str, device=None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{fn_name}: {name} must be a device tensor, got device {t.device}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{fn_name}: {name} is on {t.device}, the others on {device}")
+
+
+def _mx_layer(mx_layer, halves: int, num_heads: int, head_size: int, fn_name: str,
+              device) -> int:
+    """Check one layer's view [K|V, block, chunk bytes] of a 4-bit cache;
+    returns its tokens per block."""
+    _require_device(mx_layer, "mx_layer", fn_name, device)
+    if mx_layer.dtype != torch.uint8 or mx_layer.dim() != 3 or mx_layer.stride(2) != 1:
+        raise ValueError(f"{fn_name}: mx_layer must be a uint8 tensor [K|V, block, chunk bytes] "
+                         f"with neighbouring bytes, got {mx_layer.dtype} "
+                         f"{tuple(mx_layer.shape)} {mx_layer.stride()}")
+    if mx_layer.shape[0] != halves:
+        raise ValueError(f"{fn_name}: mx_layer has {mx_layer.shape[0]} halves, needs {halves}")
+    if head_size < 32 or head_size % 32:
+        raise ValueError(f"{fn_name}: head_size must be a multiple of 32, got {head_size}")
+    token = num_heads * (head_size // 32) * 17
+    tokens, rest = divmod(mx_layer.shape[2], token)
+    if rest or tokens < 16 or tokens % 16:
+        raise ValueError(f"{fn_name}: mx_layer's chunks of {mx_layer.shape[2]} bytes do not hold "
+                         f"a multiple of 16 tokens of {num_heads} heads of {head_size}")
+    return tokens
+
+
+def _on_device(device: torch.device):
+    """A context in which `device` is the current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def quantize_kv_tokens(key: torch.Tensor, value, mx_layer: torch.Tensor,
+                       slots: torch.Tensor) -> None:
+    """Quantise new tokens of one layer into their slots of a 4-bit cache
+    (extension; fkv_quantize_kv_tokens).  ``key`` and ``value``: [token, head,
+    head_size], of any token and head stride (value None for one latent half);
+    ``mx_layer``: uint8 [K|V, block, chunk bytes], a view of the cache's layer;
+    ``slots``: int64 or int32, block * tokens_per_block + offset, one below 0 or
+    past the cache being padding.  Slots have to differ.  Asynchronous on the
+    current torch stream; may be captured into a graph."""
+    fn = "quantize_kv_tokens"
+    _require_device(key, "key", fn)
+    device = key.device
+    if key.dim() != 3 or key.stride(2) != 1:
+        raise ValueError(f"{fn}: key must be [token, head, head_size] with neighbouring elements, "
+                         f"got {tuple(key.shape)} {key.stride()}")
+    code = _dtype_code(key.dtype, fn)
+    if value is not None:
+        _require_device(value, "value", fn, device)
+        if value.shape != key.shape or value.dtype != key.dtype or value.stride(2) != 1:
+            raise ValueError(f"{fn}: value must be as key is, {tuple(key.shape)} {key.dtype}, got "
+                             f"{tuple(value.shape)} {value.dtype} {value.stride()}")
+    n, heads, dim = key.shape
+    tokens = _mx_layer(mx_layer, 1 if value is None else 2, heads, dim, fn, device)
+    _require_device(slots, "slots", fn, device)
+    if slots.dtype not in (torch.int64, torch.int32) or slots.shape != (n,) \
+            or not slots.is_contiguous():
+        raise ValueError(f"{fn}: slots must be {n} contiguous int64 or int32 values, got "
+                         f"{slots.dtype} {tuple(slots.shape)}")
+    es = key.element_size()
+    with _on_device(device):
+        rc = _lib.load().fkv_quantize_kv_tokens(
+            n, key.data_ptr(), key.stride(0) * es, key.stride(1) * es,
+            value.data_ptr() if value is not None else None,
+            value.stride(0) * es if value is not None else 0,
+            value.stride(1) * es if value is not None else 0,
+            slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0, mx_layer.data_ptr(),
+            mx_layer.stride(0), mx_layer.stride(1), mx_layer.shape[1], tokens, heads, dim, code,
+            _stream_handle(fn))
+    if rc != 0:
+        raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
+
+
+def mx4_attention(query: torch.Tensor, mx_layer: torch.Tensor, num_kv_heads: int,
+                  block_table: torch.Tensor, seq_lens: torch.Tensor, query_starts=None,
+                  scale: float = None, causal: bool = True, out: torch.Tensor = None,
+                  lse: torch.Tensor = None) -> torch.Tensor:
+    """Attention of packed queries over one layer of a paged 4-bit cache
+    (extension; fkv_mx4_attention).  ``query``: bf16 or fp16 [row, head,
+    head_size] of any row and head stride, ``num_kv_heads`` times the group heads;
+    ``mx_layer`` as in quantize_kv_tokens; ``block_table`` [sequence, blocks] and
+    ``seq_lens`` [sequence] give each sequence's blocks and keys, the queries'
+    own included; ``query_starts`` [sequences + 1] the rows of each, its last
+    tokens (None: row b is sequence b's one query); all three int32 or all int64.
+    ``scale`` defaults to head_size ** -0.5.  With ``causal`` a query sees the keys
+    up to its own position.  Rows that see none give zeros (lse -inf); rows of no
+    sequence are left as they were (not written in a given ``out``, unset in a new
+    one).  ``lse``: float32 [row, head], receives the log of the sum of exp.
+    Returns ``out``.  Asynchronous on the current torch stream; may be captured
+    into a graph."""
+    fn = "mx4_attention"
+    _require_device(query, "query", fn)
+    device = query.device
+    if query.dim() != 3 or query.stride(2) != 1 or query.dtype not in (torch.bfloat16,
+                                                                       torch.float16):
+        raise ValueError(f"{fn}: query must be bf16 or fp16 [row, head, head_size] with "
+                         f"neighbouring elements, got {query.dtype} {tuple(query.shape)} "
+                         f"{query.stride()}")
+    rows, heads, dim = query.shape
+    num_kv_heads = operator.index(num_kv_heads)
+    if num_kv_heads < 1 or heads < 1 or heads % num_kv_heads:
+        raise ValueError(f"{fn}: {heads} query heads are no multiple of {num_kv_heads} K/V heads")
+    tokens = _mx_layer(mx_layer, 2, num_kv_heads, dim, fn, device)
+    _require_device(block_table, "block_table", fn, device)
+    _require_device(seq_lens, "seq_lens", fn, device)
+    index = seq_lens.dtype
+    if index not in (torch.int32, torch.int64) or block_table.dtype != index or \
+            (query_starts is not None and getattr(query_starts, "dtype", None) != index):
+        raise ValueError(f"{fn}: block_table, seq_lens and query_starts must be all int32 or all "
+                         f"int64")
+    if seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+        raise ValueError(f"{fn}: seq_lens must be a contiguous vector, got {tuple(seq_lens.shape)}")
+    batch = seq_lens.shape[0]
+    if block_table.dim() != 2 or block_table.shape[0] != batch or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"{fn}: block_table must be [{batch}, blocks] with neighbouring entries, "
+                         f"got {tuple(block_table.shape)} {block_table.stride()}")
+    if query_starts is None:
+        if rows < batch:
+            raise ValueError(f"{fn}: {batch} sequences of one query each, but {rows} rows")
+    else:
+        _require_device(query_starts, "query_starts", fn, device)
+        if query_starts.shape != (batch + 1,) or not query_starts.is_contiguous():
+            raise ValueError(f"{fn}: query_starts must hold {batch + 1} contiguous values, got "
+                             f"{tuple(query_starts.shape)}")
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=query.dtype, device=device)
+    else:
+        _require_device(out, "out", fn, device)
+        if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
+            raise ValueError(f"{fn}: out must be as query is, {tuple(query.shape)} {query.dtype}, "
+                             f"got {tuple(out.shape)} {out.dtype} {out.stride()}")
+    if lse is not None:
+        _require_device(lse, "lse", fn, device)
+        if lse.shape != (rows, heads) or lse.dtype != torch.float32:
+            raise ValueError(f"{fn}: lse must be float32 {(rows, heads)}, got {lse.dtype} "
+                             f"{tuple(lse.shape)}")
+    es = query.element_size()
+    args = _lib.Mx4AttentionArgs(
+        query.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
+        query.stride(0) * es, query.stride(1) * es, out.stride(0) * es, out.stride(1) * es,
+        lse.stride(0) if lse is not None else 0, lse.stride(1) if lse is not None else 0,
+        mx_layer.data_ptr(), mx_layer.stride(0), mx_layer.stride(1), mx_layer.shape[1],
+        block_table.data_ptr(), seq_lens.data_ptr(),
+        query_starts.data_ptr() if query_starts is not None else None, block_table.stride(0),
+        1 if index is torch.int64 else 0, block_table.shape[1], batch, rows, tokens, num_kv_heads,
+        heads // num_kv_heads, dim, _lib.DTYPES[query.dtype], 1 if causal else 0,
+        float(dim ** -0.5 if scale is None else scale))
+    with _on_device(device):
+        rc = _lib.load().fkv_mx4_attention(args, _stream_handle(fn))
+    if rc != 0:
+        raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
+    return out
 
 
 class LayerwiseTransfer:

@@ -96,6 +96,17 @@ class KVCacheLayout:
             f"num_head {self.num_head} must be divisible by num_chunks {num_chunks}"
         return self._replace(num_head=self.num_head // num_chunks)
 
+    def mx4(self) -> "KVCacheLayout":
+        """The layout of this cache held in 4 bits, to be read with torch.uint8
+        elements: a head takes 17 bytes for 32 elements.  Within a chunk the
+        bytes are [head][token][head_size / 2] codes, then
+        [head][head_size / 32][token] scales."""
+        if self.head_size % 32 or self.tokens_per_block % 16:
+            raise ValueError("a 4-bit cache needs head_size in multiples of 32 and "
+                             f"tokens_per_block in multiples of 16, got {self.head_size} and "
+                             f"{self.tokens_per_block}")
+        return self._replace(head_size=self.head_size // 32 * 17)
+
     def get_chunk_size(self) -> int:
         return self.tokens_per_block * self.num_head * self.head_size
 

@@ -369,6 +369,110 @@ int fkv_tp_group_transfer(fkv_tp_group_t group, int num_blocks, const int64_t* g
                           int layer_granularity, int is_mla);
 int fkv_tp_group_destroy(fkv_tp_group_t group);
 
+/* ---------------------------------------------------------------------------
+ * A KV cache held in 4 bits (OCP MXFP4).  No counterpart in the reference.
+ *
+ * A chunk (the tokens_per_block = T tokens of one block of K or V of one layer, H
+ * heads of D elements) is
+ *     [head][token][D / 2]    codes: element 2i in the low half of byte i; sign, two
+ *                             exponent bits, one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6)
+ *     [head][D / 32][token]   a scale byte b for 32 neighbouring elements: 2^(b - 127)
+ * that is T * H * (D / 32) * 17 bytes, 17/64 of 16-bit elements.  T is a multiple
+ * of 16 up to 4096, D of 32 up to 1024, H at most 1024.  The chunks of a cache lie
+ * at strides of their own, as those of any cache here: fkv_transfer_kv_blocks and the
+ * SSD tier move them as bytes.
+ *
+ * Quantising: with a the largest magnitude of a group, E = floor(log2 a), one more
+ * where a's mantissa is over 1.75 and at most 127, the scale is 2^(E - 2), at least
+ * 2^-127; every element is rounded once, to the nearest, ties to the even code, and
+ * is within one scale of its value.  A group that holds an infinity or a NaN gets
+ * scale byte 255 and reads back as NaN.  Reading back is exact, but for values past
+ * the destination type's largest finite one, which become that one. */
+
+/* Element types of the wide side. */
+enum { FKV_DTYPE_BF16 = 0, FKV_DTYPE_FP16 = 1, FKV_DTYPE_FP32 = 2 };
+
+/* Quantise the blocks gpu_block_ids of the per-layer GPU cache (arguments as
+ * fkv_transfer_kv_blocks: layer l, half k, block b at gpu_layer_ptrs[l] +
+ * k * gpu_kv_stride_bytes + b * gpu_block_stride_bytes, [token][head][D] elements of
+ * `dtype`) into the blocks mx_block_ids of a 4-bit cache: chunk (l, k, i) at mx_ptr +
+ * (l + start_layer_id) * mx_layer_stride_bytes + k * mx_kv_stride_bytes +
+ * mx_block_ids[i] * mx_block_stride_bytes.  mx_ptr is device memory or pinned host
+ * memory.  fkv_dequantize_kv_blocks is the way back.  Pointers, strides: multiples
+ * of 16 bytes; ids and pointers are checked against their allocations as there.
+ * An id of the written side that comes twice leaves one of the two or a mixture.
+ * Synchronous, on `stream`; a stream under HIP graph capture is refused
+ * (hipErrorStreamCaptureUnsupported). */
+int fkv_quantize_kv_blocks(int num_blocks, int start_layer_id, int num_layers,
+                           const int64_t* gpu_block_ids, void* const* gpu_layer_ptrs,
+                           int64_t gpu_kv_stride_bytes, int64_t gpu_block_stride_bytes,
+                           const int64_t* mx_block_ids, void* mx_ptr, int64_t mx_kv_stride_bytes,
+                           int64_t mx_layer_stride_bytes, int64_t mx_block_stride_bytes,
+                           int tokens_per_block, int num_heads, int head_size, int dtype,
+                           fkv_stream_t stream, int is_mla);
+int fkv_dequantize_kv_blocks(int num_blocks, int start_layer_id, int num_layers,
+                             const int64_t* gpu_block_ids, void* const* gpu_layer_ptrs,
+                             int64_t gpu_kv_stride_bytes, int64_t gpu_block_stride_bytes,
+                             const int64_t* mx_block_ids, const void* mx_ptr,
+                             int64_t mx_kv_stride_bytes, int64_t mx_layer_stride_bytes,
+                             int64_t mx_block_stride_bytes, int tokens_per_block, int num_heads,
+                             int head_size, int dtype, fkv_stream_t stream, int is_mla);
+
+/* Quantise new tokens of one layer into their slots of the 4-bit cache: row n of
+ * `key` and `value` (head h at key + n * key_token_stride + h * key_head_stride, D
+ * neighbouring elements of `dtype`) goes to token slots[n] % T of block
+ * slots[n] / T, half k of block b being at mx_ptr + k * mx_kv_stride_bytes +
+ * b * mx_block_stride_bytes, b < num_mx_blocks.  `value` is null for a cache with
+ * one latent half.  slots: device memory, int64 or int32 (slots_are_64bit); a slot
+ * below 0 or past the cache is padding and writes nothing.  Slots of one call have
+ * to differ: one that comes twice leaves a mixture.  Pointers and strides: multiples
+ * of 16 bytes.  Asynchronous on `stream`, and may be captured into a graph. */
+int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_stride_bytes,
+                           int64_t key_head_stride_bytes, const void* value,
+                           int64_t value_token_stride_bytes, int64_t value_head_stride_bytes,
+                           const void* slots, int slots_are_64bit, void* mx_ptr,
+                           int64_t mx_kv_stride_bytes, int64_t mx_block_stride_bytes,
+                           int64_t num_mx_blocks, int tokens_per_block, int num_heads,
+                           int head_size, int dtype, fkv_stream_t stream);
+
+/* Attention of queries over one layer of a paged 4-bit cache.  Sequence b has
+ * seq_lens[b] keys, token t of it in block block_table[b][t / T] at t % T, and the queries
+ * query_starts[b] .. query_starts[b + 1] of the packed rows (null: row b alone), which
+ * are its last tokens.  For query row i and head hq, with K/V head hq / group_size,
+ *     out = softmax(scale * q . k) v   over the sequence's keys,
+ * or with `causal` over those up to the query's own position, seq_lens[b] - its
+ * queries + its index.  A row that sees no key gives zeros, and lse -infinity.
+ * lse (may be null): log of the sum of exp(scale * q . k).
+ *
+ * head_size 64, 128 or 256; dtype (of query and out) FKV_DTYPE_BF16 or _FP16.  Sums,
+ * maximum and normalisation are held in 32 bits; the queries enter exactly, and the
+ * weights p with 8 significant bits for bf16, 16 for fp16.  Block ids, lengths and starts are device memory, all int32 or all
+ * int64 (index_is_64bit), read by the kernels: a block id outside the cache or a
+ * length past the table's row makes that sequence's rows NaN, and nothing outside
+ * the cache is read.  Starts have to ascend; rows of no sequence are left as they
+ * were.  A NaN in a key or value reaches the rows that see that token and no
+ * other.  A query row that holds an infinity or a NaN gives NaN.
+ * Asynchronous on `stream`, and may be captured into a graph. */
+typedef struct fkv_mx4_attention_args {
+  const void* query;                 /* [num_queries][num_heads * group_size][head_size] */
+  void* out;                         /* as query; may not overlap it */
+  float* lse;                        /* [num_queries][num_heads * group_size], or null */
+  int64_t query_row_stride_bytes, query_head_stride_bytes;   /* multiples of 16, as pointers */
+  int64_t out_row_stride_bytes, out_head_stride_bytes;
+  int64_t lse_row_stride, lse_head_stride;                   /* in elements */
+  const void* mx_ptr;                /* half k of block b at + k * kv stride + b * block stride */
+  int64_t mx_kv_stride_bytes, mx_block_stride_bytes, num_mx_blocks;
+  const void* block_table;           /* [batch][table_width] */
+  const void* seq_lens;              /* [batch] */
+  const void* query_starts;          /* [batch + 1], or null: one query a sequence */
+  int64_t table_row_stride;          /* in elements */
+  int index_is_64bit;
+  int table_width, batch, num_queries;
+  int tokens_per_block, num_heads, group_size, head_size, dtype, causal;
+  float scale;
+} fkv_mx4_attention_args;
+int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream);
+
 /* How copy-engine mode (use_ce_transfer = FKV_XFER_CE) chooses between the
  * SDMA engines and the zero-copy kernel, process-wide.  No counterpart in
  * the reference, whose CE mode always copies on the engines.
