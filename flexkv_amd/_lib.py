@@ -43,6 +43,7 @@ EXPORTED_SYMBOLS = (
     "fkv_quantize_kv_blocks",
     "fkv_dequantize_kv_blocks",
     "fkv_quantize_kv_tokens",
+    "fkv_mx4_attention_workspace",
     "fkv_mx4_attention",
     "fkv_transfer_kv_blocks_layerwise",
     "fkv_handle_num_groups",
@@ -141,6 +142,8 @@ class Mx4AttentionArgs(ctypes.Structure):
         ("dtype", ctypes.c_int),
         ("causal", ctypes.c_int),
         ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -178,6 +181,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     f.restype = c_int
     f.argtypes = [c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_int, c_vp, c_i64, c_i64,
                   c_i64, c_int, c_int, c_int, c_int, c_vp]
+    f = lib.fkv_mx4_attention_workspace
+    f.restype = c_int
+    f.argtypes = [ctypes.POINTER(Mx4AttentionArgs), ctypes.POINTER(c_sz)]
     f = lib.fkv_mx4_attention
     f.restype = c_int
     f.argtypes = [ctypes.POINTER(Mx4AttentionArgs), c_vp]

@@ -10,6 +10,7 @@ the HIP C-ABI entry ``fkv_transfer_kv_blocks``.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import operator
 
 import torch
@@ -431,8 +432,17 @@ def mx4_attention(query: torch.Tensor, mx_layer: torch.Tensor, num_kv_heads: int
         1 if index is torch.int64 else 0, block_table.shape[1], batch, rows, tokens, num_kv_heads,
         heads // num_kv_heads, dim, _lib.DTYPES[query.dtype], 1 if causal else 0,
         float(dim ** -0.5 if scale is None else scale))
-    with _on_device(device):
-        rc = _lib.load().fkv_mx4_attention(args, _stream_handle(fn))
+    lib = _lib.load()
+    need = ctypes.c_size_t()
+    rc = lib.fkv_mx4_attention_workspace(args, need)
+    if rc == 0:
+        with _on_device(device):
+            if need.value:
+                # the allocator orders its reuse on the current stream
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+                args.workspace = workspace.data_ptr()
+                args.workspace_bytes = need.value
+            rc = lib.fkv_mx4_attention(args, _stream_handle(fn))
     if rc != 0:
         raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
     return out

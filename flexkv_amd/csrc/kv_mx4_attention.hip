@@ -19,6 +19,13 @@
 // register by byte permutes.
 //
 // Softmax: one pass, running maximum and sum per row in 32 bits, in units of log2.
+// The maximum is a reference that follows only when a score passes it by 2^8, so
+// most steps neither compare across lanes nor scale the sums.
+//
+// A workgroup's four wavefronts take the 32-token steps of its tile in turn, each
+// loading its next step while it computes one, and add up in LDS.  With few
+// tiles the keys are cut among workgroups as well (Plan), whose sums a second
+// kernel joins in a fixed order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -41,6 +48,10 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 16;          // rows of a tile: columns of a matrix instruction
 constexpr int kStep = 32;          // tokens of a step: two tiles of 16, k of the second product
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kMinSteps = 4;       // of a workgroup, where the keys are cut
+constexpr float kSlack = 8.f;      // log2 by which a score may pass the reference
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -50,20 +61,18 @@ __device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
   return __builtin_amdgcn_perm(hi, lo, sel);
 }
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ inline int64_t uniform64(int64_t v) {
-  const uint64_t u = static_cast<uint64_t>(v);
-  const uint64_t lo = static_cast<uint32_t>(uniform(static_cast<int>(u)));
-  const uint64_t hi = static_cast<uint32_t>(uniform(static_cast<int>(u >> 32)));
-  return static_cast<int64_t>(hi << 32 | lo);
-}
-// the larger of a lane's value and those 16, 32 and 48 lanes away
+// quads: the 4 groups of 16 lanes
 __device__ inline float max_over_quads(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  auto r = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+  v = fmaxf(bits_f32(r[0]), bits_f32(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+  return fmaxf(bits_f32(r[0]), bits_f32(r[1]));
 }
 __device__ inline float sum_over_quads(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  auto r = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+  v = bits_f32(r[0]) + bits_f32(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+  return bits_f32(r[0]) + bits_f32(r[1]);
 }
 
 struct Args {
@@ -83,8 +92,11 @@ struct Args {
   int batch, heads, group, queries;
   int tokens;                        // of a block
   int causal;
+  int target;                        // workgroups to cut the keys into; 0: uncut
   float scale_log2;
-  FastDiv tiles_per_block, group_div;
+  float2* part_ml;                   // [workgroup][row]: maximum and sum of a cut
+  v4f* part_o;                       // [workgroup][register][lane]
+  FastDiv tiles_per_block, group_div, heads_div;
 };
 
 __device__ inline int64_t index_at(const void* p, int64_t i, int is64) {
@@ -113,14 +125,75 @@ __device__ inline Seq sequence(const Args& a, int b) {
   return s;
 }
 
-// Row tiles are numbered so that sequence b's start at first(b) * group / kRows + b,
-// which leaves room for its last, partly filled one, and needs no lengths
-// but its own: tile `t` belongs to the last sequence that starts at or before it.
-__device__ inline int tile_base(const Args& a, int b) {
-  if (!a.starts) return b * ((a.group + kRows - 1) / kRows);
-  int64_t lo = index_at(a.starts, b, a.index64);
-  lo = lo < 0 ? 0 : lo > a.queries ? a.queries : lo;
-  return static_cast<int>(lo * a.group / kRows) + b;
+// How the workgroups are dealt out.  A sequence has ceil(queries * group / rows a tile)
+// tiles; where the keys are cut, every tile's into cuts of the same number of
+// steps, chosen from the lengths on the device so that there are about `target`
+// of them in all however uneven the sequences are.  Every wavefront works this out
+// for itself: sequence b = lane, then 64 further on.
+struct Work {
+  int seq, tile, cut, cuts;   // seq < 0: none
+  int steps;                  // of a cut
+  int first;                  // the tile's first cut's number
+};
+__device__ inline int tiles_of(const Args& a, const Seq& s, int rows_a_tile) {
+  return (s.count * a.group + rows_a_tile - 1) / rows_a_tile;
+}
+__device__ inline int steps_of(const Seq& s) { return (max(s.keys, 0) + kStep - 1) / kStep; }
+
+__device__ inline int64_t sum_over_lanes(int64_t v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+  return v;
+}
+
+// Item `item` of the plan; by_tile: `item` counts tiles, the answer is its first cut.
+__device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool by_tile) {
+  const int lane = threadIdx.x & 63;
+  int per_cut = 1 << 30;
+  Seq s{0, 0, 0};
+  if (a.target) {
+    int64_t total = 0;
+    for (int b = lane; b < a.batch; b += 64) {
+      s = sequence(a, b);
+      total += static_cast<int64_t>(tiles_of(a, s, rows_a_tile)) * steps_of(s);
+    }
+    total = sum_over_lanes(total) * a.heads;
+    const int64_t even = (total + a.target - 1) / a.target;
+    per_cut = static_cast<int>(max(even, static_cast<int64_t>(kMinSteps)));
+  }
+  Work w{-1, 0, 0, 0, per_cut, 0};
+  int before = 0, cuts_before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    int tiles = 0, cuts = 0;
+    if (b < a.batch) {
+      if (!a.target || a.batch > 64) s = sequence(a, b);
+      tiles = tiles_of(a, s, rows_a_tile);
+      cuts = max(1, (steps_of(s) + per_cut - 1) / per_cut);
+    }
+    int ends = by_tile ? tiles : tiles * cuts, cut_ends = tiles * cuts;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int e = __shfl_up(ends, d), c = __shfl_up(cut_ends, d);
+      if (lane >= d) ends += e, cut_ends += c;
+    }
+    const uint64_t later = __ballot(before + ends > item);
+    if (later) {
+      const int at = __ffsll(static_cast<unsigned long long>(later)) - 1;
+      const int n = uniform(__shfl(tiles, at)), c = uniform(__shfl(cuts, at));
+      const int start = before + uniform(__shfl(ends, at)) - (by_tile ? n : n * c);
+      const int local = item - start;
+      w.seq = b0 + at;
+      w.cuts = c;
+      w.tile = by_tile ? local : local / c;
+      w.cut = by_tile ? 0 : local - w.tile * c;
+      w.first = cuts_before + uniform(__shfl(cut_ends, at)) - n * c + w.tile * c;
+      return w;
+    }
+    before += uniform(__shfl(ends, 63));
+    cuts_before += uniform(__shfl(cut_ends, 63));
+  }
+  return w;
 }
 
 // The queries of one row as e4m3 parts: operand registers for each part and
@@ -293,93 +366,103 @@ __device__ inline uint32_t pack_bf16(float a, float b) {
 template <int D>
 struct State {
   v4f o[D / 16];   // o[j][i]: element (D / 16) * (quad * 4 + i) + j
-  float m, l;      // l: of this lane's tokens
+  float m, l;      // the reference; the sum of this lane's tokens
 };
 
-// Two tiles of 16 tokens from token `at` on.  MASKED: some row does not see
-// all of them.  `visible`: the keys this lane's row sees; `keys`: those there are.
-// P of bf16 has 8 significant bits, as flash attention's has; where the output has
-// 11 (SPLIT_P) the rest of P is a second bf16 operand.
-template <int D, int PARTS, bool MASKED, bool SPLIT_P>
-__device__ inline void attend(const Query<D, PARTS>& q, Tile<D> (&t)[2], int at, int visible,
-                              int keys, float scale_log2, int quad, State<D>& st) {
+// Byte i of `scales` as the scale of a conversion, which reads its exponent
+// field and nothing else (every sign and mantissa tried gave the same).
+__device__ inline float byte_scale(uint32_t scales, int i) {
+  return bits_f32(i == 0 ? scales << 23 : i == 1 ? scales << 15 : i == 2 ? scales << 7
+                                                                        : scales >> 1);
+}
+
+// Two tiles of 16 tokens from token `at` on, for R row tiles.  MASKED: some row does
+// not see all of them.  `visible`: the keys this lane's rows see; `keys`: those there are.
+// P of bf16 has 8 significant bits, its rounding averaging out over the keys;
+// where the output has 11 (SPLIT_P) the rest of P is a second bf16 operand.
+template <int D, int PARTS, int R, bool MASKED, bool SPLIT_P>
+__device__ inline void attend(const Query<D, PARTS> (&q)[R], Tile<D> (&t)[2], int at,
+                              const int (&visible)[R], int keys, float scale_log2, int quad,
+                              State<D> (&st)[R]) {
   constexpr int NT = D / 16;
-  float s[2][4];
+  v8bf p_hi[R], p_lo[R];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < R; ++r) {
+    float s[2][4];
 #pragma unroll
-    for (int k = 0; k < Query<D, PARTS>::kSteps; ++k) {
-      v8i kc = {static_cast<int>(t[h].k[k].x), static_cast<int>(t[h].k[k].y),
-                static_cast<int>(t[h].k[k].z), static_cast<int>(t[h].k[k].w), 0, 0, 0, 0};
+    for (int h = 0; h < 2; ++h) {
+      v4f acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int p = PARTS - 1; p >= 0; --p)
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            kc, q.part[p][k], acc, 4, 0, 0, t[h].k_scale[k], 0, q.scale[p]);
+      for (int k = 0; k < Query<D, PARTS>::kSteps; ++k) {
+        v8i kc = {static_cast<int>(t[h].k[k].x), static_cast<int>(t[h].k[k].y),
+                  static_cast<int>(t[h].k[k].z), static_cast<int>(t[h].k[k].w), 0, 0, 0, 0};
+#pragma unroll
+        for (int p = PARTS - 1; p >= 0; --p)
+          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              kc, q[r].part[p][k], acc, 4, 0, 0, t[h].k_scale[k], 0, q[r].scale[p]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[h][i] = acc[i] * scale_log2;
+        if (MASKED && at + 16 * h + quad * 4 + i >= visible[r]) s[h][i] = -INFINITY;
+      }
     }
+    float top = s[0][0];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[h][i] = acc[i] * scale_log2;
-      if (MASKED && at + 16 * h + quad * 4 + i >= visible) s[h][i] = -INFINITY;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
+    if (__any(top > st[r].m + kSlack)) {
+      const float m = fmaxf(st[r].m, max_over_quads(top));
+      const float fade = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st[r].m - m);
+      st[r].m = m;
+      st[r].l *= fade;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
     }
-  }
-  float top = s[0][0];
+    const float ref = MASKED && st[r].m == -INFINITY ? 0.f : st[r].m;   // nothing seen yet
+    uint32_t hi[4], lo[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      float p[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
-  top = max_over_quads(top);
-  const float m = fmaxf(st.m, top);
-  const float ref = m == -INFINITY ? 0.f : m;     // a row that sees nothing yet
-  const float fade = __builtin_amdgcn_exp2f(st.m - ref);
-  st.m = m;
-  st.l *= fade;
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(s[h][i] - ref);
+        st[r].l += p[i];
+      }
 #pragma unroll
-  for (int j = 0; j < NT; ++j) st.o[j] *= fade;
-  uint32_t p_hi[4], p_lo[4];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(s[h][i] - ref);
-      st.l += p[i];
-    }
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const uint32_t u = pack_bf16(p[2 * w], p[2 * w + 1]);
-      p_hi[2 * h + w] = u;
-      if constexpr (SPLIT_P)
-        p_lo[2 * h + w] = pack_bf16(p[2 * w] - bits_f32(u << 16),
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t u = pack_bf16(p[2 * w], p[2 * w + 1]);
+        hi[2 * h + w] = u;
+        if constexpr (SPLIT_P)
+          lo[2 * h + w] = pack_bf16(p[2 * w] - bits_f32(u << 16),
                                     p[2 * w + 1] - bits_f32(u & 0xffff0000u));
+      }
     }
+    p_hi[r] = __builtin_bit_cast(v8bf, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+    if constexpr (SPLIT_P)
+      p_lo[r] = __builtin_bit_cast(v8bf, make_uint4(lo[0], lo[1], lo[2], lo[3]));
   }
   // V: masked tokens hold nothing, whatever their bytes are
   bool any_lost = false;
   uint32_t lost[2] = {0, 0};     // byte i: 255 where token i's group is NaN
-  float vs[2][4];
+  if constexpr (MASKED) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t b = (t[h].v_scale >> (8 * i)) & 255u;
-      if constexpr (MASKED) {
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t byte = 255u << (8 * i);
         const bool there = at + 16 * h + quad * 4 + i < keys;
-        const bool nan = there && b == 255u;
-        if (nan) lost[h] |= 255u << (8 * i);
+        const bool nan = there && (t[h].v_scale & byte) == byte;
+        if (nan) lost[h] |= byte;
         any_lost |= nan;
         if (!there || nan) {
-          b = 127;
+          t[h].v_scale &= ~byte;
 #pragma unroll
           for (int w = 0; w < Tile<D>::kWords; ++w) t[h].v[i][w] = 0;
         }
       }
-      vs[h][i] = bits_f32(b << 23);
-    }
-  const v8bf ph = __builtin_bit_cast(v8bf, make_uint4(p_hi[0], p_hi[1], p_hi[2], p_hi[3]));
-  v8bf pl;
-  if constexpr (SPLIT_P)
-    pl = __builtin_bit_cast(v8bf, make_uint4(p_lo[0], p_lo[1], p_lo[2], p_lo[3]));
+  }
 #pragma unroll
   for (int j = 0; j < NT; j += 2) {
     uint32_t w[2][4];     // elements j, j + 1 of each token
@@ -387,7 +470,8 @@ __device__ inline void attend(const Query<D, PARTS>& q, Tile<D> (&t)[2], int at,
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        w[h][i] = cvt_bf16(t[h].v[i][D >= 128 ? j / 8 : 0], vs[h][i], (j / 2) % 4);
+        w[h][i] = cvt_bf16(t[h].v[i][D >= 128 ? j / 8 : 0], byte_scale(t[h].v_scale, i),
+                           (j / 2) % 4);
     uint4 even, odd;
     even.x = perm(w[0][1], w[0][0], 0x05040100u);
     even.y = perm(w[0][3], w[0][2], 0x05040100u);
@@ -398,11 +482,16 @@ __device__ inline void attend(const Query<D, PARTS>& q, Tile<D> (&t)[2], int at,
     odd.z = perm(w[1][1], w[1][0], 0x07060302u);
     odd.w = perm(w[1][3], w[1][2], 0x07060302u);
     const v8bf ve = __builtin_bit_cast(v8bf, even), vo = __builtin_bit_cast(v8bf, odd);
-    st.o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, ph, st.o[j], 0, 0, 0);
-    st.o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, ph, st.o[j + 1], 0, 0, 0);
-    if constexpr (SPLIT_P) {
-      st.o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, pl, st.o[j], 0, 0, 0);
-      st.o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, pl, st.o[j + 1], 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      st[r].o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, p_hi[r], st[r].o[j], 0, 0, 0);
+      st[r].o[j + 1] =
+          __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, p_hi[r], st[r].o[j + 1], 0, 0, 0);
+      if constexpr (SPLIT_P) {
+        st[r].o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, p_lo[r], st[r].o[j], 0, 0, 0);
+        st[r].o[j + 1] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, p_lo[r], st[r].o[j + 1], 0, 0, 0);
+      }
     }
   }
   if constexpr (MASKED) {
@@ -410,8 +499,6 @@ __device__ inline void attend(const Query<D, PARTS>& q, Tile<D> (&t)[2], int at,
     // reach those that do not, so the product took zeros, and the rows that see
     // it become NaN here.
     if (__any(any_lost)) {
-      const int row = (threadIdx.x & 15);
-      (void)row;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         for (int tok = 0; tok < 16; ++tok)
@@ -419,10 +506,12 @@ __device__ inline void attend(const Query<D, PARTS>& q, Tile<D> (&t)[2], int at,
           for (int i = 0; i < 4; ++i) {
             const uint32_t f = static_cast<uint32_t>(
                 __shfl(static_cast<int>(lost[h]), (tok / 4) * 16 + quad * 4 + i));
-            if (((f >> (8 * (tok % 4))) & 255u) && at + 16 * h + tok < visible) {
 #pragma unroll
-              for (int j = 0; j < NT; ++j) st.o[j][i] = bits_f32(0x7fc00000u);
-            }
+            for (int r = 0; r < R; ++r)
+              if (((f >> (8 * (tok % 4))) & 255u) && at + 16 * h + tok < visible[r]) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) st[r].o[j][i] = bits_f32(0x7fc00000u);
+              }
           }
     }
   }
@@ -438,89 +527,257 @@ __device__ inline uint32_t narrow2(float a, float b) {
   return __builtin_bit_cast(uint32_t, r);
 }
 
-// One wavefront for a row tile of one K/V head.
+// Row r of a tile: the packed query row, its head and the keys it sees.
+struct Row {
+  int64_t at;
+  int head, visible;
+};
+__device__ inline Row row_of(const Args& a, const Seq& s, int r, int kv_head) {
+  const int pos = a.group_div.div(r);
+  Row row;
+  row.at = static_cast<int64_t>(s.first) + pos;
+  row.head = kv_head * a.group + (r - pos * a.group);
+  const int keys = max(s.keys, 0);
+  row.visible = a.causal ? max(0, keys - s.count + pos + 1) : keys;
+  return row;
+}
+
+// A row's elements (D / 16) * 4 quad .. as the output's type, and its lse.
 template <class T, int D>
-__global__ __launch_bounds__(64) void mx4_attention_kernel(const Args a) {
-  constexpr int PARTS = __is_same(T, __bf16) ? 2 : 3;
-  constexpr bool SPLIT_P = !__is_same(T, __bf16);
+__device__ inline void write_row(const Args& a, const Row& row, int quad, const v4f (&o)[D / 16],
+                                 float m, float l) {
   constexpr int NT = D / 16;
-  const int head = blockIdx.x % a.heads;
-  const int tile = blockIdx.x / a.heads;
-  int lo = 0, hi = a.batch;        // the last sequence whose tiles start at or before `tile`
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (tile_base(a, mid) <= tile) lo = mid;
-    else hi = mid;
-  }
-  const int b = uniform(lo);
-  const Seq seq = sequence(a, b);
-  const int first = (tile - tile_base(a, b)) * kRows;
-  const int rows = min(kRows, seq.count * a.group - first);
-  if (rows <= 0) return;
-  const int lane = threadIdx.x, quad = lane >> 4;
-  const int r = first + min(lane & 15, rows - 1);
-  const int pos = a.group_div.div(r), in_group = r - pos * a.group;
-  const bool valid = (lane & 15) < rows;
-  const int keys = max(seq.keys, 0);
-  const int visible = a.causal ? max(0, keys - seq.count + pos + 1) : keys;
-  // of the tile's rows, in order: the first sees the fewest, the last the most
-  const int fewest = __shfl(visible, 0), most = uniform(__shfl(visible, rows - 1));
-  const int64_t q_at = static_cast<int64_t>(seq.first + pos);
-  const int64_t hq = static_cast<int64_t>(head) * a.group + in_group;
-  Query<D, PARTS> q;
-  load_query<T, D, PARTS>(a.q + q_at * a.q_row + hq * a.q_head, valid, quad, a.scale_log2 < 0.f, q);
-  State<D> st;
-  st.m = -INFINITY;
-  st.l = 0.f;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) st.o[j] = {0.f, 0.f, 0.f, 0.f};
-  const Lanes<D> o = lane_offsets<D>(lane, a.tokens);
-  const float scale_log2 = fabsf(a.scale_log2);
-  bool bad = seq.keys < 0;
-  const int last_tile = (most - 1) / kMx4TokenTile;
-  for (int at = 0; at < most; at += kStep) {
-    Tile<D> t[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // past the last tile: that one again, masked as a whole
-      const int i = min(at / kMx4TokenTile + h, last_tile);
-      const int page = a.tiles_per_block.div(i);
-      int64_t block = index_at(a.table, b * a.table_row + page, a.index64);
-      if (block < 0 || block >= a.num_blocks) {
-        bad = true;
-        block = 0;
-      }
-      block = uniform64(block);
-      const int offset = (i - page * static_cast<int>(a.tiles_per_block.d)) * kMx4TokenTile;
-      load_tile<D>(a, o, block, head, offset, quad, t[h]);
-    }
-    if (at + kStep <= fewest)
-      attend<D, PARTS, false, SPLIT_P>(q, t, at, visible, keys, scale_log2, quad, st);
-    else
-      attend<D, PARTS, true, SPLIT_P>(q, t, at, visible, keys, scale_log2, quad, st);
-  }
-  const float l = bad ? bits_f32(0x7fc00000u) : sum_over_quads(st.l);
-  if (!valid) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* const out = a.out + q_at * a.out_row + hq * a.out_head + quad * 4 * NT * 2;
+  char* const out = a.out + row.at * a.out_row + row.head * a.out_head + quad * 4 * NT * 2;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t w[NT / 2];
 #pragma unroll
-    for (int j = 0; j < NT; j += 2) w[j / 2] = narrow2<T>(st.o[j][i] * inv, st.o[j + 1][i] * inv);
+    for (int j = 0; j < NT; j += 2) w[j / 2] = narrow2<T>(o[j][i] * inv, o[j + 1][i] * inv);
 #pragma unroll
     for (int x = 0; x < NT / 2; x += 2)
       *reinterpret_cast<uint2*>(out + (i * NT + 2 * x) * 2) = make_uint2(w[x], w[x + 1]);
   }
   if (a.lse && quad == 0)
-    a.lse[q_at * a.lse_row + hq * a.lse_head] =
-        l == 0.f ? -INFINITY : (st.m + __builtin_amdgcn_logf(l)) * kLn2;
+    a.lse[row.at * a.lse_row + row.head * a.lse_head] =
+        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// One workgroup for a cut of the keys of a tile of 16 R rows of one K/V head.
+template <class T, int D, int R>
+__global__ __launch_bounds__(kThreads) void mx4_attention_kernel(const Args a) {
+  constexpr int PARTS = __is_same(T, __bf16) ? 2 : 3;
+  constexpr bool SPLIT_P = !__is_same(T, __bf16);
+  constexpr int NT = D / 16;
+  __shared__ v4f sum_o[2][R * NT][64];
+  __shared__ float sum_m[kWaves][R][16], sum_l[kWaves][R][16];
+  const int item = a.heads_div.div(blockIdx.x);
+  const int kv_head = blockIdx.x - item * a.heads;
+  const Work w = find_work(a, item, kRows * R, false);
+  if (w.seq < 0) return;
+  const Seq seq = sequence(a, w.seq);
+  const int first = w.tile * kRows * R;
+  const int rows = min(kRows * R, seq.count * a.group - first);
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
+  const int keys = max(seq.keys, 0);
+  Query<D, PARTS> q[R];
+  State<D> st[R];
+  int visible[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int n = 16 * r + (lane & 15);
+    const Row row = row_of(a, seq, first + min(n, rows - 1), kv_head);
+    visible[r] = row.visible;
+    load_query<T, D, PARTS>(a.q + row.at * a.q_row + row.head * a.q_head, n < rows, quad,
+                            a.scale_log2 < 0.f, q[r]);
+    st[r].m = -INFINITY;
+    st[r].l = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) st[r].o[j] = {0.f, 0.f, 0.f, 0.f};
+  }
+  // of the tile's rows, in order, the first sees the fewest, the last the most
+  const int fewest = uniform(visible[0]);
+  const int most = uniform(__shfl(visible[R - 1], 15));
+  const Lanes<D> o = lane_offsets<D>(lane, a.tokens);
+  const float scale_log2 = fabsf(a.scale_log2);
+  bool bad = seq.keys < 0;
+  const int last_tile = (most - 1) / kMx4TokenTile;
+  const int all_steps = (most + kStep - 1) / kStep;
+  const int end = w.cuts > 1 ? min(all_steps, (w.cut + 1) * w.steps) : all_steps;
+  // the block ids of the next 32 steps of this wavefront, two tiles each, a lane a tile
+  int ids = 0;
+  auto load_ids = [&](int step) {
+    const int i = (step + (lane >> 1) * kWaves) * 2 + (lane & 1);
+    const int tile = min(i, last_tile);
+    const int page = a.tiles_per_block.div(tile);
+    int64_t id = 0;
+    if (i < 2 * end) id = index_at(a.table, w.seq * a.table_row + page, a.index64);
+    if (id < 0 || id >= a.num_blocks) {
+      bad = true;
+      id = 0;
+    }
+    ids = static_cast<int>(id);
+  };
+  auto load_step = [&](int step, int nth, Tile<D> (&t)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // past the last tile: that one again, masked as a whole
+      const int i = min(2 * step + h, last_tile);
+      const int page = a.tiles_per_block.div(i);
+      const int offset = (i - page * static_cast<int>(a.tiles_per_block.d)) * kMx4TokenTile;
+      load_tile<D>(a, o, __builtin_amdgcn_readlane(ids, 2 * nth + h), kv_head, offset, quad, t[h]);
+    }
+  };
+  int step = (w.cuts > 1 ? w.cut * w.steps : 0) + wave;
+  if (step < end) {
+    Tile<D> t[2], next[2];
+    load_ids(step);
+    load_step(step, 0, next);
+    for (int nth = 1; step < end; ++nth) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) t[h] = next[h];
+      const int at = step * kStep;
+      step += kWaves;
+      if (step < end) {
+        if (nth == 32) {
+          load_ids(step);
+          nth = 0;
+        }
+        load_step(step, nth, next);
+      }
+      if (at + kStep <= fewest)
+        attend<D, PARTS, R, false, SPLIT_P>(q, t, at, visible, keys, scale_log2, quad, st);
+      else
+        attend<D, PARTS, R, true, SPLIT_P>(q, t, at, visible, keys, scale_log2, quad, st);
+    }
+  }
+  // The four wavefronts' sums: each to the common reference, then 2 and 3 onto
+  // 0 and 1, then 1 onto 0.
+  const bool any_bad = __any(bad);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float l = sum_over_quads(st[r].l);
+    if (quad == 0) {
+      sum_m[wave][r][lane] = st[r].m;
+      sum_l[wave][r][lane] = any_bad ? bits_f32(0x7fc00000u) : l;
+    }
+  }
+  __syncthreads();
+  float m_all[R], l_all[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) m = fmaxf(m, sum_m[x][r][lane & 15]);
+    m_all[r] = m;
+    const float ref = m == -INFINITY ? 0.f : m;
+    l_all[r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x)
+      l_all[r] += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - ref);
+    const float f = __builtin_amdgcn_exp2f(st[r].m - ref);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) st[r].o[j] *= f;
+  }
+#pragma unroll
+  for (int half = kWaves / 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sum_o[wave - half][r * NT + j][lane] = st[r].o[j];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) st[r].o[j] += sum_o[wave][r * NT + j][lane];
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int n = 16 * r + (lane & 15);
+    if (n >= rows) continue;
+    if (w.cuts == 1) {
+      const Row row = row_of(a, seq, first + n, kv_head);
+      write_row<T, D>(a, row, quad, st[r].o, m_all[r], l_all[r]);
+    } else {
+      if (quad == 0)
+        a.part_ml[static_cast<int64_t>(blockIdx.x) * kRows * R + n] = make_float2(m_all[r], l_all[r]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        a.part_o[(static_cast<int64_t>(blockIdx.x) * R * NT + r * NT + j) * 64 + lane] = st[r].o[j];
+    }
+  }
+}
+
+// Joins the cuts of 16 rows: a wavefront takes every fourth cut of the rows' elements
+// of 4 registers, so cuts are read 4 at a time; the workgroup's sums are added in
+// the order of its wavefronts.
+template <class T, int D, int R>
+__global__ __launch_bounds__(kThreads) void mx4_join_kernel(const Args a) {
+  constexpr int NT = D / 16;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
+  const int item = a.heads_div.div(blockIdx.x);
+  const int kv_head = blockIdx.x - item * a.heads;
+  const Work w = find_work(a, item, kRows * R, true);
+  if (w.seq < 0 || w.cuts == 1) return;
+  const Seq seq = sequence(a, w.seq);
+  const int r = blockIdx.y;
+  const int first = (w.tile * R + r) * kRows;
+  const int rows = min(kRows, seq.count * a.group - first);
+  if (rows <= 0) return;
+  const bool valid = (lane & 15) < rows;
+  __shared__ v4f sum_o[kWaves][NT][64];
+  __shared__ float sum_m[kWaves][16], sum_l[kWaves][16];
+  v4f o[NT];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) o[j] = {0.f, 0.f, 0.f, 0.f};
+  if (valid) {
+    for (int c = wave; c < w.cuts; c += kWaves) {
+      const int64_t at = static_cast<int64_t>(w.first + c) * a.heads + kv_head;
+      const float2 ml = a.part_ml[at * kRows * R + 16 * r + (lane & 15)];
+      const float top = fmaxf(m, ml.x);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(ml.x - ref);
+      m = top;
+      l = l * f + ml.y * g;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        o[j] = o[j] * f + a.part_o[(at * R * NT + r * NT + j) * 64 + lane] * g;
+    }
+  }
+  if (quad == 0) sum_m[wave][lane] = m, sum_l[wave][lane] = l;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) sum_o[wave][j][lane] = o[j];
+  __syncthreads();
+  if (wave || !valid) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x) top = fmaxf(top, sum_m[x][lane & 15]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  l = 0.f;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) o[j] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x) {
+    const float f = __builtin_amdgcn_exp2f(sum_m[x][lane & 15] - ref);
+    l += sum_l[x][lane & 15] * f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[j] += sum_o[x][j][lane] * f;
+  }
+  const Row row = row_of(a, seq, first + (lane & 15), kv_head);
+  write_row<T, D>(a, row, quad, o, top, l);
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 
-int check_attention(const fkv_mx4_attention_args& c) {
+int check_sizes(const fkv_mx4_attention_args& c) {
   int rc;
   if (c.batch < 0 || c.num_queries < 0)
     return fail(kInval, "negative count: batch=%d num_queries=%d", c.batch, c.num_queries);
@@ -541,9 +798,14 @@ int check_attention(const fkv_mx4_attention_args& c) {
   if (static_cast<int64_t>(c.num_queries) * c.group_size >= int64_t(1) << 30)
     return fail(kInval, "%d queries of %d heads a K/V head are too many for one call",
                 c.num_queries, c.group_size);
-  if (c.batch == 0 || c.num_queries == 0) return 0;
-  if (!c.query_starts && c.num_queries < c.batch)
+  if (!c.query_starts && c.num_queries < c.batch && c.num_queries > 0)
     return fail(kInval, "%d sequences of one query each, but %d queries", c.batch, c.num_queries);
+  return 0;
+}
+
+int check_attention(const fkv_mx4_attention_args& c) {
+  const int rc = check_sizes(c);
+  if (rc || c.batch == 0 || c.num_queries == 0) return rc;
   if (!c.query || !c.out || !c.seq_lens || (!c.block_table && c.table_width > 0))
     return fail(kInval, "null pointer argument");
   const int64_t aligned[] = {c.query_row_stride_bytes, c.query_head_stride_bytes,
@@ -557,16 +819,68 @@ int check_attention(const fkv_mx4_attention_args& c) {
                          2, mx4_chunk_bytes(c.tokens_per_block, c.num_heads, c.head_size));
 }
 
+// Workgroups the keys are cut into where there are few tiles: 8 a compute unit,
+// so that those of uneven sequences even out.
+constexpr int kCutTarget = 2048;
+
+struct LaunchPlan {
+  int row_tiles;          // R
+  int64_t tiles;          // times heads: the most there can be
+  int target;
+  int64_t workgroups;
+  size_t ml_bytes, o_bytes;
+};
+
+LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
+  LaunchPlan p;
+  const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
+  p.row_tiles = rows <= static_cast<int64_t>(c.batch) * kRows ? 1 : 2;
+  const int rows_a_tile = kRows * p.row_tiles;
+  const int64_t tiles = c.query_starts
+      ? rows / rows_a_tile + c.batch
+      : static_cast<int64_t>(c.batch) * ((c.group_size + rows_a_tile - 1) / rows_a_tile);
+  p.tiles = tiles * c.num_heads;
+  const int64_t most_steps =
+      (static_cast<int64_t>(c.table_width) * c.tokens_per_block + kStep - 1) / kStep;
+  p.target = p.tiles < kCutTarget && most_steps > kMinSteps ? kCutTarget : 0;
+  p.workgroups = p.tiles + p.target;
+  p.ml_bytes = p.target ? p.workgroups * rows_a_tile * sizeof(float2) : 0;
+  p.o_bytes = p.target ? p.workgroups * rows_a_tile * static_cast<int64_t>(c.head_size) * 4 : 0;
+  return p;
+}
+
+template <class T, int D, int R>
+void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
+  hipLaunchKernelGGL((mx4_attention_kernel<T, D, R>), dim3(p.workgroups), dim3(kThreads), 0, s, a);
+  if (p.target)
+    hipLaunchKernelGGL((mx4_join_kernel<T, D, R>), dim3(p.tiles, R), dim3(kThreads), 0, s, a);
+}
+template <class T, int D>
+void launch_rows(const Args& a, const LaunchPlan& p, hipStream_t s) {
+  if (p.row_tiles == 1) launch<T, D, 1>(a, p, s);
+  else launch<T, D, 2>(a, p, s);
+}
 template <class T>
-void launch_attention(const Args& a, int dim, dim3 grid, hipStream_t s) {
-  if (dim == 64) hipLaunchKernelGGL((mx4_attention_kernel<T, 64>), grid, dim3(64), 0, s, a);
-  else if (dim == 128) hipLaunchKernelGGL((mx4_attention_kernel<T, 128>), grid, dim3(64), 0, s, a);
-  else hipLaunchKernelGGL((mx4_attention_kernel<T, 256>), grid, dim3(64), 0, s, a);
+void launch_attention(const Args& a, const LaunchPlan& p, int dim, hipStream_t s) {
+  if (dim == 64) launch_rows<T, 64>(a, p, s);
+  else if (dim == 128) launch_rows<T, 128>(a, p, s);
+  else launch_rows<T, 256>(a, p, s);
 }
 
 }  // namespace
 
 extern "C" {
+
+int fkv_mx4_attention_workspace(const fkv_mx4_attention_args* args, size_t* bytes) {
+  last_error().clear();
+  if (!args || !bytes) return fail(kInval, "null pointer argument");
+  *bytes = 0;
+  const int rc = check_sizes(*args);
+  if (rc || args->batch == 0 || args->num_queries == 0) return rc;
+  const LaunchPlan p = launch_plan(*args);
+  *bytes = p.ml_bytes + p.o_bytes;
+  return 0;
+}
 
 int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
   try {
@@ -575,6 +889,11 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
     const fkv_mx4_attention_args& c = *args;
     int rc = check_attention(c);
     if (rc || c.batch == 0 || c.num_queries == 0) return rc;
+    const LaunchPlan p = launch_plan(c);
+    if (p.target && (!c.workspace || c.workspace_bytes < p.ml_bytes + p.o_bytes ||
+                     reinterpret_cast<uintptr_t>(c.workspace) % 16))
+      return fail(kInval, "the workspace must hold %zu bytes on a multiple of 16, got %zu",
+                  p.ml_bytes + p.o_bytes, c.workspace ? c.workspace_bytes : 0);
     Args a;
     a.q = static_cast<const char*>(c.query);
     a.out = static_cast<char*>(c.out);
@@ -590,23 +909,23 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
     a.num_blocks = static_cast<int>(c.num_mx_blocks), a.width = c.table_width;
     a.batch = c.batch, a.heads = c.num_heads, a.group = c.group_size, a.queries = c.num_queries;
     a.tokens = c.tokens_per_block, a.causal = c.causal;
+    a.target = p.target;
     a.scale_log2 = c.scale * kLog2e;
+    a.part_o = static_cast<v4f*>(c.workspace);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.workspace) + p.o_bytes);
     a.tiles_per_block = FastDiv(c.tokens_per_block / kMx4TokenTile);
     a.group_div = FastDiv(c.group_size);
-    const int64_t tiles = c.query_starts
-        ? static_cast<int64_t>(c.num_queries) * c.group_size / kRows + c.batch
-        : static_cast<int64_t>(c.batch) * ((c.group_size + kRows - 1) / kRows);
-    if (tiles * c.num_heads >= int64_t(1) << 31)
+    a.heads_div = FastDiv(c.num_heads);
+    if (p.workgroups >= int64_t(1) << 31)
       return fail(kInval, "%d queries of %d K/V heads are too many for one call", c.num_queries,
                   c.num_heads);
     hipStream_t s = static_cast<hipStream_t>(stream);
     int dev = 0;
     DeviceGuard guard;
     if ((rc = stream_device(s, &dev)) || (rc = guard.set(dev))) return rc;
-    const dim3 grid(static_cast<uint32_t>(tiles * c.num_heads));
     (void)hipGetLastError();
-    if (c.dtype == FKV_DTYPE_BF16) launch_attention<__bf16>(a, c.head_size, grid, s);
-    else launch_attention<_Float16>(a, c.head_size, grid, s);
+    if (c.dtype == FKV_DTYPE_BF16) launch_attention<__bf16>(a, p, c.head_size, s);
+    else launch_attention<_Float16>(a, p, c.head_size, s);
     FKV_HIP(hipGetLastError());
     return 0;
   } catch (const std::exception& e) {

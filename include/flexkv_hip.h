@@ -470,7 +470,13 @@ typedef struct fkv_mx4_attention_args {
   int table_width, batch, num_queries;
   int tokens_per_block, num_heads, group_size, head_size, dtype, causal;
   float scale;
+  void* workspace;                   /* device memory, on a multiple of 16; see below */
+  size_t workspace_bytes;
 } fkv_mx4_attention_args;
+/* The workspace a call of these sizes needs (pointers and strides are not looked
+ * at, but for whether query_starts is null); 0 for none.  It holds nothing between calls, and no
+ * two that may run at the same time may share one. */
+int fkv_mx4_attention_workspace(const fkv_mx4_attention_args* args, size_t* bytes);
 int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream);
 
 /* How copy-engine mode (use_ce_transfer = FKV_XFER_CE) chooses between the
