@@ -22,16 +22,17 @@
 // The maximum is a reference that follows only when a score passes it by 2^8, so
 // most steps neither compare across lanes nor scale the sums.
 //
-// A workgroup's four wavefronts take the 32-token steps of its tile in turn, each
-// loading its next step while it computes one, and add up in LDS.  With few
-// tiles the keys are cut among workgroups as well (Plan), whose sums a second
-// kernel joins in a fixed order.
+// A workgroup's wavefronts take the 32-token steps of its tile in turn, each loading
+// its next step while it computes one, and add up in LDS.  With few tiles the keys
+// are cut among workgroups as well (find_work), whose sums a second kernel joins
+// in a fixed order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <type_traits>
 
 #include "kv_mx4.h"
 
@@ -41,6 +42,8 @@ namespace {
 
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t Vec2 __attribute__((ext_vector_type(2)));
+typedef uint32_t Vec4 __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -48,10 +51,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 16;          // rows of a tile: columns of a matrix instruction
 constexpr int kStep = 32;          // tokens of a step: two tiles of 16, k of the second product
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kMinSteps = 4;       // of a workgroup, where the keys are cut
-constexpr float kSlack = 8.f;      // log2 by which a score may pass the reference
+constexpr int kMinSteps = 16;      // of a workgroup, where the keys are cut
+constexpr float kSlack = 256.f;    // weight up to which a score may pass the reference
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -61,6 +62,16 @@ __device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
   return __builtin_amdgcn_perm(hi, lo, sel);
 }
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// A chunk of the cache as a buffer: its address is scalar, a lane adds 32 bits of
+// offset, and nothing outside the chunk is read.
+typedef __amdgpu_buffer_rsrc_t Chunk;
+__device__ inline Chunk chunk_at(const char* p, int bytes) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint64_t lo = static_cast<uint32_t>(uniform(static_cast<int>(u)));
+  const uint64_t hi = static_cast<uint32_t>(uniform(static_cast<int>(u >> 32)));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(hi << 32 | lo), 0, bytes,
+                                           0x00027000);
+}
 // quads: the 4 groups of 16 lanes
 __device__ inline float max_over_quads(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
@@ -90,7 +101,7 @@ struct Args {
   int index64;                       // table, lens and starts are int64
   int num_blocks, width;             // of the cache; of a table row
   int batch, heads, group, queries;
-  int tokens;                        // of a block
+  int tokens, chunk;                 // of a block; bytes of a chunk
   int causal;
   int target;                        // workgroups to cut the keys into; 0: uncut
   float scale_log2;
@@ -125,26 +136,41 @@ __device__ inline Seq sequence(const Args& a, int b) {
   return s;
 }
 
+// Inclusive sums over the lanes of a wavefront.
+template <class V>
+__device__ inline V scan_lanes(V v) {
+  auto add = [&v](auto ctrl, auto rows) {
+    v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
+                                                           decltype(ctrl)::value,
+                                                           decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());   // 1, 2, 4, 8 lanes before
+  add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());   // lane 15 of the row before
+  add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());   // lane 31
+  return v;
+}
+__device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
 // How the workgroups are dealt out.  A sequence has ceil(queries * group / rows a tile)
 // tiles; where the keys are cut, every tile's into cuts of the same number of
-// steps, chosen from the lengths on the device so that there are about `target`
-// of them in all however uneven the sequences are.  Every wavefront works this out
-// for itself: sequence b = lane, then 64 further on.
+// steps, chosen from the lengths on the device so that there are at most `target`
+// more of them than tiles, however uneven the sequences are.  Every wavefront works
+// this out for itself: sequence b = lane, then 64 further on.
 struct Work {
-  int seq, tile, cut, cuts;   // seq < 0: none
+  int seq;                    // < 0: none
+  int tile, cut, cuts;
   int steps;                  // of a cut
-  int first;                  // the tile's first cut's number
+  int first;                  // the number of the tile's first cut
+  Seq s;
 };
 __device__ inline int tiles_of(const Args& a, const Seq& s, int rows_a_tile) {
   return (s.count * a.group + rows_a_tile - 1) / rows_a_tile;
 }
 __device__ inline int steps_of(const Seq& s) { return (max(s.keys, 0) + kStep - 1) / kStep; }
-
-__device__ inline int64_t sum_over_lanes(int64_t v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  return v;
-}
 
 // Item `item` of the plan; by_tile: `item` counts tiles, the answer is its first cut.
 __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool by_tile) {
@@ -152,16 +178,17 @@ __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool 
   int per_cut = 1 << 30;
   Seq s{0, 0, 0};
   if (a.target) {
-    int64_t total = 0;
+    float total = 0.f;
     for (int b = lane; b < a.batch; b += 64) {
       s = sequence(a, b);
-      total += static_cast<int64_t>(tiles_of(a, s, rows_a_tile)) * steps_of(s);
+      total += static_cast<float>(tiles_of(a, s, rows_a_tile)) * static_cast<float>(steps_of(s));
     }
-    total = sum_over_lanes(total) * a.heads;
-    const int64_t even = (total + a.target - 1) / a.target;
-    per_cut = static_cast<int>(max(even, static_cast<int64_t>(kMinSteps)));
+    total = bits_f32(lane_value(f32_bits(scan_lanes(total)), 63));
+    // rounded up by more than the sum's error
+    const float even = total * a.heads / a.target * 1.0001f;
+    per_cut = max(kMinSteps, static_cast<int>(fminf(even, 1e9f)) + 1);
   }
-  Work w{-1, 0, 0, 0, per_cut, 0};
+  Work w{-1, 0, 0, 0, per_cut, 0, Seq{0, 0, 0}};
   int before = 0, cuts_before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int b = b0 + lane;
@@ -169,40 +196,37 @@ __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool 
     if (b < a.batch) {
       if (!a.target || a.batch > 64) s = sequence(a, b);
       tiles = tiles_of(a, s, rows_a_tile);
-      cuts = max(1, (steps_of(s) + per_cut - 1) / per_cut);
+      cuts = a.target ? max(1, (steps_of(s) + per_cut - 1) / per_cut) : 1;
     }
-    int ends = by_tile ? tiles : tiles * cuts, cut_ends = tiles * cuts;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int e = __shfl_up(ends, d), c = __shfl_up(cut_ends, d);
-      if (lane >= d) ends += e, cut_ends += c;
-    }
+    const int cut_ends = scan_lanes(tiles * cuts);
+    const int ends = by_tile ? scan_lanes(tiles) : cut_ends;
     const uint64_t later = __ballot(before + ends > item);
     if (later) {
-      const int at = __ffsll(static_cast<unsigned long long>(later)) - 1;
-      const int n = uniform(__shfl(tiles, at)), c = uniform(__shfl(cuts, at));
-      const int start = before + uniform(__shfl(ends, at)) - (by_tile ? n : n * c);
-      const int local = item - start;
+      const int at = __builtin_ctzll(later);
+      const int n = lane_value(tiles, at), c = lane_value(cuts, at);
+      const int local = item - (before + lane_value(ends, at) - (by_tile ? n : n * c));
       w.seq = b0 + at;
       w.cuts = c;
-      w.tile = by_tile ? local : local / c;
+      w.tile = by_tile || c == 1 ? local : local / c;
       w.cut = by_tile ? 0 : local - w.tile * c;
-      w.first = cuts_before + uniform(__shfl(cut_ends, at)) - n * c + w.tile * c;
+      w.first = cuts_before + lane_value(cut_ends, at) - n * c + w.tile * c;
+      w.s = {lane_value(s.first, at), lane_value(s.count, at), lane_value(s.keys, at)};
       return w;
     }
-    before += uniform(__shfl(ends, 63));
-    cuts_before += uniform(__shfl(cut_ends, 63));
+    before += lane_value(ends, 63);
+    cuts_before += lane_value(cut_ends, 63);
   }
   return w;
 }
 
-// The queries of one row as e4m3 parts: operand registers for each part and
-// 128-element step, and the scale bytes.
+// The queries of 16 rows as e4m3 parts: operand registers for each part and
+// 128-element step, and the scale bytes, part p's in byte p.
 template <int D, int PARTS>
 struct Query {
   static constexpr int kSteps = (D + 127) / 128;
+  static constexpr int kVectors = PARTS * kSteps * 2;   // of 16 bytes a lane
   v8i part[PARTS][kSteps];
-  int scale[PARTS];
+  int scale;
 };
 
 template <class T>
@@ -253,8 +277,9 @@ __device__ inline void load_query(const char* row, bool valid, int quad, bool ne
   const bool lost = top >= 0x7f800000u;
   const int e = max(static_cast<int>(top >> 23) - 7, 4 * (PARTS - 1));
   const float up = lost ? 0.f : bits_f32(static_cast<uint32_t>(254 - e) << 23);
+  q.scale = 0;
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) q.scale[p] = lost ? 255 : e - 4 * p;
+  for (int p = 0; p < PARTS; ++p) q.scale |= (lost ? 255 : e - 4 * p) << (8 * p);
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
@@ -290,7 +315,7 @@ template <int D>
 struct Tile {
   static constexpr int kSteps = (D + 127) / 128;
   static constexpr int kWords = D >= 128 ? D / 128 : 1;   // of V a token: D / 16 codes
-  uint4 k[kSteps];
+  Vec4 k[kSteps];
   int k_scale[kSteps];
   uint32_t v[4][kWords];
   uint32_t v_scale;     // of 4 tokens
@@ -315,33 +340,31 @@ __device__ inline Lanes<D> lane_offsets(int lane, int tokens) {
 }
 
 template <int D>
-__device__ inline void load_tile(const Args& a, const Lanes<D>& o, int64_t block, int head,
-                                 int offset, int quad, Tile<D>& t) {
-  const int64_t plane = static_cast<int64_t>(a.heads) * a.tokens * (D / 2);
-  const char* const k = a.mx + block * a.mbs;
-  const char* const kc = k + (static_cast<int64_t>(head) * a.tokens + offset) * (D / 2);
-  const char* const ks = k + plane + static_cast<int64_t>(head) * (D / 32) * a.tokens + offset;
-  const char* const vc = kc + a.mks;
-  const char* const vs = ks + a.mks;
+__device__ inline void load_tile(const Args& a, const Lanes<D>& o, int block, int head, int offset,
+                                 int quad, Tile<D>& t) {
+  const char* const page = a.mx + block * a.mbs;
+  const Chunk k = chunk_at(page, a.chunk), v = chunk_at(page + a.mks, a.chunk);
+  const int codes = (head * a.tokens + offset) * (D / 2);
+  const int scales = (a.heads * (D / 2) + head * (D / 32)) * a.tokens + offset;
 #pragma unroll
   for (int s = 0; s < Tile<D>::kSteps; ++s) {
-    t.k[s] = *reinterpret_cast<const uint4*>(kc + o.k_code + 64 * s);
-    t.k_scale[s] = *reinterpret_cast<const uint8_t*>(ks + o.k_scale + 4 * s * a.tokens);
+    t.k[s] = __builtin_amdgcn_raw_buffer_load_b128(k, o.k_code + 64 * s, codes, 0);
+    t.k_scale[s] = __builtin_amdgcn_raw_buffer_load_b8(k, o.k_scale, scales + 4 * s * a.tokens, 0);
     if (D == 64 && quad >= 2) t.k_scale[s] = 127;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (D == 64) {
-      t.v[i][0] = *reinterpret_cast<const uint16_t*>(vc + o.v_code + i * (D / 2));
+      t.v[i][0] = __builtin_amdgcn_raw_buffer_load_b16(v, o.v_code + i * (D / 2), codes, 0);
     } else if constexpr (D == 128) {
-      t.v[i][0] = *reinterpret_cast<const uint32_t*>(vc + o.v_code + i * (D / 2));
+      t.v[i][0] = __builtin_amdgcn_raw_buffer_load_b32(v, o.v_code + i * (D / 2), codes, 0);
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(vc + o.v_code + i * (D / 2));
-      t.v[i][0] = w.x;
-      t.v[i][1] = w.y;
+      const Vec2 w = __builtin_amdgcn_raw_buffer_load_b64(v, o.v_code + i * (D / 2), codes, 0);
+      t.v[i][0] = w[0];
+      t.v[i][1] = w[1];
     }
   }
-  t.v_scale = *reinterpret_cast<const uint32_t*>(vs + o.v_scale);
+  t.v_scale = __builtin_amdgcn_raw_buffer_load_b32(v, o.v_scale, scales, 0);
 }
 
 __device__ inline uint32_t cvt_bf16(uint32_t codes, float scale, int byte) {
@@ -367,6 +390,7 @@ template <int D>
 struct State {
   v4f o[D / 16];   // o[j][i]: element (D / 16) * (quad * 4 + i) + j
   float m, l;      // the reference; the sum of this lane's tokens
+  uint32_t lost;   // bit i: o[][i] is NaN
 };
 
 // Byte i of `scales` as the scale of a conversion, which reads its exponent
@@ -376,68 +400,100 @@ __device__ inline float byte_scale(uint32_t scales, int i) {
                                                                         : scales >> 1);
 }
 
+__device__ inline v4f multiply_keys(v8i k, v8i q, v4f acc, int k_scale, int q_scale, int part) {
+  switch (part) {
+    case 0:
+      return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, acc, 4, 0, 0, k_scale, 0,
+                                                              q_scale);
+    case 1:
+      return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, acc, 4, 0, 0, k_scale, 1,
+                                                              q_scale);
+    default:
+      return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, acc, 4, 0, 0, k_scale, 2,
+                                                              q_scale);
+  }
+}
+
 // Two tiles of 16 tokens from token `at` on, for R row tiles.  MASKED: some row does
 // not see all of them.  `visible`: the keys this lane's rows see; `keys`: those there are.
 // P of bf16 has 8 significant bits, its rounding averaging out over the keys;
 // where the output has 11 (SPLIT_P) the rest of P is a second bf16 operand.
-template <int D, int PARTS, int R, bool MASKED, bool SPLIT_P>
-__device__ inline void attend(const Query<D, PARTS> (&q)[R], Tile<D> (&t)[2], int at,
-                              const int (&visible)[R], int keys, float scale_log2, int quad,
-                              State<D> (&st)[R]) {
+// query(r): the queries of row tile r.
+template <int D, int PARTS, int R, bool MASKED, bool SPLIT_P, class GetQuery>
+__device__ inline void attend(GetQuery query, Tile<D> (&t)[2], int at, const int (&visible)[R],
+                              int keys, float scale_log2, int quad, State<D> (&st)[R]) {
   constexpr int NT = D / 16;
-  v8bf p_hi[R], p_lo[R];
+  v4f s[R][2];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float s[2][4];
+    const Query<D, PARTS> q = query(r);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      v4f acc = {0.f, 0.f, 0.f, 0.f};
+      s[r][h] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < Query<D, PARTS>::kSteps; ++k) {
-        v8i kc = {static_cast<int>(t[h].k[k].x), static_cast<int>(t[h].k[k].y),
-                  static_cast<int>(t[h].k[k].z), static_cast<int>(t[h].k[k].w), 0, 0, 0, 0};
+        const Vec4 c = t[h].k[k];
+        const v8i kc = {static_cast<int>(c[0]), static_cast<int>(c[1]), static_cast<int>(c[2]),
+                        static_cast<int>(c[3]), 0, 0, 0, 0};
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p)
-          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              kc, q[r].part[p][k], acc, 4, 0, 0, t[h].k_scale[k], 0, q[r].scale[p]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[h][i] = acc[i] * scale_log2;
-        if (MASKED && at + 16 * h + quad * 4 + i >= visible[r]) s[h][i] = -INFINITY;
+          s[r][h] = multiply_keys(kc, q.part[p][k], s[r][h], t[h].k_scale[k], q.scale, p);
       }
     }
-    float top = s[0][0];
+  }
+  auto hidden = [&](int r, int h, int i) { return at + 16 * h + quad * 4 + i >= visible[r]; };
+  // the scores become weights; a reference of -infinity, before the first, makes
+  // them infinite, so that they count as passing it
+  auto weigh = [&](int r, v4f (&p)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[h][i]);
-    if (__any(top > st[r].m + kSlack)) {
+      for (int i = 0; i < 4; ++i) {
+        p[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][h][i], scale_log2, -st[r].m));
+        if (MASKED && hidden(r, h, i)) p[h][i] = 0.f;
+      }
+  };
+  v4f p[R][2];
+  bool grows = false;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    weigh(r, p[r]);
+    float top = p[r][0][0];
+#pragma unroll
+    for (int x = 1; x < 8; ++x) top = fmaxf(top, p[r][x / 4][x % 4]);
+    grows |= top > kSlack;
+  }
+  if (__any(grows)) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float v = s[r][x / 4][x % 4] * scale_log2;
+        top = MASKED && hidden(r, x / 4, x % 4) ? top : fmaxf(top, v);
+      }
       const float m = fmaxf(st[r].m, max_over_quads(top));
       const float fade = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st[r].m - m);
       st[r].m = m;
       st[r].l *= fade;
 #pragma unroll
       for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
+      weigh(r, p[r]);
     }
-    const float ref = MASKED && st[r].m == -INFINITY ? 0.f : st[r].m;   // nothing seen yet
+  }
+  v8bf p_hi[R], p_lo[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float p[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(s[h][i] - ref);
-        st[r].l += p[i];
-      }
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const uint32_t u = pack_bf16(p[2 * w], p[2 * w + 1]);
-        hi[2 * h + w] = u;
-        if constexpr (SPLIT_P)
-          lo[2 * h + w] = pack_bf16(p[2 * w] - bits_f32(u << 16),
-                                    p[2 * w + 1] - bits_f32(u & 0xffff0000u));
-      }
+    for (int w = 0; w < 4; ++w) {
+      const float x = p[r][w / 2][2 * (w % 2)], y = p[r][w / 2][2 * (w % 2) + 1];
+      st[r].l += x;
+      st[r].l += y;
+      const uint32_t u = pack_bf16(x, y);
+      hi[w] = u;
+      if constexpr (SPLIT_P)
+        lo[w] = pack_bf16(x - bits_f32(u << 16), y - bits_f32(u & 0xffff0000u));
     }
     p_hi[r] = __builtin_bit_cast(v8bf, make_uint4(hi[0], hi[1], hi[2], hi[3]));
     if constexpr (SPLIT_P)
@@ -496,23 +552,22 @@ __device__ inline void attend(const Query<D, PARTS> (&q)[R], Tile<D> (&t)[2], in
   }
   if constexpr (MASKED) {
     // A NaN group of V that some rows see and others do not: 0 x NaN must not
-    // reach those that do not, so the product took zeros, and the rows that see
-    // it become NaN here.
+    // reach those that do not, so the product took zeros, and what the rows that
+    // see it hold is marked.
     if (__any(any_lost)) {
+#pragma unroll 1
+      for (int tok = 0; tok < 32; ++tok) {
+        const uint32_t mine = tok < 16 ? lost[0] : lost[1];
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t f = static_cast<uint32_t>(
+              __shfl(static_cast<int>(mine), (tok / 4 % 4) * 16 + quad * 4 + i));
+          const bool is = (f >> (8 * (tok % 4))) & 255u;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        for (int tok = 0; tok < 16; ++tok)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t f = static_cast<uint32_t>(
-                __shfl(static_cast<int>(lost[h]), (tok / 4) * 16 + quad * 4 + i));
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-              if (((f >> (8 * (tok % 4))) & 255u) && at + 16 * h + tok < visible[r]) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) st[r].o[j][i] = bits_f32(0x7fc00000u);
-              }
-          }
+          for (int r = 0; r < R; ++r)
+            if (is && at + tok < visible[r]) st[r].lost |= 1u << i;
+        }
+      }
     }
   }
 }
@@ -542,6 +597,11 @@ __device__ inline Row row_of(const Args& a, const Seq& s, int r, int kv_head) {
   return row;
 }
 
+__device__ inline void write_lse(const Args& a, const Row& row, float m, float l) {
+  a.lse[row.at * a.lse_row + row.head * a.lse_head] =
+      l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
 // A row's elements (D / 16) * 4 quad .. as the output's type, and its lse.
 template <class T, int D>
 __device__ inline void write_row(const Args& a, const Row& row, int quad, const v4f (&o)[D / 16],
@@ -558,46 +618,52 @@ __device__ inline void write_row(const Args& a, const Row& row, int quad, const 
     for (int x = 0; x < NT / 2; x += 2)
       *reinterpret_cast<uint2*>(out + (i * NT + 2 * x) * 2) = make_uint2(w[x], w[x + 1]);
   }
-  if (a.lse && quad == 0)
-    a.lse[row.at * a.lse_row + row.head * a.lse_head] =
-        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (a.lse && quad == 0) write_lse(a, row, m, l);
 }
+
+// Wavefronts of a workgroup, and how many of them a SIMD is to hold, by the
+// row tiles they carry: those of one tile are short of loads in flight, those of more
+// of registers.
+constexpr int waves_of(int row_tiles) { return row_tiles == 1 ? 8 : 4; }
+constexpr int waves_a_simd(int row_tiles, int dim) { return row_tiles == 1 && dim <= 128 ? 4 : 2; }
 
 // One workgroup for a cut of the keys of a tile of 16 R rows of one K/V head.
 template <class T, int D, int R>
-__global__ __launch_bounds__(kThreads) void mx4_attention_kernel(const Args a) {
+__global__ __launch_bounds__(64 * waves_of(R), waves_a_simd(R, D)) void mx4_attention_kernel(
+    const Args a) {
   constexpr int PARTS = __is_same(T, __bf16) ? 2 : 3;
   constexpr bool SPLIT_P = !__is_same(T, __bf16);
-  constexpr int NT = D / 16;
-  __shared__ v4f sum_o[2][R * NT][64];
-  __shared__ float sum_m[kWaves][R][16], sum_l[kWaves][R][16];
+  constexpr int NT = D / 16, W = waves_of(R);
+  using Q = Query<D, PARTS>;
+  constexpr bool kQueryInRegisters = R * D <= 256;
+  // the queries, then (W / 2) x NT vectors of a lane for the sums
+  constexpr int kVectors = std::max(R * Q::kVectors, W / 2 * NT);
+  __shared__ uint4 shared[kVectors][64];
+  __shared__ int shared_scale[R][64];
+  __shared__ float sum_m[W][R][16], sum_l[W][R][16];
   const int item = a.heads_div.div(blockIdx.x);
   const int kv_head = blockIdx.x - item * a.heads;
   const Work w = find_work(a, item, kRows * R, false);
   if (w.seq < 0) return;
-  const Seq seq = sequence(a, w.seq);
+  const Seq seq = w.s;
   const int first = w.tile * kRows * R;
   const int rows = min(kRows * R, seq.count * a.group - first);
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
   const int keys = max(seq.keys, 0);
-  Query<D, PARTS> q[R];
   State<D> st[R];
   int visible[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int n = 16 * r + (lane & 15);
-    const Row row = row_of(a, seq, first + min(n, rows - 1), kv_head);
-    visible[r] = row.visible;
-    load_query<T, D, PARTS>(a.q + row.at * a.q_row + row.head * a.q_head, n < rows, quad,
-                            a.scale_log2 < 0.f, q[r]);
+    visible[r] = row_of(a, seq, first + min(16 * r + (lane & 15), rows - 1), kv_head).visible;
     st[r].m = -INFINITY;
     st[r].l = 0.f;
+    st[r].lost = 0;
 #pragma unroll
     for (int j = 0; j < NT; ++j) st[r].o[j] = {0.f, 0.f, 0.f, 0.f};
   }
   // of the tile's rows, in order, the first sees the fewest, the last the most
   const int fewest = uniform(visible[0]);
-  const int most = uniform(__shfl(visible[R - 1], 15));
+  const int most = lane_value(visible[R - 1], 15);
   const Lanes<D> o = lane_offsets<D>(lane, a.tokens);
   const float scale_log2 = fabsf(a.scale_log2);
   bool bad = seq.keys < 0;
@@ -607,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void mx4_attention_kernel(const Args a) {
   // the block ids of the next 32 steps of this wavefront, two tiles each, a lane a tile
   int ids = 0;
   auto load_ids = [&](int step) {
-    const int i = (step + (lane >> 1) * kWaves) * 2 + (lane & 1);
+    const int i = (step + (lane >> 1) * W) * 2 + (lane & 1);
     const int tile = min(i, last_tile);
     const int page = a.tiles_per_block.div(tile);
     int64_t id = 0;
@@ -625,34 +691,85 @@ __global__ __launch_bounds__(kThreads) void mx4_attention_kernel(const Args a) {
       const int i = min(2 * step + h, last_tile);
       const int page = a.tiles_per_block.div(i);
       const int offset = (i - page * static_cast<int>(a.tiles_per_block.d)) * kMx4TokenTile;
-      load_tile<D>(a, o, __builtin_amdgcn_readlane(ids, 2 * nth + h), kv_head, offset, quad, t[h]);
+      load_tile<D>(a, o, lane_value(ids, 2 * nth + h), kv_head, offset, quad, t[h]);
     }
   };
   int step = (w.cuts > 1 ? w.cut * w.steps : 0) + wave;
+  Tile<D> next[2];
   if (step < end) {
-    Tile<D> t[2], next[2];
     load_ids(step);
     load_step(step, 0, next);
-    for (int nth = 1; step < end; ++nth) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) t[h] = next[h];
-      const int at = step * kStep;
-      step += kWaves;
-      if (step < end) {
-        if (nth == 32) {
-          load_ids(step);
-          nth = 0;
-        }
-        load_step(step, nth, next);
-      }
-      if (at + kStep <= fewest)
-        attend<D, PARTS, R, false, SPLIT_P>(q, t, at, visible, keys, scale_log2, quad, st);
-      else
-        attend<D, PARTS, R, true, SPLIT_P>(q, t, at, visible, keys, scale_log2, quad, st);
-    }
   }
-  // The four wavefronts' sums: each to the common reference, then 2 and 3 onto
-  // 0 and 1, then 1 onto 0.
+  // a wavefront prepares a row tile's queries, for all of them
+  for (int r = wave; r < R; r += W) {
+    const int n = 16 * r + (lane & 15);
+    const Row row = row_of(a, seq, first + min(n, rows - 1), kv_head);
+    Q q;
+    load_query<T, D, PARTS>(a.q + row.at * a.q_row + row.head * a.q_head, n < rows, quad,
+                            a.scale_log2 < 0.f, q);
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+      for (int k = 0; k < Q::kSteps; ++k) {
+        uint4 v[2];
+        __builtin_memcpy(v, &q.part[p][k], 32);
+        shared[r * Q::kVectors + (p * Q::kSteps + k) * 2][lane] = v[0];
+        shared[r * Q::kVectors + (p * Q::kSteps + k) * 2 + 1][lane] = v[1];
+      }
+    shared_scale[r][lane] = q.scale;
+  }
+  __syncthreads();
+  auto read_query = [&](int r) {
+    Q q;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+      for (int k = 0; k < Q::kSteps; ++k) {
+        const uint4 v[2] = {shared[r * Q::kVectors + (p * Q::kSteps + k) * 2][lane],
+                            shared[r * Q::kVectors + (p * Q::kSteps + k) * 2 + 1][lane]};
+        __builtin_memcpy(&q.part[p][k], v, 32);
+      }
+    q.scale = shared_scale[r][lane];
+    return q;
+  };
+  Q kept[R];
+  if constexpr (kQueryInRegisters) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) kept[r] = read_query(r);
+  }
+  auto query = [&](int r) {
+    if constexpr (kQueryInRegisters) return kept[r];
+    // every step anew: held, they would be 2^6 registers
+    if (r == 0) asm volatile("" ::: "memory");
+    return read_query(r);
+  };
+  int nth = 0;
+  auto advance = [&](Tile<D> (&t)[2]) {
+    t[0] = next[0], t[1] = next[1];
+    step += W;
+    if (step < end) {
+      if (++nth == 32) {
+        load_ids(step);
+        nth = 0;
+      }
+      load_step(step, nth, next);
+    }
+  };
+  const int all_seen = min(end, fewest / kStep);    // steps before it: every row sees all
+  while (step < all_seen) {
+    const int at = step * kStep;
+    Tile<D> t[2];
+    advance(t);
+    attend<D, PARTS, R, false, SPLIT_P>(query, t, at, visible, keys, scale_log2, quad, st);
+  }
+  while (step < end) {
+    const int at = step * kStep;
+    Tile<D> t[2];
+    advance(t);
+    attend<D, PARTS, R, true, SPLIT_P>(query, t, at, visible, keys, scale_log2, quad, st);
+  }
+  // The wavefronts' sums: each to the common reference, then the upper half onto
+  // the lower until one is left, a row tile at a time.
   const bool any_bad = __any(bad);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -663,50 +780,43 @@ __global__ __launch_bounds__(kThreads) void mx4_attention_kernel(const Args a) {
     }
   }
   __syncthreads();
-  float m_all[R], l_all[R];
+  v4f(*const sum_o)[64] = reinterpret_cast<v4f(*)[64]>(shared);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float m = -INFINITY;
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) m = fmaxf(m, sum_m[x][r][lane & 15]);
-    m_all[r] = m;
+    for (int x = 0; x < W; ++x) m = fmaxf(m, sum_m[x][r][lane & 15]);
     const float ref = m == -INFINITY ? 0.f : m;
-    l_all[r] = 0.f;
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x)
-      l_all[r] += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - ref);
+    for (int x = 0; x < W; ++x)
+      l += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - ref);
     const float f = __builtin_amdgcn_exp2f(st[r].m - ref);
+    v4f factor;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) st[r].o[j] *= f;
-  }
+    for (int i = 0; i < 4; ++i) factor[i] = st[r].lost >> i & 1 ? bits_f32(0x7fc00000u) : f;
 #pragma unroll
-  for (int half = kWaves / 2; half > 0; half /= 2) {
-    if (wave >= half && wave < 2 * half) {
+    for (int j = 0; j < NT; ++j) st[r].o[j] *= factor;
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+    for (int half = W / 2; half > 0; half /= 2) {
+      if (wave >= half && wave < 2 * half) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) sum_o[wave - half][r * NT + j][lane] = st[r].o[j];
+        for (int j = 0; j < NT; ++j) sum_o[(wave - half) * NT + j][lane] = st[r].o[j];
+      }
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) st[r].o[j] += sum_o[wave * NT + j][lane];
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    if (wave < half) {
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) st[r].o[j] += sum_o[wave][r * NT + j][lane];
-    }
-    __syncthreads();
-  }
-  if (wave) return;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
     const int n = 16 * r + (lane & 15);
-    if (n >= rows) continue;
+    if (wave || n >= rows) continue;
     if (w.cuts == 1) {
       const Row row = row_of(a, seq, first + n, kv_head);
-      write_row<T, D>(a, row, quad, st[r].o, m_all[r], l_all[r]);
+      write_row<T, D>(a, row, quad, st[r].o, m, l);
     } else {
       if (quad == 0)
-        a.part_ml[static_cast<int64_t>(blockIdx.x) * kRows * R + n] = make_float2(m_all[r], l_all[r]);
+        a.part_ml[static_cast<int64_t>(blockIdx.x) * kRows * R + n] = make_float2(m, l);
 #pragma unroll
       for (int j = 0; j < NT; ++j)
         a.part_o[(static_cast<int64_t>(blockIdx.x) * R * NT + r * NT + j) * 64 + lane] = st[r].o[j];
@@ -714,64 +824,83 @@ __global__ __launch_bounds__(kThreads) void mx4_attention_kernel(const Args a) {
   }
 }
 
-// Joins the cuts of 16 rows: a wavefront takes every fourth cut of the rows' elements
-// of 4 registers, so cuts are read 4 at a time; the workgroup's sums are added in
-// the order of its wavefronts.
+// Joins the cuts of 16 rows, two of a lane's NT vectors (blockIdx.y: row tile and
+// which two): each of the four wavefronts takes every fourth cut, four at a time in
+// flight; their sums are added in their order.
 template <class T, int D, int R>
-__global__ __launch_bounds__(kThreads) void mx4_join_kernel(const Args a) {
-  constexpr int NT = D / 16;
+__global__ __launch_bounds__(256) void mx4_join_kernel(const Args a) {
+  constexpr int NT = D / 16, W = 4, kAhead = 4;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
   const int item = a.heads_div.div(blockIdx.x);
   const int kv_head = blockIdx.x - item * a.heads;
   const Work w = find_work(a, item, kRows * R, true);
   if (w.seq < 0 || w.cuts == 1) return;
-  const Seq seq = sequence(a, w.seq);
-  const int r = blockIdx.y;
+  const int r = blockIdx.y / (NT / 2), j = blockIdx.y % (NT / 2) * 2;
   const int first = (w.tile * R + r) * kRows;
-  const int rows = min(kRows, seq.count * a.group - first);
+  const int rows = min(kRows, w.s.count * a.group - first);
   if (rows <= 0) return;
   const bool valid = (lane & 15) < rows;
-  __shared__ v4f sum_o[kWaves][NT][64];
-  __shared__ float sum_m[kWaves][16], sum_l[kWaves][16];
-  v4f o[NT];
+  __shared__ v4f sum_o[W][2][64];
+  __shared__ float sum_m[W][16], sum_l[W][16];
+  v4f o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   float m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) o[j] = {0.f, 0.f, 0.f, 0.f};
   if (valid) {
-    for (int c = wave; c < w.cuts; c += kWaves) {
-      const int64_t at = static_cast<int64_t>(w.first + c) * a.heads + kv_head;
-      const float2 ml = a.part_ml[at * kRows * R + 16 * r + (lane & 15)];
-      const float top = fmaxf(m, ml.x);
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(ml.x - ref);
-      m = top;
-      l = l * f + ml.y * g;
+    const int64_t cut = static_cast<int64_t>(w.first) * a.heads + kv_head;
+    const float2* const ml = a.part_ml + cut * kRows * R + 16 * r + (lane & 15);
+    const v4f* const part = a.part_o + (cut * R * NT + r * NT + j) * 64 + lane;
+    const int64_t ml_step = static_cast<int64_t>(a.heads) * kRows * R;
+    const int64_t part_step = static_cast<int64_t>(a.heads) * R * NT * 64;
+    for (int c0 = wave; c0 < w.cuts; c0 += W * kAhead) {
+      float2 x[kAhead];
+      v4f y[kAhead][2];
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        o[j] = o[j] * f + a.part_o[(at * R * NT + r * NT + j) * 64 + lane] * g;
+      for (int n = 0; n < kAhead; ++n) {
+        const int c = c0 + n * W;
+        x[n] = make_float2(-INFINITY, 0.f);
+        y[n][0] = y[n][1] = {0.f, 0.f, 0.f, 0.f};
+        if (c < w.cuts) {
+          x[n] = ml[c * ml_step];
+          y[n][0] = part[c * part_step];
+          y[n][1] = part[c * part_step + 64];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const float top = fmaxf(m, x[n].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(x[n].x - ref);
+        m = top;
+        l = l * f + x[n].y * g;
+        o[0] = o[0] * f + y[n][0] * g;
+        o[1] = o[1] * f + y[n][1] * g;
+      }
     }
   }
   if (quad == 0) sum_m[wave][lane] = m, sum_l[wave][lane] = l;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) sum_o[wave][j][lane] = o[j];
+  sum_o[wave][0][lane] = o[0];
+  sum_o[wave][1][lane] = o[1];
   __syncthreads();
   if (wave || !valid) return;
   float top = -INFINITY;
 #pragma unroll
-  for (int x = 0; x < kWaves; ++x) top = fmaxf(top, sum_m[x][lane & 15]);
+  for (int x = 0; x < W; ++x) top = fmaxf(top, sum_m[x][lane & 15]);
   const float ref = top == -INFINITY ? 0.f : top;
   l = 0.f;
+  o[0] = o[1] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < NT; ++j) o[j] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int x = 0; x < kWaves; ++x) {
+  for (int x = 0; x < W; ++x) {
     const float f = __builtin_amdgcn_exp2f(sum_m[x][lane & 15] - ref);
     l += sum_l[x][lane & 15] * f;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) o[j] += sum_o[x][j][lane] * f;
+    o[0] += sum_o[x][0][lane] * f;
+    o[1] += sum_o[x][1][lane] * f;
   }
-  const Row row = row_of(a, seq, first + (lane & 15), kv_head);
-  write_row<T, D>(a, row, quad, o, top, l);
+  const Row row = row_of(a, w.s, first + (lane & 15), kv_head);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  char* const out = a.out + row.at * a.out_row + row.head * a.out_head + (quad * 4 * NT + j) * 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<uint32_t*>(out + i * NT * 2) = narrow2<T>(o[0][i] * inv, o[1][i] * inv);
+  if (a.lse && quad == 0 && j == 0) write_lse(a, row, top, l);
 }
 
 // ---------------------------------------------------------------------------
@@ -819,9 +948,9 @@ int check_attention(const fkv_mx4_attention_args& c) {
                          2, mx4_chunk_bytes(c.tokens_per_block, c.num_heads, c.head_size));
 }
 
-// Workgroups the keys are cut into where there are few tiles: 8 a compute unit,
-// so that those of uneven sequences even out.
-constexpr int kCutTarget = 2048;
+// Workgroups the keys are cut into where there are few tiles: as many as the device
+// holds at a time (256 compute units), since cuts are of one size.
+constexpr int kCutTarget = 512;
 
 struct LaunchPlan {
   int row_tiles;          // R
@@ -834,7 +963,8 @@ struct LaunchPlan {
 LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   LaunchPlan p;
   const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
-  p.row_tiles = rows <= static_cast<int64_t>(c.batch) * kRows ? 1 : 2;
+  const int64_t rows_a_seq = (rows + c.batch - 1) / c.batch;
+  p.row_tiles = rows_a_seq <= kRows ? 1 : rows_a_seq <= 2 * kRows || c.head_size > 128 ? 2 : 4;
   const int rows_a_tile = kRows * p.row_tiles;
   const int64_t tiles = c.query_starts
       ? rows / rows_a_tile + c.batch
@@ -851,14 +981,16 @@ LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
 
 template <class T, int D, int R>
 void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_attention_kernel<T, D, R>), dim3(p.workgroups), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL((mx4_attention_kernel<T, D, R>), dim3(p.workgroups), dim3(64 * waves_of(R)),
+                     0, s, a);
   if (p.target)
-    hipLaunchKernelGGL((mx4_join_kernel<T, D, R>), dim3(p.tiles, R), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((mx4_join_kernel<T, D, R>), dim3(p.tiles, R * D / 32), dim3(256), 0, s, a);
 }
 template <class T, int D>
 void launch_rows(const Args& a, const LaunchPlan& p, hipStream_t s) {
   if (p.row_tiles == 1) launch<T, D, 1>(a, p, s);
-  else launch<T, D, 2>(a, p, s);
+  else if (p.row_tiles == 2) launch<T, D, 2>(a, p, s);
+  else if constexpr (D <= 128) launch<T, D, 4>(a, p, s);
 }
 template <class T>
 void launch_attention(const Args& a, const LaunchPlan& p, int dim, hipStream_t s) {
@@ -909,6 +1041,7 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
     a.num_blocks = static_cast<int>(c.num_mx_blocks), a.width = c.table_width;
     a.batch = c.batch, a.heads = c.num_heads, a.group = c.group_size, a.queries = c.num_queries;
     a.tokens = c.tokens_per_block, a.causal = c.causal;
+    a.chunk = static_cast<int>(mx4_chunk_bytes(c.tokens_per_block, c.num_heads, c.head_size));
     a.target = p.target;
     a.scale_log2 = c.scale * kLog2e;
     a.part_o = static_cast<v4f*>(c.workspace);
