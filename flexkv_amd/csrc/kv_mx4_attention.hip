@@ -51,8 +51,11 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 16;          // rows of a tile: columns of a matrix instruction
 constexpr int kStep = 32;          // tokens of a step: two tiles of 16, k of the second product
-constexpr int kMinSteps = 16;      // of a workgroup, where the keys are cut
+constexpr int kMinSteps = 32;      // of a workgroup, where the keys are cut
 constexpr float kSlack = 256.f;    // weight up to which a score may pass the reference
+// The reference of a row that has seen nothing.  Any score passes it, and so does
+// not -infinity, which a score that a row does not see becomes.
+constexpr float kNothing = -3e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -103,10 +106,11 @@ struct Args {
   int batch, heads, group, queries;
   int tokens, chunk;                 // of a block; bytes of a chunk
   int causal;
-  int target;                        // workgroups to cut the keys into; 0: uncut
+  int slots;                         // workgroups to cut the keys into; 0: uncut
   float scale_log2;
   float2* part_ml;                   // [workgroup][row]: maximum and sum of a cut
-  v4f* part_o;                       // [workgroup][register][lane]
+  float* part_o;                     // [workgroup][row tile][i][j][lane], see State
+  int* any_cut;                      // whether some tile has more than one cut
   FastDiv tiles_per_block, group_div, heads_div;
 };
 
@@ -156,13 +160,18 @@ __device__ inline V scan_lanes(V v) {
 __device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 // How the workgroups are dealt out.  A sequence has ceil(queries * group / rows a tile)
-// tiles; where the keys are cut, every tile's into cuts of the same number of
-// steps, chosen from the lengths on the device so that there are at most `target`
-// more of them than tiles, however uneven the sequences are.  Every wavefront works
-// this out for itself: sequence b = lane, then 64 further on.
+// tiles; where the keys are cut, every tile of a sequence is cut alike, the
+// longer the sequence the more often, so that all cuts together fill the
+// `slots` the device has at a time and do not start a second round; with more tiles
+// than slots only sequences of twice a slot's share are cut.  The lengths are
+// read here, on the device: every wavefront works the plan out for itself, sequence
+// b = lane, then 64 further on.  The first 64 sequences go longest first, and a
+// sequence's tiles last first, as causal rows see more the later they are.
 struct Work {
   int seq;                    // < 0: none
   int tile, cut, cuts;
+  bool any_cut;               // whether some tile of the first 64 sequences is cut, or
+                              // there are more sequences
   int steps;                  // of a cut
   int first;                  // the number of the tile's first cut
   Seq s;
@@ -171,33 +180,69 @@ __device__ inline int tiles_of(const Args& a, const Seq& s, int rows_a_tile) {
   return (s.count * a.group + rows_a_tile - 1) / rows_a_tile;
 }
 __device__ inline int steps_of(const Seq& s) { return (max(s.keys, 0) + kStep - 1) / kStep; }
+// ceil(steps / per_cut), at least 1; in floats, so perhaps one more
+__device__ inline int cuts_of(int steps, float inv_per_cut) {
+  return max(1, static_cast<int>(steps * inv_per_cut + 0.9999f));
+}
 
 // Item `item` of the plan; by_tile: `item` counts tiles, the answer is its first cut.
 __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool by_tile) {
   const int lane = threadIdx.x & 63;
-  int per_cut = 1 << 30;
   Seq s{0, 0, 0};
-  if (a.target) {
+  int tiles = 0, b = lane;
+  if (lane < a.batch) {
+    s = sequence(a, lane);
+    tiles = tiles_of(a, s, rows_a_tile);
+  }
+  const bool few = a.batch <= 64;
+  if (few && a.batch > 1) {
+    int rank = 0;
+    for (int j = 0; j < a.batch; ++j) {
+      const int k = lane_value(s.keys, j);
+      rank += k > s.keys || (k == s.keys && j < lane);
+    }
+    if (lane >= a.batch) rank = lane;
+    auto move = [&](int v) { return __builtin_amdgcn_ds_permute(rank * 4, v); };
+    s.first = move(s.first), s.count = move(s.count), s.keys = move(s.keys);
+    tiles = move(tiles), b = move(b);
+  }
+  float inv_per_cut = 0.f;     // one cut
+  if (a.slots) {
     float total = 0.f;
-    for (int b = lane; b < a.batch; b += 64) {
-      s = sequence(a, b);
-      total += static_cast<float>(tiles_of(a, s, rows_a_tile)) * static_cast<float>(steps_of(s));
+    if (few) {
+      total = static_cast<float>(tiles) * static_cast<float>(steps_of(s));
+    } else {
+      for (int i = lane; i < a.batch; i += 64) {
+        const Seq x = sequence(a, i);
+        total += static_cast<float>(tiles_of(a, x, rows_a_tile)) * static_cast<float>(steps_of(x));
+      }
     }
     total = bits_f32(lane_value(f32_bits(scan_lanes(total)), 63));
-    // rounded up by more than the sum's error
-    const float even = total * a.heads / a.target * 1.0001f;
-    per_cut = max(kMinSteps, static_cast<int>(fminf(even, 1e9f)) + 1);
+    // at least this many steps a cut; the sum's error and cuts_of's are less than 1 %
+    const float even = fmaxf(total * a.heads / a.slots * 1.01f, kMinSteps);
+    // cuts of even size overflow the slots by the last, short ones: longer cuts until
+    // they do not, or to twice the size
+    inv_per_cut = 0.5f / even;
+    for (int i = 0; few && i < 8; ++i) {
+      inv_per_cut = 1.f / (even * (1.f + i * 0.125f));
+      const int n = lane_value(scan_lanes(tiles * cuts_of(steps_of(s), inv_per_cut)), 63);
+      if (static_cast<int64_t>(n) * a.heads <= a.slots) break;
+    }
   }
-  Work w{-1, 0, 0, 0, per_cut, 0, Seq{0, 0, 0}};
+  Work w{-1, 0, 0, 0, false, 0, 0, Seq{0, 0, 0}};
   int before = 0, cuts_before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int b = b0 + lane;
-    int tiles = 0, cuts = 0;
-    if (b < a.batch) {
-      if (!a.target || a.batch > 64) s = sequence(a, b);
-      tiles = tiles_of(a, s, rows_a_tile);
-      cuts = a.target ? max(1, (steps_of(s) + per_cut - 1) / per_cut) : 1;
+    if (b0) {
+      b = b0 + lane;
+      tiles = 0;
+      if (b < a.batch) {
+        s = sequence(a, b);
+        tiles = tiles_of(a, s, rows_a_tile);
+      }
     }
+    const int steps = steps_of(s);
+    const int cuts = cuts_of(steps, inv_per_cut);
+    if (!b0) w.any_cut = !few || __any(tiles && cuts > 1);
     const int cut_ends = scan_lanes(tiles * cuts);
     const int ends = by_tile ? scan_lanes(tiles) : cut_ends;
     const uint64_t later = __ballot(before + ends > item);
@@ -205,17 +250,33 @@ __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool 
       const int at = __builtin_ctzll(later);
       const int n = lane_value(tiles, at), c = lane_value(cuts, at);
       const int local = item - (before + lane_value(ends, at) - (by_tile ? n : n * c));
-      w.seq = b0 + at;
+      const int nth = by_tile || c == 1 ? local : uniform(local / c);
+      w.seq = lane_value(b, at);
       w.cuts = c;
-      w.tile = by_tile || c == 1 ? local : local / c;
-      w.cut = by_tile ? 0 : local - w.tile * c;
-      w.first = cuts_before + lane_value(cut_ends, at) - n * c + w.tile * c;
+      w.tile = n - 1 - nth;
+      w.cut = by_tile ? 0 : local - nth * c;
+      w.steps = uniform((lane_value(steps, at) + c - 1) / c);
+      w.first = cuts_before + lane_value(cut_ends, at) - n * c + nth * c;
       w.s = {lane_value(s.first, at), lane_value(s.count, at), lane_value(s.keys, at)};
       return w;
     }
     before += lane_value(ends, 63);
     cuts_before += lane_value(cut_ends, 63);
   }
+  return w;
+}
+
+// The same where the keys are uncut and every sequence has one query: nothing
+// but the sequence's own length is read.
+__device__ inline Work find_single(const Args& a, int item, int rows_a_tile) {
+  Work w{item, 0, 0, 1, false, 0, 0, Seq{0, 0, 0}};
+  const int tiles = (a.group + rows_a_tile - 1) / rows_a_tile;
+  if (tiles > 1) {
+    w.seq = uniform(item / tiles);
+    w.tile = item - w.seq * tiles;
+  }
+  w.s = sequence(a, w.seq);
+  w.s.keys = uniform(w.s.keys);
   return w;
 }
 
@@ -339,16 +400,21 @@ __device__ inline Lanes<D> lane_offsets(int lane, int tokens) {
   return o;
 }
 
+// K's codes are read whole by one load and not again by this compute unit: past the
+// L1 (96 sequences of 8192 keys 157 -> 148 us; V's, a cache line of which takes four
+// loads, gain nothing).
+constexpr int kOnce = 2;
+
 template <int D>
 __device__ inline void load_tile(const Args& a, const Lanes<D>& o, int block, int head, int offset,
                                  int quad, Tile<D>& t) {
   const char* const page = a.mx + block * a.mbs;
   const Chunk k = chunk_at(page, a.chunk), v = chunk_at(page + a.mks, a.chunk);
-  const int codes = (head * a.tokens + offset) * (D / 2);
-  const int scales = (a.heads * (D / 2) + head * (D / 32)) * a.tokens + offset;
+  const int codes = uniform((head * a.tokens + offset) * (D / 2));
+  const int scales = uniform((a.heads * (D / 2) + head * (D / 32)) * a.tokens + offset);
 #pragma unroll
   for (int s = 0; s < Tile<D>::kSteps; ++s) {
-    t.k[s] = __builtin_amdgcn_raw_buffer_load_b128(k, o.k_code + 64 * s, codes, 0);
+    t.k[s] = __builtin_amdgcn_raw_buffer_load_b128(k, o.k_code + 64 * s, codes, kOnce);
     t.k_scale[s] = __builtin_amdgcn_raw_buffer_load_b8(k, o.k_scale, scales + 4 * s * a.tokens, 0);
     if (D == 64 && quad >= 2) t.k_scale[s] = 127;
   }
@@ -414,14 +480,15 @@ __device__ inline v4f multiply_keys(v8i k, v8i q, v4f acc, int k_scale, int q_sc
   }
 }
 
-// Two tiles of 16 tokens from token `at` on, for R row tiles.  MASKED: some row does
+// Two tiles of 16 tokens from token `at` on, for R row tiles.  `partial`: some row does
 // not see all of them.  `visible`: the keys this lane's rows see; `keys`: those there are.
 // P of bf16 has 8 significant bits, its rounding averaging out over the keys;
 // where the output has 11 (SPLIT_P) the rest of P is a second bf16 operand.
 // query(r): the queries of row tile r.
-template <int D, int PARTS, int R, bool MASKED, bool SPLIT_P, class GetQuery>
-__device__ inline void attend(GetQuery query, Tile<D> (&t)[2], int at, const int (&visible)[R],
-                              int keys, float scale_log2, int quad, State<D> (&st)[R]) {
+template <int D, int PARTS, int R, bool SPLIT_P, class GetQuery>
+__device__ inline void attend(GetQuery query, Tile<D> (&t)[2], int at, bool partial,
+                              const int (&visible)[R], int keys, float scale_log2, int quad,
+                              State<D> (&st)[R]) {
   constexpr int NT = D / 16;
   v4f s[R][2];
 #pragma unroll
@@ -441,83 +508,100 @@ __device__ inline void attend(GetQuery query, Tile<D> (&t)[2], int at, const int
       }
     }
   }
-  auto hidden = [&](int r, int h, int i) { return at + 16 * h + quad * 4 + i >= visible[r]; };
-  // the scores become weights; a reference of -infinity, before the first, makes
-  // them infinite, so that they count as passing it
-  auto weigh = [&](int r, v4f (&p)[2]) {
+  if (partial) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][h][i], scale_log2, -st[r].m));
-        if (MASKED && hidden(r, h, i)) p[h][i] = 0.f;
-      }
-  };
-  v4f p[R][2];
-  bool grows = false;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    weigh(r, p[r]);
-    float top = p[r][0][0];
-#pragma unroll
-    for (int x = 1; x < 8; ++x) top = fmaxf(top, p[r][x / 4][x % 4]);
-    grows |= top > kSlack;
-  }
-  if (__any(grows)) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const float v = s[r][x / 4][x % 4] * scale_log2;
-        top = MASKED && hidden(r, x / 4, x % 4) ? top : fmaxf(top, v);
-      }
-      const float m = fmaxf(st[r].m, max_over_quads(top));
-      const float fade = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st[r].m - m);
-      st[r].m = m;
-      st[r].l *= fade;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
-      weigh(r, p[r]);
-    }
+        for (int i = 0; i < 4; ++i)
+          if (at + 16 * h + quad * 4 + i >= visible[r]) s[r][h][i] = -INFINITY;
   }
   v8bf p_hi[R], p_lo[R];
+  float l[R];
+  // the scores of row tile r as weights; returns the largest
+  auto weigh = [&](int r) {
+    float p[8];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+    for (int x = 0; x < 8; ++x)
+      p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][x / 4][x % 4], scale_log2, -st[r].m));
+    float top = p[0];
+    l[r] = st[r].l + p[0];
+#pragma unroll
+    for (int x = 1; x < 8; ++x) {
+      top = fmaxf(top, p[x]);
+      l[r] += p[x];
+    }
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float x = p[r][w / 2][2 * (w % 2)], y = p[r][w / 2][2 * (w % 2) + 1];
-      st[r].l += x;
-      st[r].l += y;
-      const uint32_t u = pack_bf16(x, y);
-      hi[w] = u;
+      hi[w] = pack_bf16(p[2 * w], p[2 * w + 1]);
       if constexpr (SPLIT_P)
-        lo[w] = pack_bf16(x - bits_f32(u << 16), y - bits_f32(u & 0xffff0000u));
+        lo[w] = pack_bf16(p[2 * w] - bits_f32(hi[w] << 16),
+                          p[2 * w + 1] - bits_f32(hi[w] & 0xffff0000u));
     }
     p_hi[r] = __builtin_bit_cast(v8bf, make_uint4(hi[0], hi[1], hi[2], hi[3]));
     if constexpr (SPLIT_P)
       p_lo[r] = __builtin_bit_cast(v8bf, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    return top;
+  };
+  bool grows = false;
+#pragma unroll
+  for (int r = 0; r < R; ++r) grows |= weigh(r) > kSlack;
+  if (__any(grows)) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = st[r].m;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) top = fmaxf(top, s[r][x / 4][x % 4] * scale_log2);
+      const float m = max_over_quads(top);
+      const float fade = __builtin_amdgcn_exp2f(st[r].m - m);
+      st[r].m = m;
+      st[r].l *= fade;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
+      weigh(r);
+    }
   }
-  // V: masked tokens hold nothing, whatever their bytes are
-  bool any_lost = false;
-  uint32_t lost[2] = {0, 0};     // byte i: 255 where token i's group is NaN
-  if constexpr (MASKED) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) st[r].l = l[r];
+  // Weights of 0 leave out what a row does not see only while V is finite, which
+  // it is in bf16 unless a scale byte is over 252: NaN, or bytes of a block that
+  // nothing was written to.  Those tokens are taken out here, and what the rows
+  // that do see them hold is marked as NaN.
+  auto over_252 = [](uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x03030303u) & x & 0x80808080u); };
+  if (__any((over_252(t[0].v_scale) | over_252(t[1].v_scale)) != 0)) {
+    bool any_lost = false;
+    uint32_t lost[2] = {0, 0};     // byte i: token i's group
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t byte = 255u << (8 * i);
         const bool there = at + 16 * h + quad * 4 + i < keys;
-        const bool nan = there && (t[h].v_scale & byte) == byte;
-        if (nan) lost[h] |= byte;
-        any_lost |= nan;
-        if (!there || nan) {
-          t[h].v_scale &= ~byte;
+        const bool over = over_252(t[h].v_scale) >> (8 * i) & 0x80u;
+        if (there && over) lost[h] |= 255u << (8 * i);
+        any_lost |= there && over;
+        if (over) {
+          t[h].v_scale &= ~(255u << (8 * i));
 #pragma unroll
           for (int w = 0; w < Tile<D>::kWords; ++w) t[h].v[i][w] = 0;
         }
       }
+    if (__any(any_lost)) {
+#pragma unroll 1
+      for (int tok = 0; tok < 32; ++tok) {
+        const uint32_t mine = tok < 16 ? lost[0] : lost[1];
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t f = static_cast<uint32_t>(
+              __shfl(static_cast<int>(mine), (tok / 4 % 4) * 16 + quad * 4 + i));
+          const bool is = (f >> (8 * (tok % 4))) & 255u;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (is && at + tok < visible[r]) st[r].lost |= 1u << i;
+        }
+      }
+    }
   }
 #pragma unroll
   for (int j = 0; j < NT; j += 2) {
@@ -547,26 +631,6 @@ __device__ inline void attend(GetQuery query, Tile<D> (&t)[2], int at, const int
         st[r].o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, p_lo[r], st[r].o[j], 0, 0, 0);
         st[r].o[j + 1] =
             __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, p_lo[r], st[r].o[j + 1], 0, 0, 0);
-      }
-    }
-  }
-  if constexpr (MASKED) {
-    // A NaN group of V that some rows see and others do not: 0 x NaN must not
-    // reach those that do not, so the product took zeros, and what the rows that
-    // see it hold is marked.
-    if (__any(any_lost)) {
-#pragma unroll 1
-      for (int tok = 0; tok < 32; ++tok) {
-        const uint32_t mine = tok < 16 ? lost[0] : lost[1];
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t f = static_cast<uint32_t>(
-              __shfl(static_cast<int>(mine), (tok / 4 % 4) * 16 + quad * 4 + i));
-          const bool is = (f >> (8 * (tok % 4))) & 255u;
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (is && at + tok < visible[r]) st[r].lost |= 1u << i;
-        }
       }
     }
   }
@@ -602,60 +666,106 @@ __device__ inline void write_lse(const Args& a, const Row& row, float m, float l
       l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// A row's elements (D / 16) * 4 quad .. as the output's type, and its lse.
-template <class T, int D>
-__device__ inline void write_row(const Args& a, const Row& row, int quad, const v4f (&o)[D / 16],
-                                 float m, float l) {
+// NJ elements from (D / 16) * (4 quad + i) + j0 of a row on as the output's type, and
+// its lse.
+template <class T, int D, int NJ>
+__device__ inline void write_row(const Args& a, const Row& row, int quad, int i, int j0,
+                                 const float (&o)[NJ], float m, float l) {
   constexpr int NT = D / 16;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* const out = a.out + row.at * a.out_row + row.head * a.out_head + quad * 4 * NT * 2;
+  uint32_t w[NJ / 2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t w[NT / 2];
+  for (int j = 0; j < NJ; j += 2) w[j / 2] = narrow2<T>(o[j] * inv, o[j + 1] * inv);
+  char* const out =
+      a.out + row.at * a.out_row + row.head * a.out_head + ((quad * 4 + i) * NT + j0) * 2;
+  if constexpr (NJ == 2) {
+    *reinterpret_cast<uint32_t*>(out) = w[0];
+  } else {
 #pragma unroll
-    for (int j = 0; j < NT; j += 2) w[j / 2] = narrow2<T>(o[j][i] * inv, o[j + 1][i] * inv);
-#pragma unroll
-    for (int x = 0; x < NT / 2; x += 2)
-      *reinterpret_cast<uint2*>(out + (i * NT + 2 * x) * 2) = make_uint2(w[x], w[x + 1]);
+    for (int x = 0; x < NJ / 2; x += 2)
+      *reinterpret_cast<uint2*>(out + x * 4) = make_uint2(w[x], w[x + 1]);
   }
-  if (a.lse && quad == 0) write_lse(a, row, m, l);
+  if (a.lse && quad == 0 && i == 0 && j0 == 0) write_lse(a, row, m, l);
 }
 
-// Wavefronts of a workgroup, and how many of them a SIMD is to hold, by the
-// row tiles they carry: those of one tile are short of loads in flight, those of more
-// of registers.
-constexpr int waves_of(int row_tiles) { return row_tiles == 1 ? 8 : 4; }
-constexpr int waves_a_simd(int row_tiles, int dim) { return row_tiles == 1 && dim <= 128 ? 4 : 2; }
+// Wavefronts a SIMD is to hold: more than these cost spilled registers.
+constexpr int waves_a_simd(int row_tiles, int dim) { return row_tiles == 1 && dim <= 128 ? 3 : 2; }
+// Wavefronts of a workgroup: all that a compute unit holds for a single row tile,
+// so that few sequences need no cuts; half of them for more.
+constexpr int waves_of(int row_tiles, int dim) {
+  return row_tiles == 1 ? 4 * waves_a_simd(row_tiles, dim) : 4;
+}
+// Steps whose loads a wavefront has in flight beside the one it computes.
+constexpr int steps_ahead(int row_tiles) { return row_tiles == 1 ? 2 : 1; }
+
+// Which item of the plan, and which K/V head, a workgroup has.  Workgroups go round the
+// 8 XCDs.  Where K and V are read once (R = 1), an item's heads are on one XCD, so
+// that a block is read whole by one L2 at about one time.  Where many tiles read
+// them, a head's tiles are on one XCD if there are 8 heads.
+constexpr int kXcds = 8;
+struct Place {
+  int item, head;
+};
+template <int R>
+__device__ inline Place place_of(const Args& a, int block) {
+  if constexpr (R > 1) {
+    const int item = a.heads_div.div(block);
+    return {item, block - item * a.heads};
+  }
+  const int nth = block / kXcds, group = a.heads_div.div(nth);
+  return {group * kXcds + block % kXcds, nth - group * a.heads};
+}
+// The number that a cut's part of the workspace has.
+__device__ inline int64_t part_of(const Args& a, int item, int head) {
+  return static_cast<int64_t>(item) * a.heads + head;
+}
 
 // One workgroup for a cut of the keys of a tile of 16 R rows of one K/V head.
 template <class T, int D, int R>
-__global__ __launch_bounds__(64 * waves_of(R), waves_a_simd(R, D)) void mx4_attention_kernel(
+__global__ __launch_bounds__(64 * waves_of(R, D), waves_a_simd(R, D)) void mx4_attention_kernel(
     const Args a) {
   constexpr int PARTS = __is_same(T, __bf16) ? 2 : 3;
   constexpr bool SPLIT_P = !__is_same(T, __bf16);
-  constexpr int NT = D / 16, W = waves_of(R);
+  constexpr int NT = D / 16, W = waves_of(R, D);
   using Q = Query<D, PARTS>;
   constexpr bool kQueryInRegisters = R * D <= 256;
-  // the queries, then (W / 2) x NT vectors of a lane for the sums
-  constexpr int kVectors = std::max(R * Q::kVectors, W / 2 * NT);
+  // the queries, then a row tile's sums of every wavefront
+  constexpr int kVectors = std::max(R * Q::kVectors, W * NT);
   __shared__ uint4 shared[kVectors][64];
   __shared__ int shared_scale[R][64];
   __shared__ float sum_m[W][R][16], sum_l[W][R][16];
-  const int item = a.heads_div.div(blockIdx.x);
-  const int kv_head = blockIdx.x - item * a.heads;
-  const Work w = find_work(a, item, kRows * R, false);
+  const Place at = place_of<R>(a, blockIdx.x);
+  const int kv_head = at.head;
+  const Work w = a.slots || a.starts ? find_work(a, at.item, kRows * R, false)
+                                     : find_single(a, at.item, kRows * R);
+  if (a.slots && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = w.any_cut;
   if (w.seq < 0) return;
   const Seq seq = w.s;
   const int first = w.tile * kRows * R;
   const int rows = min(kRows * R, seq.count * a.group - first);
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
+  // the block ids of this wavefront's next 32 steps, two tiles each, a lane a tile
+  int ids = 0;
+  bool bad = false;
+  auto load_ids = [&](int step) {
+    const int tile = (step + (lane >> 1) * W) * 2 + (lane & 1);
+    const int page = a.tiles_per_block.div(tile);
+    const int64_t id = a.width ? index_at(a.table, w.seq * a.table_row + min(page, a.width - 1),
+                                          a.index64) : -1;
+    const bool outside = id < 0 || id >= a.num_blocks;
+    ids = outside ? 0 : static_cast<int>(id);
+    return outside;
+  };
+  int step = (w.cuts > 1 ? w.cut * w.steps : 0) + wave;
+  bool outside = load_ids(step);
   const int keys = max(seq.keys, 0);
+  bad = seq.keys < 0;
   State<D> st[R];
   int visible[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     visible[r] = row_of(a, seq, first + min(16 * r + (lane & 15), rows - 1), kv_head).visible;
-    st[r].m = -INFINITY;
+    st[r].m = kNothing;
     st[r].l = 0.f;
     st[r].lost = 0;
 #pragma unroll
@@ -665,40 +775,39 @@ __global__ __launch_bounds__(64 * waves_of(R), waves_a_simd(R, D)) void mx4_atte
   const int fewest = uniform(visible[0]);
   const int most = lane_value(visible[R - 1], 15);
   const Lanes<D> o = lane_offsets<D>(lane, a.tokens);
-  const float scale_log2 = fabsf(a.scale_log2);
-  bool bad = seq.keys < 0;
+  // not 0, so that -infinity stays that
+  const float scale_log2 = fmaxf(fabsf(a.scale_log2), 1e-30f);
   const int last_tile = (most - 1) / kMx4TokenTile;
   const int all_steps = (most + kStep - 1) / kStep;
   const int end = w.cuts > 1 ? min(all_steps, (w.cut + 1) * w.steps) : all_steps;
-  // the block ids of the next 32 steps of this wavefront, two tiles each, a lane a tile
-  int ids = 0;
-  auto load_ids = [&](int step) {
-    const int i = (step + (lane >> 1) * W) * 2 + (lane & 1);
-    const int tile = min(i, last_tile);
-    const int page = a.tiles_per_block.div(tile);
-    int64_t id = 0;
-    if (i < 2 * end) id = index_at(a.table, w.seq * a.table_row + page, a.index64);
-    if (id < 0 || id >= a.num_blocks) {
-      bad = true;
-      id = 0;
-    }
-    ids = static_cast<int>(id);
+  // whether a tile that holds keys of this cut is in no block of the cache
+  auto check_ids = [&](int from, bool out) {
+    const int tile = (from + (lane >> 1) * W) * 2 + (lane & 1);
+    bad |= out && tile <= last_tile && tile < 2 * end;
   };
-  auto load_step = [&](int step, int nth, Tile<D> (&t)[2]) {
+  check_ids(step, outside);
+  int from = step;     // the first of the 32
+  auto load_step = [&](int s, Tile<D> (&t)[2]) {
+    if (s >= from + 32 * W) {
+      from += 32 * W;
+      check_ids(from, load_ids(from));
+    }
+    // of the last step of all, which may be another wavefront's, some block
+    const int place = min((s - from) / W, 31);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      // past the last tile: that one again, masked as a whole
-      const int i = min(2 * step + h, last_tile);
-      const int page = a.tiles_per_block.div(i);
-      const int offset = (i - page * static_cast<int>(a.tiles_per_block.d)) * kMx4TokenTile;
-      load_tile<D>(a, o, lane_value(ids, 2 * nth + h), kv_head, offset, quad, t[h]);
+      // a step's second tile may lie past the last: some block, masked as a whole
+      const int i = 2 * s + h;
+      const int offset =
+          (i - a.tiles_per_block.div(i) * static_cast<int>(a.tiles_per_block.d)) * kMx4TokenTile;
+      load_tile<D>(a, o, lane_value(ids, 2 * place + h), kv_head, offset, quad, t[h]);
     }
   };
-  int step = (w.cuts > 1 ? w.cut * w.steps : 0) + wave;
-  Tile<D> next[2];
+  constexpr int kAhead = steps_ahead(R), N = kAhead + 1;
+  Tile<D> t[N][2];
   if (step < end) {
-    load_ids(step);
-    load_step(step, 0, next);
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) load_step(min(step + n * W, end - 1), t[n]);
   }
   // a wavefront prepares a row tile's queries, for all of them
   for (int r = wave; r < R; r += W) {
@@ -743,33 +852,22 @@ __global__ __launch_bounds__(64 * waves_of(R), waves_a_simd(R, D)) void mx4_atte
     if (r == 0) asm volatile("" ::: "memory");
     return read_query(r);
   };
-  int nth = 0;
-  auto advance = [&](Tile<D> (&t)[2]) {
-    t[0] = next[0], t[1] = next[1];
-    step += W;
-    if (step < end) {
-      if (++nth == 32) {
-        load_ids(step);
-        nth = 0;
-      }
-      load_step(step, nth, next);
+  // N steps at a time: a step's registers are named by its place, so that no copy
+  // of them waits for their loads.  Past the last step it is loaded again: were the
+  // loads conditional, no wait could be for a number of them and each would be for all.
+  for (bool more = step < end; more;) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!more) break;
+      load_step(min(step + kAhead * W, end - 1), t[(n + kAhead) % N]);
+      attend<D, PARTS, R, SPLIT_P>(query, t[n], step * kStep, (step + 1) * kStep > fewest, visible,
+                                   keys, scale_log2, quad, st);
+      step += W;
+      more = step < end;
     }
-  };
-  const int all_seen = min(end, fewest / kStep);    // steps before it: every row sees all
-  while (step < all_seen) {
-    const int at = step * kStep;
-    Tile<D> t[2];
-    advance(t);
-    attend<D, PARTS, R, false, SPLIT_P>(query, t, at, visible, keys, scale_log2, quad, st);
   }
-  while (step < end) {
-    const int at = step * kStep;
-    Tile<D> t[2];
-    advance(t);
-    attend<D, PARTS, R, true, SPLIT_P>(query, t, at, visible, keys, scale_log2, quad, st);
-  }
-  // The wavefronts' sums: each to the common reference, then the upper half onto
-  // the lower until one is left, a row tile at a time.
+  // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
+  // each) adds up the elements [][i] of all.
   const bool any_bad = __any(bad);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -779,128 +877,125 @@ __global__ __launch_bounds__(64 * waves_of(R), waves_a_simd(R, D)) void mx4_atte
       sum_l[wave][r][lane] = any_bad ? bits_f32(0x7fc00000u) : l;
     }
   }
-  __syncthreads();
-  v4f(*const sum_o)[64] = reinterpret_cast<v4f(*)[64]>(shared);
+  __syncthreads();     // and the queries have been read
+  constexpr int kParts = W >= 8 ? 2 : 1, NJ = NT / kParts;
+  const int i = wave & 3, j0 = wave / 4 * NJ;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float m = -INFINITY, l = 0.f;
+    float m = kNothing, l = 0.f;
 #pragma unroll
     for (int x = 0; x < W; ++x) m = fmaxf(m, sum_m[x][r][lane & 15]);
-    const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int x = 0; x < W; ++x)
-      l += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - ref);
-    const float f = __builtin_amdgcn_exp2f(st[r].m - ref);
+      l += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - m);
+    const float f = __builtin_amdgcn_exp2f(st[r].m - m);
     v4f factor;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) factor[i] = st[r].lost >> i & 1 ? bits_f32(0x7fc00000u) : f;
+    for (int y = 0; y < 4; ++y) factor[y] = st[r].lost >> y & 1 ? bits_f32(0x7fc00000u) : f;
+    if (r) __syncthreads();
 #pragma unroll
-    for (int j = 0; j < NT; ++j) st[r].o[j] *= factor;
+    for (int j = 0; j < NT; ++j)
+      reinterpret_cast<v4f*>(shared[wave * NT + j])[lane] = st[r].o[j] * factor;
+    __syncthreads();
+    if (wave >= 4 * kParts) continue;
+    float sum[NJ];
 #pragma unroll
-    for (int half = W / 2; half > 0; half /= 2) {
-      if (wave >= half && wave < 2 * half) {
+    for (int j = 0; j < NJ; ++j) {
+      sum[j] = 0.f;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) sum_o[(wave - half) * NT + j][lane] = st[r].o[j];
-      }
-      __syncthreads();
-      if (wave < half) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) st[r].o[j] += sum_o[wave * NT + j][lane];
-      }
-      __syncthreads();
+      for (int x = 0; x < W; ++x)
+        sum[j] += reinterpret_cast<const float*>(shared[x * NT + j0 + j])[lane * 4 + i];
     }
     const int n = 16 * r + (lane & 15);
-    if (wave || n >= rows) continue;
+    if (n >= rows) continue;
     if (w.cuts == 1) {
       const Row row = row_of(a, seq, first + n, kv_head);
-      write_row<T, D>(a, row, quad, st[r].o, m, l);
+      write_row<T, D, NJ>(a, row, quad, i, j0, sum, m, l);
     } else {
-      if (quad == 0)
-        a.part_ml[static_cast<int64_t>(blockIdx.x) * kRows * R + n] = make_float2(m, l);
+      const int64_t part = part_of(a, at.item, kv_head) * R + r;
+      if (wave == 0 && quad == 0) a.part_ml[part * kRows + lane] = make_float2(m, l);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        a.part_o[(static_cast<int64_t>(blockIdx.x) * R * NT + r * NT + j) * 64 + lane] = st[r].o[j];
+      for (int j = 0; j < NJ; ++j)
+        a.part_o[((part * 4 + i) * NT + j0 + j) * 64 + lane] = sum[j];
     }
   }
 }
 
-// Joins the cuts of 16 rows, two of a lane's NT vectors (blockIdx.y: row tile and
-// which two): each of the four wavefronts takes every fourth cut, four at a time in
-// flight; their sums are added in their order.
+// Joins the cuts of a tile: of the 16 wavefronts, i + 4 g takes the elements [][i] of
+// State of every fourth cut from g on, some at a time in flight; their sums are
+// added in the order of g.
 template <class T, int D, int R>
-__global__ __launch_bounds__(256) void mx4_join_kernel(const Args a) {
-  constexpr int NT = D / 16, W = 4, kAhead = 4;
+__global__ __launch_bounds__(1024) void mx4_join_kernel(const Args a) {
+  constexpr int NT = D / 16, G = 4, kAhead = D == 256 ? 2 : 4;
+  if (!*a.any_cut) return;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
-  const int item = a.heads_div.div(blockIdx.x);
-  const int kv_head = blockIdx.x - item * a.heads;
-  const Work w = find_work(a, item, kRows * R, true);
+  const int i = wave & 3, g = wave >> 2;
+  const int tile = a.heads_div.div(blockIdx.x);
+  const int kv_head = blockIdx.x - tile * a.heads;
+  const Work w = find_work(a, tile, kRows * R, true);
   if (w.seq < 0 || w.cuts == 1) return;
-  const int r = blockIdx.y / (NT / 2), j = blockIdx.y % (NT / 2) * 2;
-  const int first = (w.tile * R + r) * kRows;
-  const int rows = min(kRows, w.s.count * a.group - first);
-  if (rows <= 0) return;
-  const bool valid = (lane & 15) < rows;
-  __shared__ v4f sum_o[W][2][64];
-  __shared__ float sum_m[W][16], sum_l[W][16];
-  v4f o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  float m = -INFINITY, l = 0.f;
-  if (valid) {
-    const int64_t cut = static_cast<int64_t>(w.first) * a.heads + kv_head;
-    const float2* const ml = a.part_ml + cut * kRows * R + 16 * r + (lane & 15);
-    const v4f* const part = a.part_o + (cut * R * NT + r * NT + j) * 64 + lane;
-    const int64_t ml_step = static_cast<int64_t>(a.heads) * kRows * R;
-    const int64_t part_step = static_cast<int64_t>(a.heads) * R * NT * 64;
-    for (int c0 = wave; c0 < w.cuts; c0 += W * kAhead) {
-      float2 x[kAhead];
-      v4f y[kAhead][2];
+  __shared__ float sum_o[G * 4][NT][64];
+  __shared__ float sum_m[G][16], sum_l[G][16];
+  for (int r = 0; r < R; ++r) {
+    const int first = (w.tile * R + r) * kRows;
+    const int rows = min(kRows, w.s.count * a.group - first);
+    if (rows <= 0) break;
+    const bool valid = (lane & 15) < rows;
+    float o[NT], m = kNothing, l = 0.f;
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const int c = c0 + n * W;
-        x[n] = make_float2(-INFINITY, 0.f);
-        y[n][0] = y[n][1] = {0.f, 0.f, 0.f, 0.f};
-        if (c < w.cuts) {
-          x[n] = ml[c * ml_step];
-          y[n][0] = part[c * part_step];
-          y[n][1] = part[c * part_step + 64];
+    for (int j = 0; j < NT; ++j) o[j] = 0.f;
+    if (valid) {
+      const int64_t part = part_of(a, w.first, kv_head) * R + r;
+      const float2* const ml = a.part_ml + part * kRows + (lane & 15);
+      const float* const po = a.part_o + (part * 4 + i) * NT * 64 + lane;
+      const int64_t next = static_cast<int64_t>(a.heads) * R;
+      for (int c0 = g; c0 < w.cuts; c0 += G * kAhead) {
+        float2 x[kAhead];
+        float y[kAhead][NT];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+          const int c = c0 + n * G;
+          x[n] = make_float2(kNothing, 0.f);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) y[n][j] = 0.f;
+          if (c < w.cuts) {
+            x[n] = ml[c * next * kRows];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) y[n][j] = po[(c * next * 4 * NT + j) * 64];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+          const float top = fmaxf(m, x[n].x);
+          const float f = __builtin_amdgcn_exp2f(m - top), h = __builtin_amdgcn_exp2f(x[n].x - top);
+          m = top;
+          l = l * f + x[n].y * h;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) o[j] = o[j] * f + y[n][j] * h;
         }
       }
-#pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const float top = fmaxf(m, x[n].x);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(x[n].x - ref);
-        m = top;
-        l = l * f + x[n].y * g;
-        o[0] = o[0] * f + y[n][0] * g;
-        o[1] = o[1] * f + y[n][1] * g;
-      }
     }
+    if (r) __syncthreads();
+    if (i == 0 && quad == 0) sum_m[g][lane] = m, sum_l[g][lane] = l;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sum_o[wave][j][lane] = o[j];
+    __syncthreads();
+    if (g || !valid) continue;
+    float top = kNothing;
+#pragma unroll
+    for (int x = 0; x < G; ++x) top = fmaxf(top, sum_m[x][lane & 15]);
+    l = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[j] = 0.f;
+#pragma unroll
+    for (int x = 0; x < G; ++x) {
+      const float f = __builtin_amdgcn_exp2f(sum_m[x][lane & 15] - top);
+      l += sum_l[x][lane & 15] * f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) o[j] += sum_o[x * 4 + i][j][lane] * f;
+    }
+    write_row<T, D, NT>(a, row_of(a, w.s, first + (lane & 15), kv_head), quad, i, 0, o, top, l);
   }
-  if (quad == 0) sum_m[wave][lane] = m, sum_l[wave][lane] = l;
-  sum_o[wave][0][lane] = o[0];
-  sum_o[wave][1][lane] = o[1];
-  __syncthreads();
-  if (wave || !valid) return;
-  float top = -INFINITY;
-#pragma unroll
-  for (int x = 0; x < W; ++x) top = fmaxf(top, sum_m[x][lane & 15]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  l = 0.f;
-  o[0] = o[1] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int x = 0; x < W; ++x) {
-    const float f = __builtin_amdgcn_exp2f(sum_m[x][lane & 15] - ref);
-    l += sum_l[x][lane & 15] * f;
-    o[0] += sum_o[x][0][lane] * f;
-    o[1] += sum_o[x][1][lane] * f;
-  }
-  const Row row = row_of(a, w.s, first + (lane & 15), kv_head);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* const out = a.out + row.at * a.out_row + row.head * a.out_head + (quad * 4 * NT + j) * 2;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint32_t*>(out + i * NT * 2) = narrow2<T>(o[0][i] * inv, o[1][i] * inv);
-  if (a.lse && quad == 0 && j == 0) write_lse(a, row, top, l);
 }
 
 // ---------------------------------------------------------------------------
@@ -948,49 +1043,61 @@ int check_attention(const fkv_mx4_attention_args& c) {
                          2, mx4_chunk_bytes(c.tokens_per_block, c.num_heads, c.head_size));
 }
 
-// Workgroups the keys are cut into where there are few tiles: as many as the device
-// holds at a time (256 compute units), since cuts are of one size.
-constexpr int kCutTarget = 512;
-
 struct LaunchPlan {
   int row_tiles;          // R
   int64_t tiles;          // times heads: the most there can be
-  int target;
+  int slots;
   int64_t workgroups;
   size_t ml_bytes, o_bytes;
 };
+
+// Workgroups that 256 compute units hold at a time.
+int slots_of(int row_tiles, int dim) {
+  return 256 * 4 * waves_a_simd(row_tiles, dim) / waves_of(row_tiles, dim);
+}
 
 LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   LaunchPlan p;
   const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
   const int64_t rows_a_seq = (rows + c.batch - 1) / c.batch;
-  p.row_tiles = rows_a_seq <= kRows ? 1 : rows_a_seq <= 2 * kRows || c.head_size > 128 ? 2 : 4;
-  const int rows_a_tile = kRows * p.row_tiles;
-  const int64_t tiles = c.query_starts
-      ? rows / rows_a_tile + c.batch
-      : static_cast<int64_t>(c.batch) * ((c.group_size + rows_a_tile - 1) / rows_a_tile);
-  p.tiles = tiles * c.num_heads;
+  auto tiles = [&](int row_tiles) {
+    const int n = kRows * row_tiles;
+    return (c.query_starts ? rows / n + c.batch
+                           : static_cast<int64_t>(c.batch) * ((c.group_size + n - 1) / n)) *
+           c.num_heads;
+  };
+  // The more rows a tile, the fewer times K and V are loaded and converted, as long
+  // as the rows fill it and the tiles the device.
+  p.row_tiles = c.head_size > 128 ? 2 : 3;
+  while (p.row_tiles > 1 && (rows_a_seq <= kRows * (p.row_tiles - 1) ||
+                             tiles(p.row_tiles) < slots_of(p.row_tiles, c.head_size)))
+    --p.row_tiles;
+  p.tiles = tiles(p.row_tiles);
   const int64_t most_steps =
       (static_cast<int64_t>(c.table_width) * c.tokens_per_block + kStep - 1) / kStep;
-  p.target = p.tiles < kCutTarget && most_steps > kMinSteps ? kCutTarget : 0;
-  p.workgroups = p.tiles + p.target;
-  p.ml_bytes = p.target ? p.workgroups * rows_a_tile * sizeof(float2) : 0;
-  p.o_bytes = p.target ? p.workgroups * rows_a_tile * static_cast<int64_t>(c.head_size) * 4 : 0;
+  const int slots = slots_of(p.row_tiles, c.head_size);
+  p.slots = most_steps > kMinSteps && p.tiles <= 2 * slots ? slots : 0;
+  // items (cuts of a tile, of all heads), in whole rounds of the XCDs
+  const int64_t items = (p.tiles + p.slots + c.num_heads - 1) / c.num_heads;
+  p.workgroups = (items + kXcds - 1) / kXcds * kXcds * c.num_heads;
+  const int64_t part_rows = p.slots ? p.workgroups * kRows * p.row_tiles : 0;
+  p.ml_bytes = part_rows * sizeof(float2) + (p.slots ? 16 : 0);    // and any_cut
+  p.o_bytes = part_rows * c.head_size * sizeof(float);
   return p;
 }
 
 template <class T, int D, int R>
 void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_attention_kernel<T, D, R>), dim3(p.workgroups), dim3(64 * waves_of(R)),
-                     0, s, a);
-  if (p.target)
-    hipLaunchKernelGGL((mx4_join_kernel<T, D, R>), dim3(p.tiles, R * D / 32), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((mx4_attention_kernel<T, D, R>), dim3(p.workgroups), dim3(64 * waves_of(R, D)), 0,
+                     s, a);
+  if (p.slots)
+    hipLaunchKernelGGL((mx4_join_kernel<T, D, R>), dim3(p.tiles), dim3(1024), 0, s, a);
 }
 template <class T, int D>
 void launch_rows(const Args& a, const LaunchPlan& p, hipStream_t s) {
   if (p.row_tiles == 1) launch<T, D, 1>(a, p, s);
   else if (p.row_tiles == 2) launch<T, D, 2>(a, p, s);
-  else if constexpr (D <= 128) launch<T, D, 4>(a, p, s);
+  else if constexpr (D <= 128) launch<T, D, 3>(a, p, s);
 }
 template <class T>
 void launch_attention(const Args& a, const LaunchPlan& p, int dim, hipStream_t s) {
@@ -1022,7 +1129,7 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
     int rc = check_attention(c);
     if (rc || c.batch == 0 || c.num_queries == 0) return rc;
     const LaunchPlan p = launch_plan(c);
-    if (p.target && (!c.workspace || c.workspace_bytes < p.ml_bytes + p.o_bytes ||
+    if (p.slots && (!c.workspace || c.workspace_bytes < p.ml_bytes + p.o_bytes ||
                      reinterpret_cast<uintptr_t>(c.workspace) % 16))
       return fail(kInval, "the workspace must hold %zu bytes on a multiple of 16, got %zu",
                   p.ml_bytes + p.o_bytes, c.workspace ? c.workspace_bytes : 0);
@@ -1042,10 +1149,11 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
     a.batch = c.batch, a.heads = c.num_heads, a.group = c.group_size, a.queries = c.num_queries;
     a.tokens = c.tokens_per_block, a.causal = c.causal;
     a.chunk = static_cast<int>(mx4_chunk_bytes(c.tokens_per_block, c.num_heads, c.head_size));
-    a.target = p.target;
+    a.slots = p.slots;
     a.scale_log2 = c.scale * kLog2e;
-    a.part_o = static_cast<v4f*>(c.workspace);
-    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.workspace) + p.o_bytes);
+    a.part_o = static_cast<float*>(c.workspace);
+    a.any_cut = reinterpret_cast<int*>(static_cast<char*>(c.workspace) + p.o_bytes);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.workspace) + p.o_bytes + 16);
     a.tiles_per_block = FastDiv(c.tokens_per_block / kMx4TokenTile);
     a.group_div = FastDiv(c.group_size);
     a.heads_div = FastDiv(c.num_heads);
