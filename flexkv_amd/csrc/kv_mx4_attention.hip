@@ -23,7 +23,8 @@
 // most steps neither compare across lanes nor scale the sums.
 //
 // A workgroup's wavefronts take the 32-token steps of its tile in turn, each loading
-// its next step while it computes one, and add up in LDS.  With few tiles the keys
+// its next step while it computes one, and add up in LDS.  Where there are many rows,
+// a tile is three times 16, for which a step's V is converted once.  With few tiles the keys
 // are cut among workgroups as well (find_work), whose sums a second kernel joins
 // in a fixed order.
 #include <hip/hip_runtime.h>
@@ -68,12 +69,8 @@ __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v);
 // A chunk of the cache as a buffer: its address is scalar, a lane adds 32 bits of
 // offset, and nothing outside the chunk is read.
 typedef __amdgpu_buffer_rsrc_t Chunk;
-__device__ inline Chunk chunk_at(const char* p, int bytes) {
-  const uint64_t u = reinterpret_cast<uint64_t>(p);
-  const uint64_t lo = static_cast<uint32_t>(uniform(static_cast<int>(u)));
-  const uint64_t hi = static_cast<uint32_t>(uniform(static_cast<int>(u >> 32)));
-  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(hi << 32 | lo), 0, bytes,
-                                           0x00027000);
+__device__ inline Chunk chunk_at(uint64_t address, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(address), 0, bytes, 0x00027000);
 }
 // quads: the 4 groups of 16 lanes
 __device__ inline float max_over_quads(float v) {
@@ -108,8 +105,8 @@ struct Args {
   int causal;
   int slots;                         // workgroups to cut the keys into; 0: uncut
   float scale_log2;
-  float2* part_ml;                   // [workgroup][row]: maximum and sum of a cut
-  float* part_o;                     // [workgroup][row tile][i][j][lane], see State
+  float2* part_ml;                   // [cut][row]: maximum and sum
+  float* part_o;                     // [cut][i][j][lane], see State
   int* any_cut;                      // whether some tile has more than one cut
   FastDiv tiles_per_block, group_div, heads_div;
 };
@@ -162,16 +159,15 @@ __device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_read
 // How the workgroups are dealt out.  A sequence has ceil(queries * group / rows a tile)
 // tiles; where the keys are cut, every tile of a sequence is cut alike, the
 // longer the sequence the more often, so that all cuts together fill the
-// `slots` the device has at a time and do not start a second round; with more tiles
-// than slots only sequences of twice a slot's share are cut.  The lengths are
+// `slots` the device has at a time and do not start a second round; with as many tiles
+// as slots only sequences longer than the mean are cut.  The lengths are
 // read here, on the device: every wavefront works the plan out for itself, sequence
 // b = lane, then 64 further on.  The first 64 sequences go longest first, and a
 // sequence's tiles last first, as causal rows see more the later they are.
 struct Work {
   int seq;                    // < 0: none
   int tile, cut, cuts;
-  bool any_cut;               // whether some tile of the first 64 sequences is cut, or
-                              // there are more sequences
+  bool any_cut;               // whether some tile is cut
   int steps;                  // of a cut
   int first;                  // the number of the tile's first cut
   Seq s;
@@ -207,14 +203,18 @@ __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool 
     tiles = move(tiles), b = move(b);
   }
   float inv_per_cut = 0.f;     // one cut
+  int longest = 0;             // of a lane's sequences
   if (a.slots) {
     float total = 0.f;
     if (few) {
       total = static_cast<float>(tiles) * static_cast<float>(steps_of(s));
+      longest = tiles ? steps_of(s) : 0;
     } else {
       for (int i = lane; i < a.batch; i += 64) {
         const Seq x = sequence(a, i);
-        total += static_cast<float>(tiles_of(a, x, rows_a_tile)) * static_cast<float>(steps_of(x));
+        const int n = tiles_of(a, x, rows_a_tile);
+        total += static_cast<float>(n) * static_cast<float>(steps_of(x));
+        if (n) longest = max(longest, steps_of(x));
       }
     }
     total = bits_f32(lane_value(f32_bits(scan_lanes(total)), 63));
@@ -229,7 +229,8 @@ __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool 
       if (static_cast<int64_t>(n) * a.heads <= a.slots) break;
     }
   }
-  Work w{-1, 0, 0, 0, false, 0, 0, Seq{0, 0, 0}};
+  Work w{-1, 0, 0, 0, static_cast<bool>(__any(cuts_of(longest, inv_per_cut) > 1)), 0, 0,
+         Seq{0, 0, 0}};
   int before = 0, cuts_before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (b0) {
@@ -242,7 +243,6 @@ __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool 
     }
     const int steps = steps_of(s);
     const int cuts = cuts_of(steps, inv_per_cut);
-    if (!b0) w.any_cut = !few || __any(tiles && cuts > 1);
     const int cut_ends = scan_lanes(tiles * cuts);
     const int ends = by_tile ? scan_lanes(tiles) : cut_ends;
     const uint64_t later = __ballot(before + ends > item);
@@ -274,6 +274,10 @@ __device__ inline Work find_single(const Args& a, int item, int rows_a_tile) {
   if (tiles > 1) {
     w.seq = uniform(item / tiles);
     w.tile = item - w.seq * tiles;
+  }
+  if (w.seq >= a.batch) {      // of the last round of the XCDs
+    w.seq = -1;
+    return w;
   }
   w.s = sequence(a, w.seq);
   w.s.keys = uniform(w.s.keys);
@@ -371,15 +375,18 @@ __device__ inline void load_query(const char* row, bool valid, int quad, bool ne
   }
 }
 
-// What a lane loads of one 16-token tile.
+// What a lane loads of a step's two 16-token tiles.
 template <int D>
-struct Tile {
+struct Keys {
   static constexpr int kSteps = (D + 127) / 128;
-  static constexpr int kWords = D >= 128 ? D / 128 : 1;   // of V a token: D / 16 codes
-  Vec4 k[kSteps];
-  int k_scale[kSteps];
-  uint32_t v[4][kWords];
-  uint32_t v_scale;     // of 4 tokens
+  Vec4 code[2][kSteps];
+  int scale[2][kSteps];
+};
+template <int D>
+struct Values {
+  static constexpr int kWords = D >= 128 ? D / 128 : 1;   // of a token: D / 16 codes
+  uint32_t code[2][4][kWords];
+  uint32_t scale[2];     // of 4 tokens
 };
 
 // Where a lane's parts of a tile lie, from the head's codes and scales on.
@@ -405,32 +412,59 @@ __device__ inline Lanes<D> lane_offsets(int lane, int tokens) {
 // loads, gain nothing).
 constexpr int kOnce = 2;
 
+// Where 16-token tiles lie, one a lane: the block's address and, in a chunk, the
+// head's codes and scales of the tile.  Worked out once for 64 tiles, since in the
+// steps' loop scalar arithmetic takes a wavefront's issue slots as well.
+struct Tiles {
+  uint32_t lo, hi;
+  int codes, scales;
+};
 template <int D>
-__device__ inline void load_tile(const Args& a, const Lanes<D>& o, int block, int head, int offset,
-                                 int quad, Tile<D>& t) {
-  const char* const page = a.mx + block * a.mbs;
-  const Chunk k = chunk_at(page, a.chunk), v = chunk_at(page + a.mks, a.chunk);
-  const int codes = uniform((head * a.tokens + offset) * (D / 2));
-  const int scales = uniform((a.heads * (D / 2) + head * (D / 32)) * a.tokens + offset);
+__device__ inline Tiles find_tiles(const Args& a, int tile, int64_t block, int head) {
+  const uint64_t p = reinterpret_cast<uint64_t>(a.mx) + static_cast<uint64_t>(block * a.mbs);
+  const int offset =
+      (tile - a.tiles_per_block.div(tile) * static_cast<int>(a.tiles_per_block.d)) * kMx4TokenTile;
+  return {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32),
+          (head * a.tokens + offset) * (D / 2),
+          (a.heads * (D / 2) + head * (D / 32)) * a.tokens + offset};
+}
+__device__ inline uint64_t block_of(const Tiles& t, int lane) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(lane_value(t.hi, lane))) << 32 |
+         static_cast<uint32_t>(lane_value(t.lo, lane));
+}
+
+// Tile h of a step, which `tile` of the tiles has.
+template <int D>
+__device__ inline void load_keys(const Args& a, const Lanes<D>& o, const Tiles& tiles, int tile,
+                                 int quad, int h, Keys<D>& t) {
+  const Chunk k = chunk_at(block_of(tiles, tile), a.chunk);
+  const int codes = lane_value(tiles.codes, tile), scales = lane_value(tiles.scales, tile);
 #pragma unroll
-  for (int s = 0; s < Tile<D>::kSteps; ++s) {
-    t.k[s] = __builtin_amdgcn_raw_buffer_load_b128(k, o.k_code + 64 * s, codes, kOnce);
-    t.k_scale[s] = __builtin_amdgcn_raw_buffer_load_b8(k, o.k_scale, scales + 4 * s * a.tokens, 0);
-    if (D == 64 && quad >= 2) t.k_scale[s] = 127;
+  for (int s = 0; s < Keys<D>::kSteps; ++s) {
+    t.code[h][s] = __builtin_amdgcn_raw_buffer_load_b128(k, o.k_code + 64 * s, codes, kOnce);
+    t.scale[h][s] =
+        __builtin_amdgcn_raw_buffer_load_b8(k, o.k_scale, scales + 4 * s * a.tokens, 0);
+    if (D == 64 && quad >= 2) t.scale[h][s] = 127;
   }
+}
+template <int D>
+__device__ inline void load_values(const Args& a, const Lanes<D>& o, const Tiles& tiles, int tile,
+                                   int h, Values<D>& t) {
+  const Chunk v = chunk_at(block_of(tiles, tile) + static_cast<uint64_t>(a.mks), a.chunk);
+  const int codes = lane_value(tiles.codes, tile), scales = lane_value(tiles.scales, tile);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (D == 64) {
-      t.v[i][0] = __builtin_amdgcn_raw_buffer_load_b16(v, o.v_code + i * (D / 2), codes, 0);
+      t.code[h][i][0] = __builtin_amdgcn_raw_buffer_load_b16(v, o.v_code + i * (D / 2), codes, 0);
     } else if constexpr (D == 128) {
-      t.v[i][0] = __builtin_amdgcn_raw_buffer_load_b32(v, o.v_code + i * (D / 2), codes, 0);
+      t.code[h][i][0] = __builtin_amdgcn_raw_buffer_load_b32(v, o.v_code + i * (D / 2), codes, 0);
     } else {
       const Vec2 w = __builtin_amdgcn_raw_buffer_load_b64(v, o.v_code + i * (D / 2), codes, 0);
-      t.v[i][0] = w[0];
-      t.v[i][1] = w[1];
+      t.code[h][i][0] = w[0];
+      t.code[h][i][1] = w[1];
     }
   }
-  t.v_scale = __builtin_amdgcn_raw_buffer_load_b32(v, o.v_scale, scales, 0);
+  t.scale[h] = __builtin_amdgcn_raw_buffer_load_b32(v, o.v_scale, scales, 0);
 }
 
 __device__ inline uint32_t cvt_bf16(uint32_t codes, float scale, int byte) {
@@ -480,17 +514,12 @@ __device__ inline v4f multiply_keys(v8i k, v8i q, v4f acc, int k_scale, int q_sc
   }
 }
 
-// Two tiles of 16 tokens from token `at` on, for R row tiles.  `partial`: some row does
-// not see all of them.  `visible`: the keys this lane's rows see; `keys`: those there are.
-// P of bf16 has 8 significant bits, its rounding averaging out over the keys;
-// where the output has 11 (SPLIT_P) the rest of P is a second bf16 operand.
-// query(r): the queries of row tile r.
-template <int D, int PARTS, int R, bool SPLIT_P, class GetQuery>
-__device__ inline void attend(GetQuery query, Tile<D> (&t)[2], int at, bool partial,
-                              const int (&visible)[R], int keys, float scale_log2, int quad,
-                              State<D> (&st)[R]) {
-  constexpr int NT = D / 16;
-  v4f s[R][2];
+// The parts of a step of 32 tokens from token `at` on, for R row tiles.
+// `visible`: the keys this lane's rows see; `keys`: those there are.
+
+// s[r][h][i] = q . k of row tile r and token 16 h + 4 quad + i; query(r) gives r's.
+template <int D, int PARTS, int R, class GetQuery>
+__device__ inline void scores(GetQuery query, const Keys<D>& t, v4f (&s)[R][2]) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const Query<D, PARTS> q = query(r);
@@ -498,141 +527,160 @@ __device__ inline void attend(GetQuery query, Tile<D> (&t)[2], int at, bool part
     for (int h = 0; h < 2; ++h) {
       s[r][h] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < Query<D, PARTS>::kSteps; ++k) {
-        const Vec4 c = t[h].k[k];
+      for (int k = 0; k < Keys<D>::kSteps; ++k) {
+        const Vec4 c = t.code[h][k];
         const v8i kc = {static_cast<int>(c[0]), static_cast<int>(c[1]), static_cast<int>(c[2]),
                         static_cast<int>(c[3]), 0, 0, 0, 0};
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p)
-          s[r][h] = multiply_keys(kc, q.part[p][k], s[r][h], t[h].k_scale[k], q.scale, p);
+          s[r][h] = multiply_keys(kc, q.part[p][k], s[r][h], t.scale[h][k], q.scale, p);
       }
     }
   }
-  if (partial) {
+}
+
+template <int R>
+__device__ inline void hide(v4f (&s)[R][2], int at, const int (&visible)[R], int quad) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (at + 16 * h + quad * 4 + i >= visible[r]) s[r][h][i] = -INFINITY;
-  }
-  v8bf p_hi[R], p_lo[R];
-  float l[R];
-  // the scores of row tile r as weights; returns the largest
-  auto weigh = [&](int r) {
-    float p[8];
-#pragma unroll
-    for (int x = 0; x < 8; ++x)
-      p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][x / 4][x % 4], scale_log2, -st[r].m));
-    float top = p[0];
-    l[r] = st[r].l + p[0];
-#pragma unroll
-    for (int x = 1; x < 8; ++x) {
-      top = fmaxf(top, p[x]);
-      l[r] += p[x];
-    }
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      hi[w] = pack_bf16(p[2 * w], p[2 * w + 1]);
-      if constexpr (SPLIT_P)
-        lo[w] = pack_bf16(p[2 * w] - bits_f32(hi[w] << 16),
-                          p[2 * w + 1] - bits_f32(hi[w] & 0xffff0000u));
-    }
-    p_hi[r] = __builtin_bit_cast(v8bf, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-    if constexpr (SPLIT_P)
-      p_lo[r] = __builtin_bit_cast(v8bf, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-    return top;
-  };
-  bool grows = false;
-#pragma unroll
-  for (int r = 0; r < R; ++r) grows |= weigh(r) > kSlack;
-  if (__any(grows)) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float top = st[r].m;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) top = fmaxf(top, s[r][x / 4][x % 4] * scale_log2);
-      const float m = max_over_quads(top);
-      const float fade = __builtin_amdgcn_exp2f(st[r].m - m);
-      st[r].m = m;
-      st[r].l *= fade;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
-      weigh(r);
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) st[r].l = l[r];
-  // Weights of 0 leave out what a row does not see only while V is finite, which
-  // it is in bf16 unless a scale byte is over 252: NaN, or bytes of a block that
-  // nothing was written to.  Those tokens are taken out here, and what the rows
-  // that do see them hold is marked as NaN.
-  auto over_252 = [](uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x03030303u) & x & 0x80808080u); };
-  if (__any((over_252(t[0].v_scale) | over_252(t[1].v_scale)) != 0)) {
-    bool any_lost = false;
-    uint32_t lost[2] = {0, 0};     // byte i: token i's group
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool there = at + 16 * h + quad * 4 + i < keys;
-        const bool over = over_252(t[h].v_scale) >> (8 * i) & 0x80u;
-        if (there && over) lost[h] |= 255u << (8 * i);
-        any_lost |= there && over;
-        if (over) {
-          t[h].v_scale &= ~(255u << (8 * i));
-#pragma unroll
-          for (int w = 0; w < Tile<D>::kWords; ++w) t[h].v[i][w] = 0;
-        }
-      }
-    if (__any(any_lost)) {
-#pragma unroll 1
-      for (int tok = 0; tok < 32; ++tok) {
-        const uint32_t mine = tok < 16 ? lost[0] : lost[1];
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t f = static_cast<uint32_t>(
-              __shfl(static_cast<int>(mine), (tok / 4 % 4) * 16 + quad * 4 + i));
-          const bool is = (f >> (8 * (tok % 4))) & 255u;
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (is && at + tok < visible[r]) st[r].lost |= 1u << i;
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < NT; j += 2) {
-    uint32_t w[2][4];     // elements j, j + 1 of each token
+  for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        w[h][i] = cvt_bf16(t[h].v[i][D >= 128 ? j / 8 : 0], byte_scale(t[h].v_scale, i),
-                           (j / 2) % 4);
-    uint4 even, odd;
-    even.x = perm(w[0][1], w[0][0], 0x05040100u);
-    even.y = perm(w[0][3], w[0][2], 0x05040100u);
-    even.z = perm(w[1][1], w[1][0], 0x05040100u);
-    even.w = perm(w[1][3], w[1][2], 0x05040100u);
-    odd.x = perm(w[0][1], w[0][0], 0x07060302u);
-    odd.y = perm(w[0][3], w[0][2], 0x07060302u);
-    odd.z = perm(w[1][1], w[1][0], 0x07060302u);
-    odd.w = perm(w[1][3], w[1][2], 0x07060302u);
-    const v8bf ve = __builtin_bit_cast(v8bf, even), vo = __builtin_bit_cast(v8bf, odd);
+        if (at + 16 * h + quad * 4 + i >= visible[r]) s[r][h][i] = -INFINITY;
+}
+
+// The weights p of a step as the second product's operand.  P of bf16 has 8
+// significant bits, its rounding averaging out over the keys; where the output has
+// 11 (SPLIT) the rest of P is a second operand.
+template <int R, bool SPLIT>
+struct Weights {
+  v8bf hi[R], lo[R];
+  float l[R];     // what State::l becomes
+};
+
+// Row tile r's scores as weights; returns their sum, which is over kSlack where one
+// of them passes the reference by more than that.
+template <int D, int R, bool SPLIT>
+__device__ inline float weigh(const v4f (&s)[R][2], const State<D>& st, int r, float scale_log2,
+                              Weights<R, SPLIT>& w) {
+  float p[8], sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      st[r].o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, p_hi[r], st[r].o[j], 0, 0, 0);
-      st[r].o[j + 1] =
-          __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, p_hi[r], st[r].o[j + 1], 0, 0, 0);
-      if constexpr (SPLIT_P) {
-        st[r].o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, p_lo[r], st[r].o[j], 0, 0, 0);
-        st[r].o[j + 1] =
-            __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, p_lo[r], st[r].o[j + 1], 0, 0, 0);
+  for (int x = 0; x < 8; ++x) {
+    p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][x / 4][x % 4], scale_log2, -st.m));
+    sum = x ? sum + p[x] : p[x];
+  }
+  w.l[r] = st.l + sum;
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    hi[x] = pack_bf16(p[2 * x], p[2 * x + 1]);
+    if constexpr (SPLIT)
+      lo[x] = pack_bf16(p[2 * x] - bits_f32(hi[x] << 16),
+                        p[2 * x + 1] - bits_f32(hi[x] & 0xffff0000u));
+  }
+  w.hi[r] = __builtin_bit_cast(v8bf, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+  if constexpr (SPLIT) w.lo[r] = __builtin_bit_cast(v8bf, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+  return sum;
+}
+
+// Some score passes its row's reference: the references follow, and the weights
+// are made again.
+template <int D, int R, bool SPLIT>
+__device__ inline void follow(const v4f (&s)[R][2], State<D> (&st)[R], float scale_log2,
+                              Weights<R, SPLIT>& w) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float top = st[r].m;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) top = fmaxf(top, s[r][x / 4][x % 4] * scale_log2);
+    const float m = max_over_quads(top);
+    const float fade = __builtin_amdgcn_exp2f(st[r].m - m);
+    st[r].m = m;
+    st[r].l *= fade;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) st[r].o[j] *= fade;
+    weigh(s, st[r], r, scale_log2, w);
+  }
+}
+
+// Weights of 0 leave out what a row does not see only while V is finite, which it is in
+// bf16 unless a scale byte is over 252: NaN, or bytes of a block that nothing was
+// written to.  Those tokens are taken out here, and what the rows that do see
+// them hold is marked as NaN.
+// bit 8 i + 7 of each byte i that is
+__device__ inline uint32_t over_252(uint32_t x) {
+  return ((x & 0x7f7f7f7fu) + 0x03030303u) & x & 0x80808080u;
+}
+template <int D>
+__device__ inline bool not_finite(const Values<D>& t) {
+  return (over_252(t.scale[0]) | over_252(t.scale[1])) != 0;
+}
+template <int D, int R>
+__device__ inline void take_out(Values<D>& t, int at, const int (&visible)[R], int keys, int quad,
+                                State<D> (&st)[R]) {
+  bool any_lost = false;
+  uint32_t lost[2] = {0, 0};     // byte i: token i's group
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t over = over_252(t.scale[h]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!(over >> (8 * i) & 0x80u)) continue;
+      if (at + 16 * h + quad * 4 + i < keys) {
+        lost[h] |= 255u << (8 * i);
+        any_lost = true;
       }
+      t.scale[h] &= ~(255u << (8 * i));
+#pragma unroll
+      for (int w = 0; w < Values<D>::kWords; ++w) t.code[h][i][w] = 0;
     }
+  }
+  if (!__any(any_lost)) return;
+#pragma unroll 1
+  for (int tok = 0; tok < 32; ++tok) {
+    const uint32_t mine = tok < 16 ? lost[0] : lost[1];
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t f = static_cast<uint32_t>(
+          __shfl(static_cast<int>(mine), (tok / 4 % 4) * 16 + quad * 4 + i));
+      const bool is = (f >> (8 * (tok % 4))) & 255u;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (is && at + tok < visible[r]) st[r].lost |= 1u << i;
+    }
+  }
+}
+
+// Elements j and j + 1 of a lane's 8 tokens of V as bf16 operands.
+template <int D>
+__device__ inline void widen(const Values<D>& t, int j, v8bf& even, v8bf& odd) {
+  uint32_t w[2][4];     // of each token both
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[h][i] = cvt_bf16(t.code[h][i][D >= 128 ? j / 8 : 0], byte_scale(t.scale[h], i),
+                         (j / 2) % 4);
+  uint32_t e[4], d[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const uint32_t lo = w[x / 2][2 * (x % 2)], hi = w[x / 2][2 * (x % 2) + 1];
+    e[x] = perm(hi, lo, 0x05040100u);
+    d[x] = perm(hi, lo, 0x07060302u);
+  }
+  even = __builtin_bit_cast(v8bf, make_uint4(e[0], e[1], e[2], e[3]));
+  odd = __builtin_bit_cast(v8bf, make_uint4(d[0], d[1], d[2], d[3]));
+}
+
+// o[j] += p v of element j of V
+template <int D, int R, bool SPLIT>
+__device__ inline void accumulate(v8bf v, int j, const Weights<R, SPLIT>& p, State<D> (&st)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    st[r].o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p.hi[r], st[r].o[j], 0, 0, 0);
+    if constexpr (SPLIT)
+      st[r].o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p.lo[r], st[r].o[j], 0, 0, 0);
   }
 }
 
@@ -688,193 +736,250 @@ __device__ inline void write_row(const Args& a, const Row& row, int quad, int i,
   if (a.lse && quad == 0 && i == 0 && j0 == 0) write_lse(a, row, m, l);
 }
 
-// Wavefronts a SIMD is to hold: more than these cost spilled registers.
-constexpr int waves_a_simd(int row_tiles, int dim) { return row_tiles == 1 && dim <= 128 ? 3 : 2; }
-// Wavefronts of a workgroup: all that a compute unit holds for a single row tile,
-// so that few sequences need no cuts; half of them for more.
-constexpr int waves_of(int row_tiles, int dim) {
-  return row_tiles == 1 ? 4 * waves_a_simd(row_tiles, dim) : 4;
-}
-// Steps whose loads a wavefront has in flight beside the one it computes.
-constexpr int steps_ahead(int row_tiles) { return row_tiles == 1 ? 2 : 1; }
-
 // Which item of the plan, and which K/V head, a workgroup has.  Workgroups go round the
-// 8 XCDs.  Where K and V are read once (R = 1), an item's heads are on one XCD, so
-// that a block is read whole by one L2 at about one time.  Where many tiles read
-// them, a head's tiles are on one XCD if there are 8 heads.
+// 8 XCDs.  Where K and V are read once, an item's heads are on one XCD, so that a
+// block is read whole by one L2 at about one time.  Where many tiles read them, a
+// head's tiles are on one XCD if there are 8 heads.
 constexpr int kXcds = 8;
 struct Place {
   int item, head;
 };
-template <int R>
-__device__ inline Place place_of(const Args& a, int block) {
-  if constexpr (R > 1) {
-    const int item = a.heads_div.div(block);
-    return {item, block - item * a.heads};
-  }
+__device__ inline Place heads_together(const Args& a, int block) {
   const int nth = block / kXcds, group = a.heads_div.div(nth);
   return {group * kXcds + block % kXcds, nth - group * a.heads};
+}
+__device__ inline Place heads_apart(const Args& a, int block) {
+  const int item = a.heads_div.div(block);
+  return {item, block - item * a.heads};
 }
 // The number that a cut's part of the workspace has.
 __device__ inline int64_t part_of(const Args& a, int item, int head) {
   return static_cast<int64_t>(item) * a.heads + head;
 }
 
-// One workgroup for a cut of the keys of a tile of 16 R rows of one K/V head.
-template <class T, int D, int R>
-__global__ __launch_bounds__(64 * waves_of(R, D), waves_a_simd(R, D)) void mx4_attention_kernel(
+// The tiles of the steps that a wavefront takes, every W-th from its first on, 32 steps
+// at a time: `kChunk` of them and the first two of the next, which are asked for early.
+// The next block ids are loaded a chunk ahead: in the steps' loop, a load of them
+// would be waited for with the steps' own.
+constexpr int kChunk = 30;     // a multiple of the steps' loops' 2 and 3
+constexpr int kNoTile = 0x7fffffff;
+template <int D, int W>
+struct Walk {
+  const Args& a;
+  int seq, head, lane;
+  int from;             // the chunk's first step
+  int last_tile, end;   // tiles and steps there are keys in
+  int64_t ids;          // of the chunk, then of the next
+  Tiles tiles;
+  int bad = kNoTile;    // a lane's first tile with keys whose block is outside the cache
+
+  __device__ int tile() const { return (from + (lane >> 1) * W) * 2 + (lane & 1); }
+  // before last_tile and end are known
+  __device__ void ask(int step) {
+    from = step;
+    ids = load_ids();
+  }
+  __device__ void start(int last, int ends) {
+    last_tile = last, end = ends;
+    settle();
+  }
+  __device__ void next_chunk() {
+    from += kChunk * W;
+    settle();
+  }
+  // A step that a wavefront asks for past its last is the last of all, perhaps another
+  // wavefront's, for which this gives some block's tile.
+  __device__ int place(int step) const { return 2 * min((step - from) / W, 31); }
+
+ private:
+  __device__ int64_t load_ids() const {
+    if (!a.width) return -1;
+    const int page = a.tiles_per_block.div(tile());
+    return index_at(a.table, seq * a.table_row + min(page, a.width - 1), a.index64);
+  }
+  __device__ void settle() {
+    const bool outside = ids < 0 || ids >= a.num_blocks;
+    if (outside && tile() <= last_tile && tile() < 2 * end) bad = min(bad, tile());
+    tiles = find_tiles<D>(a, tile(), outside ? 0 : ids, head);
+    from += kChunk * W;
+    ids = load_ids();
+    from -= kChunk * W;
+  }
+};
+
+template <int D>
+__device__ inline void clear(State<D>& st) {
+  st.m = kNothing;
+  st.l = 0.f;
+  st.lost = 0;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) st.o[j] = {0.f, 0.f, 0.f, 0.f};
+}
+
+// The scale of the scores; not 0, so that -infinity stays that.
+__device__ inline float score_scale(const Args& a) { return fmaxf(fabsf(a.scale_log2), 1e-30f); }
+
+// Row tiles of a workgroup for many queries, as registers allow.
+constexpr int most_row_tiles(int dim) { return dim <= 128 ? 3 : 2; }
+// Wavefronts a SIMD is to hold: more than these cost spilled registers.
+constexpr int waves_a_simd(int row_tiles, int dim) {
+  return row_tiles == 1 ? (dim <= 128 ? 3 : 2) : dim <= 128 ? 2 : 1;
+}
+// Wavefronts of a wide workgroup, which takes a compute unit for itself.
+constexpr int most_waves(int dim) { return 4 * waves_a_simd(1, dim); }
+
+// One workgroup of W wavefronts for a cut of the keys of a tile of 16 R rows of one K/V
+// head, whose wavefronts take the steps in turn.
+//
+// R = 1, single queries and few: memory bounds it, K and V being read once.  MI355X, 32
+// sequences of 8192 keys, 8 heads: 286 MB in 60 us, 64 sequences 571 MB in 97; with the
+// arithmetic left out 62 for 66 then, with K and V in the L2 41.  W = 12 where few
+// sequences have to fill a compute unit each, which then need few cuts, else 4.
+// R = 3 (2 of 256 elements), many queries: arithmetic bounds it.  A step of 16 rows is 256
+// cycles of matrix instructions, 190 of vector ones (128 for exponentials), and a third
+// of the 288 that V's conversion takes; two wavefronts a SIMD overlap about half of
+// that.  2048 queries of 32 heads over 8192 keys: 255 us; 2 row tiles 266; 4 with spilled
+// registers 243, but more where workgroups are few; V converted once for four
+// wavefronts of 32 rows each, through LDS, 257, and half as slow again for short
+// prompts, whose workgroups are then few.  256 elements: 654 us with one wavefront a
+// SIMD, 1054 with two and spilled registers.
+template <class T, int D, int R, int W>
+__global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kernel(
     const Args a) {
   constexpr int PARTS = __is_same(T, __bf16) ? 2 : 3;
   constexpr bool SPLIT_P = !__is_same(T, __bf16);
-  constexpr int NT = D / 16, W = waves_of(R, D);
+  constexpr int NT = D / 16;
   using Q = Query<D, PARTS>;
-  constexpr bool kQueryInRegisters = R * D <= 256;
   // the queries, then a row tile's sums of every wavefront
-  constexpr int kVectors = std::max(R * Q::kVectors, W * NT);
-  __shared__ uint4 shared[kVectors][64];
+  __shared__ uint4 shared[std::max(R * Q::kVectors, W * NT)][64];
   __shared__ int shared_scale[R][64];
   __shared__ float sum_m[W][R][16], sum_l[W][R][16];
-  const Place at = place_of<R>(a, blockIdx.x);
-  const int kv_head = at.head;
+  const Place at = R == 1 ? heads_together(a, blockIdx.x) : heads_apart(a, blockIdx.x);
   const Work w = a.slots || a.starts ? find_work(a, at.item, kRows * R, false)
                                      : find_single(a, at.item, kRows * R);
   if (a.slots && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = w.any_cut;
   if (w.seq < 0) return;
-  const Seq seq = w.s;
   const int first = w.tile * kRows * R;
-  const int rows = min(kRows * R, seq.count * a.group - first);
+  const int rows = min(kRows * R, w.s.count * a.group - first);
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
-  // the block ids of this wavefront's next 32 steps, two tiles each, a lane a tile
-  int ids = 0;
-  bool bad = false;
-  auto load_ids = [&](int step) {
-    const int tile = (step + (lane >> 1) * W) * 2 + (lane & 1);
-    const int page = a.tiles_per_block.div(tile);
-    const int64_t id = a.width ? index_at(a.table, w.seq * a.table_row + min(page, a.width - 1),
-                                          a.index64) : -1;
-    const bool outside = id < 0 || id >= a.num_blocks;
-    ids = outside ? 0 : static_cast<int>(id);
-    return outside;
-  };
+  auto row_at = [&](int n) { return row_of(a, w.s, first + min(n, rows - 1), at.head); };
+  Walk<D, W> walk{a, w.seq, at.head, lane};
   int step = (w.cuts > 1 ? w.cut * w.steps : 0) + wave;
-  bool outside = load_ids(step);
-  const int keys = max(seq.keys, 0);
-  bad = seq.keys < 0;
-  State<D> st[R];
+  walk.ask(step);
+  const int keys = max(w.s.keys, 0);
   int visible[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    visible[r] = row_of(a, seq, first + min(16 * r + (lane & 15), rows - 1), kv_head).visible;
-    st[r].m = kNothing;
-    st[r].l = 0.f;
-    st[r].lost = 0;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) st[r].o[j] = {0.f, 0.f, 0.f, 0.f};
-  }
-  // of the tile's rows, in order, the first sees the fewest, the last the most
-  const int fewest = uniform(visible[0]);
-  const int most = lane_value(visible[R - 1], 15);
-  const Lanes<D> o = lane_offsets<D>(lane, a.tokens);
-  // not 0, so that -infinity stays that
-  const float scale_log2 = fmaxf(fabsf(a.scale_log2), 1e-30f);
-  const int last_tile = (most - 1) / kMx4TokenTile;
+  for (int r = 0; r < R; ++r) visible[r] = row_at(16 * r + (lane & 15)).visible;
+  // of the rows, in order, the first sees the fewest, the last the most
+  const int fewest = lane_value(visible[0], 0), most = lane_value(visible[R - 1], 15);
   const int all_steps = (most + kStep - 1) / kStep;
   const int end = w.cuts > 1 ? min(all_steps, (w.cut + 1) * w.steps) : all_steps;
-  // whether a tile that holds keys of this cut is in no block of the cache
-  auto check_ids = [&](int from, bool out) {
-    const int tile = (from + (lane >> 1) * W) * 2 + (lane & 1);
-    bad |= out && tile <= last_tile && tile < 2 * end;
-  };
-  check_ids(step, outside);
-  int from = step;     // the first of the 32
-  auto load_step = [&](int s, Tile<D> (&t)[2]) {
-    if (s >= from + 32 * W) {
-      from += 32 * W;
-      check_ids(from, load_ids(from));
-    }
-    // of the last step of all, which may be another wavefront's, some block
-    const int place = min((s - from) / W, 31);
+  walk.start((most - 1) / kMx4TokenTile, end);
+  const Lanes<D> o = lane_offsets<D>(lane, a.tokens);
+  // Steps in flight beside the one that is computed (two measured as one).  Loads past
+  // the last step are of that one again: were they conditional, no wait could be for
+  // a number of them, and each would be for all.
+  constexpr int kAhead = 1, N = kAhead + 1;
+  static_assert(kChunk % N == 0, "");
+  Keys<D> k[N];
+  Values<D> v[N];
+  auto load = [&](int s, int n) {
+    s = min(s, end - 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      // a step's second tile may lie past the last: some block, masked as a whole
-      const int i = 2 * s + h;
-      const int offset =
-          (i - a.tiles_per_block.div(i) * static_cast<int>(a.tiles_per_block.d)) * kMx4TokenTile;
-      load_tile<D>(a, o, lane_value(ids, 2 * place + h), kv_head, offset, quad, t[h]);
+      load_keys<D>(a, o, walk.tiles, walk.place(s) + h, quad, h, k[n]);
+      load_values<D>(a, o, walk.tiles, walk.place(s) + h, h, v[n]);
     }
   };
-  constexpr int kAhead = steps_ahead(R), N = kAhead + 1;
-  Tile<D> t[N][2];
   if (step < end) {
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) load_step(min(step + n * W, end - 1), t[n]);
+    for (int n = 0; n < kAhead; ++n) load(step + n * W, n);
   }
   // a wavefront prepares a row tile's queries, for all of them
   for (int r = wave; r < R; r += W) {
     const int n = 16 * r + (lane & 15);
-    const Row row = row_of(a, seq, first + min(n, rows - 1), kv_head);
+    const Row row = row_at(n);
     Q q;
     load_query<T, D, PARTS>(a.q + row.at * a.q_row + row.head * a.q_head, n < rows, quad,
                             a.scale_log2 < 0.f, q);
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-      for (int k = 0; k < Q::kSteps; ++k) {
-        uint4 v[2];
-        __builtin_memcpy(v, &q.part[p][k], 32);
-        shared[r * Q::kVectors + (p * Q::kSteps + k) * 2][lane] = v[0];
-        shared[r * Q::kVectors + (p * Q::kSteps + k) * 2 + 1][lane] = v[1];
-      }
+    for (int x = 0; x < Q::kVectors; ++x) {
+      uint4 u;
+      __builtin_memcpy(&u, reinterpret_cast<const char*>(&q.part[0][0]) + 16 * x, 16);
+      shared[r * Q::kVectors + x][lane] = u;
+    }
     shared_scale[r][lane] = q.scale;
   }
   __syncthreads();
   auto read_query = [&](int r) {
     Q q;
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-      for (int k = 0; k < Q::kSteps; ++k) {
-        const uint4 v[2] = {shared[r * Q::kVectors + (p * Q::kSteps + k) * 2][lane],
-                            shared[r * Q::kVectors + (p * Q::kSteps + k) * 2 + 1][lane]};
-        __builtin_memcpy(&q.part[p][k], v, 32);
-      }
+    for (int x = 0; x < Q::kVectors; ++x) {
+      const uint4 u = shared[r * Q::kVectors + x][lane];
+      __builtin_memcpy(reinterpret_cast<char*>(&q.part[0][0]) + 16 * x, &u, 16);
+    }
     q.scale = shared_scale[r][lane];
     return q;
   };
-  Q kept[R];
-  if constexpr (kQueryInRegisters) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) kept[r] = read_query(r);
-  }
+  Q kept;
+  if constexpr (R == 1) kept = read_query(0);
   auto query = [&](int r) {
-    if constexpr (kQueryInRegisters) return kept[r];
-    // every step anew: held, they would be 2^6 registers
+    if constexpr (R == 1) return kept;
+    // every step anew: held, they would be 16 registers a tile and part
     if (r == 0) asm volatile("" ::: "memory");
     return read_query(r);
   };
-  // N steps at a time: a step's registers are named by its place, so that no copy
-  // of them waits for their loads.  Past the last step it is loaded again: were the
-  // loads conditional, no wait could be for a number of them and each would be for all.
-  for (bool more = step < end; more;) {
+  const float scale_log2 = score_scale(a);
+  State<D> st[R];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      if (!more) break;
-      load_step(min(step + kAhead * W, end - 1), t[(n + kAhead) % N]);
-      attend<D, PARTS, R, SPLIT_P>(query, t[n], step * kStep, (step + 1) * kStep > fewest, visible,
-                                   keys, scale_log2, quad, st);
-      step += W;
-      more = step < end;
+  for (int r = 0; r < R; ++r) clear(st[r]);
+  // N steps at a time: a step's registers are named by its place, so that no copy of
+  // them waits for their loads.
+  for (bool more = step < end; more;) {
+    for (int c = 0; c < kChunk / N && more; ++c) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (!more) break;
+        load(step + kAhead * W, (n + kAhead) % N);
+        v4f s[R][2];
+        scores<D, PARTS, R>(query, k[n], s);
+        const int token = step * kStep;
+        if (token + kStep > fewest) hide(s, token, visible, quad);
+        Weights<R, SPLIT_P> p;
+        bool passes = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) passes |= weigh(s, st[r], r, scale_log2, p) > kSlack;
+        if (__any(passes)) follow(s, st, scale_log2, p);
+        if (__any(not_finite(v[n]))) take_out(v[n], token, visible, keys, quad, st);
+#pragma unroll
+        for (int r = 0; r < R; ++r) st[r].l = p.l[r];
+#pragma unroll
+        for (int j = 0; j < NT; j += 2) {
+          v8bf even, odd;
+          widen(v[n], j, even, odd);
+          accumulate(even, j, p, st);
+          accumulate(odd, j + 1, p, st);
+        }
+        step += W;
+        more = step < end;
+      }
     }
+    walk.next_chunk();
   }
   // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
   // each) adds up the elements [][i] of all.
-  const bool any_bad = __any(bad);
+  int bad = kNoTile;
+  if (__any(walk.bad != kNoTile)) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) bad = min(bad, lane_value(walk.bad, i));
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float l = sum_over_quads(st[r].l);
     if (quad == 0) {
       sum_m[wave][r][lane] = st[r].m;
-      sum_l[wave][r][lane] = any_bad ? bits_f32(0x7fc00000u) : l;
+      const bool lost = w.s.keys < 0 || (visible[r] - 1) / kMx4TokenTile >= bad;
+      sum_l[wave][r][lane] = lost ? bits_f32(0x7fc00000u) : l;
     }
   }
   __syncthreads();     // and the queries have been read
@@ -898,104 +1003,97 @@ __global__ __launch_bounds__(64 * waves_of(R, D), waves_a_simd(R, D)) void mx4_a
       reinterpret_cast<v4f*>(shared[wave * NT + j])[lane] = st[r].o[j] * factor;
     __syncthreads();
     if (wave >= 4 * kParts) continue;
-    float sum[NJ];
+    float sums[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      sum[j] = 0.f;
+      sums[j] = 0.f;
 #pragma unroll
       for (int x = 0; x < W; ++x)
-        sum[j] += reinterpret_cast<const float*>(shared[x * NT + j0 + j])[lane * 4 + i];
+        sums[j] += reinterpret_cast<const float*>(shared[x * NT + j0 + j])[lane * 4 + i];
     }
     const int n = 16 * r + (lane & 15);
     if (n >= rows) continue;
-    if (w.cuts == 1) {
-      const Row row = row_of(a, seq, first + n, kv_head);
-      write_row<T, D, NJ>(a, row, quad, i, j0, sum, m, l);
+    if (R > 1 || w.cuts == 1) {
+      write_row<T, D, NJ>(a, row_at(n), quad, i, j0, sums, m, l);
     } else {
-      const int64_t part = part_of(a, at.item, kv_head) * R + r;
+      const int64_t part = part_of(a, at.item, at.head);    // one row tile
       if (wave == 0 && quad == 0) a.part_ml[part * kRows + lane] = make_float2(m, l);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        a.part_o[((part * 4 + i) * NT + j0 + j) * 64 + lane] = sum[j];
+      for (int j = 0; j < NJ; ++j) a.part_o[((part * 4 + i) * NT + j0 + j) * 64 + lane] = sums[j];
     }
   }
 }
 
-// Joins the cuts of a tile: of the 16 wavefronts, i + 4 g takes the elements [][i] of
-// State of every fourth cut from g on, some at a time in flight; their sums are
+// Joins the cuts of a tile: of the 4 G wavefronts, i + 4 g takes the elements [][i] of
+// State of every G-th cut from g on, some at a time in flight; their sums are
 // added in the order of g.
-template <class T, int D, int R>
-__global__ __launch_bounds__(1024) void mx4_join_kernel(const Args a) {
-  constexpr int NT = D / 16, G = 4, kAhead = D == 256 ? 2 : 4;
+template <class T, int D, int G>
+__global__ __launch_bounds__(256 * G) void mx4_join_kernel(const Args a) {
+  constexpr int NT = D / 16, kAhead = D == 256 ? 2 : 4;
   if (!*a.any_cut) return;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
   const int i = wave & 3, g = wave >> 2;
   const int tile = a.heads_div.div(blockIdx.x);
   const int kv_head = blockIdx.x - tile * a.heads;
-  const Work w = find_work(a, tile, kRows * R, true);
+  const Work w = find_work(a, tile, kRows, true);
   if (w.seq < 0 || w.cuts == 1) return;
   __shared__ float sum_o[G * 4][NT][64];
   __shared__ float sum_m[G][16], sum_l[G][16];
-  for (int r = 0; r < R; ++r) {
-    const int first = (w.tile * R + r) * kRows;
-    const int rows = min(kRows, w.s.count * a.group - first);
-    if (rows <= 0) break;
-    const bool valid = (lane & 15) < rows;
-    float o[NT], m = kNothing, l = 0.f;
+  const int first = w.tile * kRows;
+  const bool valid = first + (lane & 15) < w.s.count * a.group;
+  float o[NT], m = kNothing, l = 0.f;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) o[j] = 0.f;
-    if (valid) {
-      const int64_t part = part_of(a, w.first, kv_head) * R + r;
-      const float2* const ml = a.part_ml + part * kRows + (lane & 15);
-      const float* const po = a.part_o + (part * 4 + i) * NT * 64 + lane;
-      const int64_t next = static_cast<int64_t>(a.heads) * R;
-      for (int c0 = g; c0 < w.cuts; c0 += G * kAhead) {
-        float2 x[kAhead];
-        float y[kAhead][NT];
+  for (int j = 0; j < NT; ++j) o[j] = 0.f;
+  if (valid) {
+    const int64_t part = part_of(a, w.first, kv_head);
+    const float2* const ml = a.part_ml + part * kRows + (lane & 15);
+    const float* const po = a.part_o + (part * 4 + i) * NT * 64 + lane;
+    const int64_t next = a.heads;
+    for (int c0 = g; c0 < w.cuts; c0 += G * kAhead) {
+      float2 x[kAhead];
+      float y[kAhead][NT];
 #pragma unroll
-        for (int n = 0; n < kAhead; ++n) {
-          const int c = c0 + n * G;
-          x[n] = make_float2(kNothing, 0.f);
+      for (int n = 0; n < kAhead; ++n) {
+        const int c = c0 + n * G;
+        x[n] = make_float2(kNothing, 0.f);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) y[n][j] = 0.f;
-          if (c < w.cuts) {
-            x[n] = ml[c * next * kRows];
+        for (int j = 0; j < NT; ++j) y[n][j] = 0.f;
+        if (c < w.cuts) {
+          x[n] = ml[c * next * kRows];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) y[n][j] = po[(c * next * 4 * NT + j) * 64];
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < kAhead; ++n) {
-          const float top = fmaxf(m, x[n].x);
-          const float f = __builtin_amdgcn_exp2f(m - top), h = __builtin_amdgcn_exp2f(x[n].x - top);
-          m = top;
-          l = l * f + x[n].y * h;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) o[j] = o[j] * f + y[n][j] * h;
+          for (int j = 0; j < NT; ++j) y[n][j] = po[(c * next * 4 * NT + j) * 64];
         }
       }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const float top = fmaxf(m, x[n].x);
+        const float f = __builtin_amdgcn_exp2f(m - top), h = __builtin_amdgcn_exp2f(x[n].x - top);
+        m = top;
+        l = l * f + x[n].y * h;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o[j] = o[j] * f + y[n][j] * h;
+      }
     }
-    if (r) __syncthreads();
-    if (i == 0 && quad == 0) sum_m[g][lane] = m, sum_l[g][lane] = l;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) sum_o[wave][j][lane] = o[j];
-    __syncthreads();
-    if (g || !valid) continue;
-    float top = kNothing;
-#pragma unroll
-    for (int x = 0; x < G; ++x) top = fmaxf(top, sum_m[x][lane & 15]);
-    l = 0.f;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) o[j] = 0.f;
-#pragma unroll
-    for (int x = 0; x < G; ++x) {
-      const float f = __builtin_amdgcn_exp2f(sum_m[x][lane & 15] - top);
-      l += sum_l[x][lane & 15] * f;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) o[j] += sum_o[x * 4 + i][j][lane] * f;
-    }
-    write_row<T, D, NT>(a, row_of(a, w.s, first + (lane & 15), kv_head), quad, i, 0, o, top, l);
   }
+  if (i == 0 && quad == 0) sum_m[g][lane] = m, sum_l[g][lane] = l;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) sum_o[wave][j][lane] = o[j];
+  __syncthreads();
+  if (g || !valid) return;
+  float top = kNothing;
+#pragma unroll
+  for (int x = 0; x < G; ++x) top = fmaxf(top, sum_m[x][lane & 15]);
+  l = 0.f;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) o[j] = 0.f;
+#pragma unroll
+  for (int x = 0; x < G; ++x) {
+    const float f = __builtin_amdgcn_exp2f(sum_m[x][lane & 15] - top);
+    l += sum_l[x][lane & 15] * f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[j] += sum_o[x * 4 + i][j][lane] * f;
+  }
+  write_row<T, D, NT>(a, row_of(a, w.s, first + (lane & 15), kv_head), quad, i, 0, o, top, l);
 }
 
 // ---------------------------------------------------------------------------
@@ -1046,64 +1144,68 @@ int check_attention(const fkv_mx4_attention_args& c) {
 struct LaunchPlan {
   int row_tiles;          // R
   int64_t tiles;          // times heads: the most there can be
+  bool wide;              // a workgroup has all wavefronts of a compute unit, else 4
   int slots;
   int64_t workgroups;
   size_t ml_bytes, o_bytes;
 };
 
-// Workgroups that 256 compute units hold at a time.
-int slots_of(int row_tiles, int dim) {
-  return 256 * 4 * waves_a_simd(row_tiles, dim) / waves_of(row_tiles, dim);
-}
+constexpr int kComputeUnits = 256;
 
 LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   LaunchPlan p;
   const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
-  const int64_t rows_a_seq = (rows + c.batch - 1) / c.batch;
   auto tiles = [&](int row_tiles) {
     const int n = kRows * row_tiles;
     return (c.query_starts ? rows / n + c.batch
                            : static_cast<int64_t>(c.batch) * ((c.group_size + n - 1) / n)) *
            c.num_heads;
   };
-  // The more rows a tile, the fewer times K and V are loaded and converted, as long
-  // as the rows fill it and the tiles the device.
-  p.row_tiles = c.head_size > 128 ? 2 : 3;
-  while (p.row_tiles > 1 && (rows_a_seq <= kRows * (p.row_tiles - 1) ||
-                             tiles(p.row_tiles) < slots_of(p.row_tiles, c.head_size)))
-    --p.row_tiles;
+  // Many rows a tile share V's conversion, but have fewer workgroups, which are not
+  // cut along the keys: they have to fill the compute units.
+  const int many = most_row_tiles(c.head_size);
+  p.row_tiles = rows > static_cast<int64_t>(c.batch) * kRows * (many - 1) &&
+                        tiles(many) >= kComputeUnits ? many : 1;
   p.tiles = tiles(p.row_tiles);
   const int64_t most_steps =
       (static_cast<int64_t>(c.table_width) * c.tokens_per_block + kStep - 1) / kStep;
-  const int slots = slots_of(p.row_tiles, c.head_size);
-  p.slots = most_steps > kMinSteps && p.tiles <= 2 * slots ? slots : 0;
+  // Tiles for every compute unit: smaller workgroups, three a compute unit, take
+  // turns better (40 sequences of 8192 keys: 78 us; wide ones 91), and only sequences
+  // longer than the mean are cut: 64 of 2048 keys 31 us, uncut 26, but one of 16384 among
+  // 39 of 500 keys 27 us, uncut 82.  With many more tiles the plan costs more.
+  p.wide = p.tiles <= kComputeUnits;
+  p.slots = p.row_tiles > 1 || most_steps <= kMinSteps || p.tiles > 4 * kComputeUnits ? 0
+            : p.wide ? kComputeUnits : static_cast<int>(p.tiles);
   // items (cuts of a tile, of all heads), in whole rounds of the XCDs
   const int64_t items = (p.tiles + p.slots + c.num_heads - 1) / c.num_heads;
   p.workgroups = (items + kXcds - 1) / kXcds * kXcds * c.num_heads;
-  const int64_t part_rows = p.slots ? p.workgroups * kRows * p.row_tiles : 0;
+  const int64_t part_rows = p.slots ? p.workgroups * kRows : 0;
   p.ml_bytes = part_rows * sizeof(float2) + (p.slots ? 16 : 0);    // and any_cut
   p.o_bytes = part_rows * c.head_size * sizeof(float);
   return p;
 }
 
-template <class T, int D, int R>
+template <class T, int D, int R, int W>
 void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_attention_kernel<T, D, R>), dim3(p.workgroups), dim3(64 * waves_of(R, D)), 0,
-                     s, a);
-  if (p.slots)
-    hipLaunchKernelGGL((mx4_join_kernel<T, D, R>), dim3(p.tiles), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL((mx4_attention_kernel<T, D, R, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
 }
 template <class T, int D>
-void launch_rows(const Args& a, const LaunchPlan& p, hipStream_t s) {
-  if (p.row_tiles == 1) launch<T, D, 1>(a, p, s);
-  else if (p.row_tiles == 2) launch<T, D, 2>(a, p, s);
-  else if constexpr (D <= 128) launch<T, D, 3>(a, p, s);
+void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
+  if (p.row_tiles > 1) {
+    launch<T, D, most_row_tiles(D), 4>(a, p, s);
+  } else if (p.wide) {
+    launch<T, D, 1, most_waves(D)>(a, p, s);
+    if (p.slots) hipLaunchKernelGGL((mx4_join_kernel<T, D, 4>), dim3(p.tiles), dim3(1024), 0, s, a);
+  } else {
+    launch<T, D, 1, 4>(a, p, s);
+    if (p.slots) hipLaunchKernelGGL((mx4_join_kernel<T, D, 1>), dim3(p.tiles), dim3(256), 0, s, a);
+  }
 }
 template <class T>
 void launch_attention(const Args& a, const LaunchPlan& p, int dim, hipStream_t s) {
-  if (dim == 64) launch_rows<T, 64>(a, p, s);
-  else if (dim == 128) launch_rows<T, 128>(a, p, s);
-  else launch_rows<T, 256>(a, p, s);
+  if (dim == 64) launch<T, 64>(a, p, s);
+  else if (dim == 128) launch<T, 128>(a, p, s);
+  else launch<T, 256>(a, p, s);
 }
 
 }  // namespace

@@ -445,13 +445,19 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
  * lse (may be null): log of the sum of exp(scale * q . k).
  *
  * head_size 64, 128 or 256; dtype (of query and out) FKV_DTYPE_BF16 or _FP16.  Sums,
- * maximum and normalisation are held in 32 bits; the queries enter exactly, and the
- * weights p with 8 significant bits for bf16, 16 for fp16.  Block ids, lengths and starts are device memory, all int32 or all
- * int64 (index_is_64bit), read by the kernels: a block id outside the cache or a
- * length past the table's row makes that sequence's rows NaN, and nothing outside
- * the cache is read.  Starts have to ascend; rows of no sequence are left as they
- * were.  A NaN in a key or value reaches the rows that see that token and no
- * other.  A query row that holds an infinity or a NaN gives NaN.
+ * maximum and normalisation are held in 32 bits.  The queries enter exactly, but for
+ * elements 2^13 below their row's largest, which lose bits under 2^-21 of it; the
+ * weights p with 8 significant bits for bf16, 16 for fp16.  Block ids, lengths and
+ * starts are device memory, all int32 or all int64 (index_is_64bit), read by the
+ * kernels, and nothing outside the cache is read for any of them: a block id outside
+ * the cache gives NaN in the rows that see a token of that block, a length past the
+ * table's row in all rows of its sequence, and a length below 0 is taken as 0.
+ * Starts have to ascend; rows of no sequence are left as they were.
+ *
+ * A NaN in a key reaches the rows that see that token, in a value those elements of
+ * these rows, and no other.  A value group with a scale byte of 253 or 254, which
+ * quantising never writes, counts as NaN.  A query row that holds an infinity or
+ * a NaN gives NaN.
  * Asynchronous on `stream`, and may be captured into a graph. */
 typedef struct fkv_mx4_attention_args {
   const void* query;                 /* [num_queries][num_heads * group_size][head_size] */

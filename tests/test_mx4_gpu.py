@@ -405,6 +405,21 @@ PACKED = [
 ]
 
 
+@pytest.mark.parametrize("kw", DECODE, ids=lambda kw: "-".join(str(v) for v in kw.values()))
+def test_nothing_beside_the_rows_of_single_queries_is_written(kw):
+    """Whatever the number of sequences and heads, rows before and behind stay."""
+    c = Case(queries=[1] * len(kw["keys"]), seed=len(kw["keys"]), **kw)
+    c.to_device()
+    want, lse = c.run(single=True)
+    big = torch.full((c.rows + 80, c.H * c.G, c.D), 5.0, dtype=c.dtype, device=DEV)
+    bl = torch.full((c.rows + 80, c.H * c.G), 77.0, device=DEV)
+    at = slice(40, 40 + c.rows)
+    c_ext.mx4_attention(c.dq, c.dmx, c.H, c.dtable, c.dlens, None, out=big[at], lse=bl[at])
+    assert torch.equal(big[at].cpu(), want) and torch.equal(bl[at].cpu(), lse)
+    big[at], bl[at] = 5, 77
+    assert (big == 5).all() and (bl == 77).all()
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("kw", PACKED, ids=lambda kw: "-".join(str(v) for v in kw.values()))
 def test_packed_queries(kw, causal):
@@ -415,6 +430,77 @@ def test_packed_queries(kw, causal):
     c.check(got, lse, causal=causal)
     # rows of no sequence are left as they were
     assert (got[-3:] == 5).all() and (lse[-3:] == 77).all()
+
+
+# many heads and rows: several row tiles share a workgroup
+MANY_ROWS = [
+    dict(keys=[40, 0, 100, 133, 20], queries=[23, 0, 1, 90, 20], H=32, G=4, D=128),
+    dict(keys=[300, 45], queries=[61, 45], H=64, G=3, D=64, T=32, dtype=FP16),
+    dict(keys=[97, 12, 65], queries=[97, 17, 40], H=32, G=4, D=128, dtype=FP16, blockwise=True),
+    dict(keys=[150, 31], queries=[50, 31], H=48, G=2, D=256, T=48),
+    dict(keys=[71, 64], queries=[71, 50], H=32, G=3, D=256, dtype=FP16, index=torch.int64),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("kw", MANY_ROWS, ids=lambda kw: "-".join(str(v) for v in kw.values()))
+def test_packed_queries_of_many_heads(kw, causal):
+    c = Case(seed=17, spare_rows=2, **kw)
+    c.poison_unseen()
+    out = torch.full((c.rows, c.H * c.G, c.D), 5.0, dtype=c.dtype, device=DEV)
+    got, lse = c.run(causal=causal, out=out)
+    c.check(got, lse, causal=causal)
+    assert (got[-2:] == 5).all() and (lse[-2:] == 77).all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (128, BF16), (256, BF16)])
+def test_many_heads_nan_growing_scores_and_bad_pages(D, dtype):
+    c = Case(keys=[120, 90, 80], queries=[80, 90, 60], H=32, G=4, D=D, dtype=dtype, seed=23)
+    cut = c.T * c.H * D // 2
+    for half, b, t, head, group in ((0, 0, 60, 0, 1), (1, 0, 75, 31, 0), (1, 1, 0, 7, 1),
+                                    (1, 1, 89, 8, 0), (0, 1, 88, 9, 0)):
+        sc = c.mx[half, c.table[b, t // c.T], cut:].view(c.H, D // 32, c.T)
+        sc[head, group, t % c.T] = 255
+    # keys that grow by 2^12 along a sequence: the running reference follows
+    for t in range(80):
+        sc = c.mx[0, c.table[2, t // c.T], cut:].view(c.H, D // 32, c.T)
+        sc[:, :, t % c.T] = 120 + t * 12 // 80
+    out, lse = c.run()
+    c.check(out, lse)
+    c.table[2, 2] = c.N
+    bad, lse = c.run()
+    # tokens 32 and on: query i of the sequence's 60 sees 21 + i
+    assert torch.isnan(bad[182:]).all() and torch.isnan(lse[182:]).all()
+    assert _same(bad[:182], out[:182])
+
+
+@pytest.mark.parametrize("batch,H,D,dtype", [
+    (3, 1, 64, BF16), (64, 1, 64, FP16), (65, 1, 128, BF16), (130, 2, 64, BF16),
+    (40, 8, 64, FP16), (34, 8, 256, BF16), (70, 8, 64, BF16), (131, 8, 64, BF16)])
+def test_cuts_of_ragged_lengths_and_of_many_sequences(batch, H, D, dtype):
+    """Long sequences beside short ones, above and below the numbers of sequences and of
+    tiles that plan the cuts differently."""
+    g = _gen(batch)
+    keys = torch.randint(0, 40, (batch,), generator=g).tolist()
+    keys[1], keys[2], keys[-1] = 4100 // H, 1500, 2600
+    c = Case(keys=keys, queries=[1] * batch, H=H, G=3, D=D, T=32, dtype=dtype, seed=batch)
+    c.poison_unseen()
+    c.check(*c.run(single=True))
+    c.check(*c.run(single=False))
+
+
+@pytest.mark.parametrize("byte,lost", [(252, False), (253, True), (254, True), (255, True)])
+def test_value_scales_that_quantising_never_writes_count_as_nan(byte, lost):
+    for keys, queries, H in (([70], [3], 2), ([70, 33], [70, 33], 64)):
+        c = Case(keys=keys, queries=queries, H=H, G=4, D=128, seed=byte)
+        cut = c.T * H * c.D // 2
+        c.mx[1, c.table[0, 1], cut:].view(H, c.D // 32, c.T)[1, 2, 5] = byte
+        out, _ = c.run()
+        rows = queries[0]
+        hit = torch.zeros(c.rows, H, c.G, c.D, dtype=torch.bool)
+        first = max(0, 21 - (keys[0] - rows))           # the first query that sees token 21
+        hit[first:rows, 1, :, 64:96] = lost
+        assert torch.equal(torch.isnan(out.view_as(hit)), hit)
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
