@@ -298,9 +298,18 @@ _fast = None
 _INT_MAX = 2**31 - 1
 
 
+def c_int(v, what: str) -> int:
+    """An integer that the C-ABI takes as int; ctypes would cut it off."""
+    v = operator.index(v)
+    if not -_INT_MAX - 1 <= v <= _INT_MAX:
+        raise OverflowError(f"{what} {v} does not fit a C int")
+    return v
+
+
 class _CtypesCalls:
     """The per-call path of c_ext.transfer_kv_blocks and
-    transfer_kv_blocks_kv_ptrs over ctypes, with the compiled module's
+    transfer_kv_blocks_kv_ptrs over ctypes (and none for the functions on a
+    4-bit cache, whose ctypes calls c_ext makes itself), with the compiled module's
     argument conventions: the same 16 / 15 positional arguments, False
     (nothing raised) when a tensor check fails so that c_ext names the
     argument, RuntimeError with the library's message when the transfer
@@ -322,12 +331,7 @@ class _CtypesCalls:
             return FKV_XFER_CE if bool(v) else FKV_XFER_KERNEL
         return operator.index(v)
 
-    @staticmethod
-    def _c_int(v, what: str) -> int:
-        v = operator.index(v)
-        if not -_INT_MAX - 1 <= v <= _INT_MAX:
-            raise OverflowError(f"{what} {v} does not fit a C int")
-        return v
+    _c_int = staticmethod(c_int)
 
     def _stream(self, stream):
         if stream is not None:
@@ -342,6 +346,12 @@ class _CtypesCalls:
         if rc != 0:
             msg = last_error()
             raise RuntimeError(msg or f"transfer failed ({rc})")
+
+    @staticmethod
+    def mx4_blocks(*args):
+        return False
+
+    mx4_tokens = mx4_attention = mx4_blocks
 
     def transfer_kv_blocks(self, gids, ptrs, gkv, gblk, cids, cpu, ckv, clay, cblk, chunk,
                            start, sms, h2d, mode, mla, stream):
@@ -421,6 +431,9 @@ def fast():
                 return ctypes.cast(fn, ctypes.c_void_p).value
             _fkv_py.bind(addr(lib.fkv_transfer_kv_blocks), addr(lib.fkv_transfer_kv_blocks_kv_ptrs),
                          addr(lib.fkv_last_error), FKV_XFER_KERNEL, FKV_XFER_CE)
+            _fkv_py.bind_mx4(addr(lib.fkv_quantize_kv_blocks), addr(lib.fkv_dequantize_kv_blocks),
+                             addr(lib.fkv_quantize_kv_tokens),
+                             addr(lib.fkv_mx4_attention_workspace), addr(lib.fkv_mx4_attention))
             _fast = _fkv_py
     return _fast
 

@@ -78,8 +78,9 @@ def py_command() -> list:
             f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__",
             "-I", sysconfig.get_paths()["include"], "-I", os.path.join(tdir, "include"),
             "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-            "-I", os.path.join(rocm, "include"),
-            PY_SOURCE, "-o", PY_OUT + ".tmp", "-L", tlib, "-ltorch_python", "-lc10", "-lc10_hip",
+            "-I", os.path.join(rocm, "include"), "-I", os.path.join(ROOT, "include"),
+            PY_SOURCE, "-o", PY_OUT + ".tmp", "-L", tlib, "-ltorch_python", "-ltorch_cpu", "-lc10",
+            "-lc10_hip",
             f"-Wl,-rpath,{tlib}"]
 
 

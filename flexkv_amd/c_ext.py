@@ -222,6 +222,13 @@ def _mx_blocks(fn_name: str, gpu_block_id_tensor, gpu_layer_ptrs_tensor, gpu_kv_
                gpu_block_stride_in_bytes, mx_block_id_tensor, mx_tensor, mx_kv_stride_in_bytes,
                mx_layer_stride_in_bytes, mx_block_stride_in_bytes, tokens_per_block, num_heads,
                head_size, dtype, start_layer_id, is_mla) -> None:
+    if (_fast or _load_fast()).mx4_blocks(
+            fn_name == "quantize_kv_blocks", gpu_block_id_tensor, gpu_layer_ptrs_tensor,
+            gpu_kv_stride_in_bytes, gpu_block_stride_in_bytes, mx_block_id_tensor, mx_tensor,
+            mx_kv_stride_in_bytes, mx_layer_stride_in_bytes, mx_block_stride_in_bytes,
+            tokens_per_block, num_heads, head_size, _lib.DTYPES.get(dtype), start_layer_id,
+            is_mla) is not False:
+        return
     _require_int64_host(gpu_block_id_tensor, "gpu_block_id_tensor")
     _require_int64_host(gpu_layer_ptrs_tensor, "gpu_layer_ptrs_tensor")
     _require_int64_host(mx_block_id_tensor, "mx_block_id_tensor")
@@ -233,13 +240,16 @@ def _mx_blocks(fn_name: str, gpu_block_id_tensor, gpu_layer_ptrs_tensor, gpu_kv_
                            f"{mx_block_id_tensor.numel()}")
     code = _dtype_code(dtype, fn_name)
     stream = _stream_handle(fn_name)
+    ix, c_int = operator.index, _lib.c_int
     rc = getattr(_lib.load(), "fkv_" + fn_name)(
-        n, int(start_layer_id), int(gpu_layer_ptrs_tensor.numel()),
+        c_int(n, "block ids"), c_int(start_layer_id, "start_layer_id"),
+        c_int(gpu_layer_ptrs_tensor.numel(), "layer pointers"),
         gpu_block_id_tensor.data_ptr(), gpu_layer_ptrs_tensor.data_ptr(),
-        int(gpu_kv_stride_in_bytes), int(gpu_block_stride_in_bytes),
-        mx_block_id_tensor.data_ptr(), mx_tensor.data_ptr(), int(mx_kv_stride_in_bytes),
-        int(mx_layer_stride_in_bytes), int(mx_block_stride_in_bytes), int(tokens_per_block),
-        int(num_heads), int(head_size), code, stream, 1 if is_mla else 0)
+        ix(gpu_kv_stride_in_bytes), ix(gpu_block_stride_in_bytes),
+        mx_block_id_tensor.data_ptr(), mx_tensor.data_ptr(), ix(mx_kv_stride_in_bytes),
+        ix(mx_layer_stride_in_bytes), ix(mx_block_stride_in_bytes),
+        c_int(tokens_per_block, "tokens_per_block"), c_int(num_heads, "num_heads"),
+        c_int(head_size, "head_size"), code, stream, 1 if is_mla else 0)
     if rc != 0:
         raise RuntimeError(_lib.last_error() or f"{fn_name} failed ({rc})")
 
@@ -325,6 +335,8 @@ def quantize_kv_tokens(key: torch.Tensor, value, mx_layer: torch.Tensor,
     past the cache being padding.  Slots have to differ.  Asynchronous on the
     current torch stream; may be captured into a graph."""
     fn = "quantize_kv_tokens"
+    if (_fast or _load_fast()).mx4_tokens(key, value, mx_layer, slots) is not False:
+        return
     _require_device(key, "key", fn)
     device = key.device
     if key.dim() != 3 or key.stride(2) != 1:
@@ -375,6 +387,10 @@ def mx4_attention(query: torch.Tensor, mx_layer: torch.Tensor, num_kv_heads: int
     Returns ``out``.  Asynchronous on the current torch stream; may be captured
     into a graph."""
     fn = "mx4_attention"
+    done = (_fast or _load_fast()).mx4_attention(query, mx_layer, num_kv_heads, block_table,
+                                                 seq_lens, query_starts, scale, causal, out, lse)
+    if done is not False:
+        return done
     _require_device(query, "query", fn)
     device = query.device
     if query.dim() != 3 or query.stride(2) != 1 or query.dtype not in (torch.bfloat16,

@@ -726,6 +726,38 @@ def test_a_captured_step_replays_with_other_lengths_and_tokens():
         assert torch.equal(cache, c.dmx)
 
 
+def test_calls_over_ctypes_give_the_same(monkeypatch):
+    def run():
+        b = Blocks(L=2, T=16, H=2, D=64, dtype=BF16)
+        b.call(c_ext.quantize_kv_blocks, [4, 0], [6, 2])
+        b.call(c_ext.dequantize_kv_blocks, [1, 5], [2, 0])
+        with pytest.raises(RuntimeError, match="gpu block ids"):
+            b.call(c_ext.quantize_kv_blocks, [1 << 30], [0])
+        with pytest.raises(OverflowError):
+            c_ext.quantize_kv_blocks(torch.tensor([0]), b.ptrs, b.gkv, b.gblk, torch.tensor([0]),
+                                     b.mx, b.mkv, b.mlay, b.mblk, 16 + (1 << 32), 2, 64, BF16)
+        c = Case(keys=[75, 40], queries=[5, 1], seed=6)
+        c.to_device()
+        kv = c.qkv.to(DEV)
+        H, G = c.H, c.G
+        out = _step(c, kv[:, H * G:H * G + H], kv[:, H * G + H:], torch.arange(6, device=DEV))
+        single = c_ext.mx4_attention(c.dq, c.dmx, H, c.dtable, c.dlens, None, 1, True)[:2]
+        with pytest.raises(RuntimeError, match="scale"):
+            c_ext.mx4_attention(c.dq, c.dmx, H, c.dtable, c.dlens, scale=math.nan)
+        return [b.mx, *b.wide, c.dmx, out, single]
+    compiled = run()
+    assert type(_lib.fast()).__name__ == "module"
+    monkeypatch.setenv("FLEXKV_PY_FASTCALL", "0")
+    _lib.reset_fast()
+    try:
+        plain = run()
+        assert type(_lib.fast()).__name__ == "_CtypesCalls"
+    finally:
+        monkeypatch.undo()
+        _lib.reset_fast()
+    assert all(_same(x, y) for x, y in zip(compiled, plain))
+
+
 def test_two_streams_at_once():
     cases = [Case(keys=[2500, 40 + i], queries=[1, 3], H=2, G=4, seed=40 + i) for i in range(2)]
     for c in cases:
