@@ -1013,10 +1013,10 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
     }
     const int n = 16 * r + (lane & 15);
     if (n >= rows) continue;
-    if (R > 1 || w.cuts == 1) {
+    if (w.cuts == 1) {
       write_row<T, D, NJ>(a, row_at(n), quad, i, j0, sums, m, l);
     } else {
-      const int64_t part = part_of(a, at.item, at.head);    // one row tile
+      const int64_t part = part_of(a, at.item, at.head) * R + r;
       if (wave == 0 && quad == 0) a.part_ml[part * kRows + lane] = make_float2(m, l);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) a.part_o[((part * 4 + i) * NT + j0 + j) * 64 + lane] = sums[j];
@@ -1027,28 +1027,29 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
 // Joins the cuts of a tile: of the 4 G wavefronts, i + 4 g takes the elements [][i] of
 // State of every G-th cut from g on, some at a time in flight; their sums are
 // added in the order of g.
-template <class T, int D, int G>
+template <class T, int D, int R, int G>
 __global__ __launch_bounds__(256 * G) void mx4_join_kernel(const Args a) {
   constexpr int NT = D / 16, kAhead = D == 256 ? 2 : 4;
   if (!*a.any_cut) return;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
   const int i = wave & 3, g = wave >> 2;
-  const int tile = a.heads_div.div(blockIdx.x);
-  const int kv_head = blockIdx.x - tile * a.heads;
-  const Work w = find_work(a, tile, kRows, true);
+  const int block = blockIdx.x / R, r = blockIdx.x % R;
+  const int tile = a.heads_div.div(block);
+  const int kv_head = block - tile * a.heads;
+  const Work w = find_work(a, tile, kRows * R, true);
   if (w.seq < 0 || w.cuts == 1) return;
   __shared__ float sum_o[G * 4][NT][64];
   __shared__ float sum_m[G][16], sum_l[G][16];
-  const int first = w.tile * kRows;
+  const int first = (w.tile * R + r) * kRows;
   const bool valid = first + (lane & 15) < w.s.count * a.group;
   float o[NT], m = kNothing, l = 0.f;
 #pragma unroll
   for (int j = 0; j < NT; ++j) o[j] = 0.f;
   if (valid) {
-    const int64_t part = part_of(a, w.first, kv_head);
+    const int64_t part = part_of(a, w.first, kv_head) * R + r;
     const float2* const ml = a.part_ml + part * kRows + (lane & 15);
     const float* const po = a.part_o + (part * 4 + i) * NT * 64 + lane;
-    const int64_t next = a.heads;
+    const int64_t next = static_cast<int64_t>(a.heads) * R;
     for (int c0 = g; c0 < w.cuts; c0 += G * kAhead) {
       float2 x[kAhead];
       float y[kAhead][NT];
@@ -1151,6 +1152,7 @@ struct LaunchPlan {
 };
 
 constexpr int kComputeUnits = 256;
+constexpr int kLongSteps = 256;    // of a table row, from which tiles of many rows are cut
 
 LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   LaunchPlan p;
@@ -1161,25 +1163,29 @@ LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
                            : static_cast<int64_t>(c.batch) * ((c.group_size + n - 1) / n)) *
            c.num_heads;
   };
-  // Many rows a tile share V's conversion, but have fewer workgroups, which are not
-  // cut along the keys: they have to fill the compute units.
-  const int many = most_row_tiles(c.head_size);
-  p.row_tiles = rows > static_cast<int64_t>(c.batch) * kRows * (many - 1) &&
-                        tiles(many) >= kComputeUnits ? many : 1;
-  p.tiles = tiles(p.row_tiles);
   const int64_t most_steps =
       (static_cast<int64_t>(c.table_width) * c.tokens_per_block + kStep - 1) / kStep;
-  // Tiles for every compute unit: smaller workgroups, three a compute unit, take
+  // Many rows a tile share V's conversion, but have fewer workgroups.  Where these do
+  // not fill the compute units they are cut along the keys, which pays for long
+  // ones: 8 sequences of 40 rows 33 us for 42 at 8192 keys, 1024 rows 196 for 234 at
+  // 32768, but 16 sequences of 40 rows 27 for 25 at 2000.
+  const int many = most_row_tiles(c.head_size);
+  const bool fill = tiles(many) >= kComputeUnits;
+  p.row_tiles = rows > static_cast<int64_t>(c.batch) * kRows * (many - 1) &&
+                        (fill || most_steps >= kLongSteps) ? many : 1;
+  p.tiles = tiles(p.row_tiles);
+  p.wide = p.row_tiles == 1 && p.tiles <= kComputeUnits;
+  // Tiles of 16 rows for every compute unit: smaller workgroups, three a compute unit, take
   // turns better (40 sequences of 8192 keys: 78 us; wide ones 91), and only sequences
   // longer than the mean are cut: 64 of 2048 keys 31 us, uncut 26, but one of 16384 among
   // 39 of 500 keys 27 us, uncut 82.  With many more tiles the plan costs more.
-  p.wide = p.tiles <= kComputeUnits;
-  p.slots = p.row_tiles > 1 || most_steps <= kMinSteps || p.tiles > 4 * kComputeUnits ? 0
+  p.slots = most_steps <= kMinSteps || p.tiles > 4 * kComputeUnits ? 0
+            : p.row_tiles > 1 ? (fill ? 0 : 2 * kComputeUnits)
             : p.wide ? kComputeUnits : static_cast<int>(p.tiles);
   // items (cuts of a tile, of all heads), in whole rounds of the XCDs
   const int64_t items = (p.tiles + p.slots + c.num_heads - 1) / c.num_heads;
   p.workgroups = (items + kXcds - 1) / kXcds * kXcds * c.num_heads;
-  const int64_t part_rows = p.slots ? p.workgroups * kRows : 0;
+  const int64_t part_rows = p.slots ? p.workgroups * kRows * p.row_tiles : 0;
   p.ml_bytes = part_rows * sizeof(float2) + (p.slots ? 16 : 0);    // and any_cut
   p.o_bytes = part_rows * c.head_size * sizeof(float);
   return p;
@@ -1192,13 +1198,18 @@ void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
 template <class T, int D>
 void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
   if (p.row_tiles > 1) {
-    launch<T, D, most_row_tiles(D), 4>(a, p, s);
+    constexpr int R = most_row_tiles(D);
+    launch<T, D, R, 4>(a, p, s);
+    if (p.slots)
+      hipLaunchKernelGGL((mx4_join_kernel<T, D, R, 1>), dim3(p.tiles * R), dim3(256), 0, s, a);
   } else if (p.wide) {
     launch<T, D, 1, most_waves(D)>(a, p, s);
-    if (p.slots) hipLaunchKernelGGL((mx4_join_kernel<T, D, 4>), dim3(p.tiles), dim3(1024), 0, s, a);
+    if (p.slots)
+      hipLaunchKernelGGL((mx4_join_kernel<T, D, 1, 4>), dim3(p.tiles), dim3(1024), 0, s, a);
   } else {
     launch<T, D, 1, 4>(a, p, s);
-    if (p.slots) hipLaunchKernelGGL((mx4_join_kernel<T, D, 1>), dim3(p.tiles), dim3(256), 0, s, a);
+    if (p.slots)
+      hipLaunchKernelGGL((mx4_join_kernel<T, D, 1, 1>), dim3(p.tiles), dim3(256), 0, s, a);
   }
 }
 template <class T>

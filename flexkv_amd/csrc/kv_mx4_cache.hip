@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTokensPerUnit = 4;     // tokens whose group one quad of lanes handles
-constexpr int kInlinePairs = 64;      // id pairs in the kernel arguments
+constexpr int kInlinePairs = 256;     // id pairs in the kernel arguments
 constexpr int64_t kUnitsPerLaunch = int64_t(1) << 28;
 
 struct Bf16 {};
@@ -171,7 +171,7 @@ struct BlockArgs {
   int heads, tokens, dim;
   FastDiv per_chunk, per_head, groups, layers;
   uint64_t layer_ptrs[kMaxLayersPerLaunch];
-  int64_t inline_pairs[2 * kInlinePairs];
+  int32_t inline_pairs[2 * kInlinePairs];
 };
 
 // The addresses of unit `u`'s group: `wide` its elements of the first of four
@@ -188,8 +188,12 @@ __device__ inline Unit locate(const BlockArgs& a, uint32_t u) {
   const uint32_t t = a.groups.div(r2), g = r2 - t * a.groups.d;
   const uint32_t k = a.halves_log2 ? c & 1 : 0, bl = c >> a.halves_log2;
   const uint32_t i = a.layers.div(bl), l = bl - i * a.layers.d;
-  const int64_t* pairs = a.pairs ? a.pairs : a.inline_pairs;
-  const int64_t gid = pairs[2 * i], mid = pairs[2 * i + 1];
+  int64_t gid, mid;
+  if (a.pairs) {
+    gid = a.pairs[2 * i], mid = a.pairs[2 * i + 1];
+  } else {
+    gid = a.inline_pairs[2 * i], mid = a.inline_pairs[2 * i + 1];
+  }
   char* const chunk = a.mx + l * a.mls + k * a.mks + mid * a.mbs;
   const uint32_t tok = kTokensPerUnit * t;
   Unit at;
@@ -296,6 +300,7 @@ struct BlockCall {
   char* mx;
   PtrInfo mx_info;
   int tokens, heads, dim, dtype;
+  bool wide_ids;       // some id needs 64 bits
 
   int64_t wide_chunk() const {
     return static_cast<int64_t>(tokens) * heads * dim * dtype_bytes(dtype);
@@ -327,6 +332,7 @@ int check_blocks(BlockCall& c) {
     gmin = std::min(gmin, a), gmax = std::max(gmax, a);
     mmin = std::min(mmin, b), mmax = std::max(mmax, b);
   }
+  c.wide_ids = std::max(gmax, mmax) > INT32_MAX;
   if (query_ptr(c.mx, &c.mx_info) != 0)
     return fail(kInval, "mx_ptr %p is not pinned host or device memory known to HIP", c.mx);
   const __int128 lo = static_cast<__int128>(c.start_layer) * c.mls +
@@ -386,7 +392,7 @@ int run_blocks(const BlockCall& c, hipStream_t s, int dev, bool to_mx) {
   a.per_chunk = FastDiv(a.per_head.d * c.heads);
   (void)hipGetLastError();  // a stale error from elsewhere must not be blamed on these launches
   const int64_t* pairs = nullptr;
-  if (c.num_blocks > kInlinePairs) {
+  if (c.num_blocks > kInlinePairs || c.wide_ids) {
     const size_t bytes = static_cast<size_t>(c.num_blocks) * 16;
     if ((rc = ids_acquire(bytes, &host.buf))) return rc;
     for (int i = 0; i < c.num_blocks; ++i) {
@@ -424,8 +430,8 @@ int run_blocks(const BlockCall& c, hipStream_t s, int dev, bool to_mx) {
         a.pairs = pairs ? pairs + 2 * b : nullptr;
         if (!pairs)
           for (int i = 0; i < nb; ++i) {
-            a.inline_pairs[2 * i] = c.gids[b + i];
-            a.inline_pairs[2 * i + 1] = c.mids[b + i];
+            a.inline_pairs[2 * i] = static_cast<int32_t>(c.gids[b + i]);
+            a.inline_pairs[2 * i + 1] = static_cast<int32_t>(c.mids[b + i]);
           }
         if ((rc = prof.begin(s, &ev))) return rc;
         if (c.dtype == FKV_DTYPE_BF16) launch_blocks<Bf16>(a, to_mx, s);
@@ -454,7 +460,7 @@ int blocks_entry(int num_blocks, int start_layer_id, int num_layers, const int64
     if (num_blocks == 0 || num_layers == 0) return 0;
     BlockCall c{num_blocks, start_layer_id, num_layers, is_mla ? 1 : 2, gpu_block_ids,
                 mx_block_ids, gpu_layer_ptrs, gks, gbs, mks, mls, mbs,
-                static_cast<char*>(mx_ptr), PtrInfo(), tokens, heads, dim, dtype};
+                static_cast<char*>(mx_ptr), PtrInfo(), tokens, heads, dim, dtype, false};
     int rc = check_blocks(c);
     if (rc) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);

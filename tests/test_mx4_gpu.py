@@ -137,7 +137,7 @@ def test_blocks_quantise_and_come_back_bit_for_bit(kw):
 
 
 def test_many_blocks_take_the_table_on_the_device():
-    n = 200                                  # more than the kernel arguments carry
+    n = 300                                  # more than the kernel arguments carry
     c = Blocks(L=2, T=16, H=1, D=32, dtype=BF16, n_gpu=n + 9, n_mx=n + 4)
     g = _gen(5)
     gids, mids = torch.randperm(n + 9, generator=g)[:n].tolist(), torch.randperm(
@@ -148,6 +148,13 @@ def test_many_blocks_take_the_table_on_the_device():
     c.call(c_ext.dequantize_kv_blocks, gids[::-1], mids)
     for got, w in zip(c.wide, c.want_wide(gids[::-1], mids, want)):
         assert _same(got, w)
+
+
+def test_ids_past_32_bits_are_addressed():
+    c = Blocks(L=1, T=16, H=1, D=64, dtype=BF16)
+    c.gblk = 0                               # every id is the first block
+    c.call(c_ext.quantize_kv_blocks, [(1 << 40) + 3], [2])
+    assert torch.equal(c.mx.cpu(), c.want_mx([0], [2]))
 
 
 def test_every_bf16_and_fp16_pattern_is_rounded_as_the_oracle_does():
@@ -579,6 +586,24 @@ def test_strides_of_out_and_lse():
     assert got.data_ptr() == wide[:, 1].data_ptr()
     assert torch.equal(wide[:, 1].cpu(), want) and torch.equal(lt.t().cpu(), lse)
     assert (wide[:, 0] == 9).all() and (wide[:, 2] == 9).all()
+
+
+@pytest.mark.parametrize("D,dtype,T", [(64, FP16, 32), (128, BF16, 16), (256, BF16, 64)])
+def test_many_rows_over_long_tables_are_cut(D, dtype, T):
+    """Tiles of several row tiles, too few for the device, whose keys are cut: among
+    rows of one tile some see keys of few cuts."""
+    c = Case(keys=[3000, 90, 1400], queries=[40, 30, 17], H=2, G=4, D=D, T=T, dtype=dtype, seed=33,
+             width=8192 // T)
+    c.poison_unseen()
+    cut = c.T * c.H * D // 2
+    sc = c.mx[1, c.table[0, 2980 // T], cut:].view(c.H, D // 32, T)
+    sc[1, 1, 2980 % T] = 255                 # seen by the later queries alone
+    for causal in (True, False):
+        out, lse = c.run(causal=causal)
+        c.check(out, lse, causal=causal)
+        again, _ = c.run(causal=causal)
+        assert _same(out, again)
+    assert torch.isnan(out[0, 4:]).any() and not torch.isnan(c.run()[0][19, 4:]).any()
 
 
 def test_results_do_not_change_from_call_to_call():
