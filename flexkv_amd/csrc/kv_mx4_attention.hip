@@ -53,6 +53,10 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 constexpr int kRows = 16;          // rows of a tile: columns of a matrix instruction
 constexpr int kStep = 32;          // tokens of a step: two tiles of 16, k of the second product
 constexpr int kMinSteps = 32;      // of a workgroup, where the keys are cut
+// Steps that cutting has to take off the longest sequence: the plan and the join cost
+// 6 us, a wide workgroup's 12 steps 0.9.  16 sequences of 4096 keys, 8 heads: 26 us cut
+// in two, 23 uncut (21 without a plan); one of 4096: 16 cut in four, 19 uncut.
+constexpr int kCutSteps = 96;
 constexpr float kSlack = 256.f;    // weight up to which a score may pass the reference
 // The reference of a row that has seen nothing.  Any score passes it, and so does
 // not -infinity, which a score that a row does not see becomes.
@@ -222,8 +226,9 @@ __device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool 
     const float even = fmaxf(total * a.heads / a.slots * 1.01f, kMinSteps);
     // cuts of even size overflow the slots by the last, short ones: longer cuts until
     // they do not, or to twice the size
-    inv_per_cut = 0.5f / even;
-    for (int i = 0; few && i < 8; ++i) {
+    const bool pays = __any(longest >= even + kCutSteps);
+    inv_per_cut = pays ? 0.5f / even : 0.f;
+    for (int i = 0; few && pays && i < 8; ++i) {
       inv_per_cut = 1.f / (even * (1.f + i * 0.125f));
       const int n = lane_value(scan_lanes(tiles * cuts_of(steps_of(s), inv_per_cut)), 63);
       if (static_cast<int64_t>(n) * a.heads <= a.slots) break;
@@ -1179,7 +1184,7 @@ LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   // turns better (40 sequences of 8192 keys: 78 us; wide ones 91), and only sequences
   // longer than the mean are cut: 64 of 2048 keys 31 us, uncut 26, but one of 16384 among
   // 39 of 500 keys 27 us, uncut 82.  With many more tiles the plan costs more.
-  p.slots = most_steps <= kMinSteps || p.tiles > 4 * kComputeUnits ? 0
+  p.slots = most_steps < kMinSteps + kCutSteps || p.tiles > 4 * kComputeUnits ? 0
             : p.row_tiles > 1 ? (fill ? 0 : 2 * kComputeUnits)
             : p.wide ? kComputeUnits : static_cast<int>(p.tiles);
   // items (cuts of a tile, of all heads), in whole rounds of the XCDs

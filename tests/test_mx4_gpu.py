@@ -390,6 +390,8 @@ DECODE = [
     dict(keys=[200, 513], H=1, G=20, D=128, blockwise=True),
     dict(keys=[90, 33], H=8, G=1, D=128, dtype=FP16, T=64),
     dict(keys=[3000, 2050, 1], H=2, G=5, D=128, width=400),
+    dict(keys=[5000, 7777, 1, 0], H=2, G=5, D=128, width=600),
+    dict(keys=[9000, 40], H=1, G=33, D=256, T=32, dtype=FP16),
 ]
 
 
@@ -489,7 +491,7 @@ def test_cuts_of_ragged_lengths_and_of_many_sequences(batch, H, D, dtype):
     tiles that plan the cuts differently."""
     g = _gen(batch)
     keys = torch.randint(0, 40, (batch,), generator=g).tolist()
-    keys[1], keys[2], keys[-1] = 4100 // H, 1500, 2600
+    keys[1], keys[2], keys[-1] = 4900, 1500, 6100
     c = Case(keys=keys, queries=[1] * batch, H=H, G=3, D=D, T=32, dtype=dtype, seed=batch)
     c.poison_unseen()
     c.check(*c.run(single=True))
@@ -592,12 +594,12 @@ def test_strides_of_out_and_lse():
 def test_many_rows_over_long_tables_are_cut(D, dtype, T):
     """Tiles of several row tiles, too few for the device, whose keys are cut: among
     rows of one tile some see keys of few cuts."""
-    c = Case(keys=[3000, 90, 1400], queries=[40, 30, 17], H=2, G=4, D=D, T=T, dtype=dtype, seed=33,
+    c = Case(keys=[7000, 90, 5100], queries=[40, 30, 17], H=2, G=4, D=D, T=T, dtype=dtype, seed=33,
              width=8192 // T)
     c.poison_unseen()
     cut = c.T * c.H * D // 2
-    sc = c.mx[1, c.table[0, 2980 // T], cut:].view(c.H, D // 32, T)
-    sc[1, 1, 2980 % T] = 255                 # seen by the later queries alone
+    sc = c.mx[1, c.table[0, 6980 // T], cut:].view(c.H, D // 32, T)
+    sc[1, 1, 6980 % T] = 255                 # seen by the later queries alone
     for causal in (True, False):
         out, lse = c.run(causal=causal)
         c.check(out, lse, causal=causal)
@@ -607,7 +609,7 @@ def test_many_rows_over_long_tables_are_cut(D, dtype, T):
 
 
 def test_results_do_not_change_from_call_to_call():
-    c = Case(keys=[3000, 1777, 64], queries=[1, 5, 64], H=2, G=4, seed=8)
+    c = Case(keys=[6000, 4777, 64], queries=[1, 5, 64], H=2, G=4, seed=8)
     first = c.run()
     for _ in range(3):
         again = c.run()
@@ -719,7 +721,7 @@ def test_prompt_then_steps_then_blocks_leave_and_return():
 
 
 def test_a_captured_step_replays_with_other_lengths_and_tokens():
-    c = Case(keys=[900, 33, 250], queries=[1, 2, 1], H=2, G=4, seed=12, width=64)
+    c = Case(keys=[6000, 33, 250], queries=[1, 2, 1], H=2, G=4, seed=12, width=512)
     c.to_device()
     kv = c.qkv.to(DEV)
     H, G, T = c.H, c.G, c.T
@@ -733,7 +735,7 @@ def test_a_captured_step_replays_with_other_lengths_and_tokens():
     other = torch.cuda.CUDAGraph()            # a second graph over the same tensors
     with torch.cuda.graph(other):
         out2 = _step(c, key, value, slots)
-    for i, keys in enumerate(([900, 33, 250], [1, 2, 300], [640, 512, 31], [0, 1024, 1])):
+    for i, keys in enumerate(([6000, 33, 250], [1, 2, 300], [8192, 512, 31], [0, 5024, 1])):
         c.dlens.copy_(torch.tensor(keys, dtype=torch.int32))
         c.dq.normal_()
         key.normal_()
@@ -784,7 +786,7 @@ def test_calls_over_ctypes_give_the_same(monkeypatch):
 
 
 def test_two_streams_at_once():
-    cases = [Case(keys=[2500, 40 + i], queries=[1, 3], H=2, G=4, seed=40 + i) for i in range(2)]
+    cases = [Case(keys=[6500, 40 + i], queries=[1, 3], H=2, G=4, seed=40 + i) for i in range(2)]
     for c in cases:
         c.to_device()
     want = [c_ext.mx4_attention(c.dq, c.dmx, c.H, c.dtable, c.dlens, c.dstarts) for c in cases]
