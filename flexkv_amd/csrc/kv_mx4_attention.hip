@@ -290,12 +290,14 @@ __device__ inline Work find_single(const Args& a, int item, int rows_a_tile) {
 }
 
 // The queries of 16 rows as e4m3 parts: operand registers for each part and
-// 128-element step, and the scale bytes, part p's in byte p.
+// 128-element step, and the scale bytes, operand p's in byte p.  D = 64: an operand's
+// two halves hold two parts, which K's 64 elements meet twice over.
 template <int D, int PARTS>
 struct Query {
   static constexpr int kSteps = (D + 127) / 128;
-  static constexpr int kVectors = PARTS * kSteps * 2;   // of 16 bytes a lane
-  v8i part[PARTS][kSteps];
+  static constexpr int kOperands = D == 64 ? (PARTS + 1) / 2 : PARTS;
+  static constexpr int kVectors = kOperands * kSteps * 2;   // of 16 bytes a lane
+  v8i part[kOperands][kSteps];
   int scale;
 };
 
@@ -349,25 +351,29 @@ __device__ inline void load_query(const char* row, bool valid, int quad, bool ne
   const float up = lost ? 0.f : bits_f32(static_cast<uint32_t>(254 - e) << 23);
   q.scale = 0;
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) q.scale |= (lost ? 255 : e - 4 * p) << (8 * p);
+  for (int p = 0; p < Query<D, PARTS>::kOperands; ++p) {
+    // of the k that this lane's quad gives the scale for
+    const int part = D == 64 ? min(2 * p + quad / 2, PARTS - 1) : p;
+    q.scale |= (lost ? 255 : e - 4 * part) << (8 * p);
+  }
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float v = 0.f;
-          if (h < kHalves) v = lost ? 0.f : x[s][h < kHalves ? h : 0][4 * w + i] * up;
+          const float v = lost ? 0.f : x[s][h][4 * w + i] * up;
           r[i] = negate ? -v : v;
         }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
           int c = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
           c = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], c, true);
-          q.part[p][s][4 * h + w] = c;
+          if constexpr (D == 64) q.part[p / 2][s][4 * (p & 1) + w] = c;
+          else q.part[p][s][4 * h + w] = c;
           const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false);
           const v2f hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
           r[0] = (r[0] - lo[0]) * 16.f;
@@ -375,6 +381,7 @@ __device__ inline void load_query(const char* row, bool valid, int quad, bool ne
           r[2] = (r[2] - hi[0]) * 16.f;
           r[3] = (r[3] - hi[1]) * 16.f;
         }
+        if (D == 64 && PARTS % 2) q.part[PARTS / 2][s][4 + w] = 0;
       }
     }
   }
@@ -403,7 +410,7 @@ template <int D>
 __device__ inline Lanes<D> lane_offsets(int lane, int tokens) {
   const int c = lane & 15, quad = lane >> 4;
   Lanes<D> o;
-  // D = 64: quads 2 and 3 repeat what 0 and 1 load; their queries are zero
+  // D = 64: quads 2 and 3 repeat what 0 and 1 load, for the queries' second parts
   const int block = D >= 128 ? quad : quad & 1;
   o.k_code = c * (D / 2) + 16 * block;
   o.k_scale = block * tokens + c;
@@ -441,7 +448,7 @@ __device__ inline uint64_t block_of(const Tiles& t, int lane) {
 // Tile h of a step, which `tile` of the tiles has.
 template <int D>
 __device__ inline void load_keys(const Args& a, const Lanes<D>& o, const Tiles& tiles, int tile,
-                                 int quad, int h, Keys<D>& t) {
+                                 int h, Keys<D>& t) {
   const Chunk k = chunk_at(block_of(tiles, tile), a.chunk);
   const int codes = lane_value(tiles.codes, tile), scales = lane_value(tiles.scales, tile);
 #pragma unroll
@@ -449,7 +456,6 @@ __device__ inline void load_keys(const Args& a, const Lanes<D>& o, const Tiles& 
     t.code[h][s] = __builtin_amdgcn_raw_buffer_load_b128(k, o.k_code + 64 * s, codes, kOnce);
     t.scale[h][s] =
         __builtin_amdgcn_raw_buffer_load_b8(k, o.k_scale, scales + 4 * s * a.tokens, 0);
-    if (D == 64 && quad >= 2) t.scale[h][s] = 127;
   }
 }
 template <int D>
@@ -537,7 +543,7 @@ __device__ inline void scores(GetQuery query, const Keys<D>& t, v4f (&s)[R][2]) 
         const v8i kc = {static_cast<int>(c[0]), static_cast<int>(c[1]), static_cast<int>(c[2]),
                         static_cast<int>(c[3]), 0, 0, 0, 0};
 #pragma unroll
-        for (int p = PARTS - 1; p >= 0; --p)
+        for (int p = Query<D, PARTS>::kOperands - 1; p >= 0; --p)
           s[r][h] = multiply_keys(kc, q.part[p][k], s[r][h], t.scale[h][k], q.scale, p);
       }
     }
@@ -892,7 +898,7 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
     s = min(s, end - 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      load_keys<D>(a, o, walk.tiles, walk.place(s) + h, quad, h, k[n]);
+      load_keys<D>(a, o, walk.tiles, walk.place(s) + h, h, k[n]);
       load_values<D>(a, o, walk.tiles, walk.place(s) + h, h, v[n]);
     }
   };
