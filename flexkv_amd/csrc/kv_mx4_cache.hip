@@ -42,6 +42,7 @@ constexpr int kBytes = 2;
 template <>
 constexpr int kBytes<Fp32> = 4;
 
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
@@ -64,10 +65,27 @@ __device__ inline Raw<T> load_raw(const char* p) {
   if constexpr (kBytes<T> == 4) r.w = *reinterpret_cast<const uint4*>(p + 16);
   return r;
 }
+// Blocks pass through once, so they are not to displace what the caches hold: MI355X,
+// 1024 blocks of 2 MB each way 1024 us for 1072 with plain accesses, 173 blocks of 0.7 MB
+// read back 24 for 29.  (New tokens, just computed, are read from the caches: 8191 of
+// them 12.5 us, 16 by this.)
+__device__ inline uint4 load_once(const char* p) {
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p)));
+}
+__device__ inline void store_once(char* p, const uint4& v) {
+  __builtin_nontemporal_store(__builtin_bit_cast(v4u, v), reinterpret_cast<v4u*>(p));
+}
 template <class T>
-__device__ inline void store_raw(char* p, const Raw<T>& r) {
-  *reinterpret_cast<uint4*>(p) = r.v;
-  if constexpr (kBytes<T> == 4) *reinterpret_cast<uint4*>(p + 16) = r.w;
+__device__ inline Raw<T> load_raw_once(const char* p) {
+  Raw<T> r;
+  r.v = load_once(p);
+  if constexpr (kBytes<T> == 4) r.w = load_once(p + 16);
+  return r;
+}
+template <class T>
+__device__ inline void store_raw_once(char* p, const Raw<T>& r) {
+  store_once(p, r.v);
+  if constexpr (kBytes<T> == 4) store_once(p + 16, r.w);
 }
 
 __device__ inline void widen(const Raw<Bf16>& r, float (&x)[8]) {
@@ -217,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void mx4_blocks_kernel(const BlockArgs a)
   if constexpr (to_mx) {
     Raw<T> raw[kTokensPerUnit];
 #pragma unroll
-    for (int j = 0; j < kTokensPerUnit; ++j) raw[j] = load_raw<T>(wide + j * token_bytes);
+    for (int j = 0; j < kTokensPerUnit; ++j) raw[j] = load_raw_once<T>(wide + j * token_bytes);
     uint32_t scales = 0;
 #pragma unroll
     for (int j = 0; j < kTokensPerUnit; ++j) {
@@ -225,7 +243,7 @@ __global__ __launch_bounds__(kThreads) void mx4_blocks_kernel(const BlockArgs a)
       widen(raw[j], x);
       uint32_t b;
       const uint32_t c = encode(x, &b);
-      *reinterpret_cast<uint32_t*>(codes + j * (a.dim / 2)) = c;
+      __builtin_nontemporal_store(c, reinterpret_cast<uint32_t*>(codes + j * (a.dim / 2)));
       scales |= b << (8 * j);
     }
     if (s == 0) *reinterpret_cast<uint32_t*>(at.scales) = scales;
@@ -237,7 +255,7 @@ __global__ __launch_bounds__(kThreads) void mx4_blocks_kernel(const BlockArgs a)
     const uint32_t scales = *reinterpret_cast<const uint32_t*>(at.scales);
 #pragma unroll
     for (int j = 0; j < kTokensPerUnit; ++j)
-      store_raw<T>(wide + j * token_bytes, decode<T>(c[j], (scales >> (8 * j)) & 255u));
+      store_raw_once<T>(wide + j * token_bytes, decode<T>(c[j], (scales >> (8 * j)) & 255u));
   }
 }
 
