@@ -13,9 +13,13 @@
 // Both directions move bytes: 2 (4 for fp32) and 17/32 bytes an element, no
 // reuse, a handful of operations each (gfx950 rounds two elements to 4 bits in
 // one instruction), so memory bounds them.  Four neighbouring lanes hold a
-// group, 8 elements each, of four tokens in a row: 16-byte accesses on the wide
-// side, a dword of codes and a dword of the four tokens' scale bytes on the
-// narrow one, and two swaps within the quad for the group's maximum.
+// group, 8 elements each, of every fourth of 16 tokens: 16-byte accesses on the wide
+// side, a dword of codes on the narrow one, where neighbouring quads' tokens and so
+// their bytes are neighbours, a scale byte a lane, and two swaps within the quad for
+// the group's maximum.  With four tokens in a row to a quad the pieces were 64 bytes,
+// which the link to a pinned 4-bit cache minds: 128 blocks of Llama-3-8B's shape to
+// it 1320 us for 1800 (54 GB/s of the link's 57), and from it 1260 for 1440; a latent
+// of 576 elements 1160 for 1015 and 885 for 965.  On the device both measured alike.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -30,7 +34,7 @@ using namespace fkv_detail;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTokensPerUnit = 4;     // tokens whose group one quad of lanes handles
+constexpr int kTokensPerUnit = 4;     // tokens whose group one quad of lanes handles, as many apart
 constexpr int kInlinePairs = 256;     // id pairs in the kernel arguments
 constexpr int64_t kUnitsPerLaunch = int64_t(1) << 28;
 
@@ -192,8 +196,8 @@ struct BlockArgs {
   int32_t inline_pairs[2 * kInlinePairs];
 };
 
-// The addresses of unit `u`'s group: `wide` its elements of the first of four
-// tokens (token_bytes apart), `codes` (D / 2 apart) and `scales` (one byte apart).
+// The addresses of unit `u`'s group: `wide` its elements of the first of its four
+// tokens, `codes` and `scales` (a token's a byte apart).
 struct Unit {
   char* wide;
   char* codes;
@@ -213,7 +217,7 @@ __device__ inline Unit locate(const BlockArgs& a, uint32_t u) {
     gid = a.inline_pairs[2 * i], mid = a.inline_pairs[2 * i + 1];
   }
   char* const chunk = a.mx + l * a.mls + k * a.mks + mid * a.mbs;
-  const uint32_t tok = kTokensPerUnit * t;
+  const uint32_t tok = t / 4 * 16 + t % 4;
   Unit at;
   at.wide = reinterpret_cast<char*>(a.layer_ptrs[l]) + k * a.gks + gid * a.gbs +
             (static_cast<int64_t>(tok * a.heads + h) * a.dim + kMx4Group * g) * kBytes<T>;
@@ -229,33 +233,39 @@ __global__ __launch_bounds__(kThreads) void mx4_blocks_kernel(const BlockArgs a)
   const uint32_t u = thread / 4, s = thread % 4;
   if (u >= a.units) return;    // whole quads at a time
   const Unit at = locate<T>(a, u);
-  const int64_t token_bytes = static_cast<int64_t>(a.heads) * a.dim * kBytes<T>;
+  const int64_t wide_step = static_cast<int64_t>(a.heads) * a.dim * kBytes<T> * kTokensPerUnit;
+  const int64_t code_step = a.dim / 2 * kTokensPerUnit;
   char* const wide = at.wide + 8 * s * kBytes<T>;
   char* const codes = at.codes + 4 * s;
   if constexpr (to_mx) {
     Raw<T> raw[kTokensPerUnit];
 #pragma unroll
-    for (int j = 0; j < kTokensPerUnit; ++j) raw[j] = load_raw_once<T>(wide + j * token_bytes);
-    uint32_t scales = 0;
+    for (int j = 0; j < kTokensPerUnit; ++j) raw[j] = load_raw_once<T>(wide + j * wide_step);
+    uint32_t scale = 0;      // of token s of the four
 #pragma unroll
     for (int j = 0; j < kTokensPerUnit; ++j) {
       float x[8];
       widen(raw[j], x);
       uint32_t b;
       const uint32_t c = encode(x, &b);
-      __builtin_nontemporal_store(c, reinterpret_cast<uint32_t*>(codes + j * (a.dim / 2)));
-      scales |= b << (8 * j);
+      __builtin_nontemporal_store(c, reinterpret_cast<uint32_t*>(codes + j * code_step));
+      if (s == j) scale = b;
     }
-    if (s == 0) *reinterpret_cast<uint32_t*>(at.scales) = scales;
+    *reinterpret_cast<uint8_t*>(at.scales + kTokensPerUnit * s) = static_cast<uint8_t>(scale);
   } else {
     uint32_t c[kTokensPerUnit];
 #pragma unroll
     for (int j = 0; j < kTokensPerUnit; ++j)
-      c[j] = *reinterpret_cast<const uint32_t*>(codes + j * (a.dim / 2));
-    const uint32_t scales = *reinterpret_cast<const uint32_t*>(at.scales);
+      c[j] = *reinterpret_cast<const uint32_t*>(codes + j * code_step);
+    const int scale = *reinterpret_cast<const uint8_t*>(at.scales + kTokensPerUnit * s);
+    const int scales[kTokensPerUnit] = {
+        __builtin_amdgcn_mov_dpp(scale, 0x00, 0xf, 0xf, true),    // of the quad's lane 0 to 3
+        __builtin_amdgcn_mov_dpp(scale, 0x55, 0xf, 0xf, true),
+        __builtin_amdgcn_mov_dpp(scale, 0xAA, 0xf, 0xf, true),
+        __builtin_amdgcn_mov_dpp(scale, 0xFF, 0xf, 0xf, true)};
 #pragma unroll
     for (int j = 0; j < kTokensPerUnit; ++j)
-      store_raw_once<T>(wide + j * token_bytes, decode<T>(c[j], (scales >> (8 * j)) & 255u));
+      store_raw_once<T>(wide + j * wide_step, decode<T>(c[j], static_cast<uint32_t>(scales[j])));
   }
 }
 

@@ -118,6 +118,8 @@ BLOCK_SHAPES = [
     dict(L=2, T=48, H=5, D=96, dtype=FP16, start=2, mx_layers=5),
     dict(L=2, T=16, H=2, D=128, dtype=BF16, host=True),
     dict(L=130, T=16, H=1, D=32, dtype=BF16),
+    dict(L=2, T=64, H=1, D=576, dtype=BF16, mla=True, host=True),
+    dict(L=1, T=32, H=2, D=1024, dtype=FP32),
 ]
 
 
