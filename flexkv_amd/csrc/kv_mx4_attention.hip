@@ -11,7 +11,7 @@
 // lane's operand is 32 neighbouring elements of one token, which is one scale
 // group, 16 bytes and one scale byte.  The queries are the other operand, as sums
 // of two e4m3 parts (bf16: 4 + 4 significant bits, exact) or three (fp16), one
-// scale a row; parts of elements 2^13 below the row's largest lose bits under
+// scale a row (heads of 64 take two parts in one instruction); parts of elements 2^13 below the row's largest lose bits under
 // 2^-21 of it.  S comes out with 4 tokens of one row in a lane.  Those lanes are
 // the layout of the second product's operand if its 32 tokens are taken in the
 // order (quad * 4 + i of one tile, then of the next), so P never leaves its lane.
@@ -24,9 +24,9 @@
 //
 // A workgroup's wavefronts take the 32-token steps of its tile in turn, each loading
 // its next step while it computes one, and add up in LDS.  Where there are many rows,
-// a tile is three times 16, for which a step's V is converted once.  With few tiles the keys
-// are cut among workgroups as well (find_work), whose sums a second kernel joins
-// in a fixed order.
+// a tile is three times 16, for which a step's V is converted once.  With few tiles
+// the keys are cut among workgroups as well (find_work), whose sums a second
+// kernel joins in a fixed order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -610,6 +610,16 @@ def test_many_rows_over_long_tables_are_cut(D, dtype, T):
     assert torch.isnan(out[0, 4:]).any() and not torch.isnan(c.run()[0][19, 4:]).any()
 
 
+def test_many_rows_of_many_sequences_over_long_tables():
+    """More sequences than the plan ranks, their tiles of many rows cut."""
+    g = _gen(70)
+    keys = torch.randint(5, 60, (70,), generator=g).tolist()
+    keys[3], keys[69] = 6000, 4500
+    c = Case(keys=keys, queries=[9] * 70, H=1, G=4, D=64, T=32, seed=70, width=256)
+    c.poison_unseen()
+    c.check(*c.run())
+
+
 def test_results_do_not_change_from_call_to_call():
     c = Case(keys=[6000, 4777, 64], queries=[1, 5, 64], H=2, G=4, seed=8)
     first = c.run()
