@@ -11,10 +11,11 @@
 // lane's operand is 32 neighbouring elements of one token, which is one scale
 // group, 16 bytes and one scale byte.  The queries are the other operand, as sums
 // of two e4m3 parts (bf16: 4 + 4 significant bits, exact) or three (fp16), one
-// scale a row (heads of 64 take two parts in one instruction); parts of elements 2^13 below the row's largest lose bits under
-// 2^-21 of it.  S comes out with 4 tokens of one row in a lane.  Those lanes are
-// the layout of the second product's operand if its 32 tokens are taken in the
-// order (quad * 4 + i of one tile, then of the next), so P never leaves its lane.
+// scale a row (heads of 64 take two parts in one instruction); parts of elements 2^13
+// below the row's largest lose bits under 2^-21 of it.  S comes out with 4 tokens
+// of one row in a lane.  Those lanes are the layout of the second product's
+// operand if its 32 tokens are taken in the order (quad * 4 + i of one tile, then
+// of the next), so P never leaves its lane.
 // V's codes become bf16 in registers (exact: 2 significant bits), two tokens to a
 // register by byte permutes.
 //

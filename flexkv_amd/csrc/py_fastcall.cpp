@@ -1,8 +1,9 @@
 // _fkv_py: the per-call path of flexkv_amd.c_ext.transfer_kv_blocks,
 // transfer_kv_blocks_kv_ptrs and the functions on a 4-bit cache as a CPython
-// extension (vectorcall, no argument tuple).  It unpacks the torch tensors in C++, checks them, takes the current
-// torch stream and calls the C-ABI entry with the GIL released, the work that
-// csrc/bindings.cpp:25-55 does for the reference through pybind11.
+// extension (vectorcall, no argument tuple).  It unpacks the torch tensors in C++,
+// checks them, takes the current torch stream and calls the C-ABI entry with the GIL
+// released, the work that csrc/bindings.cpp:25-55 does for the reference through
+// pybind11.
 //
 // The C-ABI functions are not linked: c_ext hands over their addresses in the
 // library it already loaded (bind()), so both routes drive one copy of the
@@ -260,15 +261,10 @@ int tokens_of_layer(const at::Tensor& mx, int64_t halves, int64_t heads, int64_t
   return mx.size(2) % token || tokens % 16 || tokens > 4096 ? 0 : static_cast<int>(tokens);
 }
 
-// mx4_blocks(to_mx, gpu_block_ids, gpu_layer_ptrs, gpu_kv_stride, gpu_block_stride,
+// (to_mx, gpu_block_ids, gpu_layer_ptrs, gpu_kv_stride, gpu_block_stride,
 //            mx_block_ids, mx_tensor, mx_kv_stride, mx_layer_stride, mx_block_stride,
 //            tokens_per_block, num_heads, head_size, dtype code, start_layer, is_mla)
-PyObject* mx4_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!g_quantize_blocks) return not_bound();
-  if (n != 16) {
-    PyErr_Format(PyExc_TypeError, "mx4_blocks takes 16 arguments (%zd given)", n);
-    return nullptr;
-  }
+PyObject* mx4_blocks_of(PyObject* const* a) {
   const at::Tensor *gids, *ptrs, *mids;
   if (!int64_host(a[1], &gids) || !int64_host(a[2], &ptrs) || !int64_host(a[5], &mids) ||
       !THPVariable_Check(a[6]) || !PyLong_Check(a[13]))
@@ -303,6 +299,7 @@ PyObject* mx4_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return finish(rc);
 }
 
+// (key, value, mx_layer, slots)
 PyObject* mx4_tokens_of(PyObject* const* a) {
   const at::Tensor *key, *value = nullptr, *mx, *slots;
   if (!here(a[0], &key) || (a[1] != Py_None && !here(a[1], &value)) || !here(a[2], &mx) ||
@@ -333,8 +330,8 @@ PyObject* mx4_tokens_of(PyObject* const* a) {
   return finish(rc);
 }
 
-// mx4_attention(query, mx_layer, num_kv_heads, block_table, seq_lens, query_starts, scale,
-//               causal, out, lse)
+// (query, mx_layer, num_kv_heads, block_table, seq_lens, query_starts, scale, causal, out,
+//  lse)
 PyObject* mx4_attention_of(PyObject* const* a) {
   const at::Tensor *query, *mx, *table, *lens, *starts = nullptr, *given = nullptr, *lse = nullptr;
   if (!here(a[0], &query) || !here(a[1], &mx) || !PyLong_Check(a[2]) || !here(a[3], &table) ||
@@ -410,7 +407,7 @@ PyObject* mx4_attention_of(PyObject* const* a) {
   return THPVariable_Wrap(out);
 }
 
-// torch's errors (an allocation that fails) as Python's
+// torch's errors (an allocation that fails, a tensor without strides) as Python's
 template <PyObject* (*call)(PyObject* const*)>
 PyObject* checked(const char* name, PyObject* const* a, Py_ssize_t n, Py_ssize_t takes) {
   if (!g_attention) return not_bound();
@@ -430,6 +427,9 @@ PyObject* checked(const char* name, PyObject* const* a, Py_ssize_t n, Py_ssize_t
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
   return nullptr;
+}
+PyObject* mx4_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return checked<mx4_blocks_of>("mx4_blocks", a, n, 16);
 }
 PyObject* mx4_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return checked<mx4_tokens_of>("mx4_tokens", a, n, 4);

@@ -191,6 +191,10 @@ def test_blocks_are_refused_where_they_leave_their_allocations():
             c.call(c_ext.quantize_kv_blocks, gids, mids)
     c.call(c_ext.quantize_kv_blocks, [], [])
     assert torch.equal(c.mx.cpu(), c.before)
+    kept, c.mx = c.mx, torch.zeros(4, 4).to_sparse()         # torch's own errors come through
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        c.call(c_ext.quantize_kv_blocks, [0], [0])
+    assert torch.equal(kept.cpu(), c.before)
 
 
 def test_blocks_are_refused_under_capture():
@@ -288,6 +292,8 @@ def test_token_calls_refuse_what_they_cannot_take():
             call(*args)
     with pytest.raises(TypeError):
         call(x.to(torch.int16), x.to(torch.int16), mx, slots)
+    with pytest.raises(ValueError):
+        call(x.to_sparse(), x, mx, slots)
     with pytest.raises(RuntimeError, match="device tensor"):
         call(x, x, mx, slots.cpu())
     odd = torch.zeros(3 * 2 * 64 + 1, device=DEV, dtype=BF16)[1:].view(3, 2, 64)
