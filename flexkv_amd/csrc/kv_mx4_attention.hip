@@ -25,7 +25,7 @@
 //
 // A workgroup's wavefronts take the 32-token steps of its tile in turn, each loading
 // its next step while it computes one, and add up in LDS.  Where there are many rows,
-// a tile is three times 16, for which a step's V is converted once.  With few tiles
+// a tile is two or three times 16, for which a step's V is converted once.  With few tiles
 // the keys are cut among workgroups as well (find_work), whose sums a second
 // kernel joins in a fixed order.
 #include <hip/hip_runtime.h>
@@ -847,14 +847,16 @@ constexpr int most_waves(int dim) { return 4 * waves_a_simd(1, dim); }
 // sequences of 8192 keys, 8 heads: 286 MB in 60 us, 64 sequences 571 MB in 97; with the
 // arithmetic left out 62 for 66 then, with K and V in the L2 41.  W = 12 where few
 // sequences have to fill a compute unit each, which then need few cuts, else 4.
-// R = 3 (2 of 256 elements), many queries: arithmetic bounds it.  A step of 16 rows is 256
-// cycles of matrix instructions, 190 of vector ones (128 for exponentials), and a third
-// of the 288 that V's conversion takes; two wavefronts a SIMD overlap about half of
-// that.  2048 queries of 32 heads over 8192 keys: 255 us; 2 row tiles 266; 4 with spilled
-// registers 243, but more where workgroups are few; V converted once for four
-// wavefronts of 32 rows each, through LDS, 257, and half as slow again for short
-// prompts, whose workgroups are then few.  256 elements: 654 us with one wavefront a
-// SIMD, 1054 with two and spilled registers.
+// R = 3 (2 of 256 elements, and where 3 make too few workgroups), many queries:
+// arithmetic bounds it.  A step of 16 rows is 256 cycles of matrix instructions, 190 of
+// vector ones (128 for exponentials), and a third of the 288 that V's conversion takes;
+// counted over a prompt, matrix instructions are busy 43 % of the cycles, vector ones
+// 54 %, which two wavefronts a SIMD hardly overlap.  2048 queries of 32 heads over 8192
+// keys: 255 us (935 TFLOP/s); 2 row tiles 266; 4 with spilled registers 243, but more
+// where workgroups are few; V converted once for four wavefronts of 32 rows each,
+// through LDS, 257, and half as slow again for short prompts, whose workgroups are
+// then few.  256 elements: 654 us with one wavefront a SIMD, 1054 with two and
+// spilled registers.
 template <class T, int D, int R, int W>
 __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kernel(
     const Args a) {
@@ -1177,14 +1179,24 @@ LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   };
   const int64_t most_steps =
       (static_cast<int64_t>(c.table_width) * c.tokens_per_block + kStep - 1) / kStep;
-  // Many rows a tile share V's conversion, but have fewer workgroups.  Where these do
-  // not fill the compute units they are cut along the keys, which pays for long
-  // ones: 8 sequences of 40 rows 33 us for 42 at 8192 keys, 1024 rows 196 for 234 at
-  // 32768, but 16 sequences of 40 rows 27 for 25 at 2000.
+  // Many rows a tile share V's conversion, but have fewer workgroups, which have to fill
+  // the compute units.  Not the most there can be counts, but what to expect: of a
+  // sequence's last tile, half.  1 sequence of 400 queries of 32 heads over 8192 keys:
+  // 78 us with 2 row tiles in 400 workgroups, 98 with 3 in 272; 600 queries: 117 with 2 in
+  // 600, 98 with 3 in 400; 16 sequences of 16 queries over 4096: 34 with 2, 44 with 3.
+  // Fewer are cut along the keys, which pays for long ones: 300 queries over 8192 keys 66
+  // us for 78 with 2 row tiles uncut, 8 sequences of 40 rows 33 for 42 with 1, but 16
+  // of 40 rows over 2000 keys 27 for 25.
   const int many = most_row_tiles(c.head_size);
-  const bool fill = tiles(many) >= kComputeUnits;
-  p.row_tiles = rows > static_cast<int64_t>(c.batch) * kRows * (many - 1) &&
-                        (fill || most_steps >= kLongSteps) ? many : 1;
+  auto fills = [&](int row_tiles, int64_t workgroups) {
+    const int n = kRows * row_tiles;
+    return rows > static_cast<int64_t>(c.batch) * kRows * (row_tiles - 1) &&
+           (rows / n + c.batch / 2) * c.num_heads >= workgroups;
+  };
+  const bool three = many > 2 && fills(many, kComputeUnits + kComputeUnits / 4);
+  const bool cut = !three && most_steps >= kLongSteps && fills(many, 0) &&
+                   !fills(many, kComputeUnits);
+  p.row_tiles = three || cut ? many : fills(2, kComputeUnits) ? 2 : 1;
   p.tiles = tiles(p.row_tiles);
   p.wide = p.row_tiles == 1 && p.tiles <= kComputeUnits;
   // Tiles of 16 rows for every compute unit: smaller workgroups, three a compute unit, take
@@ -1192,7 +1204,7 @@ LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   // longer than the mean are cut: 64 of 2048 keys 31 us, uncut 26, but one of 16384 among
   // 39 of 500 keys 27 us, uncut 82.  With many more tiles the plan costs more.
   p.slots = most_steps < kMinSteps + kCutSteps || p.tiles > 4 * kComputeUnits ? 0
-            : p.row_tiles > 1 ? (fill ? 0 : 2 * kComputeUnits)
+            : p.row_tiles > 1 ? (cut ? 2 * kComputeUnits : 0)
             : p.wide ? kComputeUnits : static_cast<int>(p.tiles);
   // items (cuts of a tile, of all heads), in whole rounds of the XCDs
   const int64_t items = (p.tiles + p.slots + c.num_heads - 1) / c.num_heads;
@@ -1211,7 +1223,8 @@ template <class T, int D>
 void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
   if (p.row_tiles > 1) {
     constexpr int R = most_row_tiles(D);
-    launch<T, D, R, 4>(a, p, s);
+    if (p.row_tiles == R) launch<T, D, R, 4>(a, p, s);
+    else launch<T, D, 2, 4>(a, p, s);
     if (p.slots)
       hipLaunchKernelGGL((mx4_join_kernel<T, D, R, 1>), dim3(p.tiles * R), dim3(256), 0, s, a);
   } else if (p.wide) {

@@ -456,6 +456,10 @@ MANY_ROWS = [
     dict(keys=[97, 12, 65], queries=[97, 17, 40], H=32, G=4, D=128, dtype=FP16, blockwise=True),
     dict(keys=[150, 31], queries=[50, 31], H=48, G=2, D=256, T=48),
     dict(keys=[71, 64], queries=[71, 50], H=32, G=3, D=256, dtype=FP16, index=torch.int64),
+    # two row tiles where three would leave compute units empty
+    dict(keys=[60, 0, 133], queries=[40, 0, 20], H=32, G=4, D=128),
+    dict(keys=[90, 45], queries=[50, 14], H=48, G=3, D=64, dtype=FP16, T=48),
+    dict(keys=[300, 31, 9], queries=[31, 31, 12], H=32, G=4, D=128, dtype=FP16, blockwise=True),
 ]
 
 
