@@ -589,6 +589,20 @@ def test_bad_pages_and_lengths_make_their_rows_nan():
         assert (none[2:5] == 0).all() and torch.isinf(lse[2:5]).all()
 
 
+@pytest.mark.parametrize("keys,queries,H,width", [
+    ([100, 0, 31, 333], [1, 1, 1, 1], 2, 40), ([100, 0, 31, 6000], [1, 0, 9, 3], 2, 512),
+    ([100, 0, 31, 333], [60, 0, 31, 90], 32, 40)])
+def test_table_entries_without_keys_are_not_looked_at(keys, queries, H, width):
+    c = Case(keys=keys, queries=queries, H=H, seed=14, width=width)
+    single = queries == [1] * len(queries)
+    want, _ = c.run(single=single)
+    for fill in (-1, c.N, 2 ** 31 - 1):
+        for b, k in enumerate(keys):
+            c.table[b, -(-k // c.T):] = fill
+        got, _ = c.run(single=single)
+        assert torch.equal(got, want)
+
+
 def test_strides_of_out_and_lse():
     c = Case(keys=[77, 30], queries=[7, 9], G=2, seed=5)
     want, lse = c.run()
