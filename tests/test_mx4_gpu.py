@@ -400,6 +400,9 @@ DECODE = [
     dict(keys=[3000, 2050, 1], H=2, G=5, D=128, width=400),
     dict(keys=[5000, 7777, 1, 0], H=2, G=5, D=128, width=600),
     dict(keys=[9000, 40], H=1, G=33, D=256, T=32, dtype=FP16),
+    # groups of more rows than a row tile, over several row tiles
+    dict(keys=[33, 0, 70], H=64, G=40, D=64),
+    dict(keys=[20, 37], H=96, G=90, D=128),
 ]
 
 
