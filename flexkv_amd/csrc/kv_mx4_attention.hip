@@ -992,7 +992,8 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
     const float l = sum_over_quads(st[r].l);
     if (quad == 0) {
       sum_m[wave][r][lane] = st[r].m;
-      const bool lost = w.s.keys < 0 || (visible[r] - 1) / kMx4TokenTile >= bad;
+      const bool lost =
+          w.s.keys < 0 || (visible[r] > 0 && (visible[r] - 1) / kMx4TokenTile >= bad);
       sum_l[wave][r][lane] = lost ? bits_f32(0x7fc00000u) : l;
     }
   }

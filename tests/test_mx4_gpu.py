@@ -592,6 +592,27 @@ def test_bad_pages_and_lengths_make_their_rows_nan():
         assert (none[2:5] == 0).all() and torch.isinf(lse[2:5]).all()
 
 
+# one row tile, several, and cut keys: rows that see no key share a tile with rows that do
+KEYLESS = [dict(keys=[10], queries=[13]),
+           dict(keys=[40, 3], queries=[60, 40], H=32, G=4, D=64, dtype=FP16),
+           dict(keys=[7], queries=[30], H=64, G=4),
+           dict(keys=[20, 7000], queries=[25, 9], H=1, G=2, T=32, width=256)]
+
+
+@pytest.mark.parametrize("bad", [-1, "past"])
+@pytest.mark.parametrize("kw", KEYLESS, ids=lambda kw: "-".join(str(v) for v in kw.values()))
+def test_rows_without_keys_stay_zero_beside_a_bad_first_page(kw, bad):
+    c = Case(seed=41, **kw)
+    good, gl = c.run()
+    c.check(good, gl)
+    c.table[0, 0] = c.N if bad == "past" else bad
+    out, lse = c.run()
+    n, k = c.queries[0], c.keys[0]
+    assert (out[:n - k] == 0).all() and (lse[:n - k] == -math.inf).all()
+    assert torch.isnan(out[n - k:n]).all() and torch.isnan(lse[n - k:n]).all()
+    assert torch.equal(out[n:], good[n:]) and torch.equal(lse[n:], gl[n:])
+
+
 @pytest.mark.parametrize("keys,queries,H,width", [
     ([100, 0, 31, 333], [1, 1, 1, 1], 2, 40), ([100, 0, 31, 6000], [1, 0, 9, 3], 2, 512),
     ([100, 0, 31, 333], [60, 0, 31, 90], 32, 40)])
