@@ -62,6 +62,11 @@ constexpr float kSlack = 256.f;    // weight up to which a score may pass the re
 // The reference of a row that has seen nothing.  Any score passes it, and so does
 // not -infinity, which a score that a row does not see becomes.
 constexpr float kNothing = -3e38f;
+// From this reference on, the products of scores and scale are rounded before the reference
+// is taken off.  Below, a fused multiplication takes the exact product to it, which a
+// rounded product, the reference, differs from by at most 1; at 2^31 by 64 and more,
+// where weights overflow or vanish.
+constexpr float kCoarse = 0x1p24f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -571,15 +576,24 @@ struct Weights {
   float l[R];     // what State::l becomes
 };
 
+// s * scale rounded, then less m
+__device__ inline float rounded_less(float s, float scale, float m) {
+#pragma clang fp contract(off)
+  const float x = s * scale;
+  return x - m;
+}
+
 // Row tile r's scores as weights; returns their sum, which is over kSlack where one
 // of them passes the reference by more than that.
 template <int D, int R, bool SPLIT>
 __device__ inline float weigh(const v4f (&s)[R][2], const State<D>& st, int r, float scale_log2,
-                              Weights<R, SPLIT>& w) {
+                              Weights<R, SPLIT>& w, bool coarse = false) {
   float p[8], sum = 0.f;
 #pragma unroll
   for (int x = 0; x < 8; ++x) {
-    p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][x / 4][x % 4], scale_log2, -st.m));
+    const float score = s[r][x / 4][x % 4];
+    p[x] = __builtin_amdgcn_exp2f(coarse ? rounded_less(score, scale_log2, st.m)
+                                         : __builtin_fmaf(score, scale_log2, -st.m));
     sum = x ? sum + p[x] : p[x];
   }
   w.l[r] = st.l + sum;
@@ -597,10 +611,12 @@ __device__ inline float weigh(const v4f (&s)[R][2], const State<D>& st, int r, f
 }
 
 // Some score passes its row's reference: the references follow, and the weights
-// are made again.
+// are made again.  Returns the sum of weights past which the next step is to come here:
+// any, where a reference is kCoarse or more.
 template <int D, int R, bool SPLIT>
-__device__ inline void follow(const v4f (&s)[R][2], State<D> (&st)[R], float scale_log2,
-                              Weights<R, SPLIT>& w) {
+__device__ inline float follow(const v4f (&s)[R][2], State<D> (&st)[R], float scale_log2,
+                               Weights<R, SPLIT>& w) {
+  bool any_coarse = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float top = st[r].m;
@@ -612,8 +628,11 @@ __device__ inline void follow(const v4f (&s)[R][2], State<D> (&st)[R], float sca
     st[r].l *= fade;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) st[r].o[j] *= fade;
-    weigh(s, st[r], r, scale_log2, w);
+    const bool coarse = fabsf(m) >= kCoarse && m != kNothing;
+    any_coarse |= coarse;
+    weigh(s, st[r], r, scale_log2, w, coarse);
   }
+  return __any(any_coarse) ? -1.f : kSlack;
 }
 
 // Weights of 0 leave out what a row does not see only while V is finite, which it is in
@@ -723,16 +742,18 @@ __device__ inline Row row_of(const Args& a, const Seq& s, int r, int kv_head) {
 
 __device__ inline void write_lse(const Args& a, const Row& row, float m, float l) {
   a.lse[row.at * a.lse_row + row.head * a.lse_head] =
-      l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+      l == 0.f ? (row.visible ? bits_f32(0x7fc00000u) : -INFINITY)
+               : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // NJ elements from (D / 16) * (4 quad + i) + j0 of a row on as the output's type, and
-// its lse.
+// its lse.  No weight at all: zeros for a row that sees no key, NaN for one whose scores
+// are all below what 32 bits hold.
 template <class T, int D, int NJ>
 __device__ inline void write_row(const Args& a, const Row& row, int quad, int i, int j0,
                                  const float (&o)[NJ], float m, float l) {
   constexpr int NT = D / 16;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? (row.visible ? bits_f32(0x7fc00000u) : 0.f) : 1.f / l;
   uint32_t w[NJ / 2];
 #pragma unroll
   for (int j = 0; j < NJ; j += 2) w[j / 2] = narrow2<T>(o[j] * inv, o[j + 1] * inv);
@@ -944,6 +965,7 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
     return read_query(r);
   };
   const float scale_log2 = score_scale(a);
+  float slack = kSlack;
   State<D> st[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) clear(st[r]);
@@ -962,8 +984,8 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
         Weights<R, SPLIT_P> p;
         bool passes = false;
 #pragma unroll
-        for (int r = 0; r < R; ++r) passes |= weigh(s, st[r], r, scale_log2, p) > kSlack;
-        if (__any(passes)) follow(s, st, scale_log2, p);
+        for (int r = 0; r < R; ++r) passes |= weigh(s, st[r], r, scale_log2, p) > slack;
+        if (__any(passes)) slack = follow(s, st, scale_log2, p);
         if (__any(not_finite(v[n]))) take_out(v[n], token, visible, keys, quad, st);
 #pragma unroll
         for (int r = 0; r < R; ++r) st[r].l = p.l[r];

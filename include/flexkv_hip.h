@@ -457,7 +457,8 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
  * A NaN in a key reaches the rows that see that token, in a value those elements of
  * these rows, and no other.  A value group with a scale byte of 253 or 254, which
  * quantising never writes, counts as NaN.  A query row that holds an infinity or
- * a NaN gives NaN.
+ * a NaN gives NaN, and so does one whose largest score, in units of log 2, leaves what
+ * 32 bits hold.
  * Asynchronous on `stream`, and may be captured into a graph. */
 typedef struct fkv_mx4_attention_args {
   const void* query;                 /* [num_queries][num_heads * group_size][head_size] */

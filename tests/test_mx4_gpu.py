@@ -534,6 +534,77 @@ def test_scales_flat_sharp_and_negative(dtype, scale, spread):
     c.check(*c.run(scale=scale), scale=scale)
 
 
+FORMS = [dict(keys=[1400], queries=[1], H=1, G=8, D=128),            # a wide workgroup
+         dict(keys=[600, 500], queries=[300, 400], H=16, G=4, D=64),   # several row tiles
+         dict(keys=[400], queries=[200], H=48, G=2, D=256),
+         dict(keys=[9000, 30], queries=[1, 1], H=1, G=4, D=128, width=600),   # cut keys
+         dict(keys=[7000], queries=[40], H=2, G=4, D=64, dtype=FP16, T=32, width=256)]
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("log2", [20, 27, 30, 32, 34, 60, 100])
+@pytest.mark.parametrize("kw", FORMS, ids=lambda kw: "-".join(str(v) for v in kw.values()))
+def test_scores_of_any_size_pick_the_largest(kw, log2, sign):
+    """Scores near 2^log2: of two equal keys the largest by half, the others without weight.
+    Equal scores have equal weights, so the result is the two values' mean, within the
+    rounding of the weights and its own."""
+    c = Case(seed=43, **kw)
+    g = _gen(44)
+    T, H, D = c.T, c.H, c.D
+    direction = torch.randn(D, generator=g).clamp(-4, 4)
+    direction[direction.abs() < 2.0 ** -6] = 2.0 ** -6
+    factor = 1 + torch.rand(c.rows, H * c.G, 1, generator=g)
+    q = (direction * factor).to(c.dtype)
+    c.qkv[:, :H * c.G] = q
+    side = (sign * direction < 0).to(torch.uint8) * 8       # codes that agree in sign
+    cut = T * H * D // 2
+    top = {}
+    for b, k in enumerate(c.keys):
+        # the smallest scores are -3 or less where they are negative, the largest -0.5
+        first = max(1, k - c.queries[b])                     # all rows see tokens before it
+        top[b] = sorted({0, first // 2, first - 1})[-2:]
+        for t in range(k):
+            mag = torch.randint(0, 6, (H, D), generator=g, dtype=torch.uint8)
+            if sign < 0:
+                mag = mag % 3 + 5
+            if t in top[b]:
+                mag[:] = 7 if sign > 0 else 1
+            codes = mag | side
+            page = c.mx[0, c.table[b, t // T]]
+            page[:cut].view(H, T, D // 2)[:, t % T] = codes[:, 0::2] | codes[:, 1::2] << 4
+            page[cut:].view(H, D // 32, T)[:, :, t % T] = 127
+    scale = 0.7 * 2.0 ** log2 / float(direction.abs().sum())
+    out, lse = c.run(scale=scale)
+    at = 0
+    for b, (k, n) in enumerate(zip(c.keys, c.queries)):
+        pages = c.table[b, :-(-k // T)].long()
+        v = np.stack([mo.chunk_values(c.mx[1, p].numpy(), T, H, D) for p in pages])
+        v = torch.from_numpy(v.reshape(-1, H, D))[top[b]]
+        want = v.mean(0).repeat_interleave(c.G, 0)
+        half = torch.finfo(c.dtype).eps / 2
+        p = 2.0 ** -8 if c.dtype == BF16 else 2.0 ** -16
+        tol = (p + 2.0 ** -18) * v.abs().mean(0).repeat_interleave(c.G, 0) * (1 + half) + \
+            half * want.abs() + torch.finfo(c.dtype).smallest_normal
+        assert ((out[at:at + n].double() - want).abs() <= tol).all(), b
+        s = (q[at:at + n].double() * direction.sign() * (6 if sign > 0 else -0.5)).sum(-1) * scale
+        assert ((lse[at:at + n].double() - s).abs() <= s.abs() * 2.0 ** -14 + 1).all()
+        at += n
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("kw", FORMS, ids=lambda kw: "-".join(str(v) for v in kw.values()))
+def test_scores_past_32_bits_make_their_rows_nan(kw, sign):
+    """q . k of 2^131 and more, all of one sign, for one query and head."""
+    c = Case(seed=45, **{**kw, "dtype": BF16})
+    want, lse = c.run()
+    cut = c.T * c.H * c.D // 2
+    c.mx[0, :, :cut] = 0x66                      # 4, with scales from 2^-3 on
+    c.qkv[0, 1] = sign * 2.0 ** 124              # 64 products and more of 2^125
+    out, got = c.run()
+    assert torch.isnan(out[0, 1]).all() and torch.isnan(got[0, 1])
+    assert torch.isnan(out).sum() == c.D and torch.isnan(got).sum() == 1
+
+
 def test_extreme_scales_and_queries_stay_in_range():
     """Keys and values near the ends of what the format holds, queries whose
     elements span 2^-30 .. 2^7."""
