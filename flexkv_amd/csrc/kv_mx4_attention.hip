@@ -849,8 +849,11 @@ __device__ inline void clear(State<D>& st) {
   for (int j = 0; j < D / 16; ++j) st.o[j] = {0.f, 0.f, 0.f, 0.f};
 }
 
-// The scale of the scores; not 0, so that -infinity stays that.
-__device__ inline float score_scale(const Args& a) { return fmaxf(fabsf(a.scale_log2), 1e-30f); }
+// The scale of the scores; not 0, so that -infinity stays that, but the smallest there is,
+// with which no finite score comes to more than 2^-21.
+__device__ inline float score_scale(const Args& a) {
+  return fmaxf(fabsf(a.scale_log2), 0x1p-149f);
+}
 
 // Row tiles of a workgroup for many queries, as registers allow.
 constexpr int most_row_tiles(int dim) { return dim <= 128 ? 3 : 2; }

@@ -605,6 +605,17 @@ def test_scores_past_32_bits_make_their_rows_nan(kw, sign):
     assert torch.isnan(out).sum() == c.D and torch.isnan(got).sum() == 1
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("scale", [0.0, 1e-33, -1e-33, 1e-40])
+def test_scales_of_zero_and_near_it_beside_large_products(scale, dtype):
+    c = Case(keys=[333, 60], queries=[2, 60], G=4, dtype=dtype, seed=3)
+    cut = c.T * c.H * c.D // 2
+    up = 50 if dtype == BF16 else 0
+    c.mx[0, :, cut:] += 106 - up                 # keys of 2^(103 - up) .. 2^(106 - up)
+    c.qkv = (c.qkv.float() * 2.0 ** up).to(dtype)
+    c.check(*c.run(scale=scale), scale=scale)
+
+
 def test_extreme_scales_and_queries_stay_in_range():
     """Keys and values near the ends of what the format holds, queries whose
     elements span 2^-30 .. 2^7."""
