@@ -715,13 +715,18 @@ __device__ inline void accumulate(v8bf v, int j, const Weights<R, SPLIT>& p, Sta
   }
 }
 
+// Quantising rounds up to 65536, which reads back as fp16's largest: finite sums past that
+// are that here too.
+__device__ inline float within_fp16(float x) {
+  return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+}
 template <class T>
 __device__ inline uint32_t narrow2(float a, float b) {
   if constexpr (__is_same(T, __bf16)) return pack_bf16(a, b);
   typedef _Float16 v2h __attribute__((ext_vector_type(2)));
   v2h r;
-  r[0] = static_cast<_Float16>(a);
-  r[1] = static_cast<_Float16>(b);
+  r[0] = static_cast<_Float16>(within_fp16(a));
+  r[1] = static_cast<_Float16>(within_fp16(b));
   return __builtin_bit_cast(uint32_t, r);
 }
 

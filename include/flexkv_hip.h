@@ -447,7 +447,8 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
  * head_size 64, 128 or 256; dtype (of query and out) FKV_DTYPE_BF16 or _FP16.  Sums,
  * maximum and normalisation are held in 32 bits.  The queries enter exactly, but for
  * elements 2^13 below their row's largest, which lose bits under 2^-21 of it; the
- * weights p with 8 significant bits for bf16, 16 for fp16.  Block ids, lengths and
+ * weights p with 8 significant bits for bf16, 16 for fp16.  Finite results past fp16's
+ * largest value are that one, as when reading back.  Block ids, lengths and
  * starts are device memory, all int32 or all int64 (index_is_64bit), read by the
  * kernels, and nothing outside the cache is read for any of them: a block id outside
  * the cache gives NaN in the rows that see a token of that block, a length past the

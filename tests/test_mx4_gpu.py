@@ -527,6 +527,28 @@ def test_value_scales_that_quantising_never_writes_count_as_nan(byte, lost):
         assert torch.equal(torch.isnan(out.view_as(hit)), hit)
 
 
+@pytest.mark.parametrize("keys,queries,H,width", [([1, 40], [1, 1], 2, 0),
+                                                   ([50, 33], [50, 20], 32, 0),
+                                                   ([7000, 9], [1, 1], 1, 500)])
+def test_values_past_fp16_come_out_as_its_largest(keys, queries, H, width):
+    """Values of 65504 are held as 65536: finite when read back, and here."""
+    c = Case(keys=keys, queries=queries, H=H, G=4, D=64, dtype=FP16, seed=47, width=width)
+    c.to_device()
+    n = c.N * c.T
+    x = torch.full((n, H, c.D), 65504.0, dtype=FP16)
+    x[:, :, 1::2] = -65504.0
+    x[:, :, 32:] = 3.0
+    c_ext.quantize_kv_tokens(c.qkv.to(DEV)[:1, :H].expand(n, H, c.D).contiguous(), x.to(DEV), c.dmx,
+                             torch.arange(n, device=DEV))
+    c.mx = c.dmx.cpu()
+    out, _ = c.run()
+    # weights that sum to one within their rounding, so 65504 but for it or from beyond
+    assert torch.isfinite(out).all()
+    assert ((out[..., 0:32:2] - 65504).abs() <= 64).all()
+    assert ((out[..., 1:32:2] + 65504).abs() <= 64).all()
+    assert ((out[..., 32:].float() - 3).abs() <= 2.0 ** -8).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("scale,spread", [(0.0, 1.0), (-0.3, 1.0), (1.0, 4.0), (1e-3, 300.0)])
 def test_scales_flat_sharp_and_negative(dtype, scale, spread):
