@@ -291,6 +291,9 @@ def dequantize_kv_blocks(gpu_block_id_tensor: torch.Tensor, gpu_layer_ptrs_tenso
 def _require_device(t, name: str, fn_name: str, device=None) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{fn_name} makes no gradients, but {name} requires them: call it under "
+                           f"torch.no_grad()")
     if not t.is_cuda:
         raise RuntimeError(f"{fn_name}: {name} must be a device tensor, got device {t.device}")
     if device is not None and t.device != device:
@@ -332,7 +335,8 @@ def quantize_kv_tokens(key: torch.Tensor, value, mx_layer: torch.Tensor,
     head_size], of any token and head stride (value None for one latent half);
     ``mx_layer``: uint8 [K|V, block, chunk bytes], a view of the cache's layer;
     ``slots``: int64 or int32, block * tokens_per_block + offset, one below 0 or
-    past the cache being padding.  Slots have to differ.  Asynchronous on the
+    past the cache being padding.  Slots have to differ.  Makes no gradients: inputs that
+    require them are refused but under ``torch.no_grad()``.  Asynchronous on the
     current torch stream; may be captured into a graph."""
     fn = "quantize_kv_tokens"
     if (_fast or _load_fast()).mx4_tokens(key, value, mx_layer, slots) is not False:
@@ -384,7 +388,8 @@ def mx4_attention(query: torch.Tensor, mx_layer: torch.Tensor, num_kv_heads: int
     up to its own position.  Rows that see none give zeros (lse -inf); rows of no
     sequence are left as they were (not written in a given ``out``, unset in a new
     one).  ``lse``: float32 [row, head], receives the log of the sum of exp.
-    Returns ``out``.  Asynchronous on the current torch stream; may be captured
+    Returns ``out``.  Makes no gradients: inputs that require them are refused but under
+    ``torch.no_grad()``.  Asynchronous on the current torch stream; may be captured
     into a graph."""
     fn = "mx4_attention"
     done = (_fast or _load_fast()).mx4_attention(query, mx_layer, num_kv_heads, block_table,

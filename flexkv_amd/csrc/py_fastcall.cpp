@@ -13,6 +13,7 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -243,11 +244,12 @@ int dtype_code(at::ScalarType t) {
          : t == at::kFloat  ? FKV_DTYPE_FP32 : -1;
 }
 
-// a tensor on the current device
+// a tensor on the current device that no gradient is asked for
 bool here(PyObject* o, const at::Tensor** out) {
   if (!THPVariable_Check(o)) return false;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.get_device() != c10::hip::current_device()) return false;
+  if (t.requires_grad() && c10::GradMode::is_enabled()) return false;
   *out = &t;
   return true;
 }

@@ -209,3 +209,15 @@ def test_python_entries_refuse_host_tensors_and_types():
         c_ext.mx4_attention(x, mx, 1, ids, ids)
     with pytest.raises(TypeError):
         c_ext.mx4_attention(None, mx, 1, ids, ids)
+
+
+def test_python_entries_refuse_inputs_that_require_gradients():
+    x = torch.zeros(2, 1, 128, dtype=torch.bfloat16, requires_grad=True)
+    plain, ids = torch.zeros(2, 1, 128, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    mx = torch.zeros(4096, dtype=torch.uint8)
+    for call in (lambda: c_ext.quantize_kv_tokens(x, plain, mx, ids),
+                 lambda: c_ext.mx4_attention(x, mx, 1, ids, ids)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="device tensor"):
+            call()

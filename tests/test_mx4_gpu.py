@@ -808,6 +808,30 @@ def test_results_do_not_change_from_call_to_call():
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("compiled", [True, False])
+def test_inputs_that_require_gradients_are_refused_but_under_no_grad(compiled, monkeypatch):
+    if not compiled:
+        monkeypatch.setattr(c_ext, "_fast", _lib._CtypesCalls(_lib.load()))
+    c = Case(keys=[40, 20], queries=[1, 1])
+    want, _ = c.run()
+    kv = c.qkv.to(DEV)
+    key = kv[:, -2 * c.H:-c.H]
+    slots = torch.full((2,), -1, device=DEV)
+    with_grad = [t.clone().requires_grad_() for t in (c.dq, key)]
+    out = torch.empty_like(c.dq).requires_grad_()
+    for call in (lambda: c_ext.mx4_attention(with_grad[0], c.dmx, c.H, c.dtable, c.dlens),
+                 lambda: c_ext.mx4_attention(c.dq, c.dmx, c.H, c.dtable, c.dlens, out=out),
+                 lambda: c_ext.quantize_kv_tokens(with_grad[1], key, c.dmx, slots),
+                 lambda: c_ext.quantize_kv_tokens(key, with_grad[1], c.dmx, slots)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.inference_mode():
+        got = c_ext.mx4_attention(with_grad[0], c.dmx, c.H, c.dtable, c.dlens)
+    assert torch.equal(got.cpu(), want) and not got.requires_grad
+
+
 def test_attention_refuses_what_it_cannot_take():
     c = Case(keys=[40, 20], queries=[1, 1])
     c.to_device()
