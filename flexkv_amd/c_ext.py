@@ -328,6 +328,39 @@ def _on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether two tensors of one type and shape [row, head, element], elements next to each
+    other, share a byte."""
+    rows, heads, dim = x.shape
+    if not x.numel():
+        return False
+    size = x.element_size()
+    n, apart = dim * size, y.data_ptr() - x.data_ptr()
+    # one row or head has no stride
+    (xr, xh), (yr, yh) = ([t.stride(0) * size if rows > 1 else 0,
+                           t.stride(1) * size if heads > 1 else 0] for t in (x, y))
+    if apart >= (rows - 1) * xr + (heads - 1) * xh + n or \
+            -apart >= (rows - 1) * yr + (heads - 1) * yh + n:
+        return False
+    if (xr, xh) == (yr, yh):
+        # rows d and heads e apart, for each e the two d that bring them nearest
+        for e in range(1 - heads, heads):
+            at = apart + e * xh
+            d = -at // xr if xr else 0
+            for d in (d, d + 1):
+                if abs(at + max(1 - rows, min(d, rows - 1)) * xr) < n:
+                    return True
+        return False
+
+    def starts(r, h):
+        return (torch.arange(rows)[:, None] * r + torch.arange(heads) * h).flatten()
+    a, b = starts(xr, xh).sort().values, starts(yr, yh) + apart
+    at = torch.searchsorted(a, b)
+    after = a[at.clamp(max=a.numel() - 1)] - b
+    before = b - a[(at - 1).clamp(min=0)]
+    return bool(((after.abs() < n) | (before.abs() < n)).any())
+
+
 def quantize_kv_tokens(key: torch.Tensor, value, mx_layer: torch.Tensor,
                        slots: torch.Tensor) -> None:
     """Quantise new tokens of one layer into their slots of a 4-bit cache
@@ -387,7 +420,7 @@ def mx4_attention(query: torch.Tensor, mx_layer: torch.Tensor, num_kv_heads: int
     ``scale`` defaults to head_size ** -0.5.  With ``causal`` a query sees the keys
     up to its own position.  Rows that see none give zeros (lse -inf); rows of no
     sequence are left as they were (not written in a given ``out``, unset in a new
-    one).  ``lse``: float32 [row, head], receives the log of the sum of exp.
+    one).  ``out`` may not overlap ``query``.  ``lse``: float32 [row, head], receives the log of the sum of exp.
     Returns ``out``.  Makes no gradients: inputs that require them are refused but under
     ``torch.no_grad()``.  Asynchronous on the current torch stream; may be captured
     into a graph."""
@@ -437,6 +470,8 @@ def mx4_attention(query: torch.Tensor, mx_layer: torch.Tensor, num_kv_heads: int
         if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
             raise ValueError(f"{fn}: out must be as query is, {tuple(query.shape)} {query.dtype}, "
                              f"got {tuple(out.shape)} {out.dtype} {out.stride()}")
+        if _overlap(query, out):
+            raise ValueError(f"{fn}: out may not overlap query")
     if lse is not None:
         _require_device(lse, "lse", fn, device)
         if lse.shape != (rows, heads) or lse.dtype != torch.float32:

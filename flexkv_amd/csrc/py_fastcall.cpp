@@ -332,6 +332,18 @@ PyObject* mx4_tokens_of(PyObject* const* a) {
   return finish(rc);
 }
 
+// whether the bytes from a tensor's first element to its last meet another's
+bool ranges_meet(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return static_cast<const char*>(x.data_ptr()) < end(y) &&
+         static_cast<const char*>(y.data_ptr()) < end(x);
+}
+
 // (query, mx_layer, num_kv_heads, block_table, seq_lens, query_starts, scale, causal, out,
 //  lse)
 PyObject* mx4_attention_of(PyObject* const* a) {
@@ -361,7 +373,7 @@ PyObject* mx4_attention_of(PyObject* const* a) {
              : rows < batch)
     Py_RETURN_FALSE;
   if (given && (given->sizes() != query->sizes() || given->scalar_type() != type ||
-                given->stride(2) != 1))
+                given->stride(2) != 1 || ranges_meet(*given, *query)))
     Py_RETURN_FALSE;
   if (lse && (lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != heads ||
               lse->scalar_type() != at::kFloat))

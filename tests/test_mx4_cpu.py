@@ -221,3 +221,26 @@ def test_python_entries_refuse_inputs_that_require_gradients():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="device tensor"):
             call()
+
+
+def test_overlap_of_two_views_is_that_of_their_bytes():
+    """Every pair of views of a small buffer, strides alike or not, against sets of bytes."""
+    g = np.random.default_rng(5)
+    buf = torch.zeros(400, dtype=torch.bfloat16)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        rows, heads, dim = (int(v) for v in g.integers(1, 5, 3))
+
+        def view(strides):
+            return buf.as_strided((rows, heads, dim), (*strides, 1), int(g.integers(0, 120)))
+        strides = [tuple(int(v) for v in g.integers(0, 30, 2)) for _ in range(2)]
+        x, y = view(strides[0]), view(strides[int(g.integers(0, 2))])
+
+        def touched(t):
+            return {t.storage_offset() + i * t.stride(0) + j * t.stride(1) + k
+                    for i in range(rows) for j in range(heads) for k in range(dim)}
+        want = bool(touched(x) & touched(y))
+        assert c_ext._overlap(x, y) is want, (x.shape, x.stride(), y.stride())
+        seen[want] += 1
+    assert min(seen.values()) > 500
+    assert not c_ext._overlap(buf[:0].view(0, 1, 4), buf[:0].view(0, 1, 4))

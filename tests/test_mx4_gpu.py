@@ -832,6 +832,29 @@ def test_inputs_that_require_gradients_are_refused_but_under_no_grad(compiled, m
     assert torch.equal(got.cpu(), want) and not got.requires_grad
 
 
+def test_out_that_overlaps_query_is_refused():
+    c = Case(keys=[40, 20, 9], queries=[3, 2, 1])
+    want, _ = c.run()
+    n, HG, D = c.rows, c.H * c.G, c.D
+    def call(q, out):
+        return c_ext.mx4_attention(q, c.dmx, c.H, c.dtable, c.dlens, c.dstarts, out=out)
+    both = torch.zeros(n + 2, 2 * HG, D, dtype=c.dtype, device=DEV)
+    q = both[:n, :HG]
+    q.copy_(c.dq)
+    kept = both.clone()
+    for out in (q, both[1:n + 1, :HG], both[:n, 1:HG + 1], both[2:, :HG],
+                both.view(-1)[D // 2:D // 2 + 2 * n * HG * D].view(n, 2 * HG, D)[:, :HG]):
+        with pytest.raises(ValueError, match="overlap"):
+            call(q, out)
+    assert torch.equal(both, kept)
+    # beside it, in the same rows, or before or behind it
+    assert torch.equal(call(q, both[:n, HG:]).cpu(), want)
+    assert torch.equal(both[:n, HG:].cpu(), want) and torch.equal(both[:, :HG], kept[:, :HG])
+    pairs = torch.zeros(n, HG, 2, D, dtype=c.dtype, device=DEV)
+    pairs[:, :, 1] = c.dq
+    assert torch.equal(call(pairs[:, :, 1], pairs[:, :, 0]).cpu(), want)
+
+
 def test_attention_refuses_what_it_cannot_take():
     c = Case(keys=[40, 20], queries=[1, 1])
     c.to_device()
