@@ -1300,6 +1300,14 @@ LaunchPlan launch_plan(const fkv_mx4_attention_args& c) {
   return p;
 }
 
+// A launch has less than 2^32 threads.  Wide workgroups and joins are of few tiles.
+int check_plan(const fkv_mx4_attention_args& c, const LaunchPlan& p) {
+  if (p.workgroups >= int64_t(1) << 24)
+    return fail(kInval, "%d queries of %d K/V heads are too many for one call", c.num_queries,
+                c.num_heads);
+  return 0;
+}
+
 template <class T, int D, int R, int W>
 void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
   hipLaunchKernelGGL((mx4_attention_kernel<T, D, R, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
@@ -1337,9 +1345,10 @@ int fkv_mx4_attention_workspace(const fkv_mx4_attention_args* args, size_t* byte
   last_error().clear();
   if (!args || !bytes) return fail(kInval, "null pointer argument");
   *bytes = 0;
-  const int rc = check_sizes(*args);
+  int rc = check_sizes(*args);
   if (rc || args->batch == 0 || args->num_queries == 0) return rc;
   const LaunchPlan p = launch_plan(*args);
+  if ((rc = check_plan(*args, p))) return rc;
   *bytes = p.ml_bytes + p.o_bytes;
   return 0;
 }
@@ -1352,6 +1361,7 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
     int rc = check_attention(c);
     if (rc || c.batch == 0 || c.num_queries == 0) return rc;
     const LaunchPlan p = launch_plan(c);
+    if ((rc = check_plan(c, p))) return rc;
     if (p.slots && (!c.workspace || c.workspace_bytes < p.ml_bytes + p.o_bytes ||
                      reinterpret_cast<uintptr_t>(c.workspace) % 16))
       return fail(kInval, "the workspace must hold %zu bytes on a multiple of 16, got %zu",
@@ -1380,9 +1390,6 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream) {
     a.tiles_per_block = FastDiv(c.tokens_per_block / kMx4TokenTile);
     a.group_div = FastDiv(c.group_size);
     a.heads_div = FastDiv(c.num_heads);
-    if (p.workgroups >= int64_t(1) << 31)
-      return fail(kInval, "%d queries of %d K/V heads are too many for one call", c.num_queries,
-                  c.num_heads);
     hipStream_t s = static_cast<hipStream_t>(stream);
     int dev = 0;
     DeviceGuard guard;

@@ -554,8 +554,14 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
     const int halves = value ? 2 : 1;
     int rc;
     if ((rc = mx4_check_shape(tokens_per_block, num_heads, head_size)) ||
-        (rc = mx4_check_dtype(dtype)) ||
-        (rc = mx4_check_layer(mx_ptr, mx_kv_stride_bytes, mx_block_stride_bytes, num_mx_blocks,
+        (rc = mx4_check_dtype(dtype)))
+      return rc;
+    // less than 2^32 threads, in whole workgroups
+    const int64_t groups = head_size / kMx4Group, per_token = groups * num_heads;
+    if (per_token * num_tokens * halves > (int64_t(1) << 30) - kThreads / 4)
+      return fail(kInval, "%d tokens of %d heads of %d are too many for one call", num_tokens,
+                  num_heads, head_size);
+    if ((rc = mx4_check_layer(mx_ptr, mx_kv_stride_bytes, mx_block_stride_bytes, num_mx_blocks,
                               halves, mx4_chunk_bytes(tokens_per_block, num_heads, head_size))))
       return rc;
     if (num_tokens == 0) return 0;
@@ -576,10 +582,6 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
     a.slots = slots, a.slots64 = slots_are_64bit;
     a.num_slots = num_mx_blocks * tokens_per_block;
     a.heads = num_heads, a.tokens = tokens_per_block, a.dim = head_size;
-    const int64_t groups = head_size / kMx4Group, per_token = groups * num_heads;
-    if (per_token * num_tokens * halves >= int64_t(1) << 30)
-      return fail(kInval, "%d tokens of %d heads of %d are too many for one call", num_tokens,
-                  num_heads, head_size);
     a.groups = FastDiv(groups);
     a.per_token = FastDiv(per_token);
     a.per_half = FastDiv(per_token * num_tokens);

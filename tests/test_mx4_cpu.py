@@ -244,3 +244,24 @@ def test_overlap_of_two_views_is_that_of_their_bytes():
         seen[want] += 1
     assert min(seen.values()) > 500
     assert not c_ext._overlap(buf[:0].view(0, 1, 4), buf[:0].view(0, 1, 4))
+
+
+def test_calls_of_more_threads_than_a_launch_has_are_refused():
+    """2^32 and more: 2^24 workgroups of 256."""
+    lib, need = _lib.load(), ctypes.c_size_t()
+
+    def attend(queries, heads, dim=128):
+        a = _lib.Mx4AttentionArgs(query_starts=4096, batch=1, num_queries=queries, table_width=64,
+                                  tokens_per_block=16, num_heads=heads, group_size=48,
+                                  head_size=dim, scale=1.0)
+        return lib.fkv_mx4_attention_workspace(a, need), _lib.last_error()
+    # a tile of 48 rows for each query and one more, in eights: 2^14 - 8 tiles, then 2^14
+    assert attend((1 << 14) - 9, 1024)[0] == 0
+    for queries, heads in (((1 << 14) - 8, 1024), (1 << 20, 1024), (1 << 22, 5)):
+        rc, msg = attend(queries, heads)
+        assert rc == 1 and "too many" in msg
+    for n in ((1 << 30) - 63, 1 << 30, (1 << 31) - 1):
+        rc, msg = _tokens(n=n, dim=32, value=None)
+        assert rc == 1 and "too many" in msg
+    rc, msg = _tokens(n=(1 << 30) - 64, dim=32, value=None)
+    assert rc == 1 and "not device memory" in msg
