@@ -6,7 +6,7 @@
 // past 6, the largest element, to 8); element i becomes the nearest of 0, 0.5, 1,
 // 1.5, 2, 3, 4, 6 to |x_i| / s with its sign, ties to the even code.  Dividing by
 // a power of two is exact, so a code is one rounding of the input and every
-// element is within s of it.  E is at most 127 (biased 254), where elements
+// element is within s of it.  E is at most 127 (biased 254), where elements over 7 s
 // saturate at 6 s, and s at least 2^-127.  A group that holds an infinity or a
 // NaN gets scale byte 255 and reads back as NaN.
 //
@@ -286,7 +286,7 @@ struct TokenArgs {
   int64_t num_slots;        // of the cache
   uint32_t units;
   int heads, tokens, dim, slots64;
-  FastDiv per_half, per_token, groups, block;
+  FastDiv per_half, per_token, groups;
 };
 
 // New tokens into their slots: a quad of lanes takes one group of one row.

@@ -385,7 +385,8 @@ int fkv_tp_group_destroy(fkv_tp_group_t group);
  * Quantising: with a the largest magnitude of a group, E = floor(log2 a), one more
  * where a's mantissa is over 1.75 and at most 127, the scale is 2^(E - 2), at least
  * 2^-127; every element is rounded once, to the nearest, ties to the even code, and
- * is within one scale of its value.  A group that holds an infinity or a NaN gets
+ * is within one scale of its value (but for values past 7 * 2^125, which become 6 * 2^125).
+ * A group that holds an infinity or a NaN gets
  * scale byte 255 and reads back as NaN.  Reading back is exact, but for values past
  * the destination type's largest finite one, which become that one. */
 
@@ -446,10 +447,14 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
  *
  * head_size 64, 128 or 256; dtype (of query and out) FKV_DTYPE_BF16 or _FP16.  Sums,
  * maximum and normalisation are held in 32 bits.  The queries enter exactly, but for
- * elements 2^13 below their row's largest, which lose bits under 2^-21 of it; the
- * weights p with 8 significant bits for bf16, 16 for fp16.  Finite results past fp16's
- * largest value are that one, as when reading back.  Block ids, lengths and
- * starts are device memory, all int32 or all int64 (index_is_64bit), read by the
+ * elements 2^13 below their row's largest, which lose bits under 2^-21 of it.  The matrix
+ * instruction of the scores adds the products of eight neighbouring elements with the bits
+ * under 2^-13 of the largest of them cut off: an error of a score of 2^-15 of the sum of
+ * |scale q k| at most, 2^-20 in the mean, where a row's elements are of even size, and of
+ * 2^-13 and 2^-16 where they lie up to 2^10 apart (as measured).  The
+ * weights p enter with 8 significant bits for bf16, 16 for fp16.  Finite results past fp16's
+ * largest value are that one, as when reading back.  table_width blocks hold at most 2^28
+ * tokens.  Block ids, lengths and starts are device memory, all int32 or all int64 (index_is_64bit), read by the
  * kernels, and nothing outside the cache is read for any of them: a block id outside
  * the cache gives NaN in the rows that see a token of that block, a length past the
  * table's row in all rows of its sequence, and a length below 0 is taken as 0.

@@ -666,6 +666,32 @@ def test_scales_of_zero_and_near_it_beside_large_products(scale, dtype):
     c.check(*c.run(scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("apart", [0, 6, 10, 13])
+def test_scores_of_rows_of_uneven_elements(D, dtype, apart):
+    """The score of a single key, its lse, within what the header says: of the products of
+    eight neighbours, the bits under 2^-13 of the largest are cut, for each part of the
+    query, a part being 2^-4 of the one before."""
+    B = 300
+    c = Case(keys=[1] * B, queries=[1] * B, H=2, G=4, D=D, dtype=dtype, seed=60 + apart)
+    g = _gen(61)
+    c.qkv = (c.qkv.float() * torch.exp2(-torch.randint(0, apart + 1, c.qkv.shape,
+                                                       generator=g).float())).to(dtype)
+    scale = D ** -0.5
+    _, lse = c.run(single=True, scale=scale)
+    page = c.table[:, 0].long()
+    k = torch.from_numpy(np.stack([mo.chunk_values(c.mx[0, p].numpy(), c.T, c.H, D)[0]
+                                   for p in page])).repeat_interleave(c.G, 1)
+    q = c.qkv[:, :c.H * c.G].double()
+    s, mags = (q * k).sum(-1) * scale, (q * k).abs().sum(-1) * scale
+    cut = (q * k).abs().unflatten(-1, (-1, 8)).amax(-1).sum(-1) * scale * 7 * 2.0 ** -13
+    parts = q.abs().amax(-1) * k.abs().sum(-1) * scale * 2.0 ** -21
+    # sums and the step from log2 to log in 32 bits, exp and log of one weight
+    rest = mags * 2.0 ** -20 + 2.0 ** -20
+    assert ((lse.double() - s).abs() <= cut * (1 + 2.0 ** -4 + 2.0 ** -8) + parts + rest).all()
+
+
 def test_extreme_scales_and_queries_stay_in_range():
     """Keys and values near the ends of what the format holds, queries whose
     elements span 2^-30 .. 2^7."""
