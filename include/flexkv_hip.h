@@ -454,8 +454,8 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
  * 2^-13 and 2^-16 where they lie up to 2^10 apart (as measured).  The
  * weights p enter with 8 significant bits for bf16, 16 for fp16.  Finite results past fp16's
  * largest value are that one, as when reading back.  table_width blocks hold at most 2^28
- * tokens.  Block ids, lengths and starts are device memory, all int32 or all int64 (index_is_64bit), read by the
- * kernels, and nothing outside the cache is read for any of them: a block id outside
+ * tokens.  Block ids, lengths and starts are device memory, all int32 or all int64
+ * (index_is_64bit), read by the kernels, and nothing outside the cache is read for any of them: a block id outside
  * the cache gives NaN in the rows that see a token of that block, a length past the
  * table's row in all rows of its sequence, and a length below 0 is taken as 0.
  * Starts have to ascend; rows of no sequence are left as they were.
