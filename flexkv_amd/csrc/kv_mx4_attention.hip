@@ -70,12 +70,6 @@ constexpr float kNothing = -3e38f;
 // rounded product, the reference, differs from by at most 1; at 2^31 by 64 and more,
 // where weights overflow or vanish.
 constexpr float kCoarse = 0x1p24f;
-// Values from 6 * 2^88 on are large: weights up to kSlack for each of up to 2^28 keys make
-// sums of smaller ones up to 2^126.  Rows that see a large one raise their reference by 2^40
-// where it has a weight over 2^-32, with which sums of values up to 6 * 2^125 stay below 2^124.
-constexpr uint32_t kLargeScale = 215, kNanScale = 253;
-constexpr float kRaise = 40.f, kLight = 0x1p-32f;
-constexpr int kNoToken = 0x7fffffff;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -644,98 +638,51 @@ __device__ inline float follow(const v4f (&s)[R][2], State<D> (&st)[R], float sc
   return __any(any_coarse) ? -1.f : kSlack;
 }
 
-// Bit 8 i + 7 of each byte i that is `least` (over 128) or more.
-__device__ inline uint32_t bytes_from(uint32_t x, uint32_t least) {
-  return ((x & 0x7f7f7f7fu) + 0x01010101u * (256 - least)) & x & 0x80808080u;
+// Weights of 0 leave out what a row does not see only while V is finite, which it is in
+// bf16 unless a scale byte is over 252: NaN, or bytes of a block that nothing was
+// written to.  Those tokens are taken out here, and what the rows that do see
+// them hold is marked as NaN.
+// bit 8 i + 7 of each byte i that is
+__device__ inline uint32_t over_252(uint32_t x) {
+  return ((x & 0x7f7f7f7fu) + 0x03030303u) & x & 0x80808080u;
 }
 template <int D>
-__device__ inline bool has_large(const Values<D>& t) {
-  return (bytes_from(t.scale[0], kLargeScale) | bytes_from(t.scale[1], kLargeScale)) != 0;
+__device__ inline bool not_finite(const Values<D>& t) {
+  return (over_252(t.scale[0]) | over_252(t.scale[1])) != 0;
 }
-// The least of the lanes' numbers, for paths that are seldom taken.
-__device__ inline int least_over_lanes(int v) {
-  int least = v;
-#pragma unroll 1
-  for (int i = 0; i < 64; ++i) least = min(least, lane_value(v, i));
-  return least;
-}
-
-// Row tile r's reference 2^kRaise higher: a power of two, so that but for the reference's
-// own rounding all is as before.
-template <int D, int R, bool SPLIT>
-__device__ inline void raise(State<D>& st, int r, Weights<R, SPLIT>& w) {
-  const float m = st.m + kRaise;
-  const int by = static_cast<int>(fabsf(st.m) < kCoarse ? kRaise : m - st.m);
-  auto less = [by](float x) { return __builtin_ldexpf(x, -by); };
-  st.m = m;
-  st.l = less(st.l), w.l[r] = less(w.l[r]);
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) st.o[j][i] = less(st.o[j][i]);
-  auto weights = [&less](v8bf& p) {
-#pragma unroll
-    for (int x = 0; x < 8; ++x) p[x] = static_cast<__bf16>(less(static_cast<float>(p[x])));
-  };
-  weights(w.hi[r]);
-  if constexpr (SPLIT) weights(w.lo[r]);
-}
-
-// What a step's V needs where some scale byte is kLargeScale or more.
-// Weights of 0 leave out what a row does not see only while V is finite, which it is in
-// bf16 unless a scale byte is kNanScale or more: NaN, or bytes of a block that nothing was
-// written to.  Those tokens are taken out here, and what the rows that do see
-// them hold is marked as NaN.  Rows that see a large value have their reference raised.
-template <int D, int R, bool SPLIT>
+template <int D, int R>
 __device__ inline void take_out(Values<D>& t, int at, const int (&visible)[R], int keys, int quad,
-                                State<D> (&st)[R], Weights<R, SPLIT>& w) {
-  // so that the tokens' numbers are not worked out ahead, in every step
-  asm("" : "+s"(at));
+                                State<D> (&st)[R]) {
   bool any_lost = false;
-  int large = kNoToken;
   uint32_t lost[2] = {0, 0};     // byte i: token i's group
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t lose = bytes_from(t.scale[h], kNanScale);
-    const uint32_t big = bytes_from(t.scale[h], kLargeScale) & ~lose;
+    const uint32_t over = over_252(t.scale[h]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int token = at + 16 * h + quad * 4 + i;
-      large = min(large, big >> (8 * i) & 0x80u && token < keys ? token : kNoToken);
-      if (!(lose >> (8 * i) & 0x80u)) continue;
-      if (token < keys) {
+      if (!(over >> (8 * i) & 0x80u)) continue;
+      if (at + 16 * h + quad * 4 + i < keys) {
         lost[h] |= 255u << (8 * i);
         any_lost = true;
       }
       t.scale[h] &= ~(255u << (8 * i));
 #pragma unroll
-      for (int x = 0; x < Values<D>::kWords; ++x) t.code[h][i][x] = 0;
+      for (int w = 0; w < Values<D>::kWords; ++w) t.code[h][i][w] = 0;
     }
   }
-  if (__any(any_lost)) {
+  if (!__any(any_lost)) return;
 #pragma unroll 1
-    for (int tok = 0; tok < 32; ++tok) {
-      const uint32_t mine = tok < 16 ? lost[0] : lost[1];
+  for (int tok = 0; tok < 32; ++tok) {
+    const uint32_t mine = tok < 16 ? lost[0] : lost[1];
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t f = static_cast<uint32_t>(
-            __shfl(static_cast<int>(mine), (tok / 4 % 4) * 16 + quad * 4 + i));
-        const bool is = (f >> (8 * (tok % 4))) & 255u;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t f = static_cast<uint32_t>(
+          __shfl(static_cast<int>(mine), (tok / 4 % 4) * 16 + quad * 4 + i));
+      const bool is = (f >> (8 * (tok % 4))) & 255u;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (is && at + tok < visible[r]) st[r].lost |= 1u << i;
-      }
+      for (int r = 0; r < R; ++r)
+        if (is && at + tok < visible[r]) st[r].lost |= 1u << i;
     }
-  }
-  if (!__any(large != kNoToken)) return;
-  large = least_over_lanes(large);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    float top = 0.f;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) top = fmaxf(top, static_cast<float>(w.hi[r][x]));
-    top = max_over_quads(top);
-    if (visible[r] > large && top > kLight) raise(st[r], r, w);
   }
 }
 
@@ -1052,8 +999,7 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
 #pragma unroll
         for (int r = 0; r < R; ++r) passes |= weigh(s, st[r], r, scale_log2, p) > slack;
         if (__any(passes)) slack = follow(s, st, scale_log2, p);
-        if (__builtin_expect(__any(has_large(v[n])), 0))
-          take_out(v[n], token, visible, keys, quad, st, p);
+        if (__any(not_finite(v[n]))) take_out(v[n], token, visible, keys, quad, st);
 #pragma unroll
         for (int r = 0; r < R; ++r) st[r].l = p.l[r];
 #pragma unroll
@@ -1072,7 +1018,10 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
   // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
   // each) adds up the elements [][i] of all.
   int bad = kNoTile;
-  if (__any(walk.bad != kNoTile)) bad = least_over_lanes(walk.bad);
+  if (__any(walk.bad != kNoTile)) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) bad = min(bad, lane_value(walk.bad, i));
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float l = sum_over_quads(st[r].l);
