@@ -462,7 +462,9 @@ int fkv_quantize_kv_tokens(int num_tokens, const void* key, int64_t key_token_st
  *
  * A NaN in a key reaches the rows that see that token, in a value those elements of
  * these rows, and no other.  A value group with a scale byte of 253 or 254, which
- * quantising never writes, counts as NaN.  A query row that holds an infinity or
+ * quantising never writes, counts as NaN.  Sums of p v are in 32 bits before they are divided
+ * by that of p, whose terms reach 2^8: values up to 2^119 over the sequence's keys are
+ * safe, larger ones may give infinities or NaN.  A query row that holds an infinity or
  * a NaN gives NaN, and so does one whose largest score, in units of log 2, leaves what
  * 32 bits hold.
  * Asynchronous on `stream`, and may be captured into a graph. */

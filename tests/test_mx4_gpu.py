@@ -549,6 +549,69 @@ def test_values_past_fp16_come_out_as_its_largest(keys, queries, H, width):
     assert ((out[..., 32:].float() - 3).abs() <= 2.0 ** -8).all()
 
 
+@pytest.mark.parametrize("flat", [False, True])
+@pytest.mark.parametrize("kw", [
+    dict(keys=[70, 33], queries=[3, 1], H=2, G=4, D=128),
+    dict(keys=[1400], queries=[1], H=1, G=8, D=64),
+    dict(keys=[200, 150], queries=[90, 150], H=32, G=4, D=128),
+    dict(keys=[120], queries=[120], H=48, G=2, D=256),
+    dict(keys=[9000, 30], queries=[1, 1], H=1, G=4, D=128, width=600)],
+    ids=lambda kw: "-".join(str(v) for v in kw.values()))
+def test_large_values_do_not_overflow_the_sums(kw, flat):
+    """Values up to 2^119 over the keys, beside ordinary ones."""
+    c = Case(seed=53, **kw)
+    cut = c.T * c.H * c.D // 2
+    sc = c.mx[1, :, cut:].view(c.N, c.H, c.D // 32, c.T)
+    byte = 127 + 119 - 3 - math.ceil(math.log2(max(c.keys)))       # 6 is below 2^3
+    sc[:, -1, 1] = byte
+    sc[:, 0, 0, 3::5] = byte
+    # keys that grow, so that scores pass the first ones by a little again and again
+    if not flat:
+        for b, k in enumerate(c.keys):
+            for t in range(k):
+                ks = c.mx[0, c.table[b, t // c.T], cut:].view(c.H, c.D // 32, c.T)
+                ks[:, :, t % c.T] = 122 + t * 5 // k
+    scale = 0.0 if flat else None
+    out, lse = c.run(scale=scale)
+    assert torch.isfinite(out).all()
+    c.check(out, lse, scale=scale)
+
+
+def test_a_large_value_of_small_weight_counts():
+    """A weight of 2^-104 and a value of 2^103 and more beside one of weight 1, in one step, in
+    another and in another workgroup's: the row's result is made of it."""
+    for keys, far, width in ((30, 7, 0), (1000, 900, 0), (9000, 8000, 600)):
+        c = Case(keys=[keys], queries=[1], H=1, G=2, D=128, seed=57, width=width)
+        cut = c.T * c.D // 2
+        c.mx[0, :, :cut] = 0
+        c.mx[1, :, :cut] = 0x22                      # 1
+        c.mx[:, :, cut:] = 127
+        c.qkv[:] = 0
+        c.qkv[:, :2, 0] = 104.0
+        for t, code in ((3, 2), (far, 10)):          # scores of 104 and -104, the others 0
+            c.mx[0, c.table[0, t // c.T], (t % c.T) * c.D // 2] = code
+        page = c.mx[1, c.table[0, far // c.T]]
+        page[cut:].view(c.D // 32, c.T)[2, far % c.T] = 127 + 103
+        scale = math.log(2) / 2                      # weights 1, 2^-52 and 2^-104
+        out, lse = c.run(single=True, scale=scale)
+        c.check(out, lse, scale=scale)
+        # 2^103 2^-104, and of the others 1
+        assert ((out[0, :, 64:96] - 1.5).abs() <= 2.0 ** -6).all()
+        assert ((out[0, :, :64] - 1).abs() <= 2.0 ** -6).all()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16), (256, BF16)])
+def test_the_largest_value_of_a_single_key(dim, dtype):
+    """Scale byte 252, the last that is no NaN: the value itself, or fp16's largest."""
+    c = Case(keys=[1], queries=[1], H=2, G=2, D=dim, dtype=dtype, seed=59)
+    cut = c.T * c.H * dim // 2
+    c.mx[1, :, cut:] = 252
+    out, lse = c.run()
+    v = mo.chunk_values(c.mx[1, c.table[0, 0]].numpy(), c.T, c.H, dim)[0]
+    want = mo.as_type(v, dtype).repeat_interleave(c.G, 0)
+    assert torch.equal(out[0], want)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("scale,spread", [(0.0, 1.0), (-0.3, 1.0), (1.0, 4.0), (1e-3, 300.0)])
 def test_scales_flat_sharp_and_negative(dtype, scale, spread):
