@@ -19,6 +19,7 @@
 
 #include <cstdint>
 
+#include "kv_device.h"
 #include "kv_internal.h"
 
 namespace fkv_detail {
@@ -77,21 +78,6 @@ inline int mx4_check_layer(const void* ptr, int64_t kv_stride, int64_t block_str
                 (long long)num_blocks, info.size);
   return 0;
 }
-
-// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 as one wide multiplication.
-struct FastDiv {
-  uint32_t d = 1, mul = 1u << 31, shift = 31;
-  FastDiv() = default;
-  explicit FastDiv(uint32_t div) : d(div) {
-    uint32_t s = 0;
-    while ((uint64_t(1) << s) < div) ++s;
-    mul = static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + div - 1) / div);
-    shift = 31 + s;
-  }
-  __host__ __device__ uint32_t div(uint32_t n) const {
-    return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
-  }
-};
 
 #pragma GCC visibility pop
 }  // namespace fkv_detail

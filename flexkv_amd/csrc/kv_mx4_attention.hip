@@ -39,6 +39,7 @@
 #include <exception>
 #include <type_traits>
 
+#include "kv_attention.h"
 #include "kv_mx4.h"
 
 using namespace fkv_detail;
@@ -51,7 +52,6 @@ typedef uint32_t Vec2 __attribute__((ext_vector_type(2)));
 typedef uint32_t Vec4 __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 16;          // rows of a tile: columns of a matrix instruction
@@ -61,47 +61,20 @@ constexpr int kMinSteps = 32;      // of a workgroup, where the keys are cut
 // 6 us, a wide workgroup's 12 steps 0.9.  16 sequences of 4096 keys, 8 heads: 26 us cut
 // in two, 23 uncut (21 without a plan); one of 4096: 16 cut in four, 19 uncut.
 constexpr int kCutSteps = 96;
-// Weight up to which a score may pass the reference.  Sums of weights times values over n keys
-// come to 2^8 n times the largest value before they are divided.
-constexpr float kSlack = 256.f;
-// The reference of a row that has seen nothing.  Any score passes it, and so does
-// not -infinity, which a score that a row does not see becomes.
-constexpr float kNothing = -3e38f;
-// From this reference on, the products of scores and scale are rounded before the reference
-// is taken off.  Below, a fused multiplication takes the exact product to it, which a
-// rounded product, the reference, differs from by at most 1; at 2^31 by 64 and more,
-// where weights overflow or vanish.
-constexpr float kCoarse = 0x1p24f;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+struct Plan {
+  static constexpr int kStep = ::kStep, kMinSteps = ::kMinSteps, kCutSteps = ::kCutSteps;
+};
 
-__device__ inline float bits_f32(uint32_t u) { return __builtin_bit_cast(float, u); }
-__device__ inline uint32_t f32_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
 __device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
   return __builtin_amdgcn_perm(hi, lo, sel);
 }
-__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // A chunk of the cache as a buffer: its address is scalar, a lane adds 32 bits of
 // offset, and nothing outside the chunk is read.
 typedef __amdgpu_buffer_rsrc_t Chunk;
 __device__ inline Chunk chunk_at(uint64_t address, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(address), 0, bytes, 0x00027000);
 }
-// quads: the 4 groups of 16 lanes
-__device__ inline float max_over_quads(float v) {
-  auto r = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
-  v = fmaxf(bits_f32(r[0]), bits_f32(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
-  return fmaxf(bits_f32(r[0]), bits_f32(r[1]));
-}
-__device__ inline float sum_over_quads(float v) {
-  auto r = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
-  v = bits_f32(r[0]) + bits_f32(r[1]);
-  r = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
-  return bits_f32(r[0]) + bits_f32(r[1]);
-}
-
-struct Args {
+struct Args : Sequences {
   const char* q;
   char* out;
   float* lse;                        // null: not asked for
@@ -109,196 +82,13 @@ struct Args {
   int64_t lse_row, lse_head;         // elements
   const char* mx;
   int64_t mks, mbs;                  // 4-bit cache: half and block strides
-  const void* table;
-  const void* lens;
-  const void* starts;                // null: one query a sequence
-  int64_t table_row;                 // elements
-  int index64;                       // table, lens and starts are int64
-  int num_blocks, width;             // of the cache; of a table row
-  int batch, heads, group, queries;
-  int tokens, chunk;                 // of a block; bytes of a chunk
-  int causal;
-  int slots;                         // workgroups to cut the keys into; 0: uncut
+  int chunk;                         // bytes of a chunk
   float scale_log2;
   float2* part_ml;                   // [cut][row]: maximum and sum
   float* part_o;                     // [cut][i][j][lane], see State
   int* any_cut;                      // whether some tile has more than one cut
-  FastDiv tiles_per_block, group_div, heads_div;
+  FastDiv tiles_per_block;
 };
-
-__device__ inline int64_t index_at(const void* p, int64_t i, int is64) {
-  return is64 ? static_cast<const int64_t*>(p)[i]
-              : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
-}
-
-struct Seq {
-  int first, count;   // its queries
-  int keys;           // -1: more than its table row can hold
-};
-__device__ inline Seq sequence(const Args& a, int b) {
-  Seq s;
-  if (a.starts) {
-    const int64_t lo = index_at(a.starts, b, a.index64), hi = index_at(a.starts, b + 1, a.index64);
-    const int64_t n = a.queries;
-    s.first = static_cast<int>(lo < 0 ? 0 : lo > n ? n : lo);
-    const int64_t end = hi < s.first ? s.first : hi > n ? n : hi;
-    s.count = static_cast<int>(end) - s.first;
-  } else {
-    s.first = b;
-    s.count = 1;
-  }
-  const int64_t k = index_at(a.lens, b, a.index64);
-  s.keys = k < 0 ? 0 : k > static_cast<int64_t>(a.width) * a.tokens ? -1 : static_cast<int>(k);
-  return s;
-}
-
-// Inclusive sums over the lanes of a wavefront.
-template <class V>
-__device__ inline V scan_lanes(V v) {
-  auto add = [&v](auto ctrl, auto rows) {
-    v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
-                                                           decltype(ctrl)::value,
-                                                           decltype(rows)::value, 0xf, false));
-  };
-  using std::integral_constant;
-  add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());   // 1, 2, 4, 8 lanes before
-  add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
-  add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
-  add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
-  add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());   // lane 15 of the row before
-  add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());   // lane 31
-  return v;
-}
-__device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-
-// How the workgroups are dealt out.  A sequence has ceil(queries * group / rows a tile)
-// tiles; where the keys are cut, every tile of a sequence is cut alike, the
-// longer the sequence the more often, so that all cuts together fill the
-// `slots` the device has at a time and do not start a second round; with as many tiles
-// as slots only sequences longer than the mean are cut.  The lengths are
-// read here, on the device: every wavefront works the plan out for itself, sequence
-// b = lane, then 64 further on.  The first 64 sequences go longest first, and a
-// sequence's tiles last first, as causal rows see more the later they are.
-struct Work {
-  int seq;                    // < 0: none
-  int tile, cut, cuts;
-  bool any_cut;               // whether some tile is cut
-  int steps;                  // of a cut
-  int first;                  // the number of the tile's first cut
-  Seq s;
-};
-__device__ inline int tiles_of(const Args& a, const Seq& s, int rows_a_tile) {
-  return (s.count * a.group + rows_a_tile - 1) / rows_a_tile;
-}
-__device__ inline int steps_of(const Seq& s) { return (max(s.keys, 0) + kStep - 1) / kStep; }
-// ceil(steps / per_cut), at least 1; in floats, so perhaps one more
-__device__ inline int cuts_of(int steps, float inv_per_cut) {
-  return max(1, static_cast<int>(steps * inv_per_cut + 0.9999f));
-}
-
-// Item `item` of the plan; by_tile: `item` counts tiles, the answer is its first cut.
-__device__ inline Work find_work(const Args& a, int item, int rows_a_tile, bool by_tile) {
-  const int lane = threadIdx.x & 63;
-  Seq s{0, 0, 0};
-  int tiles = 0, b = lane;
-  if (lane < a.batch) {
-    s = sequence(a, lane);
-    tiles = tiles_of(a, s, rows_a_tile);
-  }
-  const bool few = a.batch <= 64;
-  if (few && a.batch > 1) {
-    int rank = 0;
-    for (int j = 0; j < a.batch; ++j) {
-      const int k = lane_value(s.keys, j);
-      rank += k > s.keys || (k == s.keys && j < lane);
-    }
-    if (lane >= a.batch) rank = lane;
-    auto move = [&](int v) { return __builtin_amdgcn_ds_permute(rank * 4, v); };
-    s.first = move(s.first), s.count = move(s.count), s.keys = move(s.keys);
-    tiles = move(tiles), b = move(b);
-  }
-  float inv_per_cut = 0.f;     // one cut
-  int longest = 0;             // of a lane's sequences
-  if (a.slots) {
-    float total = 0.f;
-    if (few) {
-      total = static_cast<float>(tiles) * static_cast<float>(steps_of(s));
-      longest = tiles ? steps_of(s) : 0;
-    } else {
-      for (int i = lane; i < a.batch; i += 64) {
-        const Seq x = sequence(a, i);
-        const int n = tiles_of(a, x, rows_a_tile);
-        total += static_cast<float>(n) * static_cast<float>(steps_of(x));
-        if (n) longest = max(longest, steps_of(x));
-      }
-    }
-    total = bits_f32(lane_value(f32_bits(scan_lanes(total)), 63));
-    // at least this many steps a cut; the sum's error and cuts_of's are less than 1 %
-    const float even = fmaxf(total * a.heads / a.slots * 1.01f, kMinSteps);
-    // cuts of even size overflow the slots by the last, short ones: longer cuts until
-    // they do not, or to twice the size
-    const bool pays = __any(longest >= even + kCutSteps);
-    inv_per_cut = pays ? 0.5f / even : 0.f;
-    for (int i = 0; few && pays && i < 8; ++i) {
-      inv_per_cut = 1.f / (even * (1.f + i * 0.125f));
-      const int n = lane_value(scan_lanes(tiles * cuts_of(steps_of(s), inv_per_cut)), 63);
-      if (static_cast<int64_t>(n) * a.heads <= a.slots) break;
-    }
-  }
-  Work w{-1, 0, 0, 0, static_cast<bool>(__any(cuts_of(longest, inv_per_cut) > 1)), 0, 0,
-         Seq{0, 0, 0}};
-  int before = 0, cuts_before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (b0) {
-      b = b0 + lane;
-      tiles = 0;
-      if (b < a.batch) {
-        s = sequence(a, b);
-        tiles = tiles_of(a, s, rows_a_tile);
-      }
-    }
-    const int steps = steps_of(s);
-    const int cuts = cuts_of(steps, inv_per_cut);
-    const int cut_ends = scan_lanes(tiles * cuts);
-    const int ends = by_tile ? scan_lanes(tiles) : cut_ends;
-    const uint64_t later = __ballot(before + ends > item);
-    if (later) {
-      const int at = __builtin_ctzll(later);
-      const int n = lane_value(tiles, at), c = lane_value(cuts, at);
-      const int local = item - (before + lane_value(ends, at) - (by_tile ? n : n * c));
-      const int nth = by_tile || c == 1 ? local : uniform(local / c);
-      w.seq = lane_value(b, at);
-      w.cuts = c;
-      w.tile = n - 1 - nth;
-      w.cut = by_tile ? 0 : local - nth * c;
-      w.steps = uniform((lane_value(steps, at) + c - 1) / c);
-      w.first = cuts_before + lane_value(cut_ends, at) - n * c + nth * c;
-      w.s = {lane_value(s.first, at), lane_value(s.count, at), lane_value(s.keys, at)};
-      return w;
-    }
-    before += lane_value(ends, 63);
-    cuts_before += lane_value(cut_ends, 63);
-  }
-  return w;
-}
-
-// The same where the keys are uncut and every sequence has one query: nothing
-// but the sequence's own length is read.
-__device__ inline Work find_single(const Args& a, int item, int rows_a_tile) {
-  Work w{item, 0, 0, 1, false, 0, 0, Seq{0, 0, 0}};
-  const int tiles = (a.group + rows_a_tile - 1) / rows_a_tile;
-  if (tiles > 1) {
-    w.seq = uniform(item / tiles);
-    w.tile = item - w.seq * tiles;
-  }
-  if (w.seq >= a.batch) {      // of the last round of the XCDs
-    w.seq = -1;
-    return w;
-  }
-  w.s = sequence(a, w.seq);
-  w.s.keys = uniform(w.s.keys);
-  return w;
-}
 
 // The queries of 16 rows as e4m3 parts: operand registers for each part and
 // 128-element step, and the scale bytes, operand p's in byte p.  D = 64: an operand's
@@ -500,13 +290,6 @@ __device__ inline uint32_t cvt_bf16(uint32_t codes, float scale, int byte) {
   return __builtin_bit_cast(uint32_t, r);
 }
 
-__device__ inline uint32_t pack_bf16(float a, float b) {
-  v2bf r;
-  r[0] = static_cast<__bf16>(a);
-  r[1] = static_cast<__bf16>(b);
-  return __builtin_bit_cast(uint32_t, r);
-}
-
 // A row tile's state: lane (row, quad) holds row `lane & 15`.
 template <int D>
 struct State {
@@ -580,13 +363,6 @@ struct Weights {
   v8bf hi[R], lo[R];
   float l[R];     // what State::l becomes
 };
-
-// s * scale rounded, then less m
-__device__ inline float rounded_less(float s, float scale, float m) {
-#pragma clang fp contract(off)
-  const float x = s * scale;
-  return x - m;
-}
 
 // Row tile r's scores as weights; returns their sum, which is over kSlack where one
 // of them passes the reference by more than that.
@@ -735,21 +511,6 @@ __device__ inline uint32_t narrow2(float a, float b) {
   return __builtin_bit_cast(uint32_t, r);
 }
 
-// Row r of a tile: the packed query row, its head and the keys it sees.
-struct Row {
-  int64_t at;
-  int head, visible;
-};
-__device__ inline Row row_of(const Args& a, const Seq& s, int r, int kv_head) {
-  const int pos = a.group_div.div(r);
-  Row row;
-  row.at = static_cast<int64_t>(s.first) + pos;
-  row.head = kv_head * a.group + (r - pos * a.group);
-  const int keys = max(s.keys, 0);
-  row.visible = a.causal ? max(0, keys - s.count + pos + 1) : keys;
-  return row;
-}
-
 __device__ inline void write_lse(const Args& a, const Row& row, int visible, float m, float l) {
   a.lse[row.at * a.lse_row + row.head * a.lse_head] =
       l == 0.f ? (visible ? bits_f32(0x7fc00000u) : -INFINITY)
@@ -777,27 +538,6 @@ __device__ inline void write_row(const Args& a, const Row& row, int visible, int
       *reinterpret_cast<uint2*>(out + x * 4) = make_uint2(w[x], w[x + 1]);
   }
   if (a.lse && quad == 0 && i == 0 && j0 == 0) write_lse(a, row, visible, m, l);
-}
-
-// Which item of the plan, and which K/V head, a workgroup has.  Workgroups go round the
-// 8 XCDs.  Where K and V are read once, an item's heads are on one XCD, so that a
-// block is read whole by one L2 at about one time.  Where many tiles read them, a
-// head's tiles are on one XCD if there are 8 heads.
-constexpr int kXcds = 8;
-struct Place {
-  int item, head;
-};
-__device__ inline Place heads_together(const Args& a, int block) {
-  const int nth = block / kXcds, group = a.heads_div.div(nth);
-  return {group * kXcds + block % kXcds, nth - group * a.heads};
-}
-__device__ inline Place heads_apart(const Args& a, int block) {
-  const int item = a.heads_div.div(block);
-  return {item, block - item * a.heads};
-}
-// The number that a cut's part of the workspace has.
-__device__ inline int64_t part_of(const Args& a, int item, int head) {
-  return static_cast<int64_t>(item) * a.heads + head;
 }
 
 // The tiles of the steps that a wavefront takes, every W-th from its first on, 32 steps
@@ -859,12 +599,6 @@ __device__ inline void clear(State<D>& st) {
   for (int j = 0; j < D / 16; ++j) st.o[j] = {0.f, 0.f, 0.f, 0.f};
 }
 
-// The scale of the scores; not 0, so that -infinity stays that, but the smallest there is,
-// with which no finite score comes to more than 2^-21.
-__device__ inline float score_scale(const Args& a) {
-  return fmaxf(fabsf(a.scale_log2), 0x1p-149f);
-}
-
 // Row tiles of a workgroup for many queries, as registers allow.
 constexpr int most_row_tiles(int dim) { return dim <= 128 ? 3 : 2; }
 // Wavefronts a SIMD is to hold: more than these cost spilled registers.
@@ -903,7 +637,7 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
   __shared__ int shared_scale[R][64];
   __shared__ float sum_m[W][R][16], sum_l[W][R][16];
   const Place at = R == 1 ? heads_together(a, blockIdx.x) : heads_apart(a, blockIdx.x);
-  const Work w = a.slots || a.starts ? find_work(a, at.item, kRows * R, false)
+  const Work w = a.slots || a.starts ? find_work<Plan>(a, at.item, kRows * R, false)
                                      : find_single(a, at.item, kRows * R);
   if (a.slots && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = w.any_cut;
   if (w.seq < 0) return;
@@ -977,7 +711,7 @@ __global__ __launch_bounds__(64 * W, waves_a_simd(R, D)) void mx4_attention_kern
     if (r == 0) asm volatile("" ::: "memory");
     return read_query(r);
   };
-  const float scale_log2 = score_scale(a);
+  const float scale_log2 = score_scale(a.scale_log2);
   float slack = kSlack;
   State<D> st[R];
 #pragma unroll
@@ -1090,7 +824,7 @@ __global__ __launch_bounds__(256 * G) void mx4_join_kernel(const Args a) {
   const int block = blockIdx.x / R, r = blockIdx.x % R;
   const int tile = a.heads_div.div(block);
   const int kv_head = block - tile * a.heads;
-  const Work w = find_work(a, tile, kRows * R, true);
+  const Work w = find_work<Plan>(a, tile, kRows * R, true);
   if (w.seq < 0 || w.cuts == 1) return;
   __shared__ float sum_o[G * 4][NT][64];
   __shared__ float sum_m[G][16], sum_l[G][16];
