@@ -45,6 +45,10 @@ EXPORTED_SYMBOLS = (
     "fkv_quantize_kv_tokens",
     "fkv_mx4_attention_workspace",
     "fkv_mx4_attention",
+    "fkv_write_kv_tokens",
+    "fkv_paged_attention_workspace",
+    "fkv_paged_attention",
+    "fkv_evict_kv_tokens",
     "fkv_transfer_kv_blocks_layerwise",
     "fkv_handle_num_groups",
     "fkv_handle_query",
@@ -147,6 +151,85 @@ class Mx4AttentionArgs(ctypes.Structure):
     ]
 
 
+class PagedLayer(ctypes.Structure):
+    """fkv_paged_layer."""
+    _fields_ = [
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_block_stride_bytes", ctypes.c_int64),
+        ("key_token_stride_bytes", ctypes.c_int64),
+        ("key_head_stride_bytes", ctypes.c_int64),
+        ("value_block_stride_bytes", ctypes.c_int64),
+        ("value_token_stride_bytes", ctypes.c_int64),
+        ("value_head_stride_bytes", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64),
+        ("tokens_per_block", ctypes.c_int),
+        ("num_heads", ctypes.c_int),
+        ("head_size", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """fkv_paged_attention_args."""
+    _fields_ = [
+        ("layer", PagedLayer),
+        ("query", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("query_row_stride_bytes", ctypes.c_int64),
+        ("query_head_stride_bytes", ctypes.c_int64),
+        ("out_row_stride_bytes", ctypes.c_int64),
+        ("out_head_stride_bytes", ctypes.c_int64),
+        ("lse_row_stride", ctypes.c_int64),
+        ("lse_head_stride", ctypes.c_int64),
+        ("weights", ctypes.c_void_p),
+        ("weights_seq_stride", ctypes.c_int64),
+        ("weights_head_stride", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_starts", ctypes.c_void_p),
+        ("table_row_stride", ctypes.c_int64),
+        ("index_is_64bit", ctypes.c_int),
+        ("table_width", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("num_queries", ctypes.c_int),
+        ("group_size", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("weights_width", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    """fkv_evict_args."""
+    _fields_ = [
+        ("layer", PagedLayer),
+        ("weights", ctypes.c_void_p),
+        ("new_weights", ctypes.c_void_p),
+        ("weights_seq_stride", ctypes.c_int64),
+        ("weights_head_stride", ctypes.c_int64),
+        ("new_weights_seq_stride", ctypes.c_int64),
+        ("new_weights_head_stride", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("new_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("table_row_stride", ctypes.c_int64),
+        ("new_table_row_stride", ctypes.c_int64),
+        ("kept", ctypes.c_void_p),
+        ("index_is_64bit", ctypes.c_int),
+        ("table_width", ctypes.c_int),
+        ("new_table_width", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("budget", ctypes.c_int),
+        ("recent", ctypes.c_int),
+        ("weights_width", ctypes.c_int),
+        ("new_weights_width", ctypes.c_int),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 # Counts finalize() calls: handles and streams made before the latest one
@@ -187,6 +270,19 @@ def _declare(lib: ctypes.CDLL) -> None:
     f = lib.fkv_mx4_attention
     f.restype = c_int
     f.argtypes = [ctypes.POINTER(Mx4AttentionArgs), c_vp]
+    f = lib.fkv_write_kv_tokens
+    f.restype = c_int
+    f.argtypes = [ctypes.POINTER(PagedLayer), c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp,
+                  c_int, c_vp]
+    f = lib.fkv_paged_attention_workspace
+    f.restype = c_int
+    f.argtypes = [ctypes.POINTER(PagedAttentionArgs), ctypes.POINTER(c_sz)]
+    f = lib.fkv_paged_attention
+    f.restype = c_int
+    f.argtypes = [ctypes.POINTER(PagedAttentionArgs), c_vp]
+    f = lib.fkv_evict_kv_tokens
+    f.restype = c_int
+    f.argtypes = [ctypes.POINTER(EvictArgs), c_vp]
     f = lib.fkv_transfer_kv_blocks_layerwise
     f.restype = c_int
     f.argtypes = [c_int, c_int, c_int, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64,
@@ -308,8 +404,8 @@ def c_int(v, what: str) -> int:
 
 class _CtypesCalls:
     """The per-call path of c_ext.transfer_kv_blocks and
-    transfer_kv_blocks_kv_ptrs over ctypes (and none for the functions on a
-    4-bit cache, whose ctypes calls c_ext makes itself), with the compiled module's
+    transfer_kv_blocks_kv_ptrs over ctypes (and none for the functions on a 4-bit
+    or a paged cache, whose ctypes calls c_ext makes itself), with the compiled module's
     argument conventions: the same 16 / 15 positional arguments, False
     (nothing raised) when a tensor check fails so that c_ext names the
     argument, RuntimeError with the library's message when the transfer
@@ -352,6 +448,7 @@ class _CtypesCalls:
         return False
 
     mx4_tokens = mx4_attention = mx4_blocks
+    write_kv_tokens = paged_attention = evict_kv_tokens = mx4_blocks
 
     def transfer_kv_blocks(self, gids, ptrs, gkv, gblk, cids, cpu, ckv, clay, cblk, chunk,
                            start, sms, h2d, mode, mla, stream):
@@ -434,6 +531,9 @@ def fast():
             _fkv_py.bind_mx4(addr(lib.fkv_quantize_kv_blocks), addr(lib.fkv_dequantize_kv_blocks),
                              addr(lib.fkv_quantize_kv_tokens),
                              addr(lib.fkv_mx4_attention_workspace), addr(lib.fkv_mx4_attention))
+            _fkv_py.bind_paged(addr(lib.fkv_write_kv_tokens),
+                               addr(lib.fkv_paged_attention_workspace),
+                               addr(lib.fkv_paged_attention), addr(lib.fkv_evict_kv_tokens))
             _fast = _fkv_py
     return _fast
 

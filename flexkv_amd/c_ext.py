@@ -19,7 +19,8 @@ from . import _lib
 
 __all__ = ["transfer_kv_blocks", "transfer_kv_blocks_kv_ptrs", "gather_kv_blocks",
            "scatter_kv_blocks", "mx4_chunk_bytes", "quantize_kv_blocks", "dequantize_kv_blocks",
-           "quantize_kv_tokens", "mx4_attention",
+           "quantize_kv_tokens", "mx4_attention", "write_kv_tokens", "paged_attention",
+           "evict_kv_tokens",
            "transfer_kv_blocks_layerwise", "LayerwiseTransfer", "transfer_stream",
            "release_transfer_stream", "set_copy_engine_policy", "copy_engine_policy",
            "TPTransferThreadGroup", "SSDIOCTX", "transfer_kv_blocks_ssd"]
@@ -502,6 +503,292 @@ def mx4_attention(query: torch.Tensor, mx_layer: torch.Tensor, num_kv_heads: int
     if rc != 0:
         raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
     return out
+
+
+def _paged_layer(key_cache, value_cache, fn_name: str, device=None) -> _lib.PagedLayer:
+    """Check one layer's cache, key_cache and value_cache (None: a cache of one half)
+    [block, token, head, head_size], and describe it to the library."""
+    _require_device(key_cache, "key_cache", fn_name, device)
+    device = key_cache.device
+    if key_cache.dim() != 4 or key_cache.stride(3) != 1:
+        raise ValueError(f"{fn_name}: key_cache must be [block, token, head, head_size] with "
+                         f"neighbouring elements, got {tuple(key_cache.shape)} "
+                         f"{key_cache.stride()}")
+    code = _dtype_code(key_cache.dtype, fn_name)
+    if value_cache is not None:
+        _require_device(value_cache, "value_cache", fn_name, device)
+        if value_cache.shape != key_cache.shape or value_cache.dtype != key_cache.dtype or \
+                value_cache.stride(3) != 1:
+            raise ValueError(f"{fn_name}: value_cache must be as key_cache is, "
+                             f"{tuple(key_cache.shape)} {key_cache.dtype}, got "
+                             f"{tuple(value_cache.shape)} {value_cache.dtype} "
+                             f"{value_cache.stride()}")
+    blocks, tokens, heads, dim = key_cache.shape
+    strides = [0] * 6
+    for i, t in enumerate((key_cache, value_cache)):
+        if t is not None:
+            strides[3 * i:3 * i + 3] = _strides(t)
+    c_int = _lib.c_int
+    return _lib.PagedLayer(key_cache.data_ptr(),
+                           None if value_cache is None else value_cache.data_ptr(), *strides,
+                           blocks, c_int(tokens, "tokens_per_block"), c_int(heads, "num_heads"),
+                           c_int(dim, "head_size"), code)
+
+
+def _strides(t: torch.Tensor) -> list:
+    """Bytes from one to the next in every dimension but the last; one alone has none."""
+    return [t.stride(d) * t.element_size() if t.shape[d] > 1 else 0 for d in range(t.dim() - 1)]
+
+
+def _table(fn_name: str, name: str, table, batch: int, index: torch.dtype, device) -> None:
+    _require_device(table, name, fn_name, device)
+    if table.dtype != index:
+        raise ValueError(f"{fn_name}: {name} must be as seq_lens is, {index}, got {table.dtype}")
+    if table.dim() != 2 or table.shape[0] != batch or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{fn_name}: {name} must be [{batch}, blocks] with neighbouring entries, "
+                         f"got {tuple(table.shape)} {table.stride()}")
+
+
+def _lengths(fn_name: str, seq_lens, device) -> int:
+    _require_device(seq_lens, "seq_lens", fn_name, device)
+    if seq_lens.dtype not in (torch.int32, torch.int64) or seq_lens.dim() != 1 or \
+            not seq_lens.is_contiguous():
+        raise ValueError(f"{fn_name}: seq_lens must be a contiguous vector of int32 or int64, got "
+                         f"{seq_lens.dtype} {tuple(seq_lens.shape)}")
+    return seq_lens.shape[0]
+
+
+def _weights(fn_name: str, name: str, t, batch: int, heads: int, width: int, device) -> None:
+    _require_device(t, name, fn_name, device)
+    if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (batch, heads) or \
+            t.shape[2] < width or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{fn_name}: {name} must be float32 [{batch}, {heads}, {width} or more] "
+                         f"with neighbouring entries, got {t.dtype} {tuple(t.shape)} "
+                         f"{t.stride()}")
+
+
+def write_kv_tokens(key: torch.Tensor, value, key_cache: torch.Tensor, value_cache,
+                    slots: torch.Tensor) -> None:
+    """Write new tokens of one layer into their slots of a paged cache (extension;
+    fkv_write_kv_tokens).  ``key`` and ``value``: [token, head, head_size], of any token
+    and head stride; ``key_cache`` and ``value_cache``: [block, token, head, head_size] of the
+    same type (bf16, fp16 or float32), of any block, token and head stride, such as the halves
+    of an engine's [2, blocks, tokens, heads, head_size] (value and value_cache None: one
+    latent half); ``slots``: int64 or int32, block * tokens_per_block + offset, one below 0 or
+    past the cache being padding.  Slots have to differ.  Makes no gradients: inputs that
+    require them are refused but under ``torch.no_grad()``.  Asynchronous on the current torch
+    stream; may be captured into a graph."""
+    fn = "write_kv_tokens"
+    if (_fast or _load_fast()).write_kv_tokens(key, value, key_cache, value_cache,
+                                               slots) is not False:
+        return
+    _require_device(key, "key", fn)
+    device = key.device
+    if (value is None) != (value_cache is None):
+        raise ValueError(f"{fn}: value and value_cache must both be given, or neither")
+    layer = _paged_layer(key_cache, value_cache, fn, device)
+    n = key.shape[0] if key.dim() else 0
+    for name, x in (("key", key), ("value", value)):
+        if x is None:
+            continue
+        _require_device(x, name, fn, device)
+        if x.shape != (n, *key_cache.shape[2:]) or x.dtype != key_cache.dtype or x.stride(2) != 1:
+            raise ValueError(f"{fn}: {name} must be [token, {key_cache.shape[2]}, "
+                             f"{key_cache.shape[3]}] of {key_cache.dtype} with neighbouring "
+                             f"elements, got {tuple(x.shape)} {x.dtype} {x.stride()}")
+    _require_device(slots, "slots", fn, device)
+    if slots.dtype not in (torch.int64, torch.int32) or slots.shape != (n,) \
+            or not slots.is_contiguous():
+        raise ValueError(f"{fn}: slots must be {n} contiguous int64 or int32 values, got "
+                         f"{slots.dtype} {tuple(slots.shape)}")
+    rows = [key.data_ptr(), *_strides(key)]
+    rows += [None, 0, 0] if value is None else [value.data_ptr(), *_strides(value)]
+    with _on_device(device):
+        rc = _lib.load().fkv_write_kv_tokens(
+            layer, _lib.c_int(n, "tokens"), *rows, slots.data_ptr(),
+            1 if slots.dtype == torch.int64 else 0, _stream_handle(fn))
+    if rc != 0:
+        raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
+
+
+def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                    block_table: torch.Tensor, seq_lens: torch.Tensor, query_starts=None,
+                    scale: float = None, causal: bool = True, out: torch.Tensor = None,
+                    lse: torch.Tensor = None, weights: torch.Tensor = None) -> torch.Tensor:
+    """Attention of packed queries over one layer of a paged cache (extension;
+    fkv_paged_attention).  ``query``: bf16 or fp16 [row, head, head_size] of any row and head
+    stride, a multiple of the cache's heads; ``key_cache`` and ``value_cache`` as in
+    write_kv_tokens, of the query's type; ``block_table`` [sequence, blocks] and ``seq_lens``
+    [sequence] give each sequence's blocks and keys, the queries' own included;
+    ``query_starts`` [sequences + 1] the rows of each, its last tokens (None: row b is
+    sequence b's one query); all three int32 or all int64.  ``scale`` defaults to
+    head_size ** -0.5.  With ``causal`` a query sees the keys up to its own position.  Rows
+    that see none give zeros (lse -inf); rows of no sequence are left as they were (not written
+    in a given ``out``, unset in a new one).  ``out`` may not overlap ``query``.  ``lse``:
+    float32 [row, head], receives the log of the sum of exp.  ``weights``: float32 [sequence,
+    K/V head, tokens that a row of block_table holds, or more]; entry t of a head grows by what
+    token t got of the attention of that head's queries, which is what evict_kv_tokens goes by.
+    Returns ``out``.  Makes no gradients: inputs that require them are refused but under
+    ``torch.no_grad()``.  Asynchronous on the current torch stream; may be captured into a
+    graph."""
+    fn = "paged_attention"
+    done = (_fast or _load_fast()).paged_attention(query, key_cache, value_cache, block_table,
+                                                   seq_lens, query_starts, scale, causal, out,
+                                                   lse, weights)
+    if done is not False:
+        return done
+    _require_device(query, "query", fn)
+    device = query.device
+    if query.dim() != 3 or query.stride(2) != 1 or query.dtype not in (torch.bfloat16,
+                                                                       torch.float16):
+        raise ValueError(f"{fn}: query must be bf16 or fp16 [row, head, head_size] with "
+                         f"neighbouring elements, got {query.dtype} {tuple(query.shape)} "
+                         f"{query.stride()}")
+    rows, heads, dim = query.shape
+    if value_cache is None:
+        raise TypeError(f"{fn}: value_cache must be a torch.Tensor, got NoneType")
+    layer = _paged_layer(key_cache, value_cache, fn, device)
+    kv_heads = key_cache.shape[2]
+    if key_cache.dtype != query.dtype or key_cache.shape[3] != dim:
+        raise ValueError(f"{fn}: the cache must hold rows of {dim} {query.dtype}, got "
+                         f"{tuple(key_cache.shape)} {key_cache.dtype}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{fn}: {heads} query heads are no multiple of {kv_heads} K/V heads")
+    batch = _lengths(fn, seq_lens, device)
+    index = seq_lens.dtype
+    _table(fn, "block_table", block_table, batch, index, device)
+    if query_starts is None:
+        if rows < batch:
+            raise ValueError(f"{fn}: {batch} sequences of one query each, but {rows} rows")
+    else:
+        _require_device(query_starts, "query_starts", fn, device)
+        if query_starts.dtype != index or query_starts.shape != (batch + 1,) or \
+                not query_starts.is_contiguous():
+            raise ValueError(f"{fn}: query_starts must hold {batch + 1} contiguous values of "
+                             f"{index}, got {query_starts.dtype} {tuple(query_starts.shape)}")
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=query.dtype, device=device)
+    else:
+        _require_device(out, "out", fn, device)
+        if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
+            raise ValueError(f"{fn}: out must be as query is, {tuple(query.shape)} {query.dtype}, "
+                             f"got {tuple(out.shape)} {out.dtype} {out.stride()}")
+        if _overlap(query, out):
+            raise ValueError(f"{fn}: out may not overlap query")
+    if lse is not None:
+        _require_device(lse, "lse", fn, device)
+        if lse.shape != (rows, heads) or lse.dtype != torch.float32:
+            raise ValueError(f"{fn}: lse must be float32 {(rows, heads)}, got {lse.dtype} "
+                             f"{tuple(lse.shape)}")
+    if weights is not None:
+        _weights(fn, "weights", weights, batch, kv_heads,
+                 block_table.shape[1] * key_cache.shape[1], device)
+    c_int = _lib.c_int
+    args = _lib.PagedAttentionArgs(
+        layer, query.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
+        *_strides(query), *_strides(out), *(lse.stride() if lse is not None else (0, 0)),
+        weights.data_ptr() if weights is not None else None,
+        *(weights.stride()[:2] if weights is not None else (0, 0)),
+        block_table.data_ptr(), seq_lens.data_ptr(),
+        query_starts.data_ptr() if query_starts is not None else None, block_table.stride(0),
+        1 if index is torch.int64 else 0, c_int(block_table.shape[1], "table_width"),
+        c_int(batch, "sequences"), c_int(rows, "queries"), heads // kv_heads, 1 if causal else 0,
+        min(weights.shape[2], 2**31 - 1) if weights is not None else 0,
+        float(dim ** -0.5 if scale is None else scale))
+    lib = _lib.load()
+    need = ctypes.c_size_t()
+    rc = lib.fkv_paged_attention_workspace(args, need)
+    if rc == 0:
+        with _on_device(device):
+            if need.value:
+                # the allocator orders its reuse on the current stream
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+                args.workspace = workspace.data_ptr()
+                args.workspace_bytes = need.value
+            rc = lib.fkv_paged_attention(args, _stream_handle(fn))
+    if rc != 0:
+        raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
+    return out
+
+
+def evict_kv_tokens(key_cache: torch.Tensor, value_cache, weights: torch.Tensor,
+                    block_table: torch.Tensor, seq_lens: torch.Tensor, new_table: torch.Tensor,
+                    budget: int, recent: int = 0, new_weights: torch.Tensor = None,
+                    kept: torch.Tensor = None) -> torch.Tensor:
+    """Keep ``budget`` tokens of every sequence and K/V head of one layer, in blocks of their
+    own (extension; fkv_evict_kv_tokens): the ``recent`` last, and of the others those with the
+    largest ``weights`` (float32 [sequence, head, tokens that a row of block_table holds, or
+    more], as paged_attention adds them up; of equal ones the earlier, NaN above all).
+    ``key_cache``, ``value_cache``, ``block_table`` and ``seq_lens`` as in paged_attention (any
+    type; value_cache None: one latent half).  The kept rows, in their order, become the first
+    tokens of the blocks ``new_table`` [sequence, blocks], which must be other blocks than those
+    of the sequences' tokens and differ; the old ones are only read, and may be shared.
+    ``new_weights``: float32 [sequence, head, budget or more], receives the kept tokens'
+    weights, then zeros; it may be ``weights``.  Returns ``kept``, int32 [sequence, head,
+    budget]: the places the kept tokens had, then -1; the sequences' new lengths are
+    ``seq_lens.clamp(max=budget)``.  A sequence of no more than ``budget`` tokens keeps all.
+    Asynchronous on the current torch stream; may be captured into a graph."""
+    fn = "evict_kv_tokens"
+    done = (_fast or _load_fast()).evict_kv_tokens(key_cache, value_cache, weights, block_table,
+                                                   seq_lens, new_table, budget, recent,
+                                                   new_weights, kept)
+    if done is not False:
+        return done
+    layer = _paged_layer(key_cache, value_cache, fn)
+    device = key_cache.device
+    tokens, heads = key_cache.shape[1:3]
+    batch = _lengths(fn, seq_lens, device)
+    index = seq_lens.dtype
+    _table(fn, "block_table", block_table, batch, index, device)
+    _table(fn, "new_table", new_table, batch, index, device)
+    c_int = _lib.c_int
+    budget, recent = c_int(budget, "budget"), c_int(recent, "recent")
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"{fn}: budget must be positive and recent in [0, budget], got {budget} "
+                         f"and {recent}")
+    most = block_table.shape[1] * tokens
+    _weights(fn, "weights", weights, batch, heads, most, device)
+    if new_weights is not None:
+        _weights(fn, "new_weights", new_weights, batch, heads, min(budget, most), device)
+        same = new_weights.data_ptr() == weights.data_ptr() and \
+            new_weights.stride() == weights.stride()
+        if not same and _ranges_meet(weights, new_weights):
+            raise ValueError(f"{fn}: new_weights may be weights itself, but not overlap it "
+                             f"otherwise")
+    if kept is None:
+        kept = torch.empty((batch, heads, budget), dtype=torch.int32, device=device)
+    else:
+        _require_device(kept, "kept", fn, device)
+        if kept.shape != (batch, heads, budget) or kept.dtype != torch.int32 or \
+                not kept.is_contiguous():
+            raise ValueError(f"{fn}: kept must be contiguous int32 {(batch, heads, budget)}, got "
+                             f"{kept.dtype} {tuple(kept.shape)} {kept.stride()}")
+    given = new_weights is not None
+    args = _lib.EvictArgs(
+        layer, weights.data_ptr(), new_weights.data_ptr() if given else None,
+        *weights.stride()[:2], *(new_weights.stride()[:2] if given else (0, 0)),
+        block_table.data_ptr(), new_table.data_ptr(), seq_lens.data_ptr(), block_table.stride(0),
+        new_table.stride(0), kept.data_ptr(), 1 if index is torch.int64 else 0,
+        c_int(block_table.shape[1], "table_width"), c_int(new_table.shape[1], "new_table_width"),
+        c_int(batch, "sequences"), budget, recent, min(weights.shape[2], 2**31 - 1),
+        min(new_weights.shape[2], 2**31 - 1) if given else 0)
+    with _on_device(device):
+        rc = _lib.load().fkv_evict_kv_tokens(args, _stream_handle(fn))
+    if rc != 0:
+        raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
+    return kept
+
+
+def _ranges_meet(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether the bytes from a tensor's first element to its last meet another's."""
+    if not x.numel() or not y.numel():
+        return False
+
+    def end(t):
+        return t.data_ptr() + t.element_size() * (
+            1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    return x.data_ptr() < end(y) and y.data_ptr() < end(x)
 
 
 class LayerwiseTransfer:

@@ -1,0 +1,895 @@
+// kv_paged_attention.hip - attention over a paged KV cache of bf16 or fp16, and what each
+// cached token got of it: for query i of head hq in a sequence, with K/V head h = hq / group,
+//
+//   o = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale q . k_t - max),   t <= its own position
+//   weights[h][t] += sum over those queries and heads of p_t / sum p
+//
+// The queries of a group and of neighbouring positions are the rows of one tile (row =
+// position * group + head in the group), so K and V are read once for all of them.
+//
+// Both products are matrix instructions with the tokens, then the elements, as rows of the
+// result and the query rows as columns.  S = K Q^T comes out with some tokens of one row in a
+// lane, which is the layout of the second product's operand if its tokens are taken in that
+// order, so P never leaves its lane.  bf16 weights of 8 significant bits, fp16 ones of 11
+// (of what is at least 2^-14 of the largest; 2^-25 of it below): their roundings average out
+// over the keys, and the sum they are divided by is of the unrounded ones.
+//
+// Softmax: one pass, running maximum and sum per row in 32 bits, in units of log2.
+// The maximum is a reference that follows only when a score passes it by 2^8, so
+// most steps neither compare across lanes nor scale the sums.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <exception>
+#include <type_traits>
+
+#include "kv_attention.h"
+#include "kv_paged.h"
+
+using namespace fkv_detail;
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t Vec2 __attribute__((ext_vector_type(2)));
+typedef uint32_t Vec4 __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// The matrix instructions of a type.
+template <class T>
+struct Mat;
+template <>
+struct Mat<__bf16> {
+  typedef v8bf Op;
+  static __device__ inline v4f mul16(Op a, Op b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ inline v16f mul32(Op a, Op b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ inline uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+  static __device__ inline float low(uint32_t u) { return bits_f32(u << 16); }
+  static __device__ inline float high(uint32_t u) { return bits_f32(u & 0xffff0000u); }
+  static constexpr uint32_t kExponents = 0x7f807f80u;
+};
+template <>
+struct Mat<_Float16> {
+  typedef v8h Op;
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+  static __device__ inline v4f mul16(Op a, Op b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ inline v16f mul32(Op a, Op b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ inline uint32_t pack(float a, float b) {
+    v2h r;
+    r[0] = static_cast<_Float16>(a);
+    r[1] = static_cast<_Float16>(b);
+    return __builtin_bit_cast(uint32_t, r);
+  }
+  static __device__ inline float low(uint32_t u) {
+    return static_cast<float>(__builtin_bit_cast(v2h, u)[0]);
+  }
+  static __device__ inline float high(uint32_t u) {
+    return static_cast<float>(__builtin_bit_cast(v2h, u)[1]);
+  }
+  static constexpr uint32_t kExponents = 0x7c007c00u;
+};
+
+// Whether one of the two elements of a register is an infinity or a NaN.
+template <class T>
+__device__ inline bool not_finite(uint32_t u) {
+  constexpr uint32_t lo = Mat<T>::kExponents & 0xffffu, hi = Mat<T>::kExponents & 0xffff0000u;
+  return (u & lo) == lo || (u & hi) == hi;
+}
+
+struct Args : Sequences {
+  const char* q;
+  char* out;
+  float* lse;                        // null: not asked for
+  int64_t q_row, q_head, out_row, out_head;   // bytes
+  int64_t lse_row, lse_head;         // elements
+  Half k, v;
+  float scale_log2;
+  FastDiv tokens_div;
+  float2* part_ml;                   // [cut][row]: maximum and sum
+  float* part_o;                     // [cut][row][element]
+  int* any_cut;                      // whether some tile has more than one cut
+  // for the tokens' weights, all null where they are not asked for
+  float* weights;
+  int64_t w_seq, w_head;             // elements
+  float2* stats;                     // [query][head]: reference and 1 / sum of a row
+};
+
+// 16 bytes of device memory; not a flat access, which would wait for LDS as well.
+template <class V>
+__device__ inline V load(uint64_t address) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) V*>(address);
+}
+
+// ---------------------------------------------------------------------------
+// Where the rows of tokens lie
+
+__device__ inline int64_t block_id(const Args& a, int seq, int token) {
+  return index_at(a.table, seq * a.table_row + a.tokens_div.div(token), a.index64);
+}
+// The row of a token in block `id`, of one half and head.  A block outside the cache is block 0
+// here (and noted by whoever calls).
+__device__ inline bool outside(const Args& a, int64_t id) { return id < 0 || id >= a.num_blocks; }
+__device__ inline uint64_t row_address(const Args& a, const Half& x, int64_t id, int token,
+                                       int head) {
+  const int in_block = token - a.tokens_div.div(token) * static_cast<int>(a.tokens_div.d);
+  return reinterpret_cast<uint64_t>(x.p) + (outside(a, id) ? 0 : id) * x.block +
+         in_block * x.token + head * x.head;
+}
+
+constexpr int kNoToken = 0x7fffffff;
+// The least value over the wavefront.
+__device__ inline int least(int v) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) v = min(v, __shfl_xor(v, i));
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// What a row ends with
+
+// The reference and the factor that its weights take.  No weight at all: 0 for a row that
+// sees no key, NaN for one whose scores are all below what 32 bits hold.
+__device__ inline float inverse(float l, int visible) {
+  return l == 0.f ? (visible ? bits_f32(0x7fc00000u) : 0.f) : 1.f / l;
+}
+__device__ inline void write_stats(const Args& a, const Row& row, float m, float l) {
+  if (a.lse)
+    a.lse[row.at * a.lse_row + row.head * a.lse_head] =
+        l == 0.f ? (row.visible ? bits_f32(0x7fc00000u) : -INFINITY)
+                 : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (a.stats)
+    a.stats[row.at * (a.heads * a.group) + row.head] = make_float2(m, inverse(l, row.visible));
+}
+// N neighbouring elements from `first` on as the output's type.
+template <class T, int N>
+__device__ inline void write_elements(const Args& a, const Row& row, int first, const float (&o)[N],
+                                      float inv) {
+  static_assert(N % 2 == 0, "");
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int j = 0; j < N; j += 2) w[j / 2] = Mat<T>::pack(o[j] * inv, o[j + 1] * inv);
+  char* const out = a.out + row.at * a.out_row + row.head * a.out_head + first * 2;
+  if constexpr (N == 2) {
+    *reinterpret_cast<uint32_t*>(out) = w[0];
+  } else if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int x = 0; x < N / 2; x += 4)
+      *reinterpret_cast<Vec4*>(out + x * 4) = Vec4{w[x], w[x + 1], w[x + 2], w[x + 3]};
+  } else {
+#pragma unroll
+    for (int x = 0; x < N / 2; x += 2)
+      *reinterpret_cast<Vec2*>(out + x * 4) = Vec2{w[x], w[x + 1]};
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: K and V go to registers as they are read, and the wavefronts of a workgroup take
+// the 32-token steps of its tile in turn.
+
+constexpr int kRows = 16;          // rows of a tile: columns of a matrix instruction
+struct FewPlan {
+  static constexpr int kStep = 32;       // tokens: two tiles of 16, k of the second product
+  static constexpr int kMinSteps = 32;   // of a workgroup, where the keys are cut
+  static constexpr int kCutSteps = 96;   // that cutting has to take off the longest sequence
+};
+constexpr int kStep = FewPlan::kStep;
+
+// The queries of 16 rows: lane (row, quad) holds elements 32 s + 8 quad .. + 7.
+template <class T, int D>
+struct Query {
+  typename Mat<T>::Op part[D / 32];
+};
+// What a lane loads of a step: of K token 16 h + (lane & 15), as of the queries; of V the
+// elements (D / 16) * (lane & 15) on of tokens 16 h + 4 quad + i.
+template <int D>
+struct Keys {
+  Vec4 part[2][D / 32];
+};
+template <int D>
+struct Values {
+  static constexpr int kWords = D / 32;
+  uint32_t part[2][4][kWords];
+};
+// A row tile's state: lane (row, quad) holds row `lane & 15`.
+template <int D>
+struct State {
+  v4f o[D / 16];   // o[j][i]: element (D / 16) * (4 quad + i) + j
+  float m, l;      // the reference; the sum of this lane's tokens
+};
+
+// A lane's row of a step: lanes 0 .. 31 K's of its tokens, 32 .. 63 V's.
+struct Rows {
+  uint32_t lo, hi;
+};
+__device__ inline uint64_t row_of_lane(const Rows& r, int lane) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(
+             __builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(r.hi)))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(r.lo)));
+}
+
+template <int D>
+__device__ inline void load_keys(const Rows& r, int lane, Keys<D>& k) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint64_t p = row_of_lane(r, 16 * h + (lane & 15)) + (lane >> 4) * 16;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) k.part[h][s] = load<Vec4>(p + 64 * s);
+  }
+}
+// D / 16 elements of a row
+template <int D>
+__device__ inline void load_part(uint64_t p, uint32_t (&x)[D / 32]) {
+  if constexpr (D == 64) {
+    const Vec2 u = load<Vec2>(p);
+    x[0] = u[0], x[1] = u[1];
+  } else {
+#pragma unroll
+    for (int w = 0; w < D / 32; w += 4) {
+      const Vec4 u = load<Vec4>(p + 4 * w);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[w + y] = u[y];
+    }
+  }
+}
+template <int D>
+__device__ inline void load_values(const Rows& r, int lane, Values<D>& v) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      load_part<D>(row_of_lane(r, 32 + 16 * h + 4 * (lane >> 4) + i) + (lane & 15) * (D / 8),
+                   v.part[h][i]);
+}
+
+// s[h][i] = q . k of token 16 h + 4 quad + i
+template <class T, int D>
+__device__ inline void scores(const Query<T, D>& q, const Keys<D>& k, v4f (&s)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    s[h] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+      s[h] = Mat<T>::mul16(__builtin_bit_cast(typename Mat<T>::Op, k.part[h][x]), q.part[x], s[h]);
+  }
+}
+
+__device__ inline void hide(v4f (&s)[2], int at, int visible, int quad) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + 16 * h + quad * 4 + i >= visible) s[h][i] = -INFINITY;
+}
+
+// The scores as weights p; returns their sum, which is over kSlack where one of them passes
+// the reference by more than that.
+__device__ inline float weigh(const v4f (&s)[2], float m, float scale_log2, bool coarse,
+                              float (&p)[8]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const float score = s[x / 4][x % 4];
+    p[x] = __builtin_amdgcn_exp2f(coarse ? rounded_less(score, scale_log2, m)
+                                         : __builtin_fmaf(score, scale_log2, -m));
+    sum = x ? sum + p[x] : p[x];
+  }
+  return sum;
+}
+
+// Elements j and j + 1 of a lane's 8 tokens of V as operands.
+template <class T, int D>
+__device__ inline void columns(const Values<D>& v, int j, typename Mat<T>::Op& even,
+                               typename Mat<T>::Op& odd) {
+  uint32_t e[4], d[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const uint32_t lo = v.part[x / 2][2 * (x % 2)][j / 2], hi = v.part[x / 2][2 * (x % 2) + 1][j / 2];
+    e[x] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    d[x] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+  }
+  even = __builtin_bit_cast(typename Mat<T>::Op, make_uint4(e[0], e[1], e[2], e[3]));
+  odd = __builtin_bit_cast(typename Mat<T>::Op, make_uint4(d[0], d[1], d[2], d[3]));
+}
+
+template <class T, int D>
+__device__ inline bool any_not_finite(const Values<D>& v) {
+  bool any = false;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < Values<D>::kWords; ++w) any |= not_finite<T>(v.part[h][i][w]);
+  return __any(any);
+}
+
+// A step whose values hold an infinity or a NaN that some row does not see: a weight of 0 does not
+// leave it out of a matrix product, so the products are made one by one.
+template <class T, int D>
+__device__ inline void add_one_by_one(const Args& a, int seq, int head, int at, int keys,
+                                      int visible, int lane, const float (&p)[8], State<D>& st) {
+  const int quad = lane >> 4;
+#pragma unroll 1
+  for (int x = 0; x < 32; ++x) {
+    const int token = at + x;
+    if (token >= keys) break;
+    const int at_x = x / 16 * 4 + x % 4;
+    float w = p[0];
+#pragma unroll
+    for (int y = 1; y < 8; ++y) w = y == at_x ? p[y] : w;
+    w = __shfl(w, (lane & 15) + 16 * (x / 4 % 4));
+    const uint64_t row = row_address(a, a.v, block_id(a, seq, token), token, head);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t u[D / 32];
+      load_part<D>(row + (4 * quad + i) * (D / 8), u);
+      if (token >= visible) continue;
+#pragma unroll
+      for (int j = 0; j < D / 16; j += 2) {
+        st.o[j][i] += w * Mat<T>::low(u[j / 2]);
+        st.o[j + 1][i] += w * Mat<T>::high(u[j / 2]);
+      }
+    }
+  }
+}
+
+template <int D>
+__device__ inline void clear(State<D>& st) {
+  st.m = kNothing;
+  st.l = 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) st.o[j] = {0.f, 0.f, 0.f, 0.f};
+}
+
+constexpr int few_waves_a_simd(int row_tiles, int dim) { return dim == 256 ? 1 : 2; }
+
+template <class T, int D, int R, int W>
+__global__ __launch_bounds__(64 * W, few_waves_a_simd(R, D)) void attend_few_kernel(const Args a) {
+  using Op = typename Mat<T>::Op;
+  constexpr int NT = D / 16;
+  __shared__ v4f shared[W * NT][64];
+  __shared__ float sum_m[W][R][16], sum_l[W][R][16];
+  const Place at = R == 1 ? heads_together(a, blockIdx.x) : heads_apart(a, blockIdx.x);
+  const Work w = a.slots || a.starts ? find_work<FewPlan>(a, at.item, kRows * R, false)
+                                     : find_single(a, at.item, kRows * R);
+  if (a.slots && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = w.any_cut;
+  if (w.seq < 0) return;
+  const int first = w.tile * kRows * R;
+  const int rows = min(kRows * R, w.s.count * a.group - first);
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
+  auto row_at = [&](int n) { return row_of(a, w.s, first + min(n, rows - 1), at.head); };
+  const int keys = max(w.s.keys, 0);
+  int visible[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) visible[r] = row_at(16 * r + (lane & 15)).visible;
+  // of the rows, in order, the first sees the fewest, the last the most
+  const int fewest = lane_value(visible[0], 0), most = lane_value(visible[R - 1], 15);
+  const int all_steps = (most + kStep - 1) / kStep;
+  const int end = w.cuts > 1 ? min(all_steps, (w.cut + 1) * w.steps) : all_steps;
+  int step = (w.cuts > 1 ? w.cut * w.steps : 0) + wave;
+  const bool any = step < end;
+  // the block ids are asked for a step ahead of the rows, the rows a step ahead of their use; past
+  // the last key everything is of that one again
+  int bad = kNoToken;
+  const bool of_v = lane >= 32;
+  const Half half = of_v ? a.v : a.k;
+  auto token_of = [&](int s) { return min(s * kStep + (lane & 31), keys - 1); };
+  auto find = [&](int s, int64_t id) {
+    const int t = token_of(s);
+    if (outside(a, id)) bad = min(bad, t);
+    const uint64_t p = row_address(a, half, id, t, at.head);
+    return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
+  };
+  Keys<D> k;
+  Values<D> v;
+  int64_t ids = 0;
+  if (any) {
+    ids = block_id(a, w.seq, token_of(step));
+    const Rows next = find(step, ids);
+    ids = block_id(a, w.seq, token_of(step + W));
+    load_keys<D>(next, lane, k);
+    load_values<D>(next, lane, v);
+  }
+  Query<T, D> q[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const Row row = row_at(16 * r + (lane & 15));
+    const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + quad * 16;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+      q[r].part[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 64 * x));
+  }
+  const float scale_log2 = score_scale(a.scale_log2);
+  const bool negate = a.scale_log2 < 0.f;
+  float slack = kSlack;
+  State<D> st[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) clear(st[r]);
+  for (; step < end; step += W) {
+    const Rows next = find(step + W, ids);
+    ids = block_id(a, w.seq, token_of(step + 2 * W));
+    const int token = step * kStep;
+    v4f s[R][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r) scores(q[r], k, s[r]);
+    load_keys<D>(next, lane, k);
+    float p[R][8], l[R];
+    bool passes = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (negate) s[r][0] = -s[r][0], s[r][1] = -s[r][1];
+      if (token + kStep > fewest) hide(s[r], token, visible[r], quad);
+      l[r] = weigh(s[r], st[r].m, scale_log2, false, p[r]);
+      passes |= l[r] > slack;
+    }
+    if (__any(passes)) {
+      // Some score passes its row's reference: the references follow, and the weights are made
+      // again; at every step from then on, where a reference is kCoarse or more.
+      bool any_coarse = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float top = st[r].m;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) top = fmaxf(top, s[r][x / 4][x % 4] * scale_log2);
+        const float m = max_over_quads(top);
+        const float fade = __builtin_amdgcn_exp2f(st[r].m - m);
+        st[r].m = m;
+        st[r].l *= fade;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
+        const bool coarse = fabsf(m) >= kCoarse && m != kNothing;
+        any_coarse |= coarse;
+        l[r] = weigh(s[r], m, scale_log2, coarse, p[r]);
+      }
+      slack = __any(any_coarse) ? -1.f : kSlack;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) st[r].l += l[r];
+    if (token + kStep > fewest && any_not_finite<T, D>(v)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        add_one_by_one<T, D>(a, w.seq, at.head, token, keys, visible[r], lane, p[r], st[r]);
+    } else {
+      Op weight[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        weight[r] = __builtin_bit_cast(
+            Op, make_uint4(Mat<T>::pack(p[r][0], p[r][1]), Mat<T>::pack(p[r][2], p[r][3]),
+                           Mat<T>::pack(p[r][4], p[r][5]), Mat<T>::pack(p[r][6], p[r][7])));
+#pragma unroll
+      for (int j = 0; j < NT; j += 2) {
+        Op even, odd;
+        columns<T, D>(v, j, even, odd);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          st[r].o[j] = Mat<T>::mul16(even, weight[r], st[r].o[j]);
+          st[r].o[j + 1] = Mat<T>::mul16(odd, weight[r], st[r].o[j + 1]);
+        }
+      }
+    }
+    load_values<D>(next, lane, v);
+  }
+  bad = least(bad);
+  // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
+  // each) adds up the elements [][i] of all.
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float l = sum_over_quads(st[r].l);
+    if (quad == 0) {
+      sum_m[wave][r][lane] = st[r].m;
+      const bool lost = w.s.keys < 0 || visible[r] > bad;
+      sum_l[wave][r][lane] = lost ? bits_f32(0x7fc00000u) : l;
+    }
+  }
+  __syncthreads();
+  constexpr int kParts = W >= 8 ? 2 : 1, NJ = NT / kParts;
+  const int i = wave & 3, j0 = wave / 4 * NJ;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float m = kNothing, l = 0.f;
+#pragma unroll
+    for (int x = 0; x < W; ++x) m = fmaxf(m, sum_m[x][r][lane & 15]);
+#pragma unroll
+    for (int x = 0; x < W; ++x)
+      l += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - m);
+    const float f = __builtin_amdgcn_exp2f(st[r].m - m);
+    if (r) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; ++j) shared[wave * NT + j][lane] = st[r].o[j] * f;
+    __syncthreads();
+    if (wave >= 4 * kParts) continue;
+    float sums[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      sums[j] = 0.f;
+#pragma unroll
+      for (int x = 0; x < W; ++x)
+        sums[j] += reinterpret_cast<const float*>(shared[x * NT + j0 + j])[lane * 4 + i];
+    }
+    const int n = 16 * r + (lane & 15), element = NT * (4 * quad + i) + j0;
+    if (n >= rows) continue;
+    if (w.cuts == 1) {
+      const Row row = row_at(n);
+      write_elements<T, NJ>(a, row, element, sums, inverse(l, visible[r]));
+      if (wave == 0 && quad == 0) write_stats(a, row, m, l);
+    } else {
+      const int64_t part = (part_of(a, at.item, at.head) * R + r) * kRows + (lane & 15);
+      if (wave == 0 && quad == 0) a.part_ml[part] = make_float2(m, l);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) a.part_o[part * D + element + j] = sums[j];
+    }
+  }
+}
+
+// Joins the cuts of 16 rows of a tile of ROWS: 256 threads, each D / 16 neighbouring elements of a row,
+// take every G-th cut, and their sums are added in the order of g.
+template <class T, int D, int ROWS, class P, int G>
+__global__ __launch_bounds__(256 * G) void join_kernel(const Args a) {
+  constexpr int N = D / 16, kAhead = D == 256 ? 2 : 4;
+  if (!*a.any_cut) return;
+  const int t = threadIdx.x & 255, g = threadIdx.x >> 8, n = t >> 4;
+  const int block = blockIdx.x / (ROWS / 16), r = blockIdx.x % (ROWS / 16);
+  const int tile = a.heads_div.div(block);
+  const int head = block - tile * a.heads;
+  const Work w = find_work<P>(a, tile, ROWS, true);
+  if (w.seq < 0 || w.cuts == 1) return;
+  __shared__ float sum_o[G][N][256], sum_m[G][16], sum_l[G][16];
+  const int first = w.tile * ROWS + 16 * r;
+  const bool valid = first + n < w.s.count * a.group;
+  float o[N], m = kNothing, l = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) o[j] = 0.f;
+  if (valid) {
+    const int64_t part = part_of(a, w.first, head) * ROWS + 16 * r + n;
+    const int64_t next = static_cast<int64_t>(a.heads) * ROWS;
+    for (int c0 = g; c0 < w.cuts; c0 += G * kAhead) {
+      float2 x[kAhead];
+      v4f y[kAhead][N / 4];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int c = c0 + i * G;
+        x[i] = make_float2(kNothing, 0.f);
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j) y[i][j] = {0.f, 0.f, 0.f, 0.f};
+        if (c < w.cuts) {
+          x[i] = a.part_ml[part + c * next];
+#pragma unroll
+          for (int j = 0; j < N / 4; ++j)
+            y[i][j] = reinterpret_cast<const v4f*>(a.part_o + (part + c * next) * D + (t & 15) * N)[j];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float top = fmaxf(m, x[i].x);
+        const float f = __builtin_amdgcn_exp2f(m - top), h = __builtin_amdgcn_exp2f(x[i].x - top);
+        m = top;
+        l = l * f + x[i].y * h;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = o[j] * f + y[i][j / 4][j % 4] * h;
+      }
+    }
+  }
+  if ((t & 15) == 0) sum_m[g][n] = m, sum_l[g][n] = l;
+#pragma unroll
+  for (int j = 0; j < N; ++j) sum_o[g][j][t] = o[j];
+  __syncthreads();
+  if (g || !valid) return;
+  float top = kNothing;
+#pragma unroll
+  for (int x = 0; x < G; ++x) top = fmaxf(top, sum_m[x][n]);
+  l = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) o[j] = 0.f;
+#pragma unroll
+  for (int x = 0; x < G; ++x) {
+    const float f = __builtin_amdgcn_exp2f(sum_m[x][n] - top);
+    l += sum_l[x][n] * f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] += sum_o[x][j][t] * f;
+  }
+  const Row row = row_of(a, w.s, first + n, head);
+  write_elements<T, N>(a, row, (t & 15) * N, o, inverse(l, row.visible));
+  if ((t & 15) == 0) write_stats(a, row, top, l);
+}
+
+// ---------------------------------------------------------------------------
+// What each token got: a wavefront keeps 64 tokens of K in registers and goes over the
+// queries, 32 rows at a time.  A token's sum is made by one wavefront, in the rows' order.
+
+constexpr int kWeighTokens = 256;    // of a workgroup
+
+template <class T, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args a) {
+  using Op = typename Mat<T>::Op;
+  constexpr int KS = D / 16;
+  const int head = blockIdx.y, seq = blockIdx.z;
+  const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
+  const int at = blockIdx.x * kWeighTokens + uniform(threadIdx.x >> 6) * 64;
+  const Seq s = sequence(a, seq);
+  // too long for its table row: NaN in all rows, and in the tokens of no block
+  const int keys = max(s.keys, 0), rows = s.count * a.group;
+  if (at >= keys || rows <= 0) return;
+  Op k[2][KS];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t = min(at + 32 * h + column, keys - 1);
+    const uint64_t p = row_address(a, a.k, block_id(a, seq, t), t, head) + half * 16;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) k[h][x] = __builtin_bit_cast(Op, load<Vec4>(p + 32 * x));
+  }
+  const float scale_log2 = score_scale(a.scale_log2);
+  const bool negate = a.scale_log2 < 0.f;
+  v16f sums[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sums[h][i] = 0.f;
+  // the first row that sees the first of the tokens
+  const int hidden = a.causal ? max(0, at + s.count - keys) * a.group : 0;
+  for (int r0 = hidden & ~31; r0 < rows; r0 += 32) {
+    const int n = min(r0 + column, rows - 1);
+    const Row row = row_of(a, s, n, head);
+    const int visible = r0 + column < rows ? row.visible : 0;
+    const float2 st = a.stats[row.at * (a.heads * a.group) + row.head];
+    const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + half * 16;
+    v16f acc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[h][i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      const Op q = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 32 * x));
+      acc[0] = Mat<T>::mul32(k[0][x], q, acc[0]);
+      acc[1] = Mat<T>::mul32(k[1][x], q, acc[1]);
+    }
+    const bool coarse = fabsf(st.x) >= kCoarse;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = at + 32 * h + 8 * (i / 4) + 4 * half + i % 4;
+        const float score = negate ? -acc[h][i] : acc[h][i];
+        const float e = __builtin_amdgcn_exp2f(coarse ? rounded_less(score, scale_log2, st.x)
+                                                      : __builtin_fmaf(score, scale_log2, -st.x));
+        if (t < visible) sums[h][i] += e * st.y;
+      }
+  }
+  // over the 32 rows of a half wavefront; lane `column` then has token 8 (column / 4 % 4) + 4 half
+  // + column % 4 of its h = column / 16
+  float mine = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float x = sums[h][i];
+#pragma unroll
+      for (int y = 1; y < 32; y *= 2) x += __shfl_xor(x, y);
+      if (column == 16 * h + i) mine = x;
+    }
+  const int i = column & 15;
+  const int t = at + 32 * (column >> 4) + 8 * (i / 4) + 4 * half + i % 4;
+  if (t < keys) a.weights[seq * a.w_seq + head * a.w_head + t] += mine;
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+
+int check_sizes(const fkv_paged_attention_args& c) {
+  int rc;
+  const fkv_paged_layer& layer = c.layer;
+  if (c.batch < 0 || c.num_queries < 0)
+    return fail(kInval, "negative count: batch=%d num_queries=%d", c.batch, c.num_queries);
+  if ((rc = paged_check_sizes(layer))) return rc;
+  if (layer.head_size != 64 && layer.head_size != 128 && layer.head_size != 256)
+    return fail(kInval, "attention takes a head_size of 64, 128 or 256, got %d", layer.head_size);
+  if (layer.dtype != FKV_DTYPE_BF16 && layer.dtype != FKV_DTYPE_FP16)
+    return fail(kInval, "attention takes a bf16 or fp16 cache, got dtype %d", layer.dtype);
+  if (c.group_size < 1 || c.group_size > 1024)
+    return fail(kInval, "group_size must be in [1, 1024], got %d", c.group_size);
+  if (!std::isfinite(c.scale)) return fail(kInval, "scale must be finite");
+  const int64_t most = static_cast<int64_t>(c.table_width) * layer.tokens_per_block;
+  if (c.table_width < 0 || most > int64_t(1) << 28)
+    return fail(kInval, "table_width must be non-negative and hold at most 2^28 tokens, got %d "
+                "blocks of %d", c.table_width, layer.tokens_per_block);
+  if (static_cast<int64_t>(c.num_queries) * c.group_size >= int64_t(1) << 30)
+    return fail(kInval, "%d queries of %d heads a K/V head are too many for one call",
+                c.num_queries, c.group_size);
+  if (!c.query_starts && c.num_queries < c.batch && c.num_queries > 0)
+    return fail(kInval, "%d sequences of one query each, but %d queries", c.batch, c.num_queries);
+  if (c.weights && c.weights_width < most)
+    return fail(kInval, "weights' rows of %d do not hold the %lld tokens of a row of block_table",
+                c.weights_width, (long long)most);
+  if (c.weights && c.batch > 65535)
+    return fail(kInval, "%d sequences with weights are too many for one call", c.batch);
+  return 0;
+}
+
+int check_attention(const fkv_paged_attention_args& c) {
+  if (!c.query || !c.out || !c.seq_lens || (!c.block_table && c.table_width > 0))
+    return fail(kInval, "null pointer argument");
+  if (!c.layer.value) return fail(kInval, "null cache pointer");
+  const int64_t aligned[] = {c.query_row_stride_bytes, c.query_head_stride_bytes,
+                             c.out_row_stride_bytes, c.out_head_stride_bytes,
+                             static_cast<int64_t>(reinterpret_cast<uintptr_t>(c.query)),
+                             static_cast<int64_t>(reinterpret_cast<uintptr_t>(c.out))};
+  for (int64_t v : aligned)
+    if (v % 16)
+      return fail(kInval, "query's and out's pointers and strides must be multiples of 16 bytes");
+  return paged_check_layer(c.layer);
+}
+
+struct LaunchPlan {
+  int row_tiles;          // R
+  int64_t tiles;          // times heads: the most there can be
+  bool wide;              // few tiles: more wavefronts a workgroup
+  int slots;
+  int64_t workgroups;
+  size_t ml_bytes, o_bytes, stats_bytes;
+};
+
+constexpr int kComputeUnits = 256;
+
+LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
+  LaunchPlan p;
+  const int heads = c.layer.num_heads, dim = c.layer.head_size;
+  const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
+  auto tiles = [&](int row_tiles) {
+    const int n = kRows * row_tiles;
+    return (c.query_starts ? rows / n + c.batch
+                           : static_cast<int64_t>(c.batch) * ((c.group_size + n - 1) / n)) *
+           heads;
+  };
+  const int64_t most_steps =
+      (static_cast<int64_t>(c.table_width) * c.layer.tokens_per_block + kStep - 1) / kStep;
+  p.row_tiles = rows > static_cast<int64_t>(c.batch) * kRows ? 2 : 1;
+  p.tiles = tiles(p.row_tiles);
+  p.wide = p.row_tiles == 1 && p.tiles <= kComputeUnits && dim <= 128;
+  p.slots = most_steps < FewPlan::kMinSteps + FewPlan::kCutSteps || p.tiles > 4 * kComputeUnits ||
+                    p.row_tiles > 1
+                ? 0
+            : p.wide ? kComputeUnits : static_cast<int>(p.tiles);
+  // items (cuts of a tile, of all heads), in whole rounds of the XCDs
+  const int64_t items = (p.tiles + p.slots + heads - 1) / heads;
+  p.workgroups = (items + kXcds - 1) / kXcds * kXcds * heads;
+  const int64_t part_rows = p.slots ? p.workgroups * kRows * p.row_tiles : 0;
+  p.ml_bytes = part_rows * sizeof(float2) + (p.slots ? 16 : 0);    // and any_cut
+  p.o_bytes = part_rows * dim * sizeof(float);
+  p.stats_bytes =
+      c.weights ? static_cast<size_t>(c.num_queries) * heads * c.group_size * sizeof(float2) : 0;
+  return p;
+}
+
+// A launch has less than 2^32 threads.
+int check_plan(const fkv_paged_attention_args& c, const LaunchPlan& p) {
+  const int64_t weigh = static_cast<int64_t>(c.table_width) * c.layer.tokens_per_block /
+                            kWeighTokens * c.layer.num_heads * c.batch;
+  if (p.workgroups >= int64_t(1) << 22 || (c.weights && weigh >= int64_t(1) << 23))
+    return fail(kInval, "%d queries of %d K/V heads are too many for one call", c.num_queries,
+                c.layer.num_heads);
+  return 0;
+}
+
+template <class T, int D, int R, int W>
+void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
+  hipLaunchKernelGGL((attend_few_kernel<T, D, R, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
+  if (p.slots)
+    hipLaunchKernelGGL((join_kernel<T, D, kRows * R, FewPlan, W == 8 ? 4 : 1>), dim3(p.tiles * R),
+                       dim3(256 * (W == 8 ? 4 : 1)), 0, s, a);
+}
+template <class T, int D>
+void launch(const Args& a, const LaunchPlan& p, const fkv_paged_attention_args& c, hipStream_t s) {
+  if (p.row_tiles == 2) launch<T, D, 2, 4>(a, p, s);
+  else if (p.wide) launch<T, D, 1, D == 256 ? 4 : 8>(a, p, s);
+  else launch<T, D, 1, 4>(a, p, s);
+  if (a.weights && a.width) {
+    const int64_t most = static_cast<int64_t>(a.width) * a.tokens;
+    hipLaunchKernelGGL((weigh_kernel<T, D>),
+                       dim3((most + kWeighTokens - 1) / kWeighTokens, a.heads, a.batch), dim3(256),
+                       0, s, a);
+  }
+}
+template <class T>
+void launch_attention(const Args& a, const LaunchPlan& p, const fkv_paged_attention_args& c,
+                      hipStream_t s) {
+  if (c.layer.head_size == 64) launch<T, 64>(a, p, c, s);
+  else if (c.layer.head_size == 128) launch<T, 128>(a, p, c, s);
+  else launch<T, 256>(a, p, c, s);
+}
+
+int attention(const fkv_paged_attention_args& c, fkv_stream_t stream) {
+  int rc = check_sizes(c);
+  if (rc || c.batch == 0 || c.num_queries == 0) return rc;
+  if ((rc = check_attention(c))) return rc;
+  const LaunchPlan p = launch_plan(c);
+  if ((rc = check_plan(c, p))) return rc;
+  const size_t need = p.o_bytes + p.ml_bytes + p.stats_bytes;
+  if (need && (!c.workspace || c.workspace_bytes < need ||
+               reinterpret_cast<uintptr_t>(c.workspace) % 16))
+    return fail(kInval, "the workspace must hold %zu bytes on a multiple of 16, got %zu", need,
+                c.workspace ? c.workspace_bytes : 0);
+  Args a{};
+  a.q = static_cast<const char*>(c.query);
+  a.out = static_cast<char*>(c.out);
+  a.lse = c.lse;
+  a.q_row = c.query_row_stride_bytes, a.q_head = c.query_head_stride_bytes;
+  a.out_row = c.out_row_stride_bytes, a.out_head = c.out_head_stride_bytes;
+  a.lse_row = c.lse_row_stride, a.lse_head = c.lse_head_stride;
+  a.k = key_half(c.layer), a.v = value_half(c.layer);
+  a.table = c.block_table, a.lens = c.seq_lens, a.starts = c.query_starts;
+  a.table_row = c.table_row_stride;
+  a.index64 = c.index_is_64bit;
+  a.num_blocks = static_cast<int>(c.layer.num_blocks), a.width = c.table_width;
+  a.batch = c.batch, a.heads = c.layer.num_heads, a.group = c.group_size;
+  a.queries = c.num_queries;
+  a.tokens = c.layer.tokens_per_block, a.causal = c.causal;
+  a.slots = p.slots;
+  a.scale_log2 = c.scale * kLog2e;
+  char* const space = static_cast<char*>(c.workspace);
+  a.part_o = reinterpret_cast<float*>(space);
+  a.any_cut = reinterpret_cast<int*>(space + p.o_bytes);
+  a.part_ml = reinterpret_cast<float2*>(space + p.o_bytes + 16);
+  a.weights = c.weights, a.w_seq = c.weights_seq_stride, a.w_head = c.weights_head_stride;
+  a.stats = c.weights ? reinterpret_cast<float2*>(space + p.o_bytes + p.ml_bytes) : nullptr;
+  a.tokens_div = FastDiv(a.tokens), a.group_div = FastDiv(a.group), a.heads_div = FastDiv(a.heads);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  int dev = 0;
+  DeviceGuard guard;
+  if ((rc = stream_device(s, &dev)) || (rc = guard.set(dev))) return rc;
+  (void)hipGetLastError();
+  if (c.layer.dtype == FKV_DTYPE_BF16) launch_attention<__bf16>(a, p, c, s);
+  else launch_attention<_Float16>(a, p, c, s);
+  FKV_HIP(hipGetLastError());
+  return 0;
+}
+
+// No C++ exception leaves a C entry.
+template <class F>
+int guarded(F call) {
+  try {
+    last_error().clear();
+    return call();
+  } catch (const std::exception& e) {
+    return fail(static_cast<int>(hipErrorUnknown), "exception: %s", e.what());
+  } catch (...) {
+    return fail(static_cast<int>(hipErrorUnknown), "unknown exception");
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int fkv_paged_attention_workspace(const fkv_paged_attention_args* args, size_t* bytes) {
+  return guarded([&] {
+    if (!args || !bytes) return fail(kInval, "null pointer argument");
+    *bytes = 0;
+    int rc = check_sizes(*args);
+    if (rc || args->batch == 0 || args->num_queries == 0) return rc;
+    const LaunchPlan p = launch_plan(*args);
+    if ((rc = check_plan(*args, p))) return rc;
+    *bytes = p.o_bytes + p.ml_bytes + p.stats_bytes;
+    return 0;
+  });
+}
+
+int fkv_paged_attention(const fkv_paged_attention_args* args, fkv_stream_t stream) {
+  return guarded([&] {
+    if (!args) return fail(kInval, "null pointer argument");
+    return attention(*args, stream);
+  });
+}
+
+}  // extern "C"

@@ -1,5 +1,5 @@
 // _fkv_py: the per-call path of flexkv_amd.c_ext.transfer_kv_blocks,
-// transfer_kv_blocks_kv_ptrs and the functions on a 4-bit cache as a CPython
+// transfer_kv_blocks_kv_ptrs and the functions on a 4-bit and on a paged cache as a CPython
 // extension (vectorcall, no argument tuple).  It unpacks the torch tensors in C++,
 // checks them, takes the current torch stream and calls the C-ABI entry with the GIL
 // released, the work that csrc/bindings.cpp:25-55 does for the reference through
@@ -421,10 +421,218 @@ PyObject* mx4_attention_of(PyObject* const* a) {
   return THPVariable_Wrap(out);
 }
 
+// The functions on a paged cache, with the same convention.
+decltype(&fkv_write_kv_tokens) g_write_tokens = nullptr;
+decltype(&fkv_paged_attention_workspace) g_paged_workspace = nullptr;
+decltype(&fkv_paged_attention) g_paged_attention = nullptr;
+decltype(&fkv_evict_kv_tokens) g_evict = nullptr;
+
+// bytes from one to the next in a dimension; one alone has none
+int64_t step_of(const at::Tensor& t, int64_t d) {
+  return t.size(d) > 1 ? t.stride(d) * static_cast<int64_t>(t.element_size()) : 0;
+}
+
+// key_cache and value_cache (may be null) as one layer
+bool layer_of(const at::Tensor& k, const at::Tensor* v, fkv_paged_layer* out) {
+  const int dtype = dtype_code(k.scalar_type());
+  if (dtype < 0 || k.dim() != 4 || k.stride(3) != 1 || k.size(1) > INT_MAX ||
+      k.size(2) > INT_MAX || k.size(3) > INT_MAX)
+    return false;
+  if (v && (v->sizes() != k.sizes() || v->scalar_type() != k.scalar_type() || v->stride(3) != 1))
+    return false;
+  out->key = k.data_ptr(), out->value = v ? v->data_ptr() : nullptr;
+  out->key_block_stride_bytes = step_of(k, 0), out->key_token_stride_bytes = step_of(k, 1);
+  out->key_head_stride_bytes = step_of(k, 2);
+  out->value_block_stride_bytes = v ? step_of(*v, 0) : 0;
+  out->value_token_stride_bytes = v ? step_of(*v, 1) : 0;
+  out->value_head_stride_bytes = v ? step_of(*v, 2) : 0;
+  out->num_blocks = k.size(0), out->tokens_per_block = static_cast<int>(k.size(1));
+  out->num_heads = static_cast<int>(k.size(2)), out->head_size = static_cast<int>(k.size(3));
+  out->dtype = dtype;
+  return true;
+}
+
+bool index_vector(const at::Tensor& t, int64_t n) {
+  return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.dim() == 1 &&
+         t.is_contiguous() && t.size(0) == n && n <= INT_MAX;
+}
+
+bool index_table(const at::Tensor& t, int64_t batch, at::ScalarType index) {
+  return t.scalar_type() == index && t.dim() == 2 && t.size(0) == batch && t.size(1) <= INT_MAX &&
+         (t.size(1) <= 1 || t.stride(1) == 1);
+}
+
+bool weights_of(const at::Tensor& t, int64_t batch, int64_t heads, int64_t width) {
+  return t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == batch &&
+         t.size(1) == heads && t.size(2) >= width && t.size(2) <= INT_MAX &&
+         (t.size(2) <= 1 || t.stride(2) == 1);
+}
+
+// (key, value, key_cache, value_cache, slots)
+PyObject* write_kv_tokens_of(PyObject* const* a) {
+  const at::Tensor *key, *value = nullptr, *kc, *vc = nullptr, *slots;
+  if (!here(a[0], &key) || (a[1] != Py_None && !here(a[1], &value)) || !here(a[2], &kc) ||
+      (a[3] != Py_None && !here(a[3], &vc)) || !here(a[4], &slots) || !value != !vc)
+    Py_RETURN_FALSE;
+  fkv_paged_layer layer{};
+  if (!layer_of(*kc, vc, &layer) || key->dim() != 3) Py_RETURN_FALSE;
+  const int64_t n = key->size(0);
+  for (const at::Tensor* x : {key, value})
+    if (x && (x->dim() != 3 || x->size(0) != n || x->size(1) != kc->size(2) ||
+              x->size(2) != kc->size(3) || x->scalar_type() != kc->scalar_type() ||
+              x->stride(2) != 1))
+      Py_RETURN_FALSE;
+  if (!index_vector(*slots, n)) Py_RETURN_FALSE;
+  void* stream = c10::hip::getCurrentHIPStream().stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_write_tokens(&layer, static_cast<int>(n), key->data_ptr(), step_of(*key, 0),
+                      step_of(*key, 1), value ? value->data_ptr() : nullptr,
+                      value ? step_of(*value, 0) : 0, value ? step_of(*value, 1) : 0,
+                      slots->data_ptr(), slots->scalar_type() == at::kLong, stream);
+  Py_END_ALLOW_THREADS
+  return finish(rc);
+}
+
+// (query, key_cache, value_cache, block_table, seq_lens, query_starts, scale, causal, out, lse,
+//  weights)
+PyObject* paged_attention_of(PyObject* const* a) {
+  const at::Tensor *query, *kc, *vc, *table, *lens, *starts = nullptr, *given = nullptr,
+                   *lse = nullptr, *weights = nullptr;
+  if (!here(a[0], &query) || !here(a[1], &kc) || !here(a[2], &vc) || !here(a[3], &table) ||
+      !here(a[4], &lens) || (a[5] != Py_None && !here(a[5], &starts)) ||
+      (a[6] != Py_None && !PyFloat_Check(a[6])) || (a[8] != Py_None && !here(a[8], &given)) ||
+      (a[9] != Py_None && !here(a[9], &lse)) || (a[10] != Py_None && !here(a[10], &weights)))
+    Py_RETURN_FALSE;
+  int causal;
+  if (!as_flag(a[7], &causal)) return nullptr;
+  fkv_paged_attention_args c{};
+  const at::ScalarType type = query->scalar_type();
+  if ((type != at::kBFloat16 && type != at::kHalf) || query->dim() != 3 || query->stride(2) != 1 ||
+      !layer_of(*kc, vc, &c.layer) || kc->scalar_type() != type)
+    Py_RETURN_FALSE;
+  const int64_t rows = query->size(0), heads = query->size(1), dim = query->size(2);
+  const int64_t kv_heads = kc->size(2);
+  if (kc->size(3) != dim || kv_heads < 1 || heads < 1 || heads % kv_heads || rows > INT_MAX ||
+      lens->dim() != 1)
+    Py_RETURN_FALSE;
+  const int64_t batch = lens->size(0);
+  const at::ScalarType index = lens->scalar_type();
+  if (!index_vector(*lens, batch) || !index_table(*table, batch, index) ||
+      (starts ? starts->scalar_type() != index || !index_vector(*starts, batch + 1)
+              : rows < batch))
+    Py_RETURN_FALSE;
+  if (given && (given->sizes() != query->sizes() || given->scalar_type() != type ||
+                given->stride(2) != 1 || ranges_meet(*given, *query)))
+    Py_RETURN_FALSE;
+  if (lse && (lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != heads ||
+              lse->scalar_type() != at::kFloat))
+    Py_RETURN_FALSE;
+  if (weights && !weights_of(*weights, batch, kv_heads, table->size(1) * kc->size(1)))
+    Py_RETURN_FALSE;
+  const at::Tensor out = given ? *given : at::empty({rows, heads, dim}, query->options());
+  c.query = query->data_ptr(), c.out = out.data_ptr();
+  c.lse = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+  c.query_row_stride_bytes = step_of(*query, 0), c.query_head_stride_bytes = step_of(*query, 1);
+  c.out_row_stride_bytes = step_of(out, 0), c.out_head_stride_bytes = step_of(out, 1);
+  c.lse_row_stride = lse ? lse->stride(0) : 0, c.lse_head_stride = lse ? lse->stride(1) : 0;
+  c.weights = weights ? static_cast<float*>(weights->data_ptr()) : nullptr;
+  c.weights_seq_stride = weights ? weights->stride(0) : 0;
+  c.weights_head_stride = weights ? weights->stride(1) : 0;
+  c.weights_width = weights ? static_cast<int>(weights->size(2)) : 0;
+  c.block_table = table->data_ptr(), c.seq_lens = lens->data_ptr();
+  c.query_starts = starts ? starts->data_ptr() : nullptr;
+  c.table_row_stride = table->stride(0);
+  c.index_is_64bit = index == at::kLong;
+  c.table_width = static_cast<int>(table->size(1));
+  c.batch = static_cast<int>(batch), c.num_queries = static_cast<int>(rows);
+  c.group_size = static_cast<int>(heads / kv_heads), c.causal = causal;
+  c.scale = static_cast<float>(a[6] == Py_None ? 1.0 / std::sqrt(static_cast<double>(dim))
+                                               : PyFloat_AS_DOUBLE(a[6]));
+  size_t need = 0;
+  int rc = g_paged_workspace(&c, &need);
+  at::Tensor workspace;
+  if (!rc && need) {
+    // the allocator orders its reuse on the current stream
+    workspace = at::empty({static_cast<int64_t>(need)}, query->options().dtype(at::kByte));
+    c.workspace = workspace.data_ptr(), c.workspace_bytes = need;
+  }
+  if (!rc) {
+    void* stream = c10::hip::getCurrentHIPStream().stream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_paged_attention(&c, stream);
+    Py_END_ALLOW_THREADS
+  }
+  PyObject* done = finish(rc);
+  if (!done) return nullptr;
+  Py_DECREF(done);
+  return THPVariable_Wrap(out);
+}
+
+// (key_cache, value_cache, weights, block_table, seq_lens, new_table, budget, recent,
+//  new_weights, kept)
+PyObject* evict_kv_tokens_of(PyObject* const* a) {
+  const at::Tensor *kc, *vc = nullptr, *weights, *table, *lens, *into, *nw = nullptr,
+                   *given = nullptr;
+  if (!here(a[0], &kc) || (a[1] != Py_None && !here(a[1], &vc)) || !here(a[2], &weights) ||
+      !here(a[3], &table) || !here(a[4], &lens) || !here(a[5], &into) || !PyLong_Check(a[6]) ||
+      !PyLong_Check(a[7]) || (a[8] != Py_None && !here(a[8], &nw)) ||
+      (a[9] != Py_None && !here(a[9], &given)))
+    Py_RETURN_FALSE;
+  int budget, recent;
+  if (!as_int(a[6], &budget) || !as_int(a[7], &recent)) return nullptr;
+  fkv_evict_args c{};
+  if (!layer_of(*kc, vc, &c.layer) || lens->dim() != 1 || budget < 1 || recent < 0 ||
+      recent > budget)
+    Py_RETURN_FALSE;
+  const int64_t batch = lens->size(0), heads = kc->size(2);
+  const at::ScalarType index = lens->scalar_type();
+  if (!index_vector(*lens, batch) || !index_table(*table, batch, index) ||
+      !index_table(*into, batch, index))
+    Py_RETURN_FALSE;
+  const int64_t most = table->size(1) * kc->size(1);
+  if (!weights_of(*weights, batch, heads, most)) Py_RETURN_FALSE;
+  if (nw) {
+    if (!weights_of(*nw, batch, heads, budget < most ? budget : most)) Py_RETURN_FALSE;
+    const bool same = nw->data_ptr() == weights->data_ptr() && nw->strides() == weights->strides();
+    if (!same && ranges_meet(*nw, *weights)) Py_RETURN_FALSE;
+  }
+  if (given && (given->dim() != 3 || given->size(0) != batch || given->size(1) != heads ||
+                given->size(2) != budget || given->scalar_type() != at::kInt ||
+                !given->is_contiguous()))
+    Py_RETURN_FALSE;
+  const at::Tensor kept =
+      given ? *given : at::empty({batch, heads, budget}, lens->options().dtype(at::kInt));
+  c.weights = static_cast<const float*>(weights->data_ptr());
+  c.weights_seq_stride = weights->stride(0), c.weights_head_stride = weights->stride(1);
+  c.weights_width = static_cast<int>(weights->size(2));
+  if (nw) {
+    c.new_weights = static_cast<float*>(nw->data_ptr());
+    c.new_weights_seq_stride = nw->stride(0), c.new_weights_head_stride = nw->stride(1);
+    c.new_weights_width = static_cast<int>(nw->size(2));
+  }
+  c.block_table = table->data_ptr(), c.new_table = into->data_ptr(), c.seq_lens = lens->data_ptr();
+  c.table_row_stride = table->stride(0), c.new_table_row_stride = into->stride(0);
+  c.kept = static_cast<int32_t*>(kept.data_ptr());
+  c.index_is_64bit = index == at::kLong;
+  c.table_width = static_cast<int>(table->size(1));
+  c.new_table_width = static_cast<int>(into->size(1));
+  c.batch = static_cast<int>(batch), c.budget = budget, c.recent = recent;
+  void* stream = c10::hip::getCurrentHIPStream().stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_evict(&c, stream);
+  Py_END_ALLOW_THREADS
+  PyObject* done = finish(rc);
+  if (!done) return nullptr;
+  Py_DECREF(done);
+  return THPVariable_Wrap(kept);
+}
+
 // torch's errors (an allocation that fails, a tensor without strides) as Python's
 template <PyObject* (*call)(PyObject* const*)>
 PyObject* checked(const char* name, PyObject* const* a, Py_ssize_t n, Py_ssize_t takes) {
-  if (!g_attention) return not_bound();
+  if (!g_attention || !g_paged_attention) return not_bound();
   if (n != takes) {
     PyErr_Format(PyExc_TypeError, "%s takes %zd arguments (%zd given)", name, takes, n);
     return nullptr;
@@ -450,6 +658,37 @@ PyObject* mx4_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 PyObject* mx4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return checked<mx4_attention_of>("mx4_attention", a, n, 10);
+}
+
+PyObject* write_kv_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return checked<write_kv_tokens_of>("write_kv_tokens", a, n, 5);
+}
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return checked<paged_attention_of>("paged_attention", a, n, 11);
+}
+PyObject* evict_kv_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return checked<evict_kv_tokens_of>("evict_kv_tokens", a, n, 10);
+}
+
+// bind_paged(write_kv_tokens, paged_attention_workspace, paged_attention, evict_kv_tokens)
+PyObject* bind_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "bind_paged takes 4 arguments");
+    return nullptr;
+  }
+  void* f[4];
+  for (int i = 0; i < 4; ++i) {
+    f[i] = PyLong_AsVoidPtr(a[i]);
+    if (!f[i]) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null function address");
+      return nullptr;
+    }
+  }
+  g_write_tokens = reinterpret_cast<decltype(g_write_tokens)>(f[0]);
+  g_paged_workspace = reinterpret_cast<decltype(g_paged_workspace)>(f[1]);
+  g_paged_attention = reinterpret_cast<decltype(g_paged_attention)>(f[2]);
+  g_evict = reinterpret_cast<decltype(g_evict)>(f[3]);
+  Py_RETURN_NONE;
 }
 
 // bind_mx4(quantize_blocks, dequantize_blocks, quantize_tokens, attention_workspace,
@@ -513,6 +752,17 @@ PyMethodDef kMethods[] = {
      METH_FASTCALL, "Per-call path of c_ext.quantize_kv_tokens (4 positional)."},
     {"mx4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&mx4_attention)),
      METH_FASTCALL, "Per-call path of c_ext.mx4_attention (10 positional)."},
+    {"write_kv_tokens",
+     reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&write_kv_tokens)), METH_FASTCALL,
+     "Per-call path of c_ext.write_kv_tokens (5 positional)."},
+    {"paged_attention",
+     reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&paged_attention)), METH_FASTCALL,
+     "Per-call path of c_ext.paged_attention (11 positional)."},
+    {"evict_kv_tokens",
+     reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&evict_kv_tokens)), METH_FASTCALL,
+     "Per-call path of c_ext.evict_kv_tokens (10 positional)."},
+    {"bind_paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&bind_paged)),
+     METH_FASTCALL, "Hand over the addresses of the functions on a paged cache."},
     {"bind_mx4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&bind_mx4)),
      METH_FASTCALL, "Hand over the addresses of the functions on a 4-bit cache."},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&bind)), METH_FASTCALL,

@@ -494,6 +494,119 @@ typedef struct fkv_mx4_attention_args {
 int fkv_mx4_attention_workspace(const fkv_mx4_attention_args* args, size_t* bytes);
 int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators on one layer of a paged KV cache in its own type.  No counterpart in the
+ * reference, which leaves them to the engine above it.
+ *
+ * Token t of block b, head h has its K at key + b * block stride + t * token stride +
+ * h * head stride, head_size elements of `dtype`, and its V likewise: K and V may be halves of
+ * one allocation (an engine's [2, N, T, H, D]), of each block, or two allocations, the heads before
+ * the tokens or behind.  Pointers, strides and rows: multiples of 16 bytes; head_size at most
+ * 1024, num_heads 1024, tokens_per_block 2^20.  Every block has to lie inside the allocation. */
+typedef struct fkv_paged_layer {
+  void* key;
+  void* value;                       /* null: a cache of one half (not for attention) */
+  int64_t key_block_stride_bytes, key_token_stride_bytes, key_head_stride_bytes;
+  int64_t value_block_stride_bytes, value_token_stride_bytes, value_head_stride_bytes;
+  int64_t num_blocks;
+  int tokens_per_block, num_heads, head_size, dtype;
+} fkv_paged_layer;
+
+/* Write new tokens into their slots: row n of key and value (elements of the cache's type, a
+ * head's next to each other) becomes token slots[n] % T of block slots[n] / T.  slots: device
+ * memory, int64 or int32 (slots_are_64bit); a slot below 0 or past the cache is padding and
+ * writes nothing.  Slots of one call have to differ: one that comes twice leaves a mixture.
+ * `value` is null where the cache has one half.  Pointers and strides: multiples of 16 bytes.
+ * Asynchronous on `stream`, and may be captured into a graph. */
+int fkv_write_kv_tokens(const fkv_paged_layer* layer, int num_tokens, const void* key,
+                        int64_t key_token_stride_bytes, int64_t key_head_stride_bytes,
+                        const void* value, int64_t value_token_stride_bytes,
+                        int64_t value_head_stride_bytes, const void* slots, int slots_are_64bit,
+                        fkv_stream_t stream);
+
+/* Attention of queries over one layer.  Sequence b has seq_lens[b] keys, token t of it in block
+ * block_table[b][t / T] at t % T, and the queries query_starts[b] .. query_starts[b + 1]
+ * of the packed rows (null: row b alone), which are its last tokens.  For query row i and
+ * head hq, with K/V head hq / group_size,
+ *     out = softmax(scale * q . k) v   over the sequence's keys,
+ * or with `causal` over those up to the query's own position, seq_lens[b] - its
+ * queries + its index.  A row that sees no key gives zeros, and lse -infinity.
+ * lse (may be null): log of the sum of exp(scale * q . k).
+ * weights (may be null): weights[b][h][t] grows by what token t got of the attention of K/V head
+ * h's queries, the sum over them of exp(scale * q . k - lse); of tokens past the sequence's
+ * keys nothing is read or written.  The order of its terms, and so the result, is the same
+ * from call to call.
+ *
+ * head_size 64, 128 or 256; dtype (of cache, query and out) FKV_DTYPE_BF16 or _FP16.
+ * Products enter exactly; sums, maximum, normalisation and weights are held in 32 bits.  In the
+ * second product the weights p have the type's own significant bits (8 or 11).
+ * Block ids, lengths and starts are device memory, all int32 or all int64 (index_is_64bit), read
+ * by the kernels, and nothing outside the cache is read for any of them: a block id outside the
+ * cache gives NaN in the rows that see a token of that block (and in the weights those rows give), a
+ * length past the table's row in all rows of its sequence, whose weights stay, and a length below 0
+ * is taken as 0.  Starts have to ascend; rows of no sequence are left as they were.  table_width
+ * blocks hold at most 2^28 tokens, and weights_width is at least that many.
+ *
+ * What a key or value holds reaches only the rows that see its token.  Sums of p v are in 32 bits
+ * before they are divided by that of p, whose terms reach 2^8: values up to 2^119 over the
+ * sequence's keys are safe, larger ones may give infinities or NaN.  A row whose largest score, in
+ * units of log 2, leaves what 32 bits hold gives NaN.
+ * Asynchronous on `stream`, and may be captured into a graph. */
+typedef struct fkv_paged_attention_args {
+  fkv_paged_layer layer;
+  const void* query;                 /* [num_queries][num_heads * group_size][head_size] */
+  void* out;                         /* as query; may not overlap it */
+  float* lse;                        /* [num_queries][num_heads * group_size], or null */
+  int64_t query_row_stride_bytes, query_head_stride_bytes;   /* multiples of 16, as pointers */
+  int64_t out_row_stride_bytes, out_head_stride_bytes;
+  int64_t lse_row_stride, lse_head_stride;                   /* in elements */
+  float* weights;                    /* [batch][num_heads][weights_width], or null */
+  int64_t weights_seq_stride, weights_head_stride;           /* in elements */
+  const void* block_table;           /* [batch][table_width] */
+  const void* seq_lens;              /* [batch] */
+  const void* query_starts;          /* [batch + 1], or null: one query a sequence */
+  int64_t table_row_stride;          /* in elements */
+  int index_is_64bit;
+  int table_width, batch, num_queries, group_size, causal, weights_width;
+  float scale;
+  void* workspace;                   /* device memory, on a multiple of 16; see below */
+  size_t workspace_bytes;
+} fkv_paged_attention_args;
+/* The workspace a call of these sizes needs (pointers and strides are not looked at, but for
+ * whether query_starts and weights are null); 0 for none.  It holds nothing between calls, and no
+ * two that may run at the same time may share one. */
+int fkv_paged_attention_workspace(const fkv_paged_attention_args* args, size_t* bytes);
+int fkv_paged_attention(const fkv_paged_attention_args* args, fkv_stream_t stream);
+
+/* Evict what got little attention: of sequence b's n = seq_lens[b] tokens (in the blocks
+ * block_table[b]) every head keeps min(n, budget): the `recent` last, and of the others those with
+ * the largest weights[b][h][t], of equal ones the earlier; a NaN counts as larger than all numbers.
+ * The kept tokens' rows, in their order, become tokens 0, 1, ... of the blocks new_table[b], and
+ *     kept[b][h][i]          the place that token i had, -1 past the last
+ *     new_weights[b][h][i]   its weight, 0 past the last (may be null; may be `weights` itself)
+ * Each head keeps tokens of its own.  The blocks of new_table may not be among those that
+ * block_table names for the tokens there are, nor come twice; block_table's are only read, and
+ * may be shared.  Nothing outside the cache is read or written: a token of a block outside it, or
+ * for one, is left out of the copy.  A sequence longer than its row of block_table keeps nothing:
+ * kept is -1, and its new_weights stay.  A length below 0 is taken as 0.
+ * Any dtype.  budget at least 1, recent at most budget, new_table's rows hold what may be kept.
+ * Asynchronous on `stream`, and may be captured into a graph. */
+typedef struct fkv_evict_args {
+  fkv_paged_layer layer;
+  const float* weights;              /* [batch][num_heads][weights_width] */
+  float* new_weights;                /* [batch][num_heads][new_weights_width], or null */
+  int64_t weights_seq_stride, weights_head_stride;           /* in elements */
+  int64_t new_weights_seq_stride, new_weights_head_stride;
+  const void* block_table;           /* [batch][table_width] */
+  const void* new_table;             /* [batch][new_table_width] */
+  const void* seq_lens;              /* [batch] */
+  int64_t table_row_stride, new_table_row_stride;            /* in elements */
+  int32_t* kept;                     /* [batch][num_heads][budget], without gaps */
+  int index_is_64bit;                /* of block_table, new_table and seq_lens */
+  int table_width, new_table_width, batch, budget, recent, weights_width, new_weights_width;
+} fkv_evict_args;
+int fkv_evict_kv_tokens(const fkv_evict_args* args, fkv_stream_t stream);
+
 /* How copy-engine mode (use_ce_transfer = FKV_XFER_CE) chooses between the
  * SDMA engines and the zero-copy kernel, process-wide.  No counterpart in
  * the reference, whose CE mode always copies on the engines.
