@@ -315,7 +315,7 @@ __device__ inline bool any_not_finite(const Values<D>& v) {
   return __any(any);
 }
 
-// A step whose values hold an infinity or a NaN that some row does not see: a weight of 0 does not
+// A step whose values hold an infinity or a NaN that some row may not see: a weight of 0 does not
 // leave it out of a matrix product, so the products are made one by one.
 template <class T, int D>
 __device__ inline void add_one_by_one(const Args& a, int seq, int head, int at, int keys,
@@ -353,7 +353,9 @@ __device__ inline void clear(State<D>& st) {
   for (int j = 0; j < D / 16; ++j) st.o[j] = {0.f, 0.f, 0.f, 0.f};
 }
 
-constexpr int few_waves_a_simd(int row_tiles, int dim) { return dim == 256 ? 1 : 2; }
+constexpr int few_waves_a_simd(int row_tiles, int dim) {
+  return dim == 256 ? 1 : row_tiles == 1 ? 3 : 2;
+}
 
 template <class T, int D, int R, int W>
 __global__ __launch_bounds__(64 * W, few_waves_a_simd(R, D)) void attend_few_kernel(const Args a) {
@@ -417,15 +419,15 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(R, D)) void attend_few_ker
   State<D> st[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) clear(st[r]);
-  for (; step < end; step += W) {
-    const Rows next = find(step + W, ids);
-    ids = block_id(a, w.seq, token_of(step + 2 * W));
+  float p[R][8];
+  // A step's weights and what they change of the rows' states; K makes room for the next step's.
+  auto weights = [&](const Rows& next) {
     const int token = step * kStep;
     v4f s[R][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) scores(q[r], k, s[r]);
     load_keys<D>(next, lane, k);
-    float p[R][8], l[R];
+    float l[R];
     bool passes = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -457,29 +459,42 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(R, D)) void attend_few_ker
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) st[r].l += l[r];
-    if (token + kStep > fewest && any_not_finite<T, D>(v)) {
+  };
+  auto next_rows = [&] {
+    const Rows next = find(step + W, ids);
+    ids = block_id(a, w.seq, token_of(step + 2 * W));
+    return next;
+  };
+  for (; step < end; step += W) {
+    if (step * kStep + kStep > fewest && any_not_finite<T, D>(v)) break;
+    const Rows next = next_rows();
+    weights(next);
+    Op weight[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        add_one_by_one<T, D>(a, w.seq, at.head, token, keys, visible[r], lane, p[r], st[r]);
-    } else {
-      Op weight[R];
+    for (int r = 0; r < R; ++r)
+      weight[r] = __builtin_bit_cast(
+          Op, make_uint4(Mat<T>::pack(p[r][0], p[r][1]), Mat<T>::pack(p[r][2], p[r][3]),
+                         Mat<T>::pack(p[r][4], p[r][5]), Mat<T>::pack(p[r][6], p[r][7])));
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        weight[r] = __builtin_bit_cast(
-            Op, make_uint4(Mat<T>::pack(p[r][0], p[r][1]), Mat<T>::pack(p[r][2], p[r][3]),
-                           Mat<T>::pack(p[r][4], p[r][5]), Mat<T>::pack(p[r][6], p[r][7])));
+    for (int j = 0; j < NT; j += 2) {
+      Op even, odd;
+      columns<T, D>(v, j, even, odd);
 #pragma unroll
-      for (int j = 0; j < NT; j += 2) {
-        Op even, odd;
-        columns<T, D>(v, j, even, odd);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          st[r].o[j] = Mat<T>::mul16(even, weight[r], st[r].o[j]);
-          st[r].o[j + 1] = Mat<T>::mul16(odd, weight[r], st[r].o[j + 1]);
-        }
+      for (int r = 0; r < R; ++r) {
+        st[r].o[j] = Mat<T>::mul16(even, weight[r], st[r].o[j]);
+        st[r].o[j + 1] = Mat<T>::mul16(odd, weight[r], st[r].o[j + 1]);
       }
     }
     load_values<D>(next, lane, v);
+  }
+  // From a step on whose V holds an infinity or a NaN that some row may not see: a loop of its own,
+  // as its registers would be the other's.
+#pragma unroll 1
+  for (; step < end; step += W) {
+    weights(next_rows());
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      add_one_by_one<T, D>(a, w.seq, at.head, step * kStep, keys, visible[r], lane, p[r], st[r]);
   }
   bad = least(bad);
   // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
@@ -531,6 +546,307 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(R, D)) void attend_few_ker
       for (int j = 0; j < NJ; ++j) a.part_o[part * D + element + j] = sums[j];
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: each wavefront has 32 rows, and all of a workgroup share 64 tokens of K and V at a
+// time in LDS, double-buffered; the next tile is on its way to registers meanwhile.
+
+struct ManyPlan {
+  static constexpr int kStep = 64;       // tokens of a tile
+  static constexpr int kMinSteps = 16;   // of a workgroup, where the keys are cut
+  static constexpr int kCutSteps = 16;   // that cutting has to take off the longest sequence
+};
+constexpr int kTile = ManyPlan::kStep;
+
+// A row of a tile in LDS is D / 8 pieces of 16 bytes, piece c at c ^ f(row).  K is read with 8 and
+// more neighbouring rows of one piece at a time, V (transposed) with 4 neighbouring rows of 4
+// pieces: so that either takes all banks.
+template <int D>
+__device__ constexpr int k_swizzle(int row) {
+  return D == 64 ? row & 7 : row & 15;
+}
+template <int D>
+__device__ constexpr int v_swizzle(int row) {
+  return D == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
+}
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* LdsTransposed;
+
+template <class T, int D, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(const Args a) {
+  using Op = typename Mat<T>::Op;
+  constexpr int kPieces = D / 8;              // of a row
+  constexpr int kPasses = kPieces / W;        // of the workgroup over a tile's pieces
+  constexpr int kPassRows = 64 / kPieces;     // of a wavefront in a pass
+  constexpr int kHalf = kTile * D * 2;        // bytes of a tile of K or V
+  constexpr int KS = D / 16, NT = D / 32;
+  __shared__ __attribute__((aligned(256))) char lds[2][2][kHalf];
+  __shared__ int odd[2][W];                   // whether a wavefront saw V that is not finite
+  const Place at = heads_apart(a, blockIdx.x);
+  const Work w = find_work<ManyPlan>(a, at.item, 32 * W, false);
+  if (a.slots && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = w.any_cut;
+  if (w.seq < 0) return;
+  const int first = w.tile * 32 * W;
+  const int rows = min(32 * W, w.s.count * a.group - first);
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int column = lane & 31, half = lane >> 5;
+  const int keys = max(w.s.keys, 0);
+  const int mine = 32 * wave + column;        // this lane's row of the tile
+  auto row_here = [&] { return row_of(a, w.s, first + min(mine, rows - 1), at.head); };
+  const int visible = row_here().visible;
+  // of the rows, in order, the first sees the fewest, the last the most
+  const int fewest = row_of(a, w.s, first, at.head).visible;
+  const int most = row_of(a, w.s, first + rows - 1, at.head).visible;
+  const int all_tiles = (most + kTile - 1) / kTile;
+  const int begin = w.cuts > 1 ? w.cut * w.steps : 0;
+  const int end = w.cuts > 1 ? min(all_tiles, (w.cut + 1) * w.steps) : all_tiles;
+
+  Op q[KS];
+  {
+    const Row row = row_here();
+    const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + half * 16;
+#pragma unroll
+    for (int x = 0; x < KS; ++x)
+      q[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 32 * x));
+  }
+
+  // Which rows of a tile a wavefront brings: a lane finds one of K (below 32) or V, and gets the
+  // others' from the lanes that found them.  Block ids are asked for a tile ahead of the rows, these
+  // a tile ahead of their use; past the last key everything is of that one again.
+  int bad = kNoToken;
+  Half of = lane >= 32 ? a.v : a.k;
+  of.p += at.head * of.head;
+  const int found = lane & (kPassRows * kPasses - 1);
+  const int found_row = (found / kPassRows * W + wave) * kPassRows + found % kPassRows;
+  auto token_of = [&](int tile) { return min(tile * kTile + found_row, keys - 1); };
+  auto find = [&](int tile, int64_t id) {
+    const int t = token_of(tile);
+    if (outside(a, id)) bad = min(bad, t);
+    const uint64_t p = row_address(a, of, id, t, 0);
+    return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
+  };
+  Vec4 next_k[kPasses], next_v[kPasses];
+  auto bring = [&](const Rows& r) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int from = i * kPassRows + lane / kPieces, piece = (lane % kPieces) * 16;
+      next_k[i] = load<Vec4>(row_of_lane(r, from) + piece);
+      next_v[i] = load<Vec4>(row_of_lane(r, 32 + from) + piece);
+    }
+  };
+  auto put = [&](int buffer, bool look) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = (i * W + wave) * kPassRows + lane / kPieces, piece = lane % kPieces;
+      *reinterpret_cast<Vec4*>(&lds[buffer][0][r * D * 2 + (piece ^ k_swizzle<D>(r)) * 16]) =
+          next_k[i];
+      *reinterpret_cast<Vec4*>(&lds[buffer][1][r * D * 2 + (piece ^ v_swizzle<D>(r)) * 16]) =
+          next_v[i];
+    }
+    if (look) {
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) any |= not_finite<T>(next_v[i][x]);
+      any = __any(any);
+      if (lane == 0) odd[buffer][wave] = any;
+    }
+  };
+  // a tile that some row of the workgroup does not see all of
+  auto partly = [&](int tile) { return (tile + 1) * kTile > fewest; };
+
+  const float scale_log2 = score_scale(a.scale_log2);
+  const bool negate = a.scale_log2 < 0.f;
+  float m = kNothing, l = 0.f, slack = kSlack;
+  v16f o[NT];
+#pragma unroll
+  for (int d = 0; d < NT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+
+  int64_t ids = 0;
+  Rows ahead{0, 0};
+  if (begin < end) {
+    ids = block_id(a, w.seq, token_of(begin));
+    bring(find(begin, ids));
+    ids = block_id(a, w.seq, token_of(begin + 1));
+    put(0, partly(begin));
+    ahead = find(begin + 1, ids);
+    ids = block_id(a, w.seq, token_of(begin + 2));
+  }
+  // where a lane reads: K's row `column`, piece `half`; V's rows 4 half + ((lane & 15) >> 2)
+  const int k_at = column * D * 2 + ((half ^ k_swizzle<D>(column)) << 4);
+  int v_at[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 8 * j + 4 * half + ((lane & 15) >> 2);
+    const int piece = ((lane >> 4 & 1) << 1) | (lane >> 1 & 1);
+    v_at[j] = r * D * 2 + ((piece ^ v_swizzle<D>(r)) << 4) + (lane & 1) * 8;
+  }
+  int buffer = 0, tile = begin;
+  // A tile's weights, in the place of its scores, and what they change of the row's state.
+  v16f s[2];
+  auto scores = [&] {
+    const char* const kt = lds[buffer][0];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        const Op k = __builtin_bit_cast(
+            Op, *reinterpret_cast<const Vec4*>(kt + (k_at ^ (x % 8 * 32)) + x / 8 * 256 +
+                                               32 * h * D * 2));
+        s[h] = Mat<T>::mul32(k, q[x], s[h]);
+      }
+    }
+    if (negate) s[0] = -s[0], s[1] = -s[1];
+    if (partly(tile)) {
+      int seen = visible - tile * kTile - 4 * half;
+      asm volatile("" : "+v"(seen));       // not 32 differences, one for each token, kept
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * h + 8 * (i / 4) + i % 4 >= seen) s[h][i] = -INFINITY;
+    }
+  };
+  auto weigh_all = [&](bool coarse) {
+    float sum[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[h][i] = __builtin_amdgcn_exp2f(coarse ? rounded_less(s[h][i], scale_log2, m)
+                                                : __builtin_fmaf(s[h][i], scale_log2, -m));
+        sum[h] = i ? sum[h] + s[h][i] : s[h][i];
+      }
+    return sum[0] + sum[1];
+  };
+  auto weights = [&] {
+    scores();
+    float sum = weigh_all(false);
+    if (__any(sum > slack)) {
+      // Some score passes its row's reference: the references follow, and the weights are made
+      // again, from scores made again, which would be 32 registers more if they were kept.
+      scores();
+      float top = m;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i] * scale_log2);
+      const auto other = __builtin_amdgcn_permlane32_swap(f32_bits(top), f32_bits(top), false, false);
+      top = fmaxf(bits_f32(other[0]), bits_f32(other[1]));
+      const float fade = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= fade;
+#pragma unroll
+      for (int d = 0; d < NT; ++d) o[d] *= fade;
+      const bool coarse = fabsf(m) >= kCoarse && m != kNothing;
+      sum = weigh_all(coarse);
+      slack = __any(coarse) ? -1.f : kSlack;
+    }
+    l += sum;
+  };
+  for (; tile < end; ++tile, buffer ^= 1) {
+    __syncthreads();
+    if (partly(tile)) {
+      int any = 0;
+#pragma unroll
+      for (int x = 0; x < W; ++x) any |= odd[buffer][x];
+      if (uniform(any)) break;
+    }
+    bring(ahead);
+    ahead = find(tile + 2, ids);
+    ids = block_id(a, w.seq, token_of(tile + 3));
+    weights();
+    const char* const vt = lds[buffer][1];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      uint32_t u[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        u[x] = Mat<T>::pack(s[b / 2][8 * (b % 2) + 2 * x], s[b / 2][8 * (b % 2) + 2 * x + 1]);
+      const Op weight = __builtin_bit_cast(Op, make_uint4(u[0], u[1], u[2], u[3]));
+#pragma unroll
+      for (int d = 0; d < NT; ++d) {
+        v4s x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          x[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTransposed)(
+              vt + (v_at[j] ^ (d % 4 * 64)) + d / 4 * 256 + 16 * b * D * 2));
+        const Op v =
+            __builtin_bit_cast(Op, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        o[d] = Mat<T>::mul32(v, weight, o[d]);
+      }
+    }
+    put(buffer ^ 1, partly(tile + 1));
+  }
+  // From a tile on whose V holds an infinity or a NaN that some row may not see: a weight of 0
+  // does not leave it out of a matrix product, so the products are made one by one.  A loop of its
+  // own, as its registers would be the other's.
+#pragma unroll 1
+  for (; tile < end; ++tile, buffer ^= 1) {
+    weights();
+    const char* const vt = lds[buffer][1];
+#pragma unroll 1
+    for (int t = 0; t < kTile; ++t) {
+      float x = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i)
+        x = (t / 32 * 16 + t % 32 / 8 * 4 + t % 4) == i ? s[i / 16][i % 16] : x;
+      x = __shfl(x, column + 32 * (t / 4 % 2));
+      const bool seen = tile * kTile + t < visible;
+#pragma unroll
+      for (int d = 0; d < NT; ++d) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t u = *reinterpret_cast<const uint32_t*>(
+              vt + t * D * 2 + (((4 * d + i / 4) ^ v_swizzle<D>(t)) << 4) + half * 8 + i % 4 * 2);
+          if (!seen) continue;
+          o[d][i] += x * Mat<T>::low(u);
+          o[d][i + 1] += x * Mat<T>::high(u);
+        }
+      }
+    }
+    bring(ahead);
+    ahead = find(tile + 2, ids);
+    ids = block_id(a, w.seq, token_of(tile + 3));
+    put(buffer ^ 1, false);
+    __syncthreads();
+  }
+  // the least bad token that any wavefront came across
+  bad = least(bad);
+  __shared__ int bads[W];
+  if (lane == 0) bads[wave] = bad;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < W; ++x) bad = min(bad, bads[x]);
+  const auto both = __builtin_amdgcn_permlane32_swap(f32_bits(l), f32_bits(l), false, false);
+  l = bits_f32(both[0]) + bits_f32(both[1]);
+  if (w.s.keys < 0 || visible > bad) l = bits_f32(0x7fc00000u);
+  if (mine >= rows) return;
+  const Row row = row_here();
+  const float inv = inverse(l, visible);
+  const int64_t part = part_of(a, at.item, at.head) * (32 * W) + mine;
+#pragma unroll
+  for (int d = 0; d < NT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int element = 32 * d + 8 * (i / 4) + 4 * half;
+      const float x[4] = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+      if (w.cuts == 1)
+        write_elements<T, 4>(a, row, element, x, inv);
+      else
+        *reinterpret_cast<v4f*>(a.part_o + part * D + element) = v4f{x[0], x[1], x[2], x[3]};
+    }
+  if (half) return;
+  if (w.cuts == 1) write_stats(a, row, m, l);
+  else a.part_ml[part] = make_float2(m, l);
 }
 
 // Joins the cuts of 16 rows of a tile of ROWS: 256 threads, each D / 16 neighbouring elements of a row,
@@ -732,7 +1048,8 @@ int check_attention(const fkv_paged_attention_args& c) {
 }
 
 struct LaunchPlan {
-  int row_tiles;          // R
+  int rows;               // of a tile
+  bool many;              // rows are shared out to the wavefronts, else keys are
   int64_t tiles;          // times heads: the most there can be
   bool wide;              // few tiles: more wavefronts a workgroup
   int slots;
@@ -746,25 +1063,25 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
   LaunchPlan p;
   const int heads = c.layer.num_heads, dim = c.layer.head_size;
   const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
-  auto tiles = [&](int row_tiles) {
-    const int n = kRows * row_tiles;
-    return (c.query_starts ? rows / n + c.batch
-                           : static_cast<int64_t>(c.batch) * ((c.group_size + n - 1) / n)) *
-           heads;
-  };
+  p.rows = rows > static_cast<int64_t>(c.batch) * 32 ? 128
+           : rows > static_cast<int64_t>(c.batch) * kRows ? 32 : kRows;
+  p.many = p.rows > 32;
+  p.tiles = (c.query_starts ? rows / p.rows + c.batch
+                            : static_cast<int64_t>(c.batch) * ((c.group_size + p.rows - 1) / p.rows)) *
+            heads;
+  p.wide = p.rows == kRows && p.tiles <= kComputeUnits && dim <= 128;
+  const int step = p.many ? ManyPlan::kStep : FewPlan::kStep;
+  const int least = p.many ? ManyPlan::kMinSteps + ManyPlan::kCutSteps
+                           : FewPlan::kMinSteps + FewPlan::kCutSteps;
   const int64_t most_steps =
-      (static_cast<int64_t>(c.table_width) * c.layer.tokens_per_block + kStep - 1) / kStep;
-  p.row_tiles = rows > static_cast<int64_t>(c.batch) * kRows ? 2 : 1;
-  p.tiles = tiles(p.row_tiles);
-  p.wide = p.row_tiles == 1 && p.tiles <= kComputeUnits && dim <= 128;
-  p.slots = most_steps < FewPlan::kMinSteps + FewPlan::kCutSteps || p.tiles > 4 * kComputeUnits ||
-                    p.row_tiles > 1
-                ? 0
-            : p.wide ? kComputeUnits : static_cast<int>(p.tiles);
+      (static_cast<int64_t>(c.table_width) * c.layer.tokens_per_block + step - 1) / step;
+  const int places = p.many ? 2 * kComputeUnits : kComputeUnits;
+  p.slots = most_steps < least || p.tiles > 4 * kComputeUnits || p.rows == 32 ? 0
+            : p.wide || p.many ? places : static_cast<int>(p.tiles);
   // items (cuts of a tile, of all heads), in whole rounds of the XCDs
   const int64_t items = (p.tiles + p.slots + heads - 1) / heads;
   p.workgroups = (items + kXcds - 1) / kXcds * kXcds * heads;
-  const int64_t part_rows = p.slots ? p.workgroups * kRows * p.row_tiles : 0;
+  const int64_t part_rows = p.slots ? p.workgroups * p.rows : 0;
   p.ml_bytes = part_rows * sizeof(float2) + (p.slots ? 16 : 0);    // and any_cut
   p.o_bytes = part_rows * dim * sizeof(float);
   p.stats_bytes =
@@ -782,18 +1099,28 @@ int check_plan(const fkv_paged_attention_args& c, const LaunchPlan& p) {
   return 0;
 }
 
-template <class T, int D, int R, int W>
-void launch(const Args& a, const LaunchPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((attend_few_kernel<T, D, R, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
+template <class T, int D, int ROWS, class P, int G>
+void join(const Args& a, const LaunchPlan& p, hipStream_t s) {
   if (p.slots)
-    hipLaunchKernelGGL((join_kernel<T, D, kRows * R, FewPlan, W == 8 ? 4 : 1>), dim3(p.tiles * R),
-                       dim3(256 * (W == 8 ? 4 : 1)), 0, s, a);
+    hipLaunchKernelGGL((join_kernel<T, D, ROWS, P, G>), dim3(p.tiles * (ROWS / 16)), dim3(256 * G),
+                       0, s, a);
+}
+template <class T, int D, int R, int W>
+void launch_few(const Args& a, const LaunchPlan& p, hipStream_t s) {
+  hipLaunchKernelGGL((attend_few_kernel<T, D, R, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
+  join<T, D, kRows * R, FewPlan, W == 8 ? 4 : 1>(a, p, s);
+}
+template <class T, int D, int W>
+void launch_many(const Args& a, const LaunchPlan& p, hipStream_t s) {
+  hipLaunchKernelGGL((attend_many_kernel<T, D, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
+  join<T, D, 32 * W, ManyPlan, 1>(a, p, s);
 }
 template <class T, int D>
 void launch(const Args& a, const LaunchPlan& p, const fkv_paged_attention_args& c, hipStream_t s) {
-  if (p.row_tiles == 2) launch<T, D, 2, 4>(a, p, s);
-  else if (p.wide) launch<T, D, 1, D == 256 ? 4 : 8>(a, p, s);
-  else launch<T, D, 1, 4>(a, p, s);
+  if (p.many) launch_many<T, D, 4>(a, p, s);
+  else if (p.rows == 32) launch_few<T, D, 2, 4>(a, p, s);
+  else if (p.wide) launch_few<T, D, 1, D == 256 ? 4 : 8>(a, p, s);
+  else launch_few<T, D, 1, 4>(a, p, s);
   if (a.weights && a.width) {
     const int64_t most = static_cast<int64_t>(a.width) * a.tokens;
     hipLaunchKernelGGL((weigh_kernel<T, D>),
