@@ -96,14 +96,19 @@ struct Args : Sequences {
   int64_t lse_row, lse_head;         // elements
   Half k, v;
   float scale_log2;
+  int together;                      // how heads lie on the XCDs, see Place
   FastDiv tokens_div;
-  float2* part_ml;                   // [cut][row]: maximum and sum
-  float* part_o;                     // [cut][row][element]
+  float2* part_ml;                   // [part][row]: maximum and sum
+  float* part_o;                     // [part][row][element]
   int* any_cut;                      // whether some tile has more than one cut
   // for the tokens' weights, all null where they are not asked for
   float* weights;
   int64_t w_seq, w_head;             // elements
   float2* stats;                     // [query][head]: reference and 1 / sum of a row
+  // [query][head][token]: the scores times scale, in units of log 2, where the kernel for few rows
+  // leaves them; null where they are made again
+  float* scores;
+  int64_t scores_row;
 };
 
 // 16 bytes of device memory; not a flat access, which would wait for LDS as well.
@@ -112,11 +117,35 @@ __device__ inline V load(uint64_t address) {
   return *reinterpret_cast<const __attribute__((address_space(1))) V*>(address);
 }
 
+// The same of what is read once and by one instruction: past the caches (V so: 32 sequences of 8192
+// keys, 8 heads: 188 us for 205, 5.7 TB/s for 5.3; K as well, in whole rows: 178).
+template <class V>
+__device__ inline V load_once(uint64_t address) {
+  return __builtin_nontemporal_load(
+      reinterpret_cast<const __attribute__((address_space(1))) V*>(address));
+}
+
 // ---------------------------------------------------------------------------
 // Where the rows of tokens lie
 
+// A block id as it lies in the table, two words of which the second is the first again in a table
+// of 32 bits: made a number where it is used, since what is done with a load's result where it is
+// asked for waits for all loads before it.
+struct RawId {
+  uint32_t lo, hi;
+};
+__device__ inline RawId ask_block(const Args& a, int seq, int token) {
+  const uint64_t at = reinterpret_cast<uint64_t>(a.table) +
+                      (static_cast<uint64_t>(seq * a.table_row + a.tokens_div.div(token))
+                       << (a.index64 ? 3 : 2));
+  return {load<uint32_t>(at), load<uint32_t>(at + (a.index64 ? 4 : 0))};
+}
+__device__ inline int64_t block_id(const Args& a, const RawId& r) {
+  const uint32_t hi = a.index64 ? r.hi : static_cast<uint32_t>(static_cast<int32_t>(r.lo) >> 31);
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | r.lo);
+}
 __device__ inline int64_t block_id(const Args& a, int seq, int token) {
-  return index_at(a.table, seq * a.table_row + a.tokens_div.div(token), a.index64);
+  return block_id(a, ask_block(a, seq, token));
 }
 // The row of a token in block `id`, of one half and head.  A block outside the cache is block 0
 // here (and noted by whoever calls).
@@ -181,21 +210,104 @@ __device__ inline void write_elements(const Args& a, const Row& row, int first, 
 constexpr int kRows = 16;          // rows of a tile: columns of a matrix instruction
 struct FewPlan {
   static constexpr int kStep = 32;       // tokens: two tiles of 16, k of the second product
-  static constexpr int kMinSteps = 32;   // of a workgroup, where the keys are cut
-  static constexpr int kCutSteps = 96;   // that cutting has to take off the longest sequence
+  static constexpr int kMinSteps = 32;   // of a workgroup, where the keys are dealt out
 };
 constexpr int kStep = FewPlan::kStep;
+
+// How the keys are dealt out, where they are: the 32-token steps of all tiles, sequence by
+// sequence, are one line for every head, and workgroup j of a head's `slots` has the steps from
+// j * per on, `per` of them.  All workgroups end at about one time, whatever the lengths; a tile that
+// several have a piece of is joined afterwards.  The lengths are read here, on the device, by
+// every wavefront, sequence b = lane, then 64 further on.  A tile has a step at least, so that its
+// rows are written.
+struct Piece {
+  int seq, tile;      // < 0: none
+  int from, steps;    // its first step in the tile, and all steps of the tile
+  int start;          // of the tile on the line
+  Seq s;
+};
+struct Line {
+  Seq s;
+  int tiles, steps;
+  __device__ Line(const Sequences& a, int b, int rows_a_tile) : s{0, 0, 0}, tiles(0), steps(1) {
+    if (b >= a.batch) return;
+    s = sequence(a, b);
+    tiles = tiles_of(a, s, rows_a_tile);
+    steps = max(1, steps_of<FewPlan>(s));
+  }
+};
+// Steps of all tiles, and those that a workgroup has: an even share, but no less than
+// kMinSteps, or the longest tile if that is shorter.  `line`: the first 64 sequences'.
+__device__ inline int deal(const Sequences& a, int rows_a_tile, const Line& line, int* total) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0, longest = 0;
+  for (int b = lane; b < a.batch; b += 64) {
+    const Line x = b == lane ? line : Line(a, b, rows_a_tile);
+    sum += x.tiles * x.steps;
+    if (x.tiles) longest = max(longest, x.steps);
+  }
+  *total = lane_value(scan_lanes(sum), 63);
+  longest = uniform(-least(-longest));
+  return max(uniform((*total + a.slots - 1) / a.slots), min(longest, FewPlan::kMinSteps));
+}
+// Where step `at` of the line is; by_tile: where tile `at` starts.
+__device__ inline Piece find_piece(const Sequences& a, int rows_a_tile, const Line& line, int at,
+                                   bool by_tile) {
+  const int lane = threadIdx.x & 63;
+  int before = 0, tiles_before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const Line x = b0 ? Line(a, b0 + lane, rows_a_tile) : line;
+    const int ends = scan_lanes(x.tiles * x.steps), tile_ends = scan_lanes(x.tiles);
+    const uint64_t later =
+        __ballot(by_tile ? tiles_before + tile_ends > at : before + ends > at);
+    if (later) {
+      const int l = __builtin_ctzll(later);
+      const int n = lane_value(x.tiles, l), steps = lane_value(x.steps, l);
+      const int first = before + lane_value(ends, l) - n * steps;
+      const int tile = by_tile ? at - (tiles_before + lane_value(tile_ends, l) - n)
+                               : uniform((at - first) / steps);
+      const int start = first + tile * steps;
+      return {b0 + l, tile, by_tile ? 0 : at - start, steps, start,
+              {lane_value(x.s.first, l), lane_value(x.s.count, l), lane_value(x.s.keys, l)}};
+    }
+    before += lane_value(ends, 63);
+    tiles_before += lane_value(tile_ends, 63);
+  }
+  return {-1, 0, 0, 0, 0, {0, 0, 0}};
+}
+// A tile for each workgroup, uncut, one query a sequence: nothing but that length is read.
+__device__ inline Piece find_alone(const Sequences& a, int item, int rows_a_tile) {
+  const Work w = find_single(a, item, rows_a_tile);
+  return {w.seq, w.tile, 0, max(1, steps_of<FewPlan>(w.s)), 0, w.s};
+}
+// A workgroup has parts of two tiles at most: of one that starts before it, and of one that
+// starts in it and goes on after it.
+__device__ inline int64_t part_of_piece(const Sequences& a, int slot, int head, bool starts) {
+  return (static_cast<int64_t>(slot) * a.heads + head) * 2 + (starts ? 1 : 0);
+}
+
+// A row of K or V in LDS is D / 8 pieces of 16 bytes, piece c at c ^ f(row).  K is read with 8 and
+// more neighbouring rows of one piece at a time, V (transposed) with 4 neighbouring rows of 4
+// pieces: so that either takes all banks.
+template <int D>
+__device__ constexpr int k_swizzle(int row) {
+  return D == 64 ? row & 7 : row & 15;
+}
+template <int D>
+__device__ constexpr int v_swizzle(int row) {
+  return D == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
+}
 
 // The queries of 16 rows: lane (row, quad) holds elements 32 s + 8 quad .. + 7.
 template <class T, int D>
 struct Query {
   typename Mat<T>::Op part[D / 32];
 };
-// What a lane loads of a step: of K token 16 h + (lane & 15), as of the queries; of V the
-// elements (D / 16) * (lane & 15) on of tokens 16 h + 4 quad + i.
+// What a lane loads of a step: of K whole rows, D / 8 lanes a row, which are put into the order
+// of the queries through LDS; of V the elements (D / 16) * (lane & 15) on of tokens 16 h + 4 quad + i.
 template <int D>
 struct Keys {
-  Vec4 part[2][D / 32];
+  Vec4 part[D / 16];
 };
 template <int D>
 struct Values {
@@ -221,23 +333,33 @@ __device__ inline uint64_t row_of_lane(const Rows& r, int lane) {
 
 template <int D>
 __device__ inline void load_keys(const Rows& r, int lane, Keys<D>& k) {
+  constexpr int kPieces = D / 8, kRowsAtOnce = 64 / kPieces;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint64_t p = row_of_lane(r, 16 * h + (lane & 15)) + (lane >> 4) * 16;
+  for (int j = 0; j < D / 16; ++j)
+    k.part[j] = load_once<Vec4>(row_of_lane(r, j * kRowsAtOnce + lane / kPieces) +
+                                lane % kPieces * 16);
+}
+// A wavefront's 32 rows of K in LDS.
+template <int D>
+__device__ inline void put_keys(const Keys<D>& k, int lane, char* lds) {
+  constexpr int kPieces = D / 8, kRowsAtOnce = 64 / kPieces;
 #pragma unroll
-    for (int s = 0; s < D / 32; ++s) k.part[h][s] = load<Vec4>(p + 64 * s);
+  for (int j = 0; j < D / 16; ++j) {
+    const int row = j * kRowsAtOnce + lane / kPieces;
+    *reinterpret_cast<Vec4*>(lds + row * D * 2 + ((lane % kPieces ^ k_swizzle<D>(row)) << 4)) =
+        k.part[j];
   }
 }
 // D / 16 elements of a row
 template <int D>
 __device__ inline void load_part(uint64_t p, uint32_t (&x)[D / 32]) {
   if constexpr (D == 64) {
-    const Vec2 u = load<Vec2>(p);
+    const Vec2 u = load_once<Vec2>(p);
     x[0] = u[0], x[1] = u[1];
   } else {
 #pragma unroll
     for (int w = 0; w < D / 32; w += 4) {
-      const Vec4 u = load<Vec4>(p + 4 * w);
+      const Vec4 u = load_once<Vec4>(p + 4 * w);
 #pragma unroll
       for (int y = 0; y < 4; ++y) x[w + y] = u[y];
     }
@@ -253,15 +375,24 @@ __device__ inline void load_values(const Rows& r, int lane, Values<D>& v) {
                    v.part[h][i]);
 }
 
-// s[h][i] = q . k of token 16 h + 4 quad + i
-template <class T, int D>
-__device__ inline void scores(const Query<T, D>& q, const Keys<D>& k, v4f (&s)[2]) {
+// s[r][h][i] = q[r] . k of token 16 h + 4 quad + i
+template <class T, int D, int R>
+__device__ inline void scores(const Query<T, D> (&q)[R], const char* lds, int lane,
+                              v4f (&s)[R][2]) {
+  using Op = typename Mat<T>::Op;
+  const int at = (lane & 15) * D * 2 + (((lane >> 4) ^ k_swizzle<D>(lane & 15)) << 4);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    s[h] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x)
-      s[h] = Mat<T>::mul16(__builtin_bit_cast(typename Mat<T>::Op, k.part[h][x]), q.part[x], s[h]);
+    for (int r = 0; r < R; ++r) s[r][h] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+      const Op k = __builtin_bit_cast(
+          Op, *reinterpret_cast<const Vec4*>(lds + (at ^ (x % 4 * 64)) + x / 4 * 256 +
+                                             16 * h * D * 2));
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r][h] = Mat<T>::mul16(k, q[r].part[x], s[r][h]);
+    }
   }
 }
 
@@ -353,198 +484,242 @@ __device__ inline void clear(State<D>& st) {
   for (int j = 0; j < D / 16; ++j) st.o[j] = {0.f, 0.f, 0.f, 0.f};
 }
 
-constexpr int few_waves_a_simd(int row_tiles, int dim) {
-  return dim == 256 ? 1 : row_tiles == 1 ? 3 : 2;
-}
+constexpr int few_waves_a_simd(int dim) { return dim == 256 ? 1 : 2; }
 
 template <class T, int D, int R, int W>
-__global__ __launch_bounds__(64 * W, few_waves_a_simd(R, D)) void attend_few_kernel(const Args a) {
+__global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel(const Args a) {
   using Op = typename Mat<T>::Op;
-  constexpr int NT = D / 16;
+  constexpr int NT = D / 16, kRowsATile = kRows * R;
+  // K of a wavefront's step, then a row tile's sums of every wavefront
   __shared__ v4f shared[W * NT][64];
   __shared__ float sum_m[W][R][16], sum_l[W][R][16];
-  const Place at = R == 1 ? heads_together(a, blockIdx.x) : heads_apart(a, blockIdx.x);
-  const Work w = a.slots || a.starts ? find_work<FewPlan>(a, at.item, kRows * R, false)
-                                     : find_single(a, at.item, kRows * R);
-  if (a.slots && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = w.any_cut;
-  if (w.seq < 0) return;
-  const int first = w.tile * kRows * R;
-  const int rows = min(kRows * R, w.s.count * a.group - first);
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4;
-  auto row_at = [&](int n) { return row_of(a, w.s, first + min(n, rows - 1), at.head); };
-  const int keys = max(w.s.keys, 0);
-  int visible[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) visible[r] = row_at(16 * r + (lane & 15)).visible;
-  // of the rows, in order, the first sees the fewest, the last the most
-  const int fewest = lane_value(visible[0], 0), most = lane_value(visible[R - 1], 15);
-  const int all_steps = (most + kStep - 1) / kStep;
-  const int end = w.cuts > 1 ? min(all_steps, (w.cut + 1) * w.steps) : all_steps;
-  int step = (w.cuts > 1 ? w.cut * w.steps : 0) + wave;
-  const bool any = step < end;
-  // the block ids are asked for a step ahead of the rows, the rows a step ahead of their use; past
-  // the last key everything is of that one again
-  int bad = kNoToken;
-  const bool of_v = lane >= 32;
-  const Half half = of_v ? a.v : a.k;
-  auto token_of = [&](int s) { return min(s * kStep + (lane & 31), keys - 1); };
-  auto find = [&](int s, int64_t id) {
-    const int t = token_of(s);
-    if (outside(a, id)) bad = min(bad, t);
-    const uint64_t p = row_address(a, half, id, t, at.head);
-    return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
-  };
-  Keys<D> k;
-  Values<D> v;
-  int64_t ids = 0;
-  if (any) {
-    ids = block_id(a, w.seq, token_of(step));
-    const Rows next = find(step, ids);
-    ids = block_id(a, w.seq, token_of(step + W));
-    load_keys<D>(next, lane, k);
-    load_values<D>(next, lane, v);
-  }
-  Query<T, D> q[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const Row row = row_at(16 * r + (lane & 15));
-    const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + quad * 16;
-#pragma unroll
-    for (int x = 0; x < D / 32; ++x)
-      q[r].part[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 64 * x));
-  }
+  const Place at = a.together ? heads_together(a, blockIdx.x) : heads_apart(a, blockIdx.x);
+  const int wave = uniform(threadIdx.x >> 6);
+  char* const k_lds = reinterpret_cast<char*>(shared[wave * NT]);
   const float scale_log2 = score_scale(a.scale_log2);
   const bool negate = a.scale_log2 < 0.f;
-  float slack = kSlack;
-  State<D> st[R];
+  // nothing but its own sequence's length is read where each has a tile for one workgroup
+  const bool alone = !a.slots && !a.starts;
+  const Line line(a, alone ? a.batch : threadIdx.x & 63, kRowsATile);
+  int pos = 0, pos_end = 0;
+  if (a.slots) {
+    int total;
+    const int per = deal(a, kRowsATile, line, &total);
+    // up to 2^31 steps of 2^10 workgroups: both in 64 bits
+    pos = static_cast<int>(min(static_cast<int64_t>(at.item) * per, static_cast<int64_t>(total)));
+    pos_end = static_cast<int>(min(static_cast<int64_t>(pos) + per, static_cast<int64_t>(total)));
+    if (pos == pos_end) return;
+  }
+  for (bool again = false;; again = true) {
+    if (again) __syncthreads();      // the sums of the tile before have been read
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));   // what follows from it is worked out for each tile, not kept
+    const int quad = lane >> 4;
+    const Piece w = alone ? find_alone(a, at.item, kRowsATile)
+                          : find_piece(a, kRowsATile, line, a.slots ? pos : at.item, !a.slots);
+    if (w.seq < 0) return;
+    const int to = a.slots ? min(w.steps, w.from + pos_end - pos) : w.steps;
+    const bool whole = w.from == 0 && to == w.steps;
+    const int first = w.tile * kRowsATile;
+    const int rows = min(kRowsATile, w.s.count * a.group - first);
+    auto row_at = [&](int n) { return row_of(a, w.s, first + min(n, rows - 1), at.head); };
+    const int keys = max(w.s.keys, 0);
+    int visible[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) clear(st[r]);
-  float p[R][8];
-  // A step's weights and what they change of the rows' states; K makes room for the next step's.
-  auto weights = [&](const Rows& next) {
-    const int token = step * kStep;
-    v4f s[R][2];
-#pragma unroll
-    for (int r = 0; r < R; ++r) scores(q[r], k, s[r]);
-    load_keys<D>(next, lane, k);
-    float l[R];
-    bool passes = false;
+    for (int r = 0; r < R; ++r) visible[r] = row_at(16 * r + (lane & 15)).visible;
+    // of the rows, in order, the first sees the fewest, the last the most
+    const int fewest = lane_value(visible[0], 0), most = lane_value(visible[R - 1], 15);
+    const int end = min((most + kStep - 1) / kStep, to);
+    int step = w.from + wave;
+    const bool any = step < end;
+    // the block ids are asked for a step ahead of the rows, the rows a step ahead of their use; past
+    // the last key everything is of that one again
+    int bad = kNoToken;
+    const bool of_v = lane >= 32;
+    Half half = of_v ? a.v : a.k;
+    half.p += at.head * half.head;
+    auto token_of = [&](int s) { return min(s * kStep + (lane & 31), keys - 1); };
+    auto find = [&](int s, const RawId& raw) {
+      const int t = token_of(s);
+      const int64_t id = block_id(a, raw);
+      if (outside(a, id)) bad = min(bad, t);
+      const uint64_t p = row_address(a, half, id, t, 0);
+      return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
+    };
+    Keys<D> k;
+    Values<D> v;
+    RawId ids{0, 0};
+    if (any) ids = ask_block(a, w.seq, token_of(step));
+    Query<T, D> q[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (negate) s[r][0] = -s[r][0], s[r][1] = -s[r][1];
-      if (token + kStep > fewest) hide(s[r], token, visible[r], quad);
-      l[r] = weigh(s[r], st[r].m, scale_log2, false, p[r]);
-      passes |= l[r] > slack;
+      const Row row = row_at(16 * r + (lane & 15));
+      const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + quad * 16;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x)
+        q[r].part[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 64 * x));
     }
-    if (__any(passes)) {
-      // Some score passes its row's reference: the references follow, and the weights are made
-      // again; at every step from then on, where a reference is kCoarse or more.
-      bool any_coarse = false;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float top = st[r].m;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) top = fmaxf(top, s[r][x / 4][x % 4] * scale_log2);
-        const float m = max_over_quads(top);
-        const float fade = __builtin_amdgcn_exp2f(st[r].m - m);
-        st[r].m = m;
-        st[r].l *= fade;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
-        const bool coarse = fabsf(m) >= kCoarse && m != kNothing;
-        any_coarse |= coarse;
-        l[r] = weigh(s[r], m, scale_log2, coarse, p[r]);
-      }
-      slack = __any(any_coarse) ? -1.f : kSlack;
+    if (any) {
+      const Rows next = find(step, ids);
+      ids = ask_block(a, w.seq, token_of(step + W));
+      load_keys<D>(next, lane, k);
+      load_values<D>(next, lane, v);
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) st[r].l += l[r];
-  };
-  auto next_rows = [&] {
-    const Rows next = find(step + W, ids);
-    ids = block_id(a, w.seq, token_of(step + 2 * W));
-    return next;
-  };
-  for (; step < end; step += W) {
-    if (step * kStep + kStep > fewest && any_not_finite<T, D>(v)) break;
-    const Rows next = next_rows();
-    weights(next);
-    Op weight[R];
+    // waited for here: in the loop the wait would be one for all loads, at every step
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      weight[r] = __builtin_bit_cast(
-          Op, make_uint4(Mat<T>::pack(p[r][0], p[r][1]), Mat<T>::pack(p[r][2], p[r][3]),
-                         Mat<T>::pack(p[r][4], p[r][5]), Mat<T>::pack(p[r][6], p[r][7])));
 #pragma unroll
-    for (int j = 0; j < NT; j += 2) {
-      Op even, odd;
-      columns<T, D>(v, j, even, odd);
+      for (int x = 0; x < D / 32; ++x) asm volatile("" : "+v"(q[r].part[x]));
+    float slack = kSlack;
+    State<D> st[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) clear(st[r]);
+    // where this lane's scores go
+    uint64_t scores_at[R];
+    bool scores_kept[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const Row row = row_at(16 * r + (lane & 15));
+      scores_at[r] = reinterpret_cast<uint64_t>(
+          a.scores + (row.at * (a.heads * a.group) + row.head) * a.scores_row + quad * 4);
+      scores_kept[r] = a.scores && 16 * r + (lane & 15) < rows;
+    }
+    float p[R][8];
+    // A step's weights and what they change of the rows' states; K makes room for the next step's.
+    auto weights = [&](const Rows& next) {
+      const int token = step * kStep;
+      v4f s[R][2];
+      put_keys<D>(k, lane, k_lds);
+      load_keys<D>(next, lane, k);
+      scores<T, D, R>(q, k_lds, lane, s);
+      float l[R];
+      bool passes = false;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        st[r].o[j] = Mat<T>::mul16(even, weight[r], st[r].o[j]);
-        st[r].o[j + 1] = Mat<T>::mul16(odd, weight[r], st[r].o[j + 1]);
+        if (negate) s[r][0] = -s[r][0], s[r][1] = -s[r][1];
+        if (token + kStep > fewest) hide(s[r], token, visible[r], quad);
+        if (scores_kept[r]) {
+          const uint64_t to = scores_at[r] + static_cast<uint64_t>(token) * 4;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<__attribute__((address_space(1))) v4f*>(to + 64 * h) =
+                s[r][h] * scale_log2;
+        }
+        l[r] = weigh(s[r], st[r].m, scale_log2, false, p[r]);
+        passes |= l[r] > slack;
       }
+      if (__any(passes)) {
+        // Some score passes its row's reference: the references follow, and the weights are made
+        // again; at every step from then on, where a reference is kCoarse or more.
+        bool any_coarse = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float top = st[r].m;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) top = fmaxf(top, s[r][x / 4][x % 4] * scale_log2);
+          const float m = max_over_quads(top);
+          const float fade = __builtin_amdgcn_exp2f(st[r].m - m);
+          st[r].m = m;
+          st[r].l *= fade;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) st[r].o[j] *= fade;
+          const bool coarse = fabsf(m) >= kCoarse && m != kNothing;
+          any_coarse |= coarse;
+          l[r] = weigh(s[r], m, scale_log2, coarse, p[r]);
+        }
+        slack = __any(any_coarse) ? -1.f : kSlack;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) st[r].l += l[r];
+    };
+    auto next_rows = [&] {
+      const Rows next = find(step + W, ids);
+      ids = ask_block(a, w.seq, token_of(step + 2 * W));
+      return next;
+    };
+    for (; step < end; step += W) {
+      if (step * kStep + kStep > fewest && any_not_finite<T, D>(v)) break;
+      const Rows next = next_rows();
+      weights(next);
+      Op weight[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        weight[r] = __builtin_bit_cast(
+            Op, make_uint4(Mat<T>::pack(p[r][0], p[r][1]), Mat<T>::pack(p[r][2], p[r][3]),
+                           Mat<T>::pack(p[r][4], p[r][5]), Mat<T>::pack(p[r][6], p[r][7])));
+#pragma unroll
+      for (int j = 0; j < NT; j += 2) {
+        Op even, odd;
+        columns<T, D>(v, j, even, odd);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          st[r].o[j] = Mat<T>::mul16(even, weight[r], st[r].o[j]);
+          st[r].o[j + 1] = Mat<T>::mul16(odd, weight[r], st[r].o[j + 1]);
+        }
+      }
+      load_values<D>(next, lane, v);
     }
-    load_values<D>(next, lane, v);
-  }
-  // From a step on whose V holds an infinity or a NaN that some row may not see: a loop of its own,
-  // as its registers would be the other's.
+    // From a step on whose V holds an infinity or a NaN that some row may not see: a loop of its own,
+    // as its registers would be the other's.
 #pragma unroll 1
-  for (; step < end; step += W) {
-    weights(next_rows());
+    for (; step < end; step += W) {
+      weights(next_rows());
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      add_one_by_one<T, D>(a, w.seq, at.head, step * kStep, keys, visible[r], lane, p[r], st[r]);
-  }
-  bad = least(bad);
-  // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
-  // each) adds up the elements [][i] of all.
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float l = sum_over_quads(st[r].l);
-    if (quad == 0) {
-      sum_m[wave][r][lane] = st[r].m;
-      const bool lost = w.s.keys < 0 || visible[r] > bad;
-      sum_l[wave][r][lane] = lost ? bits_f32(0x7fc00000u) : l;
+      for (int r = 0; r < R; ++r)
+        add_one_by_one<T, D>(a, w.seq, at.head, step * kStep, keys, visible[r], lane, p[r], st[r]);
     }
-  }
-  __syncthreads();
-  constexpr int kParts = W >= 8 ? 2 : 1, NJ = NT / kParts;
-  const int i = wave & 3, j0 = wave / 4 * NJ;
+    bad = least(bad);
+    // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
+    // each) adds up the elements [][i] of all.
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    float m = kNothing, l = 0.f;
-#pragma unroll
-    for (int x = 0; x < W; ++x) m = fmaxf(m, sum_m[x][r][lane & 15]);
-#pragma unroll
-    for (int x = 0; x < W; ++x)
-      l += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - m);
-    const float f = __builtin_amdgcn_exp2f(st[r].m - m);
-    if (r) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NT; ++j) shared[wave * NT + j][lane] = st[r].o[j] * f;
+    for (int r = 0; r < R; ++r) {
+      const float l = sum_over_quads(st[r].l);
+      if (quad == 0) {
+        sum_m[wave][r][lane] = st[r].m;
+        const bool lost = w.s.keys < 0 || visible[r] > bad;
+        sum_l[wave][r][lane] = lost ? bits_f32(0x7fc00000u) : l;
+      }
+    }
     __syncthreads();
-    if (wave >= 4 * kParts) continue;
-    float sums[NJ];
+    constexpr int kParts = W >= 8 ? 2 : 1, NJ = NT / kParts;
+    const int i = wave & 3, j0 = wave / 4 * NJ;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      sums[j] = 0.f;
+    for (int r = 0; r < R; ++r) {
+      float m = kNothing, l = 0.f;
+#pragma unroll
+      for (int x = 0; x < W; ++x) m = fmaxf(m, sum_m[x][r][lane & 15]);
 #pragma unroll
       for (int x = 0; x < W; ++x)
-        sums[j] += reinterpret_cast<const float*>(shared[x * NT + j0 + j])[lane * 4 + i];
-    }
-    const int n = 16 * r + (lane & 15), element = NT * (4 * quad + i) + j0;
-    if (n >= rows) continue;
-    if (w.cuts == 1) {
-      const Row row = row_at(n);
-      write_elements<T, NJ>(a, row, element, sums, inverse(l, visible[r]));
-      if (wave == 0 && quad == 0) write_stats(a, row, m, l);
-    } else {
-      const int64_t part = (part_of(a, at.item, at.head) * R + r) * kRows + (lane & 15);
-      if (wave == 0 && quad == 0) a.part_ml[part] = make_float2(m, l);
+        l += sum_l[x][r][lane & 15] * __builtin_amdgcn_exp2f(sum_m[x][r][lane & 15] - m);
+      const float f = __builtin_amdgcn_exp2f(st[r].m - m);
+      if (r) __syncthreads();
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) a.part_o[part * D + element + j] = sums[j];
+      for (int j = 0; j < NT; ++j) shared[wave * NT + j][lane] = st[r].o[j] * f;
+      __syncthreads();
+      float sums[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        sums[j] = 0.f;
+#pragma unroll
+        for (int x = 0; x < W; ++x)
+          sums[j] += reinterpret_cast<const float*>(shared[x * NT + j0 + j])[lane * 4 + i];
+      }
+      const int n = 16 * r + (lane & 15), element = NT * (4 * quad + i) + j0;
+      if (n >= rows) continue;
+      if (whole) {
+        const Row row = row_at(n);
+        write_elements<T, NJ>(a, row, element, sums, inverse(l, visible[r]));
+        if (wave == 0 && quad == 0) write_stats(a, row, m, l);
+      } else {
+        const int64_t part =
+            (part_of_piece(a, at.item, at.head, w.from == 0) * R + r) * kRows + (lane & 15);
+        if (wave == 0 && quad == 0) a.part_ml[part] = make_float2(m, l);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) a.part_o[part * D + element + j] = sums[j];
+      }
     }
+    pos += to - w.from;
+    if (pos >= pos_end) return;
   }
 }
 
@@ -558,18 +733,6 @@ struct ManyPlan {
   static constexpr int kCutSteps = 16;   // that cutting has to take off the longest sequence
 };
 constexpr int kTile = ManyPlan::kStep;
-
-// A row of a tile in LDS is D / 8 pieces of 16 bytes, piece c at c ^ f(row).  K is read with 8 and
-// more neighbouring rows of one piece at a time, V (transposed) with 4 neighbouring rows of 4
-// pieces: so that either takes all banks.
-template <int D>
-__device__ constexpr int k_swizzle(int row) {
-  return D == 64 ? row & 7 : row & 15;
-}
-template <int D>
-__device__ constexpr int v_swizzle(int row) {
-  return D == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
-}
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* LdsTransposed;
@@ -621,8 +784,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
   const int found = lane & (kPassRows * kPasses - 1);
   const int found_row = (found / kPassRows * W + wave) * kPassRows + found % kPassRows;
   auto token_of = [&](int tile) { return min(tile * kTile + found_row, keys - 1); };
-  auto find = [&](int tile, int64_t id) {
+  auto find = [&](int tile, const RawId& raw) {
     const int t = token_of(tile);
+    const int64_t id = block_id(a, raw);
     if (outside(a, id)) bad = min(bad, t);
     const uint64_t p = row_address(a, of, id, t, 0);
     return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
@@ -667,15 +831,15 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
 
-  int64_t ids = 0;
+  RawId ids{0, 0};
   Rows ahead{0, 0};
   if (begin < end) {
-    ids = block_id(a, w.seq, token_of(begin));
+    ids = ask_block(a, w.seq, token_of(begin));
     bring(find(begin, ids));
-    ids = block_id(a, w.seq, token_of(begin + 1));
+    ids = ask_block(a, w.seq, token_of(begin + 1));
     put(0, partly(begin));
     ahead = find(begin + 1, ids);
-    ids = block_id(a, w.seq, token_of(begin + 2));
+    ids = ask_block(a, w.seq, token_of(begin + 2));
   }
   // where a lane reads: K's row `column`, piece `half`; V's rows 4 half + ((lane & 15) >> 2)
   const int k_at = column * D * 2 + ((half ^ k_swizzle<D>(column)) << 4);
@@ -761,7 +925,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     }
     bring(ahead);
     ahead = find(tile + 2, ids);
-    ids = block_id(a, w.seq, token_of(tile + 3));
+    ids = ask_block(a, w.seq, token_of(tile + 3));
     weights();
     const char* const vt = lds[buffer][1];
 #pragma unroll
@@ -815,7 +979,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     }
     bring(ahead);
     ahead = find(tile + 2, ids);
-    ids = block_id(a, w.seq, token_of(tile + 3));
+    ids = ask_block(a, w.seq, token_of(tile + 3));
     put(buffer ^ 1, false);
     __syncthreads();
   }
@@ -849,28 +1013,62 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
   else a.part_ml[part] = make_float2(m, l);
 }
 
-// Joins the cuts of 16 rows of a tile of ROWS: 256 threads, each D / 16 neighbouring elements of a row,
-// take every G-th cut, and their sums are added in the order of g.
-template <class T, int D, int ROWS, class P, int G>
+// The parts of a tile as the join reads them: part(c) of `count`, of ROWS rows each.
+// Of a line: a tile's first part is in the place for those that start there.
+template <int ROWS>
+struct PiecesOfTile {
+  Piece w;
+  int first, count;        // workgroups
+  __device__ PiecesOfTile(const Args& a, int tile) {
+    int total;
+    const Line line(a, threadIdx.x & 63, ROWS);
+    const int per = deal(a, ROWS, line, &total);
+    w = find_piece(a, ROWS, line, tile, true);
+    first = uniform(w.start / per);
+    count = uniform((w.start + w.steps - 1) / per) - first + 1;
+  }
+  __device__ bool none() const { return w.seq < 0 || count == 1; }
+  __device__ int64_t part(const Args& a, int c, int head) const {
+    return part_of_piece(a, first + c, head, c == 0);
+  }
+};
+// Of a plan that cuts every tile alike.
+template <int ROWS>
+struct CutsOfTile {
+  Work w;
+  int count;
+  __device__ CutsOfTile(const Args& a, int tile) {
+    w.seq = -1;
+    if (!*a.any_cut) return;
+    w = find_work<ManyPlan>(a, tile, ROWS, true);
+    count = w.cuts;
+  }
+  __device__ bool none() const { return w.seq < 0 || count == 1; }
+  __device__ int64_t part(const Args& a, int c, int head) const {
+    return part_of(a, w.first + c, head);
+  }
+};
+
+// Joins the parts of 16 rows of a tile of ROWS: 256 threads, each D / 16 neighbouring elements of a
+// row, take every G-th part, and their sums are added in the order of g.
+template <class T, int D, int ROWS, class Parts, int G>
 __global__ __launch_bounds__(256 * G) void join_kernel(const Args a) {
   constexpr int N = D / 16, kAhead = D == 256 ? 2 : 4;
-  if (!*a.any_cut) return;
   const int t = threadIdx.x & 255, g = threadIdx.x >> 8, n = t >> 4;
   const int block = blockIdx.x / (ROWS / 16), r = blockIdx.x % (ROWS / 16);
   const int tile = a.heads_div.div(block);
   const int head = block - tile * a.heads;
-  const Work w = find_work<P>(a, tile, ROWS, true);
-  if (w.seq < 0 || w.cuts == 1) return;
+  const Parts parts(a, tile);
+  if (parts.none()) return;
+  const Seq s = parts.w.s;
   __shared__ float sum_o[G][N][256], sum_m[G][16], sum_l[G][16];
-  const int first = w.tile * ROWS + 16 * r;
-  const bool valid = first + n < w.s.count * a.group;
+  const int first = parts.w.tile * ROWS + 16 * r;
+  const bool valid = first + n < s.count * a.group;
   float o[N], m = kNothing, l = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) o[j] = 0.f;
   if (valid) {
-    const int64_t part = part_of(a, w.first, head) * ROWS + 16 * r + n;
-    const int64_t next = static_cast<int64_t>(a.heads) * ROWS;
-    for (int c0 = g; c0 < w.cuts; c0 += G * kAhead) {
+    for (int c0 = g; c0 < parts.count; c0 += G * kAhead) {
       float2 x[kAhead];
       v4f y[kAhead][N / 4];
 #pragma unroll
@@ -879,11 +1077,12 @@ __global__ __launch_bounds__(256 * G) void join_kernel(const Args a) {
         x[i] = make_float2(kNothing, 0.f);
 #pragma unroll
         for (int j = 0; j < N / 4; ++j) y[i][j] = {0.f, 0.f, 0.f, 0.f};
-        if (c < w.cuts) {
-          x[i] = a.part_ml[part + c * next];
+        if (c < parts.count) {
+          const int64_t part = parts.part(a, c, head) * ROWS + 16 * r + n;
+          x[i] = a.part_ml[part];
 #pragma unroll
           for (int j = 0; j < N / 4; ++j)
-            y[i][j] = reinterpret_cast<const v4f*>(a.part_o + (part + c * next) * D + (t & 15) * N)[j];
+            y[i][j] = reinterpret_cast<const v4f*>(a.part_o + part * D + (t & 15) * N)[j];
         }
       }
 #pragma unroll
@@ -915,13 +1114,45 @@ __global__ __launch_bounds__(256 * G) void join_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] += sum_o[x][j][t] * f;
   }
-  const Row row = row_of(a, w.s, first + n, head);
+  const Row row = row_of(a, s, first + n, head);
   write_elements<T, N>(a, row, (t & 15) * N, o, inverse(l, row.visible));
   if ((t & 15) == 0) write_stats(a, row, top, l);
 }
 
 // ---------------------------------------------------------------------------
-// What each token got: a wavefront keeps 64 tokens of K in registers and goes over the
+// What each token got, from scores that lie there: a thread adds up 4 tokens' over the rows, in
+// their order.  Bound by memory: 4 bytes a row and token (and as many to write them), where making the
+// scores again takes K's 2 D bytes a token.  32 sequences of up to 8192 keys, groups of 4: TODO us.
+
+constexpr int kAddTokens = 1024;     // of a workgroup
+
+__global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
+  const int head = blockIdx.y, seq = blockIdx.z;
+  const int at = blockIdx.x * kAddTokens + static_cast<int>(threadIdx.x) * 4;
+  const Seq s = sequence(a, seq);
+  const int keys = max(s.keys, 0), rows = s.count * a.group;
+  if (at >= keys) return;
+  float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int n = 0; n < rows; ++n) {
+    const Row row = row_of(a, s, n, head);
+    const int64_t place = row.at * (a.heads * a.group) + row.head;
+    const float2 st = a.stats[place];
+    // of steps that no row of a tile sees there are none
+    if (at >= row.visible) continue;
+    const v4f x = *reinterpret_cast<const v4f*>(a.scores + place * a.scores_row + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + i < row.visible) sums[i] += __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
+  }
+  float* const w = a.weights + seq * a.w_seq + head * a.w_head + at;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < keys) w[i] += sums[i];
+}
+
+// ---------------------------------------------------------------------------
+// What each token got, from K: a wavefront keeps 64 tokens of K in registers and goes over the
 // queries, 32 rows at a time.  A token's sum is made by one wavefront, in the rows' order.
 
 constexpr int kWeighTokens = 256;    // of a workgroup
@@ -1051,41 +1282,70 @@ struct LaunchPlan {
   int rows;               // of a tile
   bool many;              // rows are shared out to the wavefronts, else keys are
   int64_t tiles;          // times heads: the most there can be
-  bool wide;              // few tiles: more wavefronts a workgroup
-  int slots;
+  int waves;              // of a workgroup
+  int slots;              // see Sequences and Piece
+  bool together;
   int64_t workgroups;
-  size_t ml_bytes, o_bytes, stats_bytes;
+  size_t ml_bytes, o_bytes, stats_bytes, scores_bytes;
+  int64_t scores_row;     // 0: the scores are not kept
+  size_t bytes() const { return o_bytes + ml_bytes + stats_bytes + scores_bytes; }
 };
 
 constexpr int kComputeUnits = 256;
+// Scores are kept up to this size of the workspace: a table far wider than the sequences are long
+// makes it large.
+constexpr int64_t kMostScores = int64_t(1) << 30;
+// Steps of a table row from which keys are dealt out, which costs 6 to 8 us: 32 sequences of 2048 keys 43
+// us uncut and 51 dealt out; 32 of 2048 to 8192 keys 161 uncut and 133 dealt out.
+constexpr int kDealSteps = 128;
 
 LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
   LaunchPlan p;
   const int heads = c.layer.num_heads, dim = c.layer.head_size;
   const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
+  // 32 rows of 256 elements do not fit the registers
   p.rows = rows > static_cast<int64_t>(c.batch) * 32 ? 128
-           : rows > static_cast<int64_t>(c.batch) * kRows ? 32 : kRows;
+           : rows > static_cast<int64_t>(c.batch) * kRows && dim <= 128 ? 32 : kRows;
   p.many = p.rows > 32;
-  p.tiles = (c.query_starts ? rows / p.rows + c.batch
-                            : static_cast<int64_t>(c.batch) * ((c.group_size + p.rows - 1) / p.rows)) *
-            heads;
-  p.wide = p.rows == kRows && p.tiles <= kComputeUnits && dim <= 128;
+  const int64_t tiles = c.query_starts
+                            ? rows / p.rows + c.batch
+                            : static_cast<int64_t>(c.batch) * ((c.group_size + p.rows - 1) / p.rows);
+  p.tiles = tiles * heads;
   const int step = p.many ? ManyPlan::kStep : FewPlan::kStep;
-  const int least = p.many ? ManyPlan::kMinSteps + ManyPlan::kCutSteps
-                           : FewPlan::kMinSteps + FewPlan::kCutSteps;
   const int64_t most_steps =
       (static_cast<int64_t>(c.table_width) * c.layer.tokens_per_block + step - 1) / step;
-  const int places = p.many ? 2 * kComputeUnits : kComputeUnits;
-  p.slots = most_steps < least || p.tiles > 4 * kComputeUnits || p.rows == 32 ? 0
-            : p.wide || p.many ? places : static_cast<int>(p.tiles);
-  // items (cuts of a tile, of all heads), in whole rounds of the XCDs
-  const int64_t items = (p.tiles + p.slots + heads - 1) / heads;
-  p.workgroups = (items + kXcds - 1) / kXcds * kXcds * heads;
-  const int64_t part_rows = p.slots ? p.workgroups * p.rows : 0;
-  p.ml_bytes = part_rows * sizeof(float2) + (p.slots ? 16 : 0);    // and any_cut
-  p.o_bytes = part_rows * dim * sizeof(float);
-  p.stats_bytes =
-      c.weights ? static_cast<size_t>(c.num_queries) * heads * c.group_size * sizeof(float2) : 0;
+  int64_t parts;
+  p.waves = 4;
+  if (p.many) {
+    p.slots = most_steps < ManyPlan::kMinSteps + ManyPlan::kCutSteps || p.tiles > 4 * kComputeUnits
+                  ? 0 : 2 * kComputeUnits;
+    // items (cuts of a tile, of all heads), in whole rounds of the XCDs
+    const int64_t items = (p.tiles + p.slots + heads - 1) / heads;
+    p.workgroups = (items + kXcds - 1) / kXcds * kXcds * heads;
+    p.together = false;
+    parts = p.slots ? p.workgroups : 0;
+  } else {
+    // A workgroup of 8 wavefronts a compute unit, each with an even share of the steps; a tile for each
+    // workgroup where there are so many sequences that working the shares out takes long, or few keys.
+    const bool dealt = c.batch <= 4 * 64 && most_steps >= kDealSteps &&
+                       tiles * std::max<int64_t>(1, most_steps) < int64_t(1) << 31;
+    p.waves = (dealt || p.tiles <= kComputeUnits) && dim <= 128 && p.rows == kRows ? 8 : 4;
+    const int64_t places = kComputeUnits * 8 / p.waves / (dim == 256 ? 2 : 1);
+    int64_t items = dealt ? std::max<int64_t>(1, places / heads) : tiles;
+    p.together = p.rows == kRows && items >= kXcds;
+    if (p.together)                          // whole rounds of the XCDs
+      items = dealt ? items / kXcds * kXcds : (items + kXcds - 1) / kXcds * kXcds;
+    p.slots = dealt ? static_cast<int>(items) : 0;
+    p.workgroups = items * heads;
+    parts = p.slots ? 2 * p.workgroups : 0;
+  }
+  p.ml_bytes = parts * p.rows * sizeof(float2) + (parts ? 16 : 0);    // and any_cut
+  p.o_bytes = parts * p.rows * dim * sizeof(float);
+  const int64_t all_rows = static_cast<int64_t>(c.num_queries) * heads * c.group_size;
+  p.stats_bytes = c.weights ? (all_rows * sizeof(float2) + 15) / 16 * 16 : 0;
+  p.scores_row = c.weights && !p.many ? most_steps * step : 0;
+  if (static_cast<__int128>(all_rows) * p.scores_row * 4 > kMostScores) p.scores_row = 0;
+  p.scores_bytes = all_rows * p.scores_row * sizeof(float);
   return p;
 }
 
@@ -1099,30 +1359,34 @@ int check_plan(const fkv_paged_attention_args& c, const LaunchPlan& p) {
   return 0;
 }
 
-template <class T, int D, int ROWS, class P, int G>
+template <class T, int D, int ROWS, class Parts, int G>
 void join(const Args& a, const LaunchPlan& p, hipStream_t s) {
   if (p.slots)
-    hipLaunchKernelGGL((join_kernel<T, D, ROWS, P, G>), dim3(p.tiles * (ROWS / 16)), dim3(256 * G),
-                       0, s, a);
+    hipLaunchKernelGGL((join_kernel<T, D, ROWS, Parts, G>), dim3(p.tiles * (ROWS / 16)),
+                       dim3(256 * G), 0, s, a);
 }
 template <class T, int D, int R, int W>
 void launch_few(const Args& a, const LaunchPlan& p, hipStream_t s) {
   hipLaunchKernelGGL((attend_few_kernel<T, D, R, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
-  join<T, D, kRows * R, FewPlan, W == 8 ? 4 : 1>(a, p, s);
+  join<T, D, kRows * R, PiecesOfTile<kRows * R>, 4>(a, p, s);
 }
 template <class T, int D, int W>
 void launch_many(const Args& a, const LaunchPlan& p, hipStream_t s) {
   hipLaunchKernelGGL((attend_many_kernel<T, D, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
-  join<T, D, 32 * W, ManyPlan, 1>(a, p, s);
+  join<T, D, 32 * W, CutsOfTile<32 * W>, 1>(a, p, s);
 }
 template <class T, int D>
 void launch(const Args& a, const LaunchPlan& p, const fkv_paged_attention_args& c, hipStream_t s) {
   if (p.many) launch_many<T, D, 4>(a, p, s);
-  else if (p.rows == 32) launch_few<T, D, 2, 4>(a, p, s);
-  else if (p.wide) launch_few<T, D, 1, D == 256 ? 4 : 8>(a, p, s);
+  else if (p.rows == 32) launch_few<T, D, D == 256 ? 1 : 2, 4>(a, p, s);
+  else if (p.waves == 8) launch_few<T, D, 1, D == 256 ? 4 : 8>(a, p, s);
   else launch_few<T, D, 1, 4>(a, p, s);
-  if (a.weights && a.width) {
-    const int64_t most = static_cast<int64_t>(a.width) * a.tokens;
+  const int64_t most = static_cast<int64_t>(a.width) * a.tokens;
+  if (a.scores) {
+    hipLaunchKernelGGL(add_weights_kernel,
+                       dim3((most + kAddTokens - 1) / kAddTokens, a.heads, a.batch), dim3(256), 0,
+                       s, a);
+  } else if (a.weights && a.width) {
     hipLaunchKernelGGL((weigh_kernel<T, D>),
                        dim3((most + kWeighTokens - 1) / kWeighTokens, a.heads, a.batch), dim3(256),
                        0, s, a);
@@ -1142,7 +1406,7 @@ int attention(const fkv_paged_attention_args& c, fkv_stream_t stream) {
   if ((rc = check_attention(c))) return rc;
   const LaunchPlan p = launch_plan(c);
   if ((rc = check_plan(c, p))) return rc;
-  const size_t need = p.o_bytes + p.ml_bytes + p.stats_bytes;
+  const size_t need = p.bytes();
   if (need && (!c.workspace || c.workspace_bytes < need ||
                reinterpret_cast<uintptr_t>(c.workspace) % 16))
     return fail(kInval, "the workspace must hold %zu bytes on a multiple of 16, got %zu", need,
@@ -1163,6 +1427,7 @@ int attention(const fkv_paged_attention_args& c, fkv_stream_t stream) {
   a.queries = c.num_queries;
   a.tokens = c.layer.tokens_per_block, a.causal = c.causal;
   a.slots = p.slots;
+  a.together = p.together;
   a.scale_log2 = c.scale * kLog2e;
   char* const space = static_cast<char*>(c.workspace);
   a.part_o = reinterpret_cast<float*>(space);
@@ -1170,6 +1435,9 @@ int attention(const fkv_paged_attention_args& c, fkv_stream_t stream) {
   a.part_ml = reinterpret_cast<float2*>(space + p.o_bytes + 16);
   a.weights = c.weights, a.w_seq = c.weights_seq_stride, a.w_head = c.weights_head_stride;
   a.stats = c.weights ? reinterpret_cast<float2*>(space + p.o_bytes + p.ml_bytes) : nullptr;
+  a.scores_row = p.scores_row;
+  if (p.scores_row)
+    a.scores = reinterpret_cast<float*>(space + p.o_bytes + p.ml_bytes + p.stats_bytes);
   a.tokens_div = FastDiv(a.tokens), a.group_div = FastDiv(a.group), a.heads_div = FastDiv(a.heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   int dev = 0;
@@ -1207,7 +1475,7 @@ int fkv_paged_attention_workspace(const fkv_paged_attention_args* args, size_t* 
     if (rc || args->batch == 0 || args->num_queries == 0) return rc;
     const LaunchPlan p = launch_plan(*args);
     if ((rc = check_plan(*args, p))) return rc;
-    *bytes = p.o_bytes + p.ml_bytes + p.stats_bytes;
+    *bytes = p.bytes();
     return 0;
   });
 }

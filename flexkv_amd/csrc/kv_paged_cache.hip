@@ -98,6 +98,7 @@ __device__ inline uint32_t order_of(float f) {
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kRadixBits = 11;       // of a pass: three of them
 constexpr int kRounds = 8;           // of kSelectThreads tokens, between two barriers
+constexpr int kAtOnce = 16;          // loads of a thread in flight
 
 // Inclusive sums over the workgroup's threads.  `totals` holds kSelectWaves values and may not be
 // in use.
@@ -118,15 +119,35 @@ __device__ inline int scan_threads(int v, int* totals) {
 __device__ inline uint32_t threshold_of(const float* w, int n, int need, int* histogram,
                                         int* totals, int* ties) {
   __shared__ int found[2];
+  const int lane = threadIdx.x & 63;
   uint64_t prefix = 0;
   // of 33 bits, so that the digits are alike: the first has a 0 before it
   for (int shift = 2 * kRadixBits; shift >= 0; shift -= kRadixBits) {
     for (int i = threadIdx.x; i < 1 << kRadixBits; i += kSelectThreads) histogram[i] = 0;
     __syncthreads();
-    for (int t = threadIdx.x; t < n; t += kSelectThreads) {
-      const uint64_t k = order_of(w[t]);
-      if (k >> (shift + kRadixBits) == prefix)
-        atomicAdd(&histogram[(k >> shift) & ((1 << kRadixBits) - 1)], 1);
+    for (int t0 = 0; t0 < n; t0 += kAtOnce * kSelectThreads) {
+      float x[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int t = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x);
+        x[j] = w[min(t, n - 1)];
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const uint64_t k = order_of(x[j]);
+        const bool in = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x) < n &&
+                        k >> (shift + kRadixBits) == prefix;
+        const uint64_t all = __ballot(in);
+        if (!all) continue;
+        const int digit = (k >> shift) & ((1 << kRadixBits) - 1);
+        // Weights that are alike (none has got any yet) would queue for one counter.
+        const int lead = lane_value(digit, __builtin_ctzll(all));
+        if (__ballot(in && digit == lead) == all) {
+          if (lane == __builtin_ctzll(all)) atomicAdd(&histogram[lead], __popcll(all));
+        } else if (in) {
+          atomicAdd(&histogram[digit], 1);
+        }
+      }
     }
     __syncthreads();
     // a thread has two digits, the first thread the largest
