@@ -1153,7 +1153,8 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
 
 // ---------------------------------------------------------------------------
 // What each token got, from K: a wavefront keeps 64 tokens of K in registers and goes over the
-// queries, 32 rows at a time.  A token's sum is made by one wavefront, in the rows' order.
+// queries, 32 rows at a time, the next of them on their way meanwhile.  Here the tokens are the columns
+// of the products, so that a lane adds up its own token's weights, in the rows' order.
 
 constexpr int kWeighTokens = 256;    // of a workgroup
 
@@ -1161,36 +1162,55 @@ template <class T, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args a) {
   using Op = typename Mat<T>::Op;
   constexpr int KS = D / 16;
+  __shared__ float2 row_stats[4][32];          // of a wavefront's 32 rows
+  __shared__ int row_visible[4][32];
   const int head = blockIdx.y, seq = blockIdx.z;
+  const int wave = uniform(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
-  const int at = blockIdx.x * kWeighTokens + uniform(threadIdx.x >> 6) * 64;
+  const int at = blockIdx.x * kWeighTokens + wave * 64;
   const Seq s = sequence(a, seq);
   // too long for its table row: NaN in all rows, and in the tokens of no block
   const int keys = max(s.keys, 0), rows = s.count * a.group;
   if (at >= keys || rows <= 0) return;
-  Op k[2][KS];
+  Op k[2][KS], q[KS];
+  float2 stats;
+  int visible;
+  auto bring = [&](int r0) {
+    const Row row = row_of(a, s, min(r0 + column, rows - 1), head);
+    visible = r0 + column < rows ? row.visible : 0;
+    stats = a.stats[row.at * (a.heads * a.group) + row.head];
+    const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + half * 16;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int t = min(at + 32 * h + column, keys - 1);
-    const uint64_t p = row_address(a, a.k, block_id(a, seq, t), t, head) + half * 16;
+    for (int x = 0; x < KS; ++x) q[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 32 * x));
+  };
+  // the first row that sees the first of the tokens
+  const int hidden = a.causal ? max(0, at + s.count - keys) * a.group : 0;
+  int r0 = hidden & ~31;
+  {
+    const RawId id[2] = {ask_block(a, seq, min(at + column, keys - 1)),
+                         ask_block(a, seq, min(at + 32 + column, keys - 1))};
+    bring(r0);
 #pragma unroll
-    for (int x = 0; x < KS; ++x) k[h][x] = __builtin_bit_cast(Op, load<Vec4>(p + 32 * x));
+    for (int h = 0; h < 2; ++h) {
+      const int t = min(at + 32 * h + column, keys - 1);
+      const uint64_t p = row_address(a, a.k, block_id(a, id[h]), t, head) + half * 16;
+#pragma unroll
+      for (int x = 0; x < KS; ++x) k[h][x] = __builtin_bit_cast(Op, load<Vec4>(p + 32 * x));
+    }
   }
-  const float scale_log2 = score_scale(a.scale_log2);
-  const bool negate = a.scale_log2 < 0.f;
-  v16f sums[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sums[h][i] = 0.f;
-  // the first row that sees the first of the tokens
-  const int hidden = a.causal ? max(0, at + s.count - keys) * a.group : 0;
-  for (int r0 = hidden & ~31; r0 < rows; r0 += 32) {
-    const int n = min(r0 + column, rows - 1);
-    const Row row = row_of(a, s, n, head);
-    const int visible = r0 + column < rows ? row.visible : 0;
-    const float2 st = a.stats[row.at * (a.heads * a.group) + row.head];
-    const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + half * 16;
+    for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(k[h][x]));
+  const float scale_log2 = score_scale(a.scale_log2);
+  const bool negate = a.scale_log2 < 0.f;
+  float sums[2] = {0.f, 0.f};
+  for (; r0 < rows; r0 += 32) {
+    // a wavefront's own: its LDS accesses are in order
+    if (half == 0) row_stats[wave][column] = stats, row_visible[wave][column] = visible;
+    // of the rows there are, in order, the first sees the fewest; past the last nothing is seen
+    const bool all_see = r0 + 32 <= rows && lane_value(visible, 0) >= at + 64;
+    const bool any_coarse = __any(fabsf(stats.x) >= kCoarse);
     v16f acc[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -1198,37 +1218,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
       for (int i = 0; i < 16; ++i) acc[h][i] = 0.f;
 #pragma unroll
     for (int x = 0; x < KS; ++x) {
-      const Op q = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 32 * x));
-      acc[0] = Mat<T>::mul32(k[0][x], q, acc[0]);
-      acc[1] = Mat<T>::mul32(k[1][x], q, acc[1]);
+      acc[0] = Mat<T>::mul32(q[x], k[0][x], acc[0]);
+      acc[1] = Mat<T>::mul32(q[x], k[1][x], acc[1]);
     }
-    const bool coarse = fabsf(st.x) >= kCoarse;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = at + 32 * h + 8 * (i / 4) + 4 * half + i % 4;
-        const float score = negate ? -acc[h][i] : acc[h][i];
-        const float e = __builtin_amdgcn_exp2f(coarse ? rounded_less(score, scale_log2, st.x)
-                                                      : __builtin_fmaf(score, scale_log2, -st.x));
-        if (t < visible) sums[h][i] += e * st.y;
-      }
-  }
-  // over the 32 rows of a half wavefront; lane `column` then has token 8 (column / 4 % 4) + 4 half
-  // + column % 4 of its h = column / 16
-  float mine = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
+    bring(min(r0 + 32, rows - 1));
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float x = sums[h][i];
+      const int n = 8 * (i / 4) + 4 * half + i % 4;
+      const float2 st = row_stats[wave][n];
+      const int seen = all_see ? 0 : row_visible[wave][n];
 #pragma unroll
-      for (int y = 1; y < 32; y *= 2) x += __shfl_xor(x, y);
-      if (column == 16 * h + i) mine = x;
+      for (int h = 0; h < 2; ++h) {
+        const float score = negate ? -acc[h][i] : acc[h][i];
+        const float e = __builtin_amdgcn_exp2f(any_coarse && fabsf(st.x) >= kCoarse
+                                                   ? rounded_less(score, scale_log2, st.x)
+                                                   : __builtin_fmaf(score, scale_log2, -st.x));
+        if (all_see || at + 32 * h + column < seen) sums[h] += e * st.y;
+      }
     }
-  const int i = column & 15;
-  const int t = at + 32 * (column >> 4) + 8 * (i / 4) + 4 * half + i % 4;
-  if (t < keys) a.weights[seq * a.w_seq + head * a.w_head + t] += mine;
+    __builtin_amdgcn_wave_barrier();
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const auto both =
+        __builtin_amdgcn_permlane32_swap(f32_bits(sums[h]), f32_bits(sums[h]), false, false);
+    sums[h] = bits_f32(both[0]) + bits_f32(both[1]);
+  }
+  // lanes below 32 have the first 32 tokens' sums to store, the others the second's
+  const int t = at + lane;
+  if (t < keys) a.weights[seq * a.w_seq + head * a.w_head + t] += half ? sums[1] : sums[0];
 }
 
 // ---------------------------------------------------------------------------

@@ -98,7 +98,6 @@ __device__ inline uint32_t order_of(float f) {
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kRadixBits = 11;       // of a pass: three of them
 constexpr int kRounds = 8;           // of kSelectThreads tokens, between two barriers
-constexpr int kAtOnce = 16;          // loads of a thread in flight
 
 // Inclusive sums over the workgroup's threads.  `totals` holds kSelectWaves values and may not be
 // in use.
@@ -113,62 +112,106 @@ __device__ inline int scan_threads(int v, int* totals) {
   return v + before;
 }
 
-// The need-th largest weight's order among w[0 .. n), 0 < need < n: the digits of the order from
-// the highest on, each from a histogram of the values that share the digits before.
-// `ties`: how many of that order are among the need largest.
-__device__ inline uint32_t threshold_of(const float* w, int n, int need, int* histogram,
-                                        int* totals, int* ties) {
-  __shared__ int found[2];
-  const int lane = threadIdx.x & 63;
-  uint64_t prefix = 0;
-  // of 33 bits, so that the digits are alike: the first has a 0 before it
-  for (int shift = 2 * kRadixBits; shift >= 0; shift -= kRadixBits) {
-    for (int i = threadIdx.x; i < 1 << kRadixBits; i += kSelectThreads) histogram[i] = 0;
-    __syncthreads();
-    for (int t0 = 0; t0 < n; t0 += kAtOnce * kSelectThreads) {
-      float x[kAtOnce];
+// Tokens t of [0, n) and their weights' orders, kAtOnce loads of a thread in flight.
+constexpr int kAtOnce = 8;
+template <class F>
+__device__ inline void each_order(const float* w, int n, F f) {
+  for (int t0 = 0; t0 < n; t0 += kAtOnce * kSelectThreads) {
+    float x[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const int t = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x);
-        x[j] = w[min(t, n - 1)];
-      }
+    for (int j = 0; j < kAtOnce; ++j)
+      x[j] = w[min(t0 + j * kSelectThreads + static_cast<int>(threadIdx.x), n - 1)];
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const uint64_t k = order_of(x[j]);
-        const bool in = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x) < n &&
-                        k >> (shift + kRadixBits) == prefix;
-        const uint64_t all = __ballot(in);
-        if (!all) continue;
-        const int digit = (k >> shift) & ((1 << kRadixBits) - 1);
-        // Weights that are alike (none has got any yet) would queue for one counter.
-        const int lead = lane_value(digit, __builtin_ctzll(all));
-        if (__ballot(in && digit == lead) == all) {
-          if (lane == __builtin_ctzll(all)) atomicAdd(&histogram[lead], __popcll(all));
-        } else if (in) {
-          atomicAdd(&histogram[digit], 1);
-        }
-      }
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (t0 + j * kSelectThreads >= n) break;
+      f(order_of(x[j]), t0 + j * kSelectThreads + static_cast<int>(threadIdx.x) < n);
     }
-    __syncthreads();
-    // a thread has two digits, the first thread the largest
-    const int top = (1 << kRadixBits) - 1 - 2 * static_cast<int>(threadIdx.x);
-    const int c0 = histogram[top], c1 = histogram[top - 1];
-    const int upto = scan_threads(c0 + c1, totals), before = upto - c0 - c1;
-    if (before < need && need <= upto) {
-      const bool first = need <= before + c0;
-      found[0] = first ? top : top - 1;
-      found[1] = need - before - (first ? 0 : c0);
-    }
-    __syncthreads();
-    prefix = prefix << kRadixBits | static_cast<uint64_t>(found[0]);
-    need = found[1];
   }
-  *ties = need;
-  return static_cast<uint32_t>(prefix);
+}
+
+// The digit (of the 2 to the kRadixBits that `histogram` counts) where the need-th largest is, and
+// how many of those with that digit are still needed; `found` is for two threads to tell all.
+struct Digit {
+  int value, need, count;
+};
+__device__ inline Digit digit_of(const int* histogram, int need, int* totals, int* found) {
+  // a thread has two digits, the first thread the largest
+  const int top = (1 << kRadixBits) - 1 - 2 * static_cast<int>(threadIdx.x);
+  const int c0 = histogram[top], c1 = histogram[top - 1];
+  const int upto = scan_threads(c0 + c1, totals), before = upto - c0 - c1;
+  if (before < need && need <= upto) {
+    const bool first = need <= before + c0;
+    found[0] = first ? top : top - 1;
+    found[1] = need - before - (first ? 0 : c0);
+    found[2] = first ? c0 : c1;
+  }
+  __syncthreads();
+  return {found[0], found[1], found[2]};
+}
+
+// The need-th largest weight's order among w[0 .. n), 0 < need < n: the digits of the order from
+// the highest on (11, 11 and 10 bits), each from a histogram of the values that share the digits
+// before.  Those that share the first are mostly few, and then the rest is found among them alone.
+// `ties`: how many of that order are among the need largest.
+constexpr int kMostCandidates = 8192;
+struct Chooser {
+  int histogram[1 << kRadixBits];
+  int totals[kSelectWaves], found[3], fill;
+  uint32_t candidates[kMostCandidates];
+};
+__device__ inline uint32_t threshold_of(const float* w, int n, int need, Chooser& c, int* ties) {
+  auto clear = [&] {
+    for (int i = threadIdx.x; i < 1 << kRadixBits; i += kSelectThreads) c.histogram[i] = 0;
+    if (threadIdx.x == 0) c.fill = 0;
+    __syncthreads();
+  };
+  auto count = [&](uint32_t digit, bool in) {
+    // weights that are alike (none has got any yet) would queue for one counter
+    const uint64_t all = __ballot(in);
+    if (!all) return;
+    const int at = __builtin_ctzll(all);
+    const uint32_t lead = lane_value(digit, at);
+    if (__ballot(in && digit == lead) == all) {
+      if ((threadIdx.x & 63) == at) atomicAdd(&c.histogram[lead], __popcll(all));
+    } else if (in) {
+      atomicAdd(&c.histogram[digit], 1);
+    }
+  };
+  clear();
+  each_order(w, n, [&](uint32_t k, bool in) { count(k >> 21, in); });
+  __syncthreads();
+  const Digit high = digit_of(c.histogram, need, c.totals, c.found);
+  const uint32_t first = high.value;
+  clear();
+  const bool listed = high.count <= kMostCandidates;
+  if (listed) {
+    each_order(w, n, [&](uint32_t k, bool in) {
+      if (in && k >> 21 == first) c.candidates[atomicAdd(&c.fill, 1)] = k;
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < high.count; i += kSelectThreads)
+      atomicAdd(&c.histogram[c.candidates[i] >> 10 & 2047], 1);
+  } else {
+    each_order(w, n, [&](uint32_t k, bool in) { count(k >> 10 & 2047, in && k >> 21 == first); });
+  }
+  __syncthreads();
+  const Digit middle = digit_of(c.histogram, high.need, c.totals, c.found);
+  const uint32_t second = first << 11 | static_cast<uint32_t>(middle.value);
+  clear();
+  if (listed) {
+    for (int i = threadIdx.x; i < high.count; i += kSelectThreads)
+      if (c.candidates[i] >> 10 == second) atomicAdd(&c.histogram[c.candidates[i] & 1023], 1);
+  } else {
+    each_order(w, n, [&](uint32_t k, bool in) { count(k & 1023, in && k >> 10 == second); });
+  }
+  __syncthreads();
+  const Digit low = digit_of(c.histogram, middle.need, c.totals, c.found);
+  *ties = low.need;
+  return second << 10 | static_cast<uint32_t>(low.value);
 }
 
 __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const EvictArgs a) {
-  __shared__ int histogram[1 << kRadixBits], totals[kSelectWaves];
+  __shared__ Chooser chooser;
   __shared__ int counts[kRounds * kSelectWaves];
   const int b = a.heads_div.div(blockIdx.x), h = blockIdx.x - b * a.heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -180,18 +223,23 @@ __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const Evic
   const int others = max(n, 0) - recent, need = count - recent;
   uint32_t threshold = need ? 0 : 0xffffffffu;
   int ties = need;                   // all, where all stay
-  if (need && need < others) threshold = threshold_of(w, others, need, histogram, totals, &ties);
+  if (need && need < others) threshold = threshold_of(w, others, need, chooser, &ties);
   int above = 0, equal = 0;          // kept for their weight, and of the threshold's, so far
   for (int t0 = 0; t0 < n; t0 += kRounds * kSelectThreads) {
     float x[kRounds];
     uint64_t over[kRounds], same[kRounds];
 #pragma unroll
+    for (int j = 0; j < kRounds; ++j)
+      x[j] = w[min(t0 + j * kSelectThreads + static_cast<int>(threadIdx.x), n - 1)];
+#pragma unroll
     for (int j = 0; j < kRounds; ++j) {
-      const int t = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x);
-      x[j] = t < n ? w[t] : 0.f;
-      const uint32_t k = order_of(x[j]);
-      over[j] = __ballot(t < n && (t >= others || k > threshold));
-      same[j] = __ballot(t < others && k == threshold);
+      over[j] = same[j] = 0;
+      if (t0 + j * kSelectThreads < n) {
+        const int t = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x);
+        const uint32_t k = order_of(x[j]);
+        over[j] = __ballot(t < n && (t >= others || k > threshold));
+        same[j] = __ballot(t < others && k == threshold);
+      }
       if (lane == 0)
         counts[j * kSelectWaves + wave] = __popcll(over[j]) | __popcll(same[j]) << 16;
     }
@@ -202,9 +250,10 @@ __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const Evic
     const int all = lane_value(pair, 63);
 #pragma unroll
     for (int j = 0; j < kRounds; ++j) {
+      if (!(over[j] | same[j])) continue;
       const int at = j * kSelectWaves + wave;
-      int before = __shfl(pair - c0 - c1, at >> 1);
-      if (at & 1) before += __shfl(c0, at >> 1);
+      int before = lane_value(pair - c0 - c1, uniform(at >> 1));
+      if (at & 1) before += lane_value(c0, uniform(at >> 1));
       const uint64_t mine = uint64_t(1) << lane, below = mine - 1;
       const int n_over = above + (before & 0xffff) + __popcll(over[j] & below);
       const int n_same = equal + (before >> 16) + __popcll(same[j] & below);
