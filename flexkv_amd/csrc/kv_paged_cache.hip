@@ -97,8 +97,6 @@ __device__ inline uint32_t order_of(float f) {
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kRadixBits = 11;       // of a pass: three of them
-constexpr int kRounds = 8;           // of kSelectThreads tokens, between two barriers
-
 // Inclusive sums over the workgroup's threads.  `totals` holds kSelectWaves values and may not be
 // in use.
 __device__ inline int scan_threads(int v, int* totals) {
@@ -111,20 +109,38 @@ __device__ inline int scan_threads(int v, int* totals) {
   for (int i = 0; i < kSelectWaves; ++i) before += i < wave ? totals[i] : 0;
   return v + before;
 }
-
-// Tokens t of [0, n) and their weights' orders, kAtOnce loads of a thread in flight.
+// A thread's values of kAtOnce * kSelectThreads tokens from t0 on: loads in flight together.
 constexpr int kAtOnce = 8;
-template <class F>
-__device__ inline void each_order(const float* w, int n, F f) {
-  for (int t0 = 0; t0 < n; t0 += kAtOnce * kSelectThreads) {
-    float x[kAtOnce];
+struct Batch {
+  static constexpr int kTokens = kAtOnce * kSelectThreads;
+  float x[kAtOnce];
+  __device__ void load(const float* w, int t0, int n) {
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j)
       x[j] = w[min(t0 + j * kSelectThreads + static_cast<int>(threadIdx.x), n - 1)];
+  }
+  // f(order, whether there is such a token)
+  template <class F>
+  __device__ void each(int t0, int n, F f) const {
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      if (t0 + j * kSelectThreads >= n) break;
-      f(order_of(x[j]), t0 + j * kSelectThreads + static_cast<int>(threadIdx.x) < n);
+    for (int j = 0; j < kAtOnce; ++j)
+      if (t0 + j * kSelectThreads < n)
+        f(order_of(x[j]), t0 + j * kSelectThreads + static_cast<int>(threadIdx.x) < n);
+  }
+};
+// All tokens, the next two batches on their way while one is looked at.
+template <class F>
+__device__ inline void each_order(const float* w, int n, F f) {
+  Batch x[3];
+  x[0].load(w, 0, n);
+  x[1].load(w, Batch::kTokens, n);
+  for (int t0 = 0; t0 < n; t0 += 3 * Batch::kTokens) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int t = t0 + i * Batch::kTokens;
+      if (t >= n) break;
+      x[(i + 2) % 3].load(w, t + 2 * Batch::kTokens, n);
+      x[i].each(t, n, f);
     }
   }
 }
@@ -210,11 +226,13 @@ __device__ inline uint32_t threshold_of(const float* w, int n, int need, Chooser
   return second << 10 | static_cast<uint32_t>(low.value);
 }
 
+// Bound by one compute unit's instructions and two dozen barriers: 65536 tokens TODO us, 777 TODO.
 __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const EvictArgs a) {
   __shared__ Chooser chooser;
-  __shared__ int counts[kRounds * kSelectWaves];
+  __shared__ int counts[kAtOnce * kSelectWaves];
+  static_assert(kAtOnce * kSelectWaves == 2 * 64, "two a lane below");
   const int b = a.heads_div.div(blockIdx.x), h = blockIdx.x - b * a.heads;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = keys_of(a, b);
   int* const kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
   const float* const w = a.weights + b * a.w_seq + h * a.w_head;
@@ -225,31 +243,31 @@ __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const Evic
   int ties = need;                   // all, where all stay
   if (need && need < others) threshold = threshold_of(w, others, need, chooser, &ties);
   int above = 0, equal = 0;          // kept for their weight, and of the threshold's, so far
-  for (int t0 = 0; t0 < n; t0 += kRounds * kSelectThreads) {
-    float x[kRounds];
-    uint64_t over[kRounds], same[kRounds];
+  Batch x, next;
+  if (n > 0) next.load(w, 0, n);
+  for (int t0 = 0; t0 < n; t0 += Batch::kTokens) {
+    x = next;
+    next.load(w, t0 + Batch::kTokens, n);
+    uint64_t over[kAtOnce], same[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kRounds; ++j)
-      x[j] = w[min(t0 + j * kSelectThreads + static_cast<int>(threadIdx.x), n - 1)];
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
+    for (int j = 0; j < kAtOnce; ++j) {
       over[j] = same[j] = 0;
       if (t0 + j * kSelectThreads < n) {
         const int t = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x);
-        const uint32_t k = order_of(x[j]);
+        const uint32_t k = order_of(x.x[j]);
         over[j] = __ballot(t < n && (t >= others || k > threshold));
         same[j] = __ballot(t < others && k == threshold);
       }
       if (lane == 0)
         counts[j * kSelectWaves + wave] = __popcll(over[j]) | __popcll(same[j]) << 16;
     }
-    __syncthreads();
+    __syncthreads();                 // all have this batch, which the stores below may be to
     // sums over (round, wave) in the tokens' order: two of the 128 a lane, in every wave
     const int c0 = counts[2 * lane], c1 = counts[2 * lane + 1];
     const int pair = scan_lanes(c0 + c1);
     const int all = lane_value(pair, 63);
 #pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
+    for (int j = 0; j < kAtOnce; ++j) {
       if (!(over[j] | same[j])) continue;
       const int at = j * kSelectWaves + wave;
       int before = lane_value(pair - c0 - c1, uniform(at >> 1));
@@ -260,8 +278,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const Evic
       if ((over[j] & mine) || ((same[j] & mine) && n_same < ties)) {
         const int rank = n_over + min(n_same, ties);
         kept[rank] = t0 + j * kSelectThreads + static_cast<int>(threadIdx.x);
-        // may be w itself: its tokens up to here have been read by all
-        if (nw) nw[rank] = x[j];
+        if (nw) nw[rank] = x.x[j];
       }
     }
     above += all & 0xffff;
@@ -277,11 +294,10 @@ __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const Evic
 
 // A workgroup copies chunk_rows kept rows of one (sequence, head), K and V.  Where each lies and
 // goes is worked out once, a row a thread, and shared.
-constexpr int kMostRows = 128;
+constexpr int kMostRows = 64;
 __global__ __launch_bounds__(kThreads) void evict_copy_kernel(const EvictArgs a) {
   __shared__ const char* from[2][kMostRows];
   __shared__ char* to[2][kMostRows];
-  // the heads of a chunk next to each other: their rows are neighbours in the cache
   const int rest = a.heads_div.div(blockIdx.x), h = blockIdx.x - rest * a.heads;
   const int b = a.chunks_div.div(rest), first = (rest - b * a.chunks) * a.chunk_rows;
   const int count = min(max(keys_of(a, b), 0), a.budget);
@@ -308,24 +324,28 @@ __global__ __launch_bounds__(kThreads) void evict_copy_kernel(const EvictArgs a)
   __syncthreads();
   const int units = rows * static_cast<int>(a.vecs.d);
   constexpr int kAhead = 4;
-  for (int k = 0; k < a.halves; ++k)
-    for (int u0 = threadIdx.x; u0 < units; u0 += kAhead * kThreads) {
-      Vec4 x[kAhead];
-      char* p[kAhead];
+  for (int u0 = threadIdx.x; u0 < units; u0 += kAhead * kThreads) {
+    Vec4 x[2][kAhead];
+    int row[kAhead], piece[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int u = u0 + j * kThreads;
-        p[j] = nullptr;
-        if (u >= units) continue;
-        const int row = a.vecs.div(u), at = (u - row * static_cast<int>(a.vecs.d)) * 16;
-        if (!from[k][row]) continue;
-        x[j] = *reinterpret_cast<const Vec4*>(from[k][row] + at);
-        p[j] = to[k][row] + at;
-      }
+    for (int j = 0; j < kAhead; ++j) {
+      const int u = u0 + j * kThreads;
+      row[j] = a.vecs.div(u);
+      piece[j] = (u - row[j] * static_cast<int>(a.vecs.d)) * 16;
+      if (u >= units || !from[0][row[j]]) row[j] = -1;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (row[j] >= 0 && k < a.halves)
+          x[k][j] = __builtin_nontemporal_load(
+              reinterpret_cast<const Vec4*>(from[k][row[j]] + piece[j]));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
-        if (p[j]) *reinterpret_cast<Vec4*>(p[j]) = x[j];
-    }
+        if (row[j] >= 0 && k < a.halves)
+          __builtin_nontemporal_store(x[k][j], reinterpret_cast<Vec4*>(to[k][row[j]] + piece[j]));
+  }
 }
 
 int check_evict(const fkv_evict_args& c) {
