@@ -24,6 +24,7 @@
 #include <cstdint>
 #include <exception>
 #include <type_traits>
+#include <utility>
 
 #include "kv_attention.h"
 #include "kv_paged.h"
@@ -110,6 +111,14 @@ struct Args : Sequences {
   float* scores;
   int64_t scores_row;
 };
+
+// Eight elements of a query: their negatives where the scale is negative, so that it is not looked
+// at again.
+template <class T>
+__device__ inline typename Mat<T>::Op query_part(const char* p, bool negate) {
+  const uint32_t flip = negate ? 0x80008000u : 0u;
+  return __builtin_bit_cast(typename Mat<T>::Op, *reinterpret_cast<const Vec4*>(p) ^ flip);
+}
 
 // 16 bytes of device memory; not a flat access, which would wait for LDS as well.
 template <class V>
@@ -497,7 +506,6 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
   const int wave = uniform(threadIdx.x >> 6);
   char* const k_lds = reinterpret_cast<char*>(shared[wave * NT]);
   const float scale_log2 = score_scale(a.scale_log2);
-  const bool negate = a.scale_log2 < 0.f;
   // nothing but its own sequence's length is read where each has a tile for one workgroup
   const bool alone = !a.slots && !a.starts;
   const Line line(a, alone ? a.batch : threadIdx.x & 63, kRowsATile);
@@ -557,7 +565,7 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
       const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + quad * 16;
 #pragma unroll
       for (int x = 0; x < D / 32; ++x)
-        q[r].part[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 64 * x));
+        q[r].part[x] = query_part<T>(p + 64 * x, a.scale_log2 < 0.f);
     }
     if (any) {
       const Rows next = find(step, ids);
@@ -585,18 +593,15 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
       scores_kept[r] = a.scores && 16 * r + (lane & 15) < rows;
     }
     float p[R][8];
-    // A step's weights and what they change of the rows' states; K makes room for the next step's.
-    auto weights = [&](const Rows& next) {
+    // A step's scores, with K in LDS, its weights, and what these change of the rows' states.
+    auto weights = [&]() __attribute__((always_inline)) {
       const int token = step * kStep;
       v4f s[R][2];
-      put_keys<D>(k, lane, k_lds);
-      load_keys<D>(next, lane, k);
       scores<T, D, R>(q, k_lds, lane, s);
       float l[R];
       bool passes = false;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        if (negate) s[r][0] = -s[r][0], s[r][1] = -s[r][1];
         if (token + kStep > fewest) hide(s[r], token, visible[r], quad);
         if (scores_kept[r]) {
           const uint64_t to = scores_at[r] + static_cast<uint64_t>(token) * 4;
@@ -632,15 +637,7 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
 #pragma unroll
       for (int r = 0; r < R; ++r) st[r].l += l[r];
     };
-    auto next_rows = [&] {
-      const Rows next = find(step + W, ids);
-      ids = ask_block(a, w.seq, token_of(step + 2 * W));
-      return next;
-    };
-    for (; step < end; step += W) {
-      if (step * kStep + kStep > fewest && any_not_finite<T, D>(v)) break;
-      const Rows next = next_rows();
-      weights(next);
+    auto add_values = [&]() __attribute__((always_inline)) {
       Op weight[R];
 #pragma unroll
       for (int r = 0; r < R; ++r)
@@ -657,16 +654,46 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
           st[r].o[j + 1] = Mat<T>::mul16(odd, weight[r], st[r].o[j + 1]);
         }
       }
+    };
+    // a step that some row does not see all of, and whose values hold an infinity or a NaN
+    auto odd_values = [&]() __attribute__((always_inline)) {
+      return step * kStep + kStep > fewest && any_not_finite<T, D>(v);
+    };
+    bool one_by_one = false;
+    for (; step < end; step += W) {
+      if (odd_values()) {
+        one_by_one = true;
+        break;
+      }
+      const Rows next = find(step + W, ids);
+      ids = ask_block(a, w.seq, token_of(step + 2 * W));
+      put_keys<D>(k, lane, k_lds);
+      load_keys<D>(next, lane, k);
+      weights();
+      add_values();
       load_values<D>(next, lane, v);
     }
-    // From a step on whose V holds an infinity or a NaN that some row may not see: a loop of its own,
-    // as its registers would be the other's.
-#pragma unroll 1
-    for (; step < end; step += W) {
-      weights(next_rows());
+    if (one_by_one) {
+      // All over again, and without loads ahead: a loop that goes on with the sums costs the other its
+      // registers.
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        add_one_by_one<T, D>(a, w.seq, at.head, step * kStep, keys, visible[r], lane, p[r], st[r]);
+      for (int r = 0; r < R; ++r) clear(st[r]);
+      slack = kSlack;
+#pragma unroll 1
+      for (step = w.from + wave; step < end; step += W) {
+        const Rows here = find(step, ask_block(a, w.seq, token_of(step)));
+        load_keys<D>(here, lane, k);
+        load_values<D>(here, lane, v);
+        put_keys<D>(k, lane, k_lds);
+        weights();
+        if (!odd_values()) {
+          add_values();
+          continue;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          add_one_by_one<T, D>(a, w.seq, at.head, step * kStep, keys, visible[r], lane, p[r], st[r]);
+      }
     }
     bad = least(bad);
     // The wavefronts' sums, each to the common reference; wavefront i (and i + 4, half
@@ -725,7 +752,8 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
 
 // ---------------------------------------------------------------------------
 // Many rows: each wavefront has 32 rows, and all of a workgroup share 64 tokens of K and V at a
-// time in LDS, double-buffered; the next tile is on its way to registers meanwhile.
+// time in LDS.  There are two places for them, and the next tile goes straight from memory into the
+// one while the other is used.
 
 struct ManyPlan {
   static constexpr int kStep = 64;       // tokens of a tile
@@ -737,6 +765,70 @@ constexpr int kTile = ManyPlan::kStep;
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* LdsTransposed;
 
+// 16 bytes a lane from memory to LDS, lane after lane from `to` on.
+__device__ inline void load_to_lds(uint64_t from, char* to) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(from),
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+__device__ inline void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The order of the instructions from the last barrier on: AHEAD reads of LDS, then, N times, M
+// matrix instructions and R reads, so that a read's latency passes behind the products before it.
+template <int AHEAD, int N, int M, int R>
+__device__ inline void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+}
+
+// Calls f with the numbers from 0 to N - 1, as types.
+template <int N, class F, int... I>
+__device__ __attribute__((always_inline)) inline void each_index(F f,
+                                                                 std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F>
+__device__ __attribute__((always_inline)) inline void each_index(F f) {
+  each_index<N>(f, std::make_integer_sequence<int, N>());
+}
+
+// The 16 rows of a tile that a wavefront brings (of K and of V), D / 8 lanes each, in the quads of 16
+// lanes: lane e of a quad finds row e of what its quad loads, [tile][K|V][pass][row in the quad], and
+// tells it to all by a broadcast within the quad.  Rows of 256 elements take two quads, which both
+// find them.
+template <int D, int W>
+struct Places {
+  static constexpr int kPieces = D / 8, kPasses = kPieces / W;
+  static constexpr int kInQuad = kPieces < 16 ? 16 / kPieces : 1;
+  static constexpr int kOfTile = 2 * kPasses * kInQuad, kTiles = 16 / kOfTile;
+  static_assert(kTiles * kOfTile == 16 && kTiles <= 2, "");
+  int nth, value, pass, in_pass;
+  __device__ Places(int lane) {
+    const int e = lane & 15;
+    nth = e / kOfTile;
+    value = e / (kPasses * kInQuad) % 2;
+    pass = e / kInQuad % kPasses;
+    in_pass = kInQuad > 1 ? (lane >> 4) * kInQuad + e % kInQuad : (lane >> 4) * 16 / kPieces;
+  }
+  // of the tile
+  __device__ int row(int wave) const { return (pass * W + wave) * (64 / kPieces) + in_pass; }
+  template <int LANE>
+  static __device__ inline uint32_t of_quad(uint32_t x) {
+    constexpr int kBroadcast = 0x150;      // of a lane to its 16
+    const int y = __builtin_amdgcn_mov_dpp(x, kBroadcast + LANE, 0xf, 0xf, true);
+    if constexpr (kInQuad == 1) return y;
+    // the first 8 lanes the first row, the others the next
+    return __builtin_amdgcn_update_dpp(y, x, kBroadcast + LANE + kInQuad - 1, 0xf, 0xc, false);
+  }
+  template <int NTH, int PASS, int VALUE>
+  static __device__ inline uint64_t row_of_quad(const Rows& r) {
+    constexpr int kLane = NTH * kOfTile + (VALUE * kPasses + PASS) * kInQuad;
+    return __builtin_bit_cast(uint64_t, Vec2{of_quad<kLane>(r.lo), of_quad<kLane>(r.hi)});
+  }
+};
+
 template <class T, int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(const Args a) {
   using Op = typename Mat<T>::Op;
@@ -745,8 +837,11 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
   constexpr int kPassRows = 64 / kPieces;     // of a wavefront in a pass
   constexpr int kHalf = kTile * D * 2;        // bytes of a tile of K or V
   constexpr int KS = D / 16, NT = D / 32;
-  __shared__ __attribute__((aligned(256))) char lds[2][2][kHalf];
-  __shared__ int odd[2][W];                   // whether a wavefront saw V that is not finite
+  // The two places are objects of their own: were they one, every read of the one would wait for the
+  // loads into the other.
+  __shared__ __attribute__((aligned(1024))) char place0[2][kHalf];
+  __shared__ __attribute__((aligned(1024))) char place1[2][kHalf];
+  __shared__ int odd[W];                      // whether a wavefront saw V that is not finite
   const Place at = heads_apart(a, blockIdx.x);
   const Work w = find_work<ManyPlan>(a, at.item, 32 * W, false);
   if (a.slots && blockIdx.x == 0 && threadIdx.x == 0) *a.any_cut = w.any_cut;
@@ -772,75 +867,81 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + half * 16;
 #pragma unroll
     for (int x = 0; x < KS; ++x)
-      q[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 32 * x));
+      q[x] = query_part<T>(p + 32 * x, a.scale_log2 < 0.f);
   }
 
-  // Which rows of a tile a wavefront brings: a lane finds one of K (below 32) or V, and gets the
-  // others' from the lanes that found them.  Block ids are asked for a tile ahead of the rows, these
-  // a tile ahead of their use; past the last key everything is of that one again.
+  // Which rows of a tile a wavefront brings: the 16 lanes of a quad find the rows that the quad
+  // loads, in `Places`, of as many tiles as there are lanes for.  Block ids are asked for that much ahead
+  // of the rows, these as much ahead of their use; past the last key everything is of that one again.
+  using P = Places<D, W>;
   int bad = kNoToken;
-  Half of = lane >= 32 ? a.v : a.k;
+  const P mine_of(lane);
+  Half of = mine_of.value ? a.v : a.k;
   of.p += at.head * of.head;
-  const int found = lane & (kPassRows * kPasses - 1);
-  const int found_row = (found / kPassRows * W + wave) * kPassRows + found % kPassRows;
+  const int found_row = mine_of.row(wave), nth = mine_of.nth;
   auto token_of = [&](int tile) { return min(tile * kTile + found_row, keys - 1); };
-  auto find = [&](int tile, const RawId& raw) {
-    const int t = token_of(tile);
+  auto find = [&](int t, const RawId& raw) {
     const int64_t id = block_id(a, raw);
     if (outside(a, id)) bad = min(bad, t);
     const uint64_t p = row_address(a, of, id, t, 0);
     return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
   };
-  Vec4 next_k[kPasses], next_v[kPasses];
-  auto bring = [&](const Rows& r) {
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int from = i * kPassRows + lane / kPieces, piece = (lane % kPieces) * 16;
-      next_k[i] = load<Vec4>(row_of_lane(r, from) + piece);
-      next_v[i] = load<Vec4>(row_of_lane(r, 32 + from) + piece);
-    }
-  };
-  auto put = [&](int buffer, bool look) {
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int r = (i * W + wave) * kPassRows + lane / kPieces, piece = lane % kPieces;
-      *reinterpret_cast<Vec4*>(&lds[buffer][0][r * D * 2 + (piece ^ k_swizzle<D>(r)) * 16]) =
-          next_k[i];
-      *reinterpret_cast<Vec4*>(&lds[buffer][1][r * D * 2 + (piece ^ v_swizzle<D>(r)) * 16]) =
-          next_v[i];
-    }
-    if (look) {
-      bool any = false;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) any |= not_finite<T>(next_v[i][x]);
-      any = __any(any);
-      if (lane == 0) odd[buffer][wave] = any;
-    }
+  // the rows found for the n-th of kTiles tiles
+  auto bring = [&](const Rows& r, auto n, char (*place)[kHalf])__attribute__((always_inline)) {
+    each_index<kPasses>([&](auto i) __attribute__((always_inline)) {
+      const int row = (i * W + wave) * kPassRows + lane / kPieces, piece = lane % kPieces;
+      load_to_lds(P::template row_of_quad<n, i, 0>(r) + ((piece ^ k_swizzle<D>(row)) << 4),
+                  place[0] + (i * W + wave) * 1024);
+      load_to_lds(P::template row_of_quad<n, i, 1>(r) + ((piece ^ v_swizzle<D>(row)) << 4),
+                  place[1] + (i * W + wave) * 1024);
+    });
   };
   // a tile that some row of the workgroup does not see all of
   auto partly = [&](int tile) { return (tile + 1) * kTile > fewest; };
+  // whether its V holds an infinity or a NaN; the same to all
+  auto any_odd = [&](char (*place)[kHalf]) __attribute__((always_inline)) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const Vec4 x = *reinterpret_cast<const Vec4*>(place[1] + (i * W + wave) * 1024 + lane * 16);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) any |= not_finite<T>(x[y]);
+    }
+    any = __any(any);
+    if (lane == 0) odd[wave] = any;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int x = 0; x < W; ++x) all |= odd[x];
+    return uniform(all) != 0;
+  };
 
   const float scale_log2 = score_scale(a.scale_log2);
-  const bool negate = a.scale_log2 < 0.f;
-  float m = kNothing, l = 0.f, slack = kSlack;
+  float m, l, slack;
   v16f o[NT];
+  auto clear = [&]() __attribute__((always_inline)) {
+    m = kNothing, l = 0.f, slack = kSlack;
 #pragma unroll
-  for (int d = 0; d < NT; ++d)
+    for (int d = 0; d < NT; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  };
+  clear();
 
   RawId ids{0, 0};
-  Rows ahead{0, 0};
+  Rows ahead{0, 0};           // of the kTiles tiles that come next
+  constexpr std::integral_constant<int, 0> k0{};
+  constexpr std::integral_constant<int, P::kTiles - 1> k1{};
   if (begin < end) {
     ids = ask_block(a, w.seq, token_of(begin));
-    bring(find(begin, ids));
-    ids = ask_block(a, w.seq, token_of(begin + 1));
-    put(0, partly(begin));
-    ahead = find(begin + 1, ids);
-    ids = ask_block(a, w.seq, token_of(begin + 2));
+    const RawId next_ids = ask_block(a, w.seq, token_of(begin + 1 + nth));
+    bring(find(token_of(begin), ids), k0, place0);
+    ahead = find(token_of(begin + 1 + nth), next_ids);
+    ids = ask_block(a, w.seq, token_of(begin + 1 + P::kTiles + nth));
   }
+  // waited for here: in the loop the wait would be one for all loads, at every tile
+#pragma unroll
+  for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(q[x]));
   // where a lane reads: K's row `column`, piece `half`; V's rows 4 half + ((lane & 15) >> 2)
   const int k_at = column * D * 2 + ((half ^ k_swizzle<D>(column)) << 4);
   int v_at[2];
@@ -850,24 +951,25 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     const int piece = ((lane >> 4 & 1) << 1) | (lane >> 1 & 1);
     v_at[j] = r * D * 2 + ((piece ^ v_swizzle<D>(r)) << 4) + (lane & 1) * 8;
   }
-  int buffer = 0, tile = begin;
-  // A tile's weights, in the place of its scores, and what they change of the row's state.
+  int tile = begin;
+  // A tile's scores, in their place its weights, and what these change of the row's state.
   v16f s[2];
-  auto scores = [&] {
-    const char* const kt = lds[buffer][0];
+  auto scores = [&](const char* kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) {
+    for (int x = 0; x < KS; ++x)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
         const Op k = __builtin_bit_cast(
             Op, *reinterpret_cast<const Vec4*>(kt + (k_at ^ (x % 8 * 32)) + x / 8 * 256 +
                                                32 * h * D * 2));
         s[h] = Mat<T>::mul32(k, q[x], s[h]);
       }
-    }
-    if (negate) s[0] = -s[0], s[1] = -s[1];
+    reads_ahead<6, KS, 2, 2>();
+    __builtin_amdgcn_sched_barrier(0);
     if (partly(tile)) {
       int seen = visible - tile * kTile - 4 * half;
       asm volatile("" : "+v"(seen));       // not 32 differences, one for each token, kept
@@ -878,7 +980,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
           if (32 * h + 8 * (i / 4) + i % 4 >= seen) s[h][i] = -INFINITY;
     }
   };
-  auto weigh_all = [&](bool coarse) {
+  auto weigh_all = [&](bool coarse) __attribute__((always_inline)) {
     float sum[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -890,13 +992,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
       }
     return sum[0] + sum[1];
   };
-  auto weights = [&] {
-    scores();
+  auto weights = [&](const char* kt) __attribute__((always_inline)) {
     float sum = weigh_all(false);
     if (__any(sum > slack)) {
       // Some score passes its row's reference: the references follow, and the weights are made
       // again, from scores made again, which would be 32 registers more if they were kept.
-      scores();
+      scores(kt);
       float top = m;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -915,19 +1016,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     }
     l += sum;
   };
-  for (; tile < end; ++tile, buffer ^= 1) {
-    __syncthreads();
-    if (partly(tile)) {
-      int any = 0;
-#pragma unroll
-      for (int x = 0; x < W; ++x) any |= odd[buffer][x];
-      if (uniform(any)) break;
-    }
-    bring(ahead);
-    ahead = find(tile + 2, ids);
-    ids = ask_block(a, w.seq, token_of(tile + 3));
-    weights();
-    const char* const vt = lds[buffer][1];
+  auto add_values = [&](const char* vt) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       uint32_t u[4];
@@ -947,42 +1036,94 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
         o[d] = Mat<T>::mul32(v, weight, o[d]);
       }
     }
-    put(buffer ^ 1, partly(tile + 1));
+    reads_ahead<8, 4 * NT, 1, 2>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The next tile's way to `there`: of two tiles whose rows were found together the first, or the second
+  // (or only one), after which those of the next are found.
+  auto bring_next = [&](auto second_of_two, char (*there)[kHalf]) __attribute__((always_inline)) {
+    if constexpr (P::kTiles == 1 || second_of_two) {
+      bring(ahead, k1, there);
+      ahead = find(token_of(tile + 2 + nth), ids);
+      ids = ask_block(a, w.seq, token_of(tile + 2 + P::kTiles + nth));
+    } else {
+      bring(ahead, k0, there);
+    }
+  };
+  // One tile from `here`, the next one's way to `there`; false where its products may have to be made
+  // one by one.
+  auto take = [&](char (*here)[kHalf], char (*there)[kHalf],
+                  auto second_of_two) __attribute__((always_inline)) {
+    wait_for_loads();
+    __syncthreads();
+    if (partly(tile) && any_odd(here)) return false;
+    __builtin_amdgcn_sched_barrier(0);
+    scores(here[0]);
+    bring_next(second_of_two, there);
+    weights(here[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    add_values(here[1]);
+    return true;
+  };
+  bool one_by_one = false;
+  while (tile < end) {
+    if (!take(place0, place1, std::false_type())) {
+      one_by_one = true;
+      break;
+    }
+    if (++tile == end) break;
+    if (!take(place1, place0, std::true_type())) {
+      one_by_one = true;
+      break;
+    }
+    ++tile;
   }
-  // From a tile on whose V holds an infinity or a NaN that some row may not see: a weight of 0
-  // does not leave it out of a matrix product, so the products are made one by one.  A loop of its
-  // own, as its registers would be the other's.
+  if (one_by_one) {
+    // V holds an infinity or a NaN that some row may not see, and a weight of 0 does not leave it out
+    // of a matrix product: those tiles' products are made one by one.  All over again, and without
+    // loads ahead, since a loop that goes on with the sums costs the other its registers.
+    clear();
 #pragma unroll 1
-  for (; tile < end; ++tile, buffer ^= 1) {
-    weights();
-    const char* const vt = lds[buffer][1];
+    for (tile = begin; tile < end; ++tile) {
+      wait_for_loads();
+      __syncthreads();                    // the tile before has been read by all
+      ids = ask_block(a, w.seq, token_of(tile));
+      bring(find(token_of(tile), ids), k0, place0);
+      wait_for_loads();
+      __syncthreads();
+      const bool odd_values = partly(tile) && any_odd(place0);
+      scores(place0[0]);
+      weights(place0[0]);
+      if (!odd_values) {
+        add_values(place0[1]);
+        continue;
+      }
 #pragma unroll 1
-    for (int t = 0; t < kTile; ++t) {
-      float x = s[0][0];
+      for (int t = 0; t < kTile; ++t) {
+        float x = s[0][0];
 #pragma unroll
-      for (int i = 1; i < 32; ++i)
-        x = (t / 32 * 16 + t % 32 / 8 * 4 + t % 4) == i ? s[i / 16][i % 16] : x;
-      x = __shfl(x, column + 32 * (t / 4 % 2));
-      const bool seen = tile * kTile + t < visible;
+        for (int i = 1; i < 32; ++i)
+          x = (t / 32 * 16 + t % 32 / 8 * 4 + t % 4) == i ? s[i / 16][i % 16] : x;
+        x = __shfl(x, column + 32 * (t / 4 % 2));
+        const bool seen = tile * kTile + t < visible;
 #pragma unroll
-      for (int d = 0; d < NT; ++d) {
-        asm volatile("" ::: "memory");
+        for (int d = 0; d < NT; ++d) {
+          asm volatile("" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(
-              vt + t * D * 2 + (((4 * d + i / 4) ^ v_swizzle<D>(t)) << 4) + half * 8 + i % 4 * 2);
-          if (!seen) continue;
-          o[d][i] += x * Mat<T>::low(u);
-          o[d][i + 1] += x * Mat<T>::high(u);
+          for (int i = 0; i < 16; i += 2) {
+            const uint32_t u = *reinterpret_cast<const uint32_t*>(
+                place0[1] + t * D * 2 + (((4 * d + i / 4) ^ v_swizzle<D>(t)) << 4) + half * 8 +
+                i % 4 * 2);
+            if (!seen) continue;
+            o[d][i] += x * Mat<T>::low(u);
+            o[d][i + 1] += x * Mat<T>::high(u);
+          }
         }
       }
     }
-    bring(ahead);
-    ahead = find(tile + 2, ids);
-    ids = ask_block(a, w.seq, token_of(tile + 3));
-    put(buffer ^ 1, false);
-    __syncthreads();
   }
+  // nothing may still be on its way to LDS when the workgroup ends and others get it
+  wait_for_loads();
   // the least bad token that any wavefront came across
   bad = least(bad);
   __shared__ int bads[W];
@@ -1181,7 +1322,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
     stats = a.stats[row.at * (a.heads * a.group) + row.head];
     const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + half * 16;
 #pragma unroll
-    for (int x = 0; x < KS; ++x) q[x] = __builtin_bit_cast(Op, *reinterpret_cast<const Vec4*>(p + 32 * x));
+    for (int x = 0; x < KS; ++x) q[x] = query_part<T>(p + 32 * x, a.scale_log2 < 0.f);
   };
   // the first row that sees the first of the tokens
   const int hidden = a.causal ? max(0, at + s.count - keys) * a.group : 0;
@@ -1203,7 +1344,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
 #pragma unroll
     for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(k[h][x]));
   const float scale_log2 = score_scale(a.scale_log2);
-  const bool negate = a.scale_log2 < 0.f;
   float sums[2] = {0.f, 0.f};
   for (; r0 < rows; r0 += 32) {
     // a wavefront's own: its LDS accesses are in order
@@ -1230,7 +1370,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
       const int seen = all_see ? 0 : row_visible[wave][n];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float score = negate ? -acc[h][i] : acc[h][i];
+        const float score = acc[h][i];
         const float e = __builtin_amdgcn_exp2f(any_coarse && fabsf(st.x) >= kCoarse
                                                    ? rounded_less(score, scale_log2, st.x)
                                                    : __builtin_fmaf(score, scale_log2, -st.x));
