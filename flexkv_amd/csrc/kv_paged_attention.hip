@@ -330,23 +330,68 @@ struct State {
   float m, l;      // the reference; the sum of this lane's tokens
 };
 
-// A lane's row of a step: lanes 0 .. 31 K's of its tokens, 32 .. 63 V's.
+// Calls f with the numbers from 0 to N - 1, as types.
+template <int N, class F, int... I>
+__device__ __attribute__((always_inline)) inline void each_index(F f,
+                                                                 std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F>
+__device__ __attribute__((always_inline)) inline void each_index(F f) {
+  each_index<N>(f, std::make_integer_sequence<int, N>());
+}
+
+// The address of a row, which a lane finds and tells the 16 lanes of its quad: lane LANE's, or, of a
+// pair, to the first 8 lanes lane LANE's and to the others the next one's.
 struct Rows {
   uint32_t lo, hi;
 };
-__device__ inline uint64_t row_of_lane(const Rows& r, int lane) {
-  return static_cast<uint64_t>(static_cast<uint32_t>(
-             __builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(r.hi)))) << 32 |
-         static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(r.lo)));
+template <int LANE, bool PAIR>
+__device__ inline uint32_t told(uint32_t x) {
+  constexpr int kBroadcast = 0x150;      // of a lane to its 16
+  const int y = __builtin_amdgcn_mov_dpp(x, kBroadcast + LANE, 0xf, 0xf, true);
+  if constexpr (!PAIR) return y;
+  else return __builtin_amdgcn_update_dpp(y, x, kBroadcast + LANE + 1, 0xf, 0xc, false);
+}
+template <int LANE, bool PAIR>
+__device__ inline uint64_t told(const Rows& r) {
+  return __builtin_bit_cast(uint64_t, Vec2{told<LANE, PAIR>(r.lo), told<LANE, PAIR>(r.hi)});
 }
 
+// Which rows of a step's K and V the lanes of a quad find for it: lane e, below 8, one of K's loads and
+// the others V's.  Of 256 elements K's loads are 16, so K's rows and V's are found one after the other.
 template <int D>
-__device__ inline void load_keys(const Rows& r, int lane, Keys<D>& k) {
-  constexpr int kPieces = D / 8, kRowsAtOnce = 64 / kPieces;
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j)
-    k.part[j] = load_once<Vec4>(row_of_lane(r, j * kRowsAtOnce + lane / kPieces) +
-                                lane % kPieces * 16);
+struct StepPlaces {
+  static constexpr int kFinds = D == 256 ? 2 : 1;
+  // the N-th finding
+  template <int N>
+  static __device__ inline bool value(int lane) {
+    return D == 256 ? N == 1 : (lane & 8) != 0;
+  }
+  template <int N>
+  static __device__ inline int token(int lane) {
+    const int e = lane & 15, quad = lane >> 4;
+    const int of_v = 16 * (e >> 2 & 1) + 4 * quad + (e & 3);
+    if constexpr (D == 256) return N ? of_v : 2 * e + (quad >> 1);
+    const int of_k = D == 64 ? 8 * (e >> 1 & 3) + 2 * quad + (e & 1) : 4 * (e & 7) + quad;
+    return e < 8 ? of_k : of_v;
+  }
+};
+template <int D>
+struct StepRows {
+  Rows of[StepPlaces<D>::kFinds];
+};
+template <int D>
+struct StepIds {
+  RawId of[StepPlaces<D>::kFinds];
+};
+
+template <int D>
+__device__ inline void load_keys(const StepRows<D>& r, int lane, Keys<D>& k) {
+  const int piece = lane % (D / 8) * 16;
+  each_index<D / 16>([&](auto j) __attribute__((always_inline)) {
+    k.part[j] = load_once<Vec4>(told<D == 64 ? 2 * j : j, D == 64>(r.of[0]) + piece);
+  });
 }
 // A wavefront's 32 rows of K in LDS.
 template <int D>
@@ -375,13 +420,12 @@ __device__ inline void load_part(uint64_t p, uint32_t (&x)[D / 32]) {
   }
 }
 template <int D>
-__device__ inline void load_values(const Rows& r, int lane, Values<D>& v) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      load_part<D>(row_of_lane(r, 32 + 16 * h + 4 * (lane >> 4) + i) + (lane & 15) * (D / 8),
-                   v.part[h][i]);
+__device__ inline void load_values(const StepRows<D>& r, int lane, Values<D>& v) {
+  each_index<8>([&](auto x) __attribute__((always_inline)) {
+    load_part<D>(told<D == 256 ? x : 8 + x, false>(r.of[D == 256 ? 1 : 0]) +
+                     (lane & 15) * (D / 8),
+                 v.part[x / 4][x % 4]);
+  });
 }
 
 // s[r][h][i] = q[r] . k of token 16 h + 4 quad + i
@@ -522,7 +566,7 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
     if (again) __syncthreads();      // the sums of the tile before have been read
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));   // what follows from it is worked out for each tile, not kept
-    const int quad = lane >> 4;
+    int quad = lane >> 4;
     const Piece w = alone ? find_alone(a, at.item, kRowsATile)
                           : find_piece(a, kRowsATile, line, a.slots ? pos : at.item, !a.slots);
     if (w.seq < 0) return;
@@ -543,21 +587,30 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
     // the block ids are asked for a step ahead of the rows, the rows a step ahead of their use; past
     // the last key everything is of that one again
     int bad = kNoToken;
-    const bool of_v = lane >= 32;
-    Half half = of_v ? a.v : a.k;
-    half.p += at.head * half.head;
-    auto token_of = [&](int s) { return min(s * kStep + (lane & 31), keys - 1); };
-    auto find = [&](int s, const RawId& raw) {
-      const int t = token_of(s);
-      const int64_t id = block_id(a, raw);
-      if (outside(a, id)) bad = min(bad, t);
-      const uint64_t p = row_address(a, half, id, t, 0);
-      return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
+    using P = StepPlaces<D>;
+    auto ask = [&](int s) __attribute__((always_inline)) {
+      StepIds<D> ids;
+      each_index<P::kFinds>([&](auto n) __attribute__((always_inline)) {
+        ids.of[n] = ask_block(a, w.seq, min(s * kStep + P::template token<n>(lane), keys - 1));
+      });
+      return ids;
+    };
+    auto find = [&](int s, const StepIds<D>& ids) __attribute__((always_inline)) {
+      StepRows<D> rows;
+      each_index<P::kFinds>([&](auto n) __attribute__((always_inline)) {
+        const int t = min(s * kStep + P::template token<n>(lane), keys - 1);
+        const int64_t id = block_id(a, ids.of[n]);
+        if (outside(a, id)) bad = min(bad, t);
+        const uint64_t p =
+            row_address(a, P::template value<n>(lane) ? a.v : a.k, id, t, at.head);
+        rows.of[n] = {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
+      });
+      return rows;
     };
     Keys<D> k;
     Values<D> v;
-    RawId ids{0, 0};
-    if (any) ids = ask_block(a, w.seq, token_of(step));
+    StepIds<D> ids{};
+    if (any) ids = ask(step);
     Query<T, D> q[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -568,8 +621,8 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
         q[r].part[x] = query_part<T>(p + 64 * x, a.scale_log2 < 0.f);
     }
     if (any) {
-      const Rows next = find(step, ids);
-      ids = ask_block(a, w.seq, token_of(step + W));
+      const StepRows<D> next = find(step, ids);
+      ids = ask(step + W);
       load_keys<D>(next, lane, k);
       load_values<D>(next, lane, v);
     }
@@ -582,16 +635,11 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
     State<D> st[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) clear(st[r]);
-    // where this lane's scores go
-    uint64_t scores_at[R];
-    bool scores_kept[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const Row row = row_at(16 * r + (lane & 15));
-      scores_at[r] = reinterpret_cast<uint64_t>(
-          a.scores + (row.at * (a.heads * a.group) + row.head) * a.scores_row + quad * 4);
-      scores_kept[r] = a.scores && 16 * r + (lane & 15) < rows;
-    }
+    // where this lane's scores go; they are not kept of more than one tile of 16 rows
+    const bool scores_kept = R == 1 && a.scores && (lane & 15) < rows;
+    const Row scores_of = row_at(lane & 15);
+    const uint64_t scores_at = reinterpret_cast<uint64_t>(
+        a.scores + (scores_of.at * (a.heads * a.group) + scores_of.head) * a.scores_row + quad * 4);
     float p[R][8];
     // A step's scores, with K in LDS, its weights, and what these change of the rows' states.
     auto weights = [&]() __attribute__((always_inline)) {
@@ -603,8 +651,8 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (token + kStep > fewest) hide(s[r], token, visible[r], quad);
-        if (scores_kept[r]) {
-          const uint64_t to = scores_at[r] + static_cast<uint64_t>(token) * 4;
+        if (scores_kept) {
+          const uint64_t to = scores_at + static_cast<uint64_t>(token) * 4;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             *reinterpret_cast<__attribute__((address_space(1))) v4f*>(to + 64 * h) =
@@ -665,8 +713,8 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
         one_by_one = true;
         break;
       }
-      const Rows next = find(step + W, ids);
-      ids = ask_block(a, w.seq, token_of(step + 2 * W));
+      const StepRows<D> next = find(step + W, ids);
+      ids = ask(step + 2 * W);
       put_keys<D>(k, lane, k_lds);
       load_keys<D>(next, lane, k);
       weights();
@@ -676,12 +724,14 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
     if (one_by_one) {
       // All over again, and without loads ahead: a loop that goes on with the sums costs the other its
       // registers.
+      asm volatile("" : "+v"(lane));
+      quad = lane >> 4;
 #pragma unroll
       for (int r = 0; r < R; ++r) clear(st[r]);
       slack = kSlack;
 #pragma unroll 1
       for (step = w.from + wave; step < end; step += W) {
-        const Rows here = find(step, ask_block(a, w.seq, token_of(step)));
+        const StepRows<D> here = find(step, ask(step));
         load_keys<D>(here, lane, k);
         load_values<D>(here, lane, v);
         put_keys<D>(k, lane, k_lds);
@@ -783,17 +833,6 @@ __device__ inline void reads_ahead() {
   }
 }
 
-// Calls f with the numbers from 0 to N - 1, as types.
-template <int N, class F, int... I>
-__device__ __attribute__((always_inline)) inline void each_index(F f,
-                                                                 std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>()), ...);
-}
-template <int N, class F>
-__device__ __attribute__((always_inline)) inline void each_index(F f) {
-  each_index<N>(f, std::make_integer_sequence<int, N>());
-}
-
 // The 16 rows of a tile that a wavefront brings (of K and of V), D / 8 lanes each, in the quads of 16
 // lanes: lane e of a quad finds row e of what its quad loads, [tile][K|V][pass][row in the quad], and
 // tells it to all by a broadcast within the quad.  Rows of 256 elements take two quads, which both
@@ -814,18 +853,9 @@ struct Places {
   }
   // of the tile
   __device__ int row(int wave) const { return (pass * W + wave) * (64 / kPieces) + in_pass; }
-  template <int LANE>
-  static __device__ inline uint32_t of_quad(uint32_t x) {
-    constexpr int kBroadcast = 0x150;      // of a lane to its 16
-    const int y = __builtin_amdgcn_mov_dpp(x, kBroadcast + LANE, 0xf, 0xf, true);
-    if constexpr (kInQuad == 1) return y;
-    // the first 8 lanes the first row, the others the next
-    return __builtin_amdgcn_update_dpp(y, x, kBroadcast + LANE + kInQuad - 1, 0xf, 0xc, false);
-  }
   template <int NTH, int PASS, int VALUE>
   static __device__ inline uint64_t row_of_quad(const Rows& r) {
-    constexpr int kLane = NTH * kOfTile + (VALUE * kPasses + PASS) * kInQuad;
-    return __builtin_bit_cast(uint64_t, Vec2{of_quad<kLane>(r.lo), of_quad<kLane>(r.hi)});
+    return told<NTH * kOfTile + (VALUE * kPasses + PASS) * kInQuad, kInQuad == 2>(r);
   }
 };
 
@@ -1058,11 +1088,16 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     __syncthreads();
     if (partly(tile) && any_odd(here)) return false;
     __builtin_amdgcn_sched_barrier(0);
+    // the wavefront of the other workgroup on this SIMD has the vector instructions meanwhile (1 %)
+    __builtin_amdgcn_s_setprio(1);
     scores(here[0]);
+    __builtin_amdgcn_s_setprio(0);
     bring_next(second_of_two, there);
     weights(here[0]);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
     add_values(here[1]);
+    __builtin_amdgcn_s_setprio(0);
     return true;
   };
   bool one_by_one = false;
@@ -1263,7 +1298,7 @@ __global__ __launch_bounds__(256 * G) void join_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 // What each token got, from scores that lie there: a thread adds up 4 tokens' over the rows, in
 // their order.  Bound by memory: 4 bytes a row and token (and as many to write them), where making the
-// scores again takes K's 2 D bytes a token.  32 sequences of up to 8192 keys, groups of 4: TODO us.
+// scores again takes K's 2 D bytes a token.  32 sequences of up to 8192 keys, groups of 4: 9.6 us.
 
 constexpr int kAddTokens = 1024;     // of a workgroup
 
@@ -1274,17 +1309,18 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
   const int keys = max(s.keys, 0), rows = s.count * a.group;
   if (at >= keys) return;
   float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
   for (int n = 0; n < rows; ++n) {
     const Row row = row_of(a, s, n, head);
     const int64_t place = row.at * (a.heads * a.group) + row.head;
     const float2 st = a.stats[place];
-    // of steps that no row of a tile sees there are none
-    if (at >= row.visible) continue;
     const v4f x = *reinterpret_cast<const v4f*>(a.scores + place * a.scores_row + at);
+    // of steps that no row of a tile sees nothing has been written
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (at + i < row.visible) sums[i] += __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
+    for (int i = 0; i < 4; ++i) {
+      const float e = __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
+      sums[i] += at + i < row.visible ? e : 0.f;
+    }
   }
   float* const w = a.weights + seq * a.w_seq + head * a.w_head + at;
 #pragma unroll
@@ -1294,63 +1330,71 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
 
 // ---------------------------------------------------------------------------
 // What each token got, from K: a wavefront keeps 64 tokens of K in registers and goes over the
-// queries, 32 rows at a time, the next of them on their way meanwhile.  Here the tokens are the columns
-// of the products, so that a lane adds up its own token's weights, in the rows' order.
+// queries, 32 rows at a time, which the workgroup's wavefronts share in LDS.  Here the tokens are the
+// columns of the products, so that a lane adds up its own token's weights, in the rows' order.
 
 constexpr int kWeighTokens = 256;    // of a workgroup
 
 template <class T, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args a) {
   using Op = typename Mat<T>::Op;
-  constexpr int KS = D / 16;
-  __shared__ float2 row_stats[4][32];          // of a wavefront's 32 rows
-  __shared__ int row_visible[4][32];
+  constexpr int KS = D / 16, W = 4, kPieces = D / 8, kPasses = kPieces / 8;
+  // two places for 32 rows, objects of their own as the tiles of attend_many_kernel
+  __shared__ __attribute__((aligned(1024))) char place0[32 * D * 2];
+  __shared__ __attribute__((aligned(1024))) char place1[32 * D * 2];
+  __shared__ __attribute__((aligned(16))) float2 row_stats[W][32];   // of a wavefront's own reading
+  __shared__ __attribute__((aligned(16))) int row_visible[W][32];
   const int head = blockIdx.y, seq = blockIdx.z;
   const int wave = uniform(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
-  const int at = blockIdx.x * kWeighTokens + wave * 64;
+  const int first = blockIdx.x * kWeighTokens, at = first + wave * 64;
   const Seq s = sequence(a, seq);
   // too long for its table row: NaN in all rows, and in the tokens of no block
   const int keys = max(s.keys, 0), rows = s.count * a.group;
-  if (at >= keys || rows <= 0) return;
-  Op k[2][KS], q[KS];
+  if (first >= keys || rows <= 0) return;
+  Op k[2][KS];
   float2 stats;
   int visible;
-  auto bring = [&](int r0) {
+  auto bring = [&](int r0, char* place) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int n = (i * W + wave) * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
+      const Row row = row_of(a, s, min(r0 + n, rows - 1), head);
+      load_to_lds(reinterpret_cast<uint64_t>(a.q) + row.at * a.q_row + row.head * a.q_head +
+                      ((piece ^ k_swizzle<D>(n)) << 4),
+                  place + (i * W + wave) * 1024);
+    }
     const Row row = row_of(a, s, min(r0 + column, rows - 1), head);
     visible = r0 + column < rows ? row.visible : 0;
     stats = a.stats[row.at * (a.heads * a.group) + row.head];
-    const char* const p = a.q + row.at * a.q_row + row.head * a.q_head + half * 16;
-#pragma unroll
-    for (int x = 0; x < KS; ++x) q[x] = query_part<T>(p + 32 * x, a.scale_log2 < 0.f);
   };
   // the first row that sees the first of the tokens
-  const int hidden = a.causal ? max(0, at + s.count - keys) * a.group : 0;
+  const int hidden = a.causal ? max(0, first + s.count - keys) * a.group : 0;
   int r0 = hidden & ~31;
-  {
-    const RawId id[2] = {ask_block(a, seq, min(at + column, keys - 1)),
-                         ask_block(a, seq, min(at + 32 + column, keys - 1))};
-    bring(r0);
+  const RawId id[2] = {ask_block(a, seq, min(at + column, keys - 1)),
+                       ask_block(a, seq, min(at + 32 + column, keys - 1))};
+  bring(r0, place0);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = min(at + 32 * h + column, keys - 1);
-      const uint64_t p = row_address(a, a.k, block_id(a, id[h]), t, head) + half * 16;
+  for (int h = 0; h < 2; ++h) {
+    const int t = min(at + 32 * h + column, keys - 1);
+    const uint64_t p = row_address(a, a.k, block_id(a, id[h]), t, head) + half * 16;
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) k[h][x] = __builtin_bit_cast(Op, load<Vec4>(p + 32 * x));
-    }
+    for (int x = 0; x < KS; ++x)
+      k[h][x] = __builtin_bit_cast(Op, load<Vec4>(p + 32 * x) ^ flip);
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(k[h][x]));
   const float scale_log2 = score_scale(a.scale_log2);
+  const int q_at = column * D * 2 + ((half ^ k_swizzle<D>(column)) << 4);
   float sums[2] = {0.f, 0.f};
-  for (; r0 < rows; r0 += 32) {
+  auto take = [&](const char* here, char* there) __attribute__((always_inline)) {
+    wait_for_loads();
     // a wavefront's own: its LDS accesses are in order
     if (half == 0) row_stats[wave][column] = stats, row_visible[wave][column] = visible;
+    __syncthreads();
     // of the rows there are, in order, the first sees the fewest; past the last nothing is seen
     const bool all_see = r0 + 32 <= rows && lane_value(visible, 0) >= at + 64;
     const bool any_coarse = __any(fabsf(stats.x) >= kCoarse);
+    __builtin_amdgcn_sched_barrier(0);
     v16f acc[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -1358,27 +1402,40 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
       for (int i = 0; i < 16; ++i) acc[h][i] = 0.f;
 #pragma unroll
     for (int x = 0; x < KS; ++x) {
-      acc[0] = Mat<T>::mul32(q[x], k[0][x], acc[0]);
-      acc[1] = Mat<T>::mul32(q[x], k[1][x], acc[1]);
+      const Op q = __builtin_bit_cast(
+          Op, *reinterpret_cast<const Vec4*>(here + (q_at ^ (x % 8 * 32)) + x / 8 * 256));
+      acc[0] = Mat<T>::mul32(q, k[0][x], acc[0]);
+      acc[1] = Mat<T>::mul32(q, k[1][x], acc[1]);
     }
-    bring(min(r0 + 32, rows - 1));
-    __builtin_amdgcn_wave_barrier();
+    reads_ahead<3, KS, 2, 1>();
+    __builtin_amdgcn_sched_barrier(0);
+    bring(r0 + 32, there);
+    auto weigh_all = [&](bool coarse, bool masked) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int n = 8 * (i / 4) + 4 * half + i % 4;
-      const float2 st = row_stats[wave][n];
-      const int seen = all_see ? 0 : row_visible[wave][n];
+      for (int i = 0; i < 16; ++i) {
+        const int n = 8 * (i / 4) + 4 * half + i % 4;
+        const float2 st = row_stats[wave][n];
+        const int seen = masked ? row_visible[wave][n] : 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float score = acc[h][i];
-        const float e = __builtin_amdgcn_exp2f(any_coarse && fabsf(st.x) >= kCoarse
-                                                   ? rounded_less(score, scale_log2, st.x)
-                                                   : __builtin_fmaf(score, scale_log2, -st.x));
-        if (all_see || at + 32 * h + column < seen) sums[h] += e * st.y;
+        for (int h = 0; h < 2; ++h) {
+          const float e = __builtin_amdgcn_exp2f(
+              coarse && fabsf(st.x) >= kCoarse ? rounded_less(acc[h][i], scale_log2, st.x)
+                                               : __builtin_fmaf(acc[h][i], scale_log2, -st.x));
+          if (!masked || at + 32 * h + column < seen) sums[h] = __builtin_fmaf(e, st.y, sums[h]);
+        }
       }
-    }
-    __builtin_amdgcn_wave_barrier();
+    };
+    if (all_see && !any_coarse) weigh_all(false, false);
+    else weigh_all(true, true);
+    r0 += 32;
+  };
+  while (r0 < rows) {
+    take(place0, place1);
+    if (r0 >= rows) break;
+    take(place1, place0);
   }
+  // nothing may still be on its way to LDS when the workgroup ends and others get it
+  wait_for_loads();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const auto both =
@@ -1462,10 +1519,12 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
   LaunchPlan p;
   const int heads = c.layer.num_heads, dim = c.layer.head_size;
   const int64_t rows = static_cast<int64_t>(c.query_starts ? c.num_queries : c.batch) * c.group_size;
-  // 32 rows of 256 elements do not fit the registers
-  p.rows = rows > static_cast<int64_t>(c.batch) * 32 ? 128
-           : rows > static_cast<int64_t>(c.batch) * kRows && dim <= 128 ? 32 : kRows;
-  p.many = p.rows > 32;
+  // Few rows are up to 32 a sequence: a wavefront's registers hold the sums of two tiles of 16, of one
+  // where an element has 256.  16 sequences of 40 rows of 64 elements: 22 us with the kernel for many,
+  // 24 with three tiles.
+  auto over = [&](int n) { return rows > static_cast<int64_t>(c.batch) * n; };
+  p.many = over(2 * kRows);
+  p.rows = p.many ? 128 : !over(kRows) || dim == 256 ? kRows : 2 * kRows;
   const int64_t tiles = c.query_starts
                             ? rows / p.rows + c.batch
                             : static_cast<int64_t>(c.batch) * ((c.group_size + p.rows - 1) / p.rows);
@@ -1488,7 +1547,7 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
     // workgroup where there are so many sequences that working the shares out takes long, or few keys.
     const bool dealt = c.batch <= 4 * 64 && most_steps >= kDealSteps &&
                        tiles * std::max<int64_t>(1, most_steps) < int64_t(1) << 31;
-    p.waves = (dealt || p.tiles <= kComputeUnits) && dim <= 128 && p.rows == kRows ? 8 : 4;
+    p.waves = (dealt || p.tiles <= kComputeUnits) && dim <= 128 ? 8 : 4;
     const int64_t places = kComputeUnits * 8 / p.waves / (dim == 256 ? 2 : 1);
     int64_t items = dealt ? std::max<int64_t>(1, places / heads) : tiles;
     p.together = p.rows == kRows && items >= kXcds;
@@ -1502,7 +1561,9 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
   p.o_bytes = parts * p.rows * dim * sizeof(float);
   const int64_t all_rows = static_cast<int64_t>(c.num_queries) * heads * c.group_size;
   p.stats_bytes = c.weights ? (all_rows * sizeof(float2) + 15) / 16 * 16 : 0;
-  p.scores_row = c.weights && !p.many ? most_steps * step : 0;
+  // Kept of up to 16 rows a sequence: 32 sequences of 4 rows take 173 us with them, 322 where they are
+  // made again; 16 of 40 rows 55 us with them, 43 where they are made again.
+  p.scores_row = c.weights && !over(kRows) ? most_steps * step : 0;
   if (static_cast<__int128>(all_rows) * p.scores_row * 4 > kMostScores) p.scores_row = 0;
   p.scores_bytes = all_rows * p.scores_row * sizeof(float);
   return p;
@@ -1529,6 +1590,11 @@ void launch_few(const Args& a, const LaunchPlan& p, hipStream_t s) {
   hipLaunchKernelGGL((attend_few_kernel<T, D, R, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
   join<T, D, kRows * R, PiecesOfTile<kRows * R>, 4>(a, p, s);
 }
+template <class T, int D, int R>
+void launch_few(const Args& a, const LaunchPlan& p, hipStream_t s) {
+  if (p.waves == 8) launch_few<T, D, R, D == 256 ? 4 : 8>(a, p, s);
+  else launch_few<T, D, R, 4>(a, p, s);
+}
 template <class T, int D, int W>
 void launch_many(const Args& a, const LaunchPlan& p, hipStream_t s) {
   hipLaunchKernelGGL((attend_many_kernel<T, D, W>), dim3(p.workgroups), dim3(64 * W), 0, s, a);
@@ -1537,9 +1603,8 @@ void launch_many(const Args& a, const LaunchPlan& p, hipStream_t s) {
 template <class T, int D>
 void launch(const Args& a, const LaunchPlan& p, const fkv_paged_attention_args& c, hipStream_t s) {
   if (p.many) launch_many<T, D, 4>(a, p, s);
-  else if (p.rows == 32) launch_few<T, D, D == 256 ? 1 : 2, 4>(a, p, s);
-  else if (p.waves == 8) launch_few<T, D, 1, D == 256 ? 4 : 8>(a, p, s);
-  else launch_few<T, D, 1, 4>(a, p, s);
+  else if (p.rows == kRows) launch_few<T, D, 1>(a, p, s);
+  else launch_few<T, D, D == 256 ? 1 : 2>(a, p, s);
   const int64_t most = static_cast<int64_t>(a.width) * a.tokens;
   if (a.scores) {
     hipLaunchKernelGGL(add_weights_kernel,
