@@ -48,6 +48,7 @@ EXPORTED_SYMBOLS = (
     "fkv_write_kv_tokens",
     "fkv_paged_attention_workspace",
     "fkv_paged_attention",
+    "fkv_evict_kv_tokens_workspace",
     "fkv_evict_kv_tokens",
     "fkv_transfer_kv_blocks_layerwise",
     "fkv_handle_num_groups",
@@ -227,6 +228,8 @@ class EvictArgs(ctypes.Structure):
         ("recent", ctypes.c_int),
         ("weights_width", ctypes.c_int),
         ("new_weights_width", ctypes.c_int),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -280,6 +283,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     f = lib.fkv_paged_attention
     f.restype = c_int
     f.argtypes = [ctypes.POINTER(PagedAttentionArgs), c_vp]
+    f = lib.fkv_evict_kv_tokens_workspace
+    f.restype = c_int
+    f.argtypes = [ctypes.POINTER(EvictArgs), ctypes.POINTER(c_sz)]
     f = lib.fkv_evict_kv_tokens
     f.restype = c_int
     f.argtypes = [ctypes.POINTER(EvictArgs), c_vp]
@@ -533,7 +539,9 @@ def fast():
                              addr(lib.fkv_mx4_attention_workspace), addr(lib.fkv_mx4_attention))
             _fkv_py.bind_paged(addr(lib.fkv_write_kv_tokens),
                                addr(lib.fkv_paged_attention_workspace),
-                               addr(lib.fkv_paged_attention), addr(lib.fkv_evict_kv_tokens))
+                               addr(lib.fkv_paged_attention),
+                               addr(lib.fkv_evict_kv_tokens_workspace),
+                               addr(lib.fkv_evict_kv_tokens))
             _fast = _fkv_py
     return _fast
 

@@ -773,8 +773,17 @@ def evict_kv_tokens(key_cache: torch.Tensor, value_cache, weights: torch.Tensor,
         c_int(block_table.shape[1], "table_width"), c_int(new_table.shape[1], "new_table_width"),
         c_int(batch, "sequences"), budget, recent, min(weights.shape[2], 2**31 - 1),
         min(new_weights.shape[2], 2**31 - 1) if given else 0)
-    with _on_device(device):
-        rc = _lib.load().fkv_evict_kv_tokens(args, _stream_handle(fn))
+    lib = _lib.load()
+    need = ctypes.c_size_t()
+    rc = lib.fkv_evict_kv_tokens_workspace(args, need)
+    if rc == 0:
+        with _on_device(device):
+            if need.value:
+                # the allocator orders its reuse on the current stream
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+                args.workspace = workspace.data_ptr()
+                args.workspace_bytes = need.value
+            rc = lib.fkv_evict_kv_tokens(args, _stream_handle(fn))
     if rc != 0:
         raise RuntimeError(_lib.last_error() or f"{fn} failed ({rc})")
     return kept

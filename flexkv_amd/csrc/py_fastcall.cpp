@@ -425,6 +425,7 @@ PyObject* mx4_attention_of(PyObject* const* a) {
 decltype(&fkv_write_kv_tokens) g_write_tokens = nullptr;
 decltype(&fkv_paged_attention_workspace) g_paged_workspace = nullptr;
 decltype(&fkv_paged_attention) g_paged_attention = nullptr;
+decltype(&fkv_evict_kv_tokens_workspace) g_evict_workspace = nullptr;
 decltype(&fkv_evict_kv_tokens) g_evict = nullptr;
 
 // bytes from one to the next in a dimension; one alone has none
@@ -618,11 +619,20 @@ PyObject* evict_kv_tokens_of(PyObject* const* a) {
   c.table_width = static_cast<int>(table->size(1));
   c.new_table_width = static_cast<int>(into->size(1));
   c.batch = static_cast<int>(batch), c.budget = budget, c.recent = recent;
-  void* stream = c10::hip::getCurrentHIPStream().stream();
-  int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = g_evict(&c, stream);
-  Py_END_ALLOW_THREADS
+  size_t need = 0;
+  int rc = g_evict_workspace(&c, &need);
+  at::Tensor workspace;
+  if (!rc && need) {
+    // the allocator orders its reuse on the current stream
+    workspace = at::empty({static_cast<int64_t>(need)}, lens->options().dtype(at::kByte));
+    c.workspace = workspace.data_ptr(), c.workspace_bytes = need;
+  }
+  if (!rc) {
+    void* stream = c10::hip::getCurrentHIPStream().stream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_evict(&c, stream);
+    Py_END_ALLOW_THREADS
+  }
   PyObject* done = finish(rc);
   if (!done) return nullptr;
   Py_DECREF(done);
@@ -670,14 +680,15 @@ PyObject* evict_kv_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return checked<evict_kv_tokens_of>("evict_kv_tokens", a, n, 10);
 }
 
-// bind_paged(write_kv_tokens, paged_attention_workspace, paged_attention, evict_kv_tokens)
+// bind_paged(write_kv_tokens, paged_attention_workspace, paged_attention,
+//            evict_kv_tokens_workspace, evict_kv_tokens)
 PyObject* bind_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 4) {
-    PyErr_SetString(PyExc_TypeError, "bind_paged takes 4 arguments");
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "bind_paged takes 5 arguments");
     return nullptr;
   }
-  void* f[4];
-  for (int i = 0; i < 4; ++i) {
+  void* f[5];
+  for (int i = 0; i < 5; ++i) {
     f[i] = PyLong_AsVoidPtr(a[i]);
     if (!f[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null function address");
@@ -687,7 +698,8 @@ PyObject* bind_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_write_tokens = reinterpret_cast<decltype(g_write_tokens)>(f[0]);
   g_paged_workspace = reinterpret_cast<decltype(g_paged_workspace)>(f[1]);
   g_paged_attention = reinterpret_cast<decltype(g_paged_attention)>(f[2]);
-  g_evict = reinterpret_cast<decltype(g_evict)>(f[3]);
+  g_evict_workspace = reinterpret_cast<decltype(g_evict_workspace)>(f[3]);
+  g_evict = reinterpret_cast<decltype(g_evict)>(f[4]);
   Py_RETURN_NONE;
 }
 

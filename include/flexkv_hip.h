@@ -604,7 +604,13 @@ typedef struct fkv_evict_args {
   int32_t* kept;                     /* [batch][num_heads][budget], without gaps */
   int index_is_64bit;                /* of block_table, new_table and seq_lens */
   int table_width, new_table_width, batch, budget, recent, weights_width, new_weights_width;
+  void* workspace;                   /* device memory, on a multiple of 16; see below */
+  size_t workspace_bytes;
 } fkv_evict_args;
+/* The workspace a call of these sizes needs (of pointers only whether new_weights is null is looked
+ * at); 0 for none.  It holds nothing between calls, and no two that may run at the same time may
+ * share one. */
+int fkv_evict_kv_tokens_workspace(const fkv_evict_args* args, size_t* bytes);
 int fkv_evict_kv_tokens(const fkv_evict_args* args, fkv_stream_t stream);
 
 /* How copy-engine mode (use_ce_transfer = FKV_XFER_CE) chooses between the

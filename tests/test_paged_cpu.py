@@ -181,6 +181,27 @@ def test_eviction_refuses():
     assert _evict(batch=0)[0] == 0
 
 
+def test_workspace_of_an_eviction():
+    lib, need = _lib.load(), ctypes.c_size_t(1)
+
+    def of(**kw):
+        args = dict(layer=_layer({}), table_width=2, new_table_width=4096, batch=2, budget=9,
+                    recent=2, weights_width=1 << 20, new_weights_width=1 << 20)
+        args.update(kw)
+        rc = lib.fkv_evict_kv_tokens_workspace(_lib.EvictArgs(**args), need)
+        return rc, need.value
+    assert lib.fkv_evict_kv_tokens_workspace(None, need) == 1
+    assert of() == (0, 0) and of(batch=0, table_width=4096) == (0, 0)
+    assert of(budget=0, table_width=4096) == (1, 0)
+    long = of(table_width=4096)
+    assert long[0] == 0 and long[1] > 0
+    kept = of(table_width=4096, new_weights=4096)
+    heads = 2 * _layer({}).num_heads
+    assert kept == (0, long[1] + heads * 9 * 4)
+    # no more than many sequences' own workgroups need
+    assert of(table_width=4096, batch=512) == (0, 0)
+
+
 # -- refusals of the Python entries --------------------------------------------------
 
 def test_python_entries_refuse_host_tensors_and_gradients(per_call_path):

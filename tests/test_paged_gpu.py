@@ -575,6 +575,73 @@ def test_eviction_of_the_weights_in_place(kw, recent):
     c.check(c.run(recent, in_place=True), recent)
 
 
+# several workgroups choose for one sequence: few sequences, and table rows of 2^15 tokens or more
+LONG = [
+    (dict(keys=[40000, 0, 1, 20001], budget=17000, H=1, D=8, T=64), 1000),
+    (dict(keys=[16385, 1023, 16384], budget=1025, H=3, D=8, T=1, ties=True, width=33000), 1024),
+    (dict(keys=[30000, 700], budget=20000, H=2, D=8, T=32, index=torch.int64, width=2000), 20000),
+    (dict(keys=[17000, 9000], budget=9000, H=1, D=8, T=16, ties=True, width=2100), 0),
+    (dict(keys=[100], budget=40, H=1, D=64, T=16, width=2500), 3),
+    (dict(keys=[150001], budget=100, H=1, D=8, T=32, ties=True), 7),
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("kw,recent", LONG, ids=str)
+def test_eviction_of_long_sequences(kw, recent, in_place):
+    c = Evict(**kw)
+    c.check(c.run(recent, in_place), recent, in_place)
+
+
+def test_eviction_of_long_sequences_orders_every_kind_of_weight(per_call_path):
+    c = Evict([20000, 16400], 5000, D=8, T=16, width=2048)
+    hard = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, 1e-45, -1e-45, 1e38, -3.0,
+                         -math.nan, 2.0 ** -126, 0.5])
+    c.w[0, 0, :18000] = hard.repeat(1500)
+    c.w[0, 1, :20000] = 0.0
+    c.w[1, 0, :16400] = math.nan
+    c.w[1, 1, :16400] = torch.linspace(1, 0, 16400)
+    for recent in (0, 3000, 5000):
+        c.check(c.run(recent), recent)
+    kept = torch.full((2, 2, 5000), 9, dtype=torch.int32, device=DEV)
+    got, _ = c.run(7, new_weights=None, kept=kept)
+    assert torch.equal(kept.cpu(), got)
+    c.check(c.run(7), 7)
+    assert torch.equal(c.run(7)[0], got)
+    kept, nw = c.run(5, seq_lens=torch.tensor([32769, -2], dtype=torch.int32, device=DEV))
+    assert (kept == -1).all()
+    assert _same(nw[0], c.given[0]) and (nw[1] == 0).all()
+
+
+def test_eviction_of_long_sequences_in_captured_graphs():
+    """Two graphs, replayed in turn; of one the lengths change."""
+    c = [Evict([20000, 16400], 5000, H=1, D=8, T=16, seed=1, width=2048), Evict([40000], 300, D=8, seed=2)]
+    state = []
+    for e in c:
+        kc, vc = _on_device(e.cache, "layer")
+        dev = [x.to(DEV) for x in (e.w, e.table, e.lens, e.new_table)]
+        args = (kc, vc, *dev, e.budget, 20, e.given.to(DEV))
+        c_ext.evict_kv_tokens(*args)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = c_ext.evict_kv_tokens(*args)
+        state.append((e, graph, args, kept))
+    for i in range(3):
+        for e, graph, args, kept in state:
+            e.w = torch.rand(e.w.shape, generator=_gen(i))
+            args[2].copy_(e.w)
+            if len(e.keys) == 2:
+                e.keys = [20000 - 7 * i, 16400 >> 4 * i]
+                args[4].copy_(torch.tensor(e.keys))
+            args[0].copy_(e.cache[0]), args[1].copy_(e.cache[1])
+            graph.replay()
+        torch.cuda.synchronize()
+        for e, graph, args, kept in state:
+            e.kc, e.vc = args[:2]
+            e.check((kept.cpu(), args[8].cpu()), 20)
+
+
 def test_eviction_orders_every_kind_of_weight():
     c = Evict([64, 64], 20, T=8)
     hard = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, 1e-45, -1e-45, 1e38, -3.0,
