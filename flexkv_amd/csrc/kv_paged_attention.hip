@@ -807,8 +807,10 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
 
 struct ManyPlan {
   static constexpr int kStep = 64;       // tokens of a tile
-  static constexpr int kMinSteps = 16;   // of a workgroup, where the keys are cut
-  static constexpr int kCutSteps = 16;   // that cutting has to take off the longest sequence
+  // Steps of a workgroup where the keys are cut, and that cutting has to take off the longest
+  // sequence.  64 queries over 2000 keys 25 us, with 16 for both 32, with 4 23; 128 queries of two heads
+  // over 8000 keys 27, 34 and 32.
+  static constexpr int kMinSteps = 8, kCutSteps = 8;
 };
 constexpr int kTile = ManyPlan::kStep;
 
@@ -916,13 +918,20 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     const uint64_t p = row_address(a, of, id, t, 0);
     return Rows{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32)};
   };
+  // where in its row lies the piece that a lane brings; pieces are exchanged alike in every 16 rows
+  constexpr int kPeriod = W * kPassRows < 16 ? 16 / (W * kPassRows) : 1;
+  uint32_t k_piece[kPeriod], v_piece[kPeriod];
+#pragma unroll
+  for (int i = 0; i < kPeriod; ++i) {
+    const int row = (i * W + wave) * kPassRows + lane / kPieces, piece = lane % kPieces;
+    k_piece[i] = (piece ^ k_swizzle<D>(row)) << 4, v_piece[i] = (piece ^ v_swizzle<D>(row)) << 4;
+  }
   // the rows found for the n-th of kTiles tiles
   auto bring = [&](const Rows& r, auto n, char (*place)[kHalf])__attribute__((always_inline)) {
     each_index<kPasses>([&](auto i) __attribute__((always_inline)) {
-      const int row = (i * W + wave) * kPassRows + lane / kPieces, piece = lane % kPieces;
-      load_to_lds(P::template row_of_quad<n, i, 0>(r) + ((piece ^ k_swizzle<D>(row)) << 4),
+      load_to_lds(P::template row_of_quad<n, i, 0>(r) + k_piece[i % kPeriod],
                   place[0] + (i * W + wave) * 1024);
-      load_to_lds(P::template row_of_quad<n, i, 1>(r) + ((piece ^ v_swizzle<D>(row)) << 4),
+      load_to_lds(P::template row_of_quad<n, i, 1>(r) + v_piece[i % kPeriod],
                   place[1] + (i * W + wave) * 1024);
     });
   };
@@ -1022,8 +1031,21 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
       }
     return sum[0] + sum[1];
   };
+  // Of 256 elements the sums and the query are 192 registers: kept where matrix instructions alone
+  // reach them, which the compiler does not do by itself.  With them among the others it put a part
+  // of the query into scratch memory and waited there for every read (256 queries of 32 heads over
+  // up to 4906 keys of 4 sequences 141 us, 333 without; 2048 over 8192 of one 517 us).
+  auto keep_aside = [&]() __attribute__((always_inline)) {
+    if constexpr (D == 256) {
+#pragma unroll
+      for (int d = 0; d < NT; ++d) asm volatile("" : "+a"(o[d]));
+#pragma unroll
+      for (int x = 0; x < KS; ++x) asm volatile("" : "+a"(q[x]));
+    }
+  };
   auto weights = [&](const char* kt) __attribute__((always_inline)) {
     float sum = weigh_all(false);
+    keep_aside();
     if (__any(sum > slack)) {
       // Some score passes its row's reference: the references follow, and the weights are made
       // again, from scores made again, which would be 32 registers more if they were kept.
@@ -1040,9 +1062,11 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
       l *= fade;
 #pragma unroll
       for (int d = 0; d < NT; ++d) o[d] *= fade;
+      keep_aside();
       const bool coarse = fabsf(m) >= kCoarse && m != kNothing;
       sum = weigh_all(coarse);
       slack = __any(coarse) ? -1.f : kSlack;
+      keep_aside();
     }
     l += sum;
   };
@@ -1085,8 +1109,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
   auto take = [&](char (*here)[kHalf], char (*there)[kHalf],
                   auto second_of_two) __attribute__((always_inline)) {
     wait_for_loads();
+    asm volatile("" : "+v"(ids.lo), "+v"(ids.hi));   // so that these are not waited for again
     __syncthreads();
     if (partly(tile) && any_odd(here)) return false;
+    keep_aside();
     __builtin_amdgcn_sched_barrier(0);
     // the wavefront of the other workgroup on this SIMD has the vector instructions meanwhile (1 %)
     __builtin_amdgcn_s_setprio(1);
@@ -1098,10 +1124,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
     __builtin_amdgcn_s_setprio(1);
     add_values(here[1]);
     __builtin_amdgcn_s_setprio(0);
+    keep_aside();
     return true;
   };
   bool one_by_one = false;
+  keep_aside();
   while (tile < end) {
+    keep_aside();
     if (!take(place0, place1, std::false_type())) {
       one_by_one = true;
       break;
