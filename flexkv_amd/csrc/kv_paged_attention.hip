@@ -110,6 +110,12 @@ struct Args : Sequences {
   // leaves them; null where they are made again
   float* scores;
   int64_t scores_row;
+  // workgroups that share the rows where they are made again, and, of more than one, what each adds
+  // up, [sequence][head][share][token]
+  int shares;
+  FastDiv shares_div;
+  float* share_sums;
+  int64_t share_row;
 };
 
 // Eight elements of a query: their negatives where the scale is negative, so that it is not looked
@@ -1360,7 +1366,10 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 // What each token got, from K: a wavefront keeps 64 tokens of K in registers and goes over the
 // queries, 32 rows at a time, which the workgroup's wavefronts share in LDS.  Here the tokens are the
-// columns of the products, so that a lane adds up its own token's weights, in the rows' order.
+// columns of the products, so that a lane adds up its own token's weights, in the rows' order.  Where
+// there are few tokens the rows are shared out to several workgroups, whose sums are then added up.
+// Bound by the exponentials and products, of which each takes about as long (64 queries of 32 heads
+// over up to 16384 keys, 4 sequences: 58 us).
 
 constexpr int kWeighTokens = 256;    // of a workgroup
 
@@ -1376,7 +1385,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
   const int head = blockIdx.y, seq = blockIdx.z;
   const int wave = uniform(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
-  const int first = blockIdx.x * kWeighTokens, at = first + wave * 64;
+  const int tile = a.shares_div.div(blockIdx.x), share = blockIdx.x - tile * a.shares;
+  const int first = tile * kWeighTokens, at = first + wave * 64;
   const Seq s = sequence(a, seq);
   // too long for its table row: NaN in all rows, and in the tokens of no block
   const int keys = max(s.keys, 0), rows = s.count * a.group;
@@ -1399,7 +1409,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
   };
   // the first row that sees the first of the tokens
   const int hidden = a.causal ? max(0, first + s.count - keys) * a.group : 0;
-  int r0 = hidden & ~31;
+  const int shown = hidden & ~31;
+  const int per_share = a.shares_div.div((rows - shown + 31) / 32 + a.shares - 1) * 32;
+  int r0 = shown + share * per_share;
+  const int stop = min(rows, r0 + per_share);
   const RawId id[2] = {ask_block(a, seq, min(at + column, keys - 1)),
                        ask_block(a, seq, min(at + 32 + column, keys - 1))};
   bring(r0, place0);
@@ -1458,9 +1471,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
     else weigh_all(true, true);
     r0 += 32;
   };
-  while (r0 < rows) {
+  while (r0 < stop) {
     take(place0, place1);
-    if (r0 >= rows) break;
+    if (r0 >= stop) break;
     take(place1, place0);
   }
   // nothing may still be on its way to LDS when the workgroup ends and others get it
@@ -1473,7 +1486,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_kernel(const Args
   }
   // lanes below 32 have the first 32 tokens' sums to store, the others the second's
   const int t = at + lane;
-  if (t < keys) a.weights[seq * a.w_seq + head * a.w_head + t] += half ? sums[1] : sums[0];
+  const float sum = half ? sums[1] : sums[0];
+  if (a.shares > 1)
+    a.share_sums[((static_cast<int64_t>(seq) * a.heads + head) * a.shares + share) * a.share_row + t] =
+        sum;
+  else if (t < keys)
+    a.weights[seq * a.w_seq + head * a.w_head + t] += sum;
+}
+
+// The shares' sums added up, in their order: a token a thread.
+__global__ __launch_bounds__(256) void add_shares_kernel(const Args a) {
+  const int head = blockIdx.y, seq = blockIdx.z;
+  const int t = blockIdx.x * 256 + static_cast<int>(threadIdx.x);
+  const Seq s = sequence(a, seq);
+  if (t >= s.keys || s.count <= 0) return;
+  const float* const from =
+      a.share_sums + (static_cast<int64_t>(seq) * a.heads + head) * a.shares * a.share_row + t;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < a.shares; ++i) sum += from[i * a.share_row];
+  a.weights[seq * a.w_seq + head * a.w_head + t] += sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -1531,9 +1563,11 @@ struct LaunchPlan {
   int slots;              // see Sequences and Piece
   bool together;
   int64_t workgroups;
-  size_t ml_bytes, o_bytes, stats_bytes, scores_bytes;
+  size_t ml_bytes, o_bytes, stats_bytes, scores_bytes, shares_bytes;
   int64_t scores_row;     // 0: the scores are not kept
-  size_t bytes() const { return o_bytes + ml_bytes + stats_bytes + scores_bytes; }
+  int shares;             // of the rows, where the scores are made again
+  int64_t share_row;
+  size_t bytes() const { return o_bytes + ml_bytes + stats_bytes + scores_bytes + shares_bytes; }
 };
 
 constexpr int kComputeUnits = 256;
@@ -1595,6 +1629,20 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
   p.scores_row = c.weights && !over(kRows) ? most_steps * step : 0;
   if (static_cast<__int128>(all_rows) * p.scores_row * 4 > kMostScores) p.scores_row = 0;
   p.scores_bytes = all_rows * p.scores_row * sizeof(float);
+  // As many as give each compute unit six workgroups (three are there at a time), of at least 64 rows,
+  // a step for each of the two places: 8 sequences of up to 390 queries of 10 heads of 64 elements over
+  // up to 620 keys take 33 us with the attention, 103 without shares, and 38 with shares of 128 rows; 2000
+  // queries of 32 heads over themselves 114 us, 324 without, and 122 with three workgroups.
+  const int64_t weigh_tiles =
+      (static_cast<int64_t>(c.table_width) * c.layer.tokens_per_block + kWeighTokens - 1) /
+      kWeighTokens;
+  const int64_t weigh_items = std::max<int64_t>(1, weigh_tiles * heads * c.batch);
+  p.share_row = weigh_tiles * kWeighTokens;
+  p.shares = p.scores_row ? 1 : static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({32, 6 * kComputeUnits / weigh_items, rows / c.batch / 64})));
+  p.shares_bytes = c.weights && p.shares > 1
+                       ? static_cast<int64_t>(c.batch) * heads * p.shares * p.share_row * sizeof(float)
+                       : 0;
   return p;
 }
 
@@ -1640,9 +1688,12 @@ void launch(const Args& a, const LaunchPlan& p, const fkv_paged_attention_args& 
                        dim3((most + kAddTokens - 1) / kAddTokens, a.heads, a.batch), dim3(256), 0,
                        s, a);
   } else if (a.weights && a.width) {
-    hipLaunchKernelGGL((weigh_kernel<T, D>),
-                       dim3((most + kWeighTokens - 1) / kWeighTokens, a.heads, a.batch), dim3(256),
-                       0, s, a);
+    const int64_t tiles = (most + kWeighTokens - 1) / kWeighTokens;
+    hipLaunchKernelGGL((weigh_kernel<T, D>), dim3(tiles * a.shares, a.heads, a.batch), dim3(256), 0,
+                       s, a);
+    if (a.shares > 1)
+      hipLaunchKernelGGL(add_shares_kernel, dim3((most + 255) / 256, a.heads, a.batch), dim3(256), 0,
+                         s, a);
   }
 }
 template <class T>
@@ -1691,6 +1742,8 @@ int attention(const fkv_paged_attention_args& c, fkv_stream_t stream) {
   a.scores_row = p.scores_row;
   if (p.scores_row)
     a.scores = reinterpret_cast<float*>(space + p.o_bytes + p.ml_bytes + p.stats_bytes);
+  a.shares = p.shares, a.shares_div = FastDiv(p.shares), a.share_row = p.share_row;
+  a.share_sums = reinterpret_cast<float*>(space + p.o_bytes + p.ml_bytes + p.stats_bytes);
   a.tokens_div = FastDiv(a.tokens), a.group_div = FastDiv(a.group), a.heads_div = FastDiv(a.heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   int dev = 0;
