@@ -1575,7 +1575,10 @@ constexpr int kComputeUnits = 256;
 // makes it large.
 constexpr int64_t kMostScores = int64_t(1) << 30;
 // Steps of a table row from which keys are dealt out, which costs 6 to 8 us: 32 sequences of 2048 keys 43
-// us uncut and 51 dealt out; 32 of 2048 to 8192 keys 161 uncut and 133 dealt out.
+// us uncut and 51 dealt out; 32 of 2048 to 8192 keys 161 uncut and 133 dealt out.  Half of them where
+// uncut tiles leave half of the compute units without work (one sequence of 3114 keys 34 uncut and 24
+// dealt out, 32 of them 55 and 58), or have four wavefronts, as those of 256 elements (71 and 39, 108 and
+// 100).
 constexpr int kDealSteps = 128;
 
 LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
@@ -1608,7 +1611,9 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
   } else {
     // A workgroup of 8 wavefronts a compute unit, each with an even share of the steps; a tile for each
     // workgroup where there are so many sequences that working the shares out takes long, or few keys.
-    const bool dealt = c.batch <= 4 * 64 && most_steps >= kDealSteps &&
+    const int deal_steps =
+        dim == 256 || p.tiles <= kComputeUnits / 2 ? kDealSteps / 2 : kDealSteps;
+    const bool dealt = c.batch <= 4 * 64 && most_steps >= deal_steps &&
                        tiles * std::max<int64_t>(1, most_steps) < int64_t(1) << 31;
     p.waves = (dealt || p.tiles <= kComputeUnits) && dim <= 128 ? 8 : 4;
     const int64_t places = kComputeUnits * 8 / p.waves / (dim == 256 ? 2 : 1);

@@ -250,6 +250,20 @@ SHAPES = [
     dict(keys=[8200, 40, 7000], queries=[1, 1, 1], H=2, G=4),
     dict(keys=[12000, 100], queries=[5, 3], H=1, G=8, T=64),
     dict(keys=[7000], queries=[60], H=1, G=4),
+    # dealt out among more than 64 sequences, and more than are dealt out; cut among more than 64
+    dict(keys=[3000, *range(1, 70)], queries=[1] * 70, H=1, G=3, D=64),
+    dict(keys=[40 - n % 40 for n in range(260)], queries=[1] * 260, H=1, G=2, T=8, width=300),
+    dict(keys=[3000, *range(10, 79)], queries=[10] * 70, H=1, D=64, dtype=FP16),
+    # two tiles of 16 rows for a wavefront, dealt out; two for each sequence
+    dict(keys=[4200, 90], queries=[6, 7], H=1),
+    dict(keys=[2300], queries=[4], H=2, G=7, D=64, dtype=FP16),
+    dict(keys=[2600, 31], queries=[1, 1], H=1, G=23, D=256),
+    dict(keys=[70, 5], queries=[3, 2], H=1, G=9, D=256, dtype=FP16),
+    # a table so wide that the scores are not kept
+    dict(keys=[3000], queries=[2], H=1, G=8, T=1024, width=16500),
+    # one row for each share of the rows that weigh, and rows that nothing is seen by
+    dict(keys=[30, 257], queries=[100, 200], H=1, G=1, D=64),
+    dict(keys=[1100], queries=[700], H=1, G=1, D=256, dtype=FP16, T=128),
 ]
 
 
