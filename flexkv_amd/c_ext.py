@@ -568,6 +568,15 @@ def _weights(fn_name: str, name: str, t, batch: int, heads: int, width: int, dev
                          f"{t.stride()}")
 
 
+def _require_apart(fn_name: str, name: str, t: torch.Tensor) -> None:
+    """Refuse a tensor to write to with entries that share memory, as an expanded one's do."""
+    end = 1
+    for step, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if step < end:
+            raise ValueError(f"{fn_name}: {name}'s entries overlap: {tuple(t.shape)} {t.stride()}")
+        end += step * (n - 1)
+
+
 def write_kv_tokens(key: torch.Tensor, value, key_cache: torch.Tensor, value_cache,
                     slots: torch.Tensor) -> None:
     """Write new tokens of one layer into their slots of a paged cache (extension;
@@ -625,8 +634,8 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     sequence b's one query); all three int32 or all int64.  ``scale`` defaults to
     head_size ** -0.5.  With ``causal`` a query sees the keys up to its own position.  Rows
     that see none give zeros (lse -inf); rows of no sequence are left as they were (not written
-    in a given ``out``, unset in a new one).  ``out`` may not overlap ``query``.  ``lse``:
-    float32 [row, head], receives the log of the sum of exp.  ``weights``: float32 [sequence,
+    in a given ``out``, unset in a new one).  ``out`` may not overlap ``query``; what is written
+    may overlap nothing else that the call uses.  ``lse``: float32 [row, head], receives the log of the sum of exp.  ``weights``: float32 [sequence,
     K/V head, tokens that a row of block_table holds, or more]; entry t of a head grows by what
     token t got of the attention of that head's queries, which is what evict_kv_tokens goes by.
     Returns ``out``.  Makes no gradients: inputs that require them are refused but under
@@ -676,14 +685,17 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
                              f"got {tuple(out.shape)} {out.dtype} {out.stride()}")
         if _overlap(query, out):
             raise ValueError(f"{fn}: out may not overlap query")
+        _require_apart(fn, "out", out)
     if lse is not None:
         _require_device(lse, "lse", fn, device)
         if lse.shape != (rows, heads) or lse.dtype != torch.float32:
             raise ValueError(f"{fn}: lse must be float32 {(rows, heads)}, got {lse.dtype} "
                              f"{tuple(lse.shape)}")
+        _require_apart(fn, "lse", lse)
     if weights is not None:
         _weights(fn, "weights", weights, batch, kv_heads,
                  block_table.shape[1] * key_cache.shape[1], device)
+        _require_apart(fn, "weights", weights)
     c_int = _lib.c_int
     args = _lib.PagedAttentionArgs(
         layer, query.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
@@ -751,6 +763,7 @@ def evict_kv_tokens(key_cache: torch.Tensor, value_cache, weights: torch.Tensor,
     _weights(fn, "weights", weights, batch, heads, most, device)
     if new_weights is not None:
         _weights(fn, "new_weights", new_weights, batch, heads, min(budget, most), device)
+        _require_apart(fn, "new_weights", new_weights)
         same = new_weights.data_ptr() == weights.data_ptr() and \
             new_weights.stride() == weights.stride()
         if not same and _ranges_meet(weights, new_weights):

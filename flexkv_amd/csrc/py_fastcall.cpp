@@ -469,6 +469,23 @@ bool weights_of(const at::Tensor& t, int64_t batch, int64_t heads, int64_t width
          (t.size(2) <= 1 || t.stride(2) == 1);
 }
 
+// whether no two entries share memory, as an expanded tensor's do
+bool apart(const at::Tensor& t) {
+  int64_t step[3], size[3], n = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) <= 1) continue;
+    int64_t i = n++;
+    for (; i > 0 && step[i - 1] > t.stride(d); --i) step[i] = step[i - 1], size[i] = size[i - 1];
+    step[i] = t.stride(d), size[i] = t.size(d);
+  }
+  int64_t end = 1;
+  for (int64_t i = 0; i < n; ++i) {
+    if (step[i] < end) return false;
+    end += step[i] * (size[i] - 1);
+  }
+  return true;
+}
+
 // (key, value, key_cache, value_cache, slots)
 PyObject* write_kv_tokens_of(PyObject* const* a) {
   const at::Tensor *key, *value = nullptr, *kc, *vc = nullptr, *slots;
@@ -524,12 +541,13 @@ PyObject* paged_attention_of(PyObject* const* a) {
               : rows < batch))
     Py_RETURN_FALSE;
   if (given && (given->sizes() != query->sizes() || given->scalar_type() != type ||
-                given->stride(2) != 1 || ranges_meet(*given, *query)))
+                given->stride(2) != 1 || ranges_meet(*given, *query) || !apart(*given)))
     Py_RETURN_FALSE;
   if (lse && (lse->dim() != 2 || lse->size(0) != rows || lse->size(1) != heads ||
-              lse->scalar_type() != at::kFloat))
+              lse->scalar_type() != at::kFloat || !apart(*lse)))
     Py_RETURN_FALSE;
-  if (weights && !weights_of(*weights, batch, kv_heads, table->size(1) * kc->size(1)))
+  if (weights && (!weights_of(*weights, batch, kv_heads, table->size(1) * kc->size(1)) ||
+                  !apart(*weights)))
     Py_RETURN_FALSE;
   const at::Tensor out = given ? *given : at::empty({rows, heads, dim}, query->options());
   c.query = query->data_ptr(), c.out = out.data_ptr();
@@ -594,7 +612,8 @@ PyObject* evict_kv_tokens_of(PyObject* const* a) {
   const int64_t most = table->size(1) * kc->size(1);
   if (!weights_of(*weights, batch, heads, most)) Py_RETURN_FALSE;
   if (nw) {
-    if (!weights_of(*nw, batch, heads, budget < most ? budget : most)) Py_RETURN_FALSE;
+    if (!weights_of(*nw, batch, heads, budget < most ? budget : most) || !apart(*nw))
+      Py_RETURN_FALSE;
     const bool same = nw->data_ptr() == weights->data_ptr() && nw->strides() == weights->strides();
     if (!same && ranges_meet(*nw, *weights)) Py_RETURN_FALSE;
   }

@@ -535,7 +535,7 @@ int fkv_write_kv_tokens(const fkv_paged_layer* layer, int num_tokens, const void
  * weights (may be null): weights[b][h][t] grows by what token t got of the attention of K/V head
  * h's queries, the sum over them of exp(scale * q . k - lse); of tokens past the sequence's
  * keys nothing is read or written.  The order of its terms, and so the result, is the same
- * from call to call.
+ * from call to call.  What is written (out, lse, weights) may overlap nothing else, nor itself.
  *
  * head_size 64, 128 or 256; dtype (of cache, query and out) FKV_DTYPE_BF16 or _FP16.
  * Products enter exactly; sums, maximum, normalisation and weights are held in 32 bits.  In the

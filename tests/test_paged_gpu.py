@@ -329,14 +329,16 @@ def test_queries_and_outputs_of_any_stride(queries):
         c.check(c.run(query=dq, out=out))
 
 
-@pytest.mark.parametrize("queries,T", [(1, 16), (3, 16), (100, 16), (100, 5)])
-def test_what_is_not_a_number_reaches_only_those_that_see_it(queries, T):
+@pytest.mark.parametrize("queries,T,D", [(1, 16, 128), (3, 16, 128), (100, 16, 128), (100, 5, 128),
+                                         (6, 16, 128), (8, 8, 64), (50, 16, 64), (4, 16, 256),
+                                         (60, 32, 256)])
+def test_what_is_not_a_number_reaches_only_those_that_see_it(queries, T, D):
     """In keys and values, at the first, some and the last token."""
     n = 150
     for half in (0, 1):
         for t in (0, n - queries // 2 - 1, n - 1):
             for x in (math.nan, math.inf):
-                c = Case([n, 40], [queries, 1], H=1, G=4, T=T, seed=t)
+                c = Case([n, 40], [queries, 1], H=1, G=4, D=D, T=T, seed=t)
                 c.cache[half, int(c.table[0, t // T]), t % T, 0, 5] = x
                 out, lse, w = c.run()
                 visible = n - queries + 1 + torch.arange(queries)
@@ -390,10 +392,10 @@ def test_starts_past_the_rows_are_cut_off():
     c.run(query_starts=torch.tensor([-7, 3, 6], device=DEV), out=out)
 
 
-@pytest.mark.parametrize("queries", [1, 30])
-def test_scores_far_from_zero(queries):
+@pytest.mark.parametrize("queries,D", [(1, 64), (10, 64), (30, 64), (1, 256), (30, 256)])
+def test_scores_far_from_zero(queries, D):
     """Products of 2^27 and more: weights as their rounded products have them."""
-    c = Case([200], [queries], H=1, G=2, D=64, seed=3)
+    c = Case([200], [queries], H=1, G=2, D=D, seed=3)
     c.q = torch.full_like(c.q, 2.0 ** 14)
     for t in range(200):
         c.cache[0, int(c.table[0, t // 16]), t % 16] = 2.0 ** 13 if t == 30 else 2.0 ** 12
@@ -447,7 +449,10 @@ def test_attention_refuses_what_it_cannot_take(per_call_path):
                dict(lse=torch.empty(4, 8, device=DEV, dtype=BF16)),
                dict(weights=w[:1]), dict(weights=w[:, :1]), dict(weights=w[..., :63]),
                dict(weights=w.double()),
-               dict(weights=torch.zeros(2, 2, 128, device=DEV)[..., ::2])):
+               dict(weights=torch.zeros(2, 2, 128, device=DEV)[..., ::2]),
+               dict(weights=w[:, :1].expand_as(w)), dict(weights=w[:1].expand_as(w)),
+               dict(lse=torch.empty(4, 1, device=DEV).expand(4, 8)),
+               dict(out=torch.empty(1, 8, 128, device=DEV, dtype=BF16).expand(4, 8, 128))):
         with pytest.raises(ValueError):
             call(**kw)
     with pytest.raises(TypeError):
@@ -468,7 +473,7 @@ def test_on_another_stream_and_in_captured_graphs():
     """Two graphs that share their memory, replayed in turn with eager calls and with other
     lengths, on a stream of their own."""
     cases = [Case([300, 41], [1, 1], H=1, seed=1), Case([700, 70], [40, 5], seed=2),
-             Case([9000], [1], H=1, G=8, seed=3)]
+             Case([9000], [1], H=1, G=8, seed=3), Case([320, 30], [150, 9], H=1, seed=4)]
     stream = torch.cuda.Stream()
     graphs, outs, pool = [], [], None
     for c in cases:
@@ -719,6 +724,7 @@ def test_eviction_refuses_what_it_cannot_take(per_call_path):
     for kw in (dict(budget=0), dict(budget=-2), dict(recent=-1), dict(recent=31),
                dict(weights=w[..., :111]), dict(weights=w[:1]), dict(weights=w.half()),
                dict(new_weights=w[..., :29]), dict(new_weights=w[..., 1:]),
+               dict(new_weights=w.clone()[:, :1].expand_as(w)),
                dict(new_table=c.new_table.long().to(DEV)), dict(new_table=c.new_table[:1].to(DEV)),
                dict(block_table=c.table.t().to(DEV)), dict(seq_lens=c.lens.float().to(DEV)),
                dict(kept=torch.empty(2, 2, 29, dtype=torch.int32, device=DEV)),
