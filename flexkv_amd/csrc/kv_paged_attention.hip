@@ -196,6 +196,14 @@ __device__ inline void write_stats(const Args& a, const Row& row, float m, float
   if (a.stats)
     a.stats[row.at * (a.heads * a.group) + row.head] = make_float2(m, inverse(l, row.visible));
 }
+// A result as the output's type holds it: the weights' roundings may carry one past the largest value
+// of V, and fp16 has no more than 65504.
+template <class T>
+__device__ inline float held(float x) {
+  if constexpr (std::is_same<T, _Float16>::value)
+    return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
+  return x;
+}
 // N neighbouring elements from `first` on as the output's type.
 template <class T, int N>
 __device__ inline void write_elements(const Args& a, const Row& row, int first, const float (&o)[N],
@@ -203,7 +211,7 @@ __device__ inline void write_elements(const Args& a, const Row& row, int first, 
   static_assert(N % 2 == 0, "");
   uint32_t w[N / 2];
 #pragma unroll
-  for (int j = 0; j < N; j += 2) w[j / 2] = Mat<T>::pack(o[j] * inv, o[j + 1] * inv);
+  for (int j = 0; j < N; j += 2) w[j / 2] = Mat<T>::pack(held<T>(o[j] * inv), held<T>(o[j + 1] * inv));
   char* const out = a.out + row.at * a.out_row + row.head * a.out_head + first * 2;
   if constexpr (N == 2) {
     *reinterpret_cast<uint32_t*>(out) = w[0];
@@ -1662,8 +1670,7 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
 
 // A launch has less than 2^32 threads.
 int check_plan(const fkv_paged_attention_args& c, const LaunchPlan& p) {
-  const int64_t weigh = static_cast<int64_t>(c.table_width) * c.layer.tokens_per_block /
-                            kWeighTokens * c.layer.num_heads * c.batch;
+  const int64_t weigh = p.share_row / kWeighTokens * c.layer.num_heads * c.batch;
   if (p.workgroups >= int64_t(1) << 22 || (c.weights && weigh >= int64_t(1) << 23))
     return fail(kInval, "%d queries of %d K/V heads are too many for one call", c.num_queries,
                 c.layer.num_heads);

@@ -409,6 +409,21 @@ def test_scores_far_from_zero(queries, D):
     assert out.isfinite().all()
 
 
+@pytest.mark.parametrize("keys,queries,D", [(70, 1, 64), (4300, 1, 128), (90, 6, 128), (300, 100, 128),
+                                            (3000, 40, 256)])
+def test_the_largest_values_of_fp16_stay_finite(keys, queries, D):
+    """All values are one of the two largest: so are results, to a rounding of the weights (2^-11, one
+    of 11 bits, and 2^-12 of the sums) and one of their own."""
+    c = Case([keys], [queries], H=1, D=D, dtype=FP16, seed=keys)
+    c.cache[1] = torch.where(c.cache[1] > 0, 65504.0, -65504.0)
+    c.cache[1, ..., 0] = 65504.0
+    c.cache[1, ..., 1] = -65472.0
+    out, _, _ = c.run()
+    assert out.isfinite().all()
+    assert ((out[..., 0].double() - 65504).abs() <= 65504 * 2.0 ** -10).all()
+    assert ((out[..., 1].double() + 65472).abs() <= 65504 * 2.0 ** -10).all()
+
+
 def test_a_cache_past_4_gib():
     T, H, D = 16, 1, 128
     N = (1 << 32) // (T * H * D * 2) + 64
