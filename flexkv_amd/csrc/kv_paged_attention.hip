@@ -11,12 +11,13 @@
 // result and the query rows as columns.  S = K Q^T comes out with some tokens of one row in a
 // lane, which is the layout of the second product's operand if its tokens are taken in that
 // order, so P never leaves its lane.  bf16 weights of 8 significant bits, fp16 ones of 11
-// (of what is at least 2^-14 of the largest; 2^-25 of it below): their roundings average out
-// over the keys, and the sum they are divided by is of the unrounded ones.
+// (of what is at least 2^-21 of the largest; below, a multiple of 2^-31 of it): a result is off by
+// half a step of its type at most, less where the roundings average out over the keys.  The sum
+// they are divided by is of the unrounded ones.
 //
 // Softmax: one pass, running maximum and sum per row in 32 bits, in units of log2.
-// The maximum is a reference that follows only when a score passes it by 2^8, so
-// most steps neither compare across lanes nor scale the sums.
+// The maximum (in fp16 a 2^7th of it, see Mat) is a reference that follows only when a score passes it
+// by 2^8, so most steps neither compare across lanes nor scale the sums.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -40,7 +41,10 @@ typedef uint32_t Vec4 __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-// The matrix instructions of a type.
+// The matrix instructions of a type, by how much (in units of log 2) a row's reference is below its
+// largest score when it is set, and the weight up to which a score may pass it.  fp16 has 2^16 above 1
+// and nothing below 2^-25, so weights start at 2^7 and may grow to 2^15: with 65536 keys of 1.4 * 2^-24
+// of the largest, references at the largest lose 29 % of what these add, and 0.2 % so.
 template <class T>
 struct Mat;
 template <>
@@ -56,6 +60,7 @@ struct Mat<__bf16> {
   static __device__ inline float low(uint32_t u) { return bits_f32(u << 16); }
   static __device__ inline float high(uint32_t u) { return bits_f32(u & 0xffff0000u); }
   static constexpr uint32_t kExponents = 0x7f807f80u;
+  static constexpr float kBelow = 0.f, kMost = kSlack;
 };
 template <>
 struct Mat<_Float16> {
@@ -80,6 +85,7 @@ struct Mat<_Float16> {
     return static_cast<float>(__builtin_bit_cast(v2h, u)[1]);
   }
   static constexpr uint32_t kExponents = 0x7c007c00u;
+  static constexpr float kBelow = 7.f, kMost = kSlack * 128.f;
 };
 
 // Whether one of the two elements of a register is an infinity or a NaN.
@@ -476,7 +482,7 @@ __device__ inline void hide(v4f (&s)[2], int at, int visible, int quad) {
       if (at + 16 * h + quad * 4 + i >= visible) s[h][i] = -INFINITY;
 }
 
-// The scores as weights p; returns their sum, which is over kSlack where one of them passes
+// The scores as weights p; returns their sum, which is over kMost where one of them passes
 // the reference by more than that.
 __device__ inline float weigh(const v4f (&s)[2], float m, float scale_log2, bool coarse,
                               float (&p)[8]) {
@@ -650,7 +656,7 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) asm volatile("" : "+v"(q[r].part[x]));
-    float slack = kSlack;
+    float slack = Mat<T>::kMost;
     State<D> st[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) clear(st[r]);
@@ -686,10 +692,10 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
         bool any_coarse = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          float top = st[r].m;
+          float top = -INFINITY;
 #pragma unroll
           for (int x = 0; x < 8; ++x) top = fmaxf(top, s[r][x / 4][x % 4] * scale_log2);
-          const float m = max_over_quads(top);
+          const float m = fmaxf(st[r].m, max_over_quads(top) - Mat<T>::kBelow);
           const float fade = __builtin_amdgcn_exp2f(st[r].m - m);
           st[r].m = m;
           st[r].l *= fade;
@@ -699,7 +705,7 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
           any_coarse |= coarse;
           l[r] = weigh(s[r], m, scale_log2, coarse, p[r]);
         }
-        slack = __any(any_coarse) ? -1.f : kSlack;
+        slack = __any(any_coarse) ? -1.f : Mat<T>::kMost;
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) st[r].l += l[r];
@@ -747,7 +753,7 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
       quad = lane >> 4;
 #pragma unroll
       for (int r = 0; r < R; ++r) clear(st[r]);
-      slack = kSlack;
+      slack = Mat<T>::kMost;
 #pragma unroll 1
       for (step = w.from + wave; step < end; step += W) {
         const StepRows<D> here = find(step, ask(step));
@@ -981,7 +987,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
   float m, l, slack;
   v16f o[NT];
   auto clear = [&]() __attribute__((always_inline)) {
-    m = kNothing, l = 0.f, slack = kSlack;
+    m = kNothing, l = 0.f, slack = Mat<T>::kMost;
 #pragma unroll
     for (int d = 0; d < NT; ++d)
 #pragma unroll
@@ -1072,13 +1078,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
       // Some score passes its row's reference: the references follow, and the weights are made
       // again, from scores made again, which would be 32 registers more if they were kept.
       scores(kt);
-      float top = m;
+      float top = -INFINITY;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i] * scale_log2);
       const auto other = __builtin_amdgcn_permlane32_swap(f32_bits(top), f32_bits(top), false, false);
-      top = fmaxf(bits_f32(other[0]), bits_f32(other[1]));
+      top = fmaxf(m, fmaxf(bits_f32(other[0]), bits_f32(other[1])) - Mat<T>::kBelow);
       const float fade = __builtin_amdgcn_exp2f(m - top);
       m = top;
       l *= fade;
@@ -1087,7 +1093,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_many_kernel(c
       keep_aside();
       const bool coarse = fabsf(m) >= kCoarse && m != kNothing;
       sum = weigh_all(coarse);
-      slack = __any(coarse) ? -1.f : kSlack;
+      slack = __any(coarse) ? -1.f : Mat<T>::kMost;
       keep_aside();
     }
     l += sum;

@@ -539,7 +539,9 @@ int fkv_write_kv_tokens(const fkv_paged_layer* layer, int num_tokens, const void
  *
  * head_size 64, 128 or 256; dtype (of cache, query and out) FKV_DTYPE_BF16 or _FP16.
  * Products enter exactly; sums, maximum, normalisation and weights are held in 32 bits.  In the
- * second product the weights p have the type's own significant bits (8 or 11).
+ * second product the weights p have the type's own significant bits (8 or 11), fp16's of at least
+ * 2^-21 of the row's largest: below they are multiples of 2^-31 of it, so that each key may be off by
+ * 2^-32 of the largest, and as many as 2^20 of them by 2^-12 of the values' size.
  * Block ids, lengths and starts are device memory, all int32 or all int64 (index_is_64bit), read
  * by the kernels, and nothing outside the cache is read for any of them: a block id outside the
  * cache gives NaN in the rows that see a token of that block (and in the weights those rows give), a
