@@ -112,8 +112,8 @@ struct Args : Sequences {
   float* weights;
   int64_t w_seq, w_head;             // elements
   float2* stats;                     // [query][head]: reference and 1 / sum of a row
-  // [query][head][token]: the scores times scale, in units of log 2, where the kernel for few rows
-  // leaves them; null where they are made again
+  // [query][head][token]: the scores before they are scaled, where the kernel for few rows leaves
+  // them; null where they are made again
   float* scores;
   int64_t scores_row;
   // workgroups that share the rows where they are made again, and, of more than one, what each adds
@@ -680,8 +680,7 @@ __global__ __launch_bounds__(64 * W, few_waves_a_simd(D)) void attend_few_kernel
           const uint64_t to = scores_at + static_cast<uint64_t>(token) * 4;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<__attribute__((address_space(1))) v4f*>(to + 64 * h) =
-                s[r][h] * scale_log2;
+            *reinterpret_cast<__attribute__((address_space(1))) v4f*>(to + 64 * h) = s[r][h];
         }
         l[r] = weigh(s[r], st[r].m, scale_log2, false, p[r]);
         passes |= l[r] > slack;
@@ -1355,8 +1354,10 @@ __global__ __launch_bounds__(256 * G) void join_kernel(const Args a) {
 
 // ---------------------------------------------------------------------------
 // What each token got, from scores that lie there: a thread adds up 4 tokens' over the rows, in
-// their order.  Bound by memory: 4 bytes a row and token (and as many to write them), where making the
-// scores again takes K's 2 D bytes a token.  32 sequences of up to 8192 keys, groups of 4: 9.6 us.
+// their order.  They are scaled as where the row's sum was made of them: rounded before the reference
+// is taken off they would be off by up to 0.5 where it is near 2^24.  Bound by memory: 4 bytes a row
+// and token (and as many to write them), where making the scores again takes K's 2 D bytes a token.
+// 32 sequences of up to 8192 keys, groups of 4: 9.6 us.
 
 constexpr int kAddTokens = 1024;     // of a workgroup
 
@@ -1366,6 +1367,7 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
   const Seq s = sequence(a, seq);
   const int keys = max(s.keys, 0), rows = s.count * a.group;
   if (at >= keys) return;
+  const float scale_log2 = score_scale(a.scale_log2);
   float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int n = 0; n < rows; ++n) {
@@ -1376,7 +1378,10 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
     // of steps that no row of a tile sees nothing has been written
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float e = __builtin_amdgcn_exp2f(x[i] - st.x) * st.y;
+      const float e = __builtin_amdgcn_exp2f(fabsf(st.x) >= kCoarse
+                                                 ? rounded_less(x[i], scale_log2, st.x)
+                                                 : __builtin_fmaf(x[i], scale_log2, -st.x)) *
+                      st.y;
       sums[i] += at + i < row.visible ? e : 0.f;
     }
   }
@@ -1389,7 +1394,9 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 // What each token got, from K: a wavefront keeps 64 tokens of K in registers and goes over the
 // queries, 32 rows at a time, which the workgroup's wavefronts share in LDS.  Here the tokens are the
-// columns of the products, so that a lane adds up its own token's weights, in the rows' order.  Where
+// columns of the products, so that a lane adds up its own token's weights, in the rows' order.  The
+// scores are the attention's bit for bit, also those of attend_few_kernel: two instructions of k = 16
+// add the products in the order of one of k = 32, and either operand may come first.  Where
 // there are few tokens the rows are shared out to several workgroups, whose sums are then added up.
 // Bound by the exponentials and products, of which each takes about as long (64 queries of 32 heads
 // over up to 16384 keys, 4 sequences: 58 us).

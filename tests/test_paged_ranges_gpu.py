@@ -62,3 +62,33 @@ def test_a_long_tail_of_small_weights_keeps_its_part_in_fp16(batch, queries, G, 
     share = (queries * G * p / total).to(DEV)
     for b in range(0, batch, 64):
         assert ((w[b, 0].double() - share).abs() <= share * (sums + 2.0 ** -14)).all()
+
+
+# -- scores far from zero --------------------------------------------------------------
+
+@pytest.mark.parametrize("scale", [2.0 ** 12, 2.0 ** 16, -2.0 ** 17, 2.0 ** 24])
+@pytest.mark.parametrize("kw", [
+    dict(keys=[400, 90], queries=[1, 1]),
+    dict(keys=[300], queries=[2], G=8, D=64, dtype=FP16),
+    dict(keys=[300], queries=[3], D=256),
+    dict(keys=[5000], queries=[1], H=1, G=8),
+    dict(keys=[400, 90], queries=[6, 7], D=64),
+    dict(keys=[300], queries=[8], dtype=FP16),
+    dict(keys=[2600, 31], queries=[1, 1], H=1, G=23, D=256),
+    dict(keys=[300], queries=[3], H=1, G=9, D=256, dtype=FP16),
+    dict(keys=[3000], queries=[2], H=1, G=8, T=1024, width=16500),
+    dict(keys=[400, 90], queries=[40, 60], D=64),
+    dict(keys=[400], queries=[70], dtype=FP16),
+    dict(keys=[2300], queries=[30], H=1, D=256),
+], ids=lambda kw: "-".join(str(v) for v in kw.values()))
+def test_the_weights_a_row_gives_add_up_to_one(kw, scale):
+    """Scores of 2^17 to 2^30 in units of log 2, whose last bits are worth up to a factor of 2^64
+    of a weight: the shares are those that the row's sum is of."""
+    c = Case(seed=7, **kw)
+    c.w = torch.zeros_like(c.w)
+    out, lse, w = c.run(scale=scale)
+    assert out.isfinite().all() and lse.isfinite().all()
+    for b, n in enumerate(c.queries):
+        # two sums of up to 5000 terms, half of 2^-24 of it each time; quotient and exponentials 2^-20
+        got = w[b].double().sum(1) / (n * c.G)
+        assert ((got - 1).abs() <= 2.0 ** -10).all(), (b, got)
