@@ -584,7 +584,7 @@ def write_kv_tokens(key: torch.Tensor, value, key_cache: torch.Tensor, value_cac
     and head stride; ``key_cache`` and ``value_cache``: [block, token, head, head_size] of the
     same type (bf16, fp16 or float32), of any block, token and head stride, such as the halves
     of an engine's [2, blocks, tokens, heads, head_size] (value and value_cache None: one
-    latent half); ``slots``: int64 or int32, block * tokens_per_block + offset, one below 0 or
+    latent half), no two rows of which may share memory; ``slots``: int64 or int32, block * tokens_per_block + offset, one below 0 or
     past the cache being padding.  Slots have to differ.  Makes no gradients: inputs that
     require them are refused but under ``torch.no_grad()``.  Asynchronous on the current torch
     stream; may be captured into a graph."""
@@ -733,7 +733,7 @@ def evict_kv_tokens(key_cache: torch.Tensor, value_cache, weights: torch.Tensor,
     largest ``weights`` (float32 [sequence, head, tokens that a row of block_table holds, or
     more], as paged_attention adds them up; of equal ones the earlier, NaN above all).
     ``key_cache``, ``value_cache``, ``block_table`` and ``seq_lens`` as in paged_attention (any
-    type; value_cache None: one latent half).  The kept rows, in their order, become the first
+    type; value_cache None: one latent half), but of rows that share no memory.  The kept rows, in their order, become the first
     tokens of the blocks ``new_table`` [sequence, blocks], which must be other blocks than those
     of the sequences' tokens and differ; the old ones are only read, and may be shared.
     ``new_weights``: float32 [sequence, head, budget or more], receives the kept tokens'

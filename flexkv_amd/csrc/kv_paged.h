@@ -9,6 +9,7 @@
 
 #include "kv_device.h"
 #include "kv_internal.h"
+#include "kv_overlap.h"
 
 namespace fkv_detail {
 #pragma GCC visibility push(hidden)
@@ -63,6 +64,24 @@ inline int paged_check_layer(const fkv_paged_layer& c) {
       return fail(kInval, "%lld blocks of the %s cache reach outside its allocation (%zu bytes)",
                   (long long)c.num_blocks, name, info.size);
   }
+  return 0;
+}
+
+// Of a layer that is written to no two rows share memory: what two of them got would be a mixture.
+inline int paged_check_written(const fkv_paged_layer& c) {
+  const int64_t counts[3] = {c.num_blocks, c.tokens_per_block, c.num_heads};
+  const int64_t bytes = c.head_size * paged_element_bytes(c.dtype);
+  const RowSet k(c.key, bytes,
+                 {c.key_block_stride_bytes, c.key_token_stride_bytes, c.key_head_stride_bytes},
+                 counts);
+  if (!rows_apart(k)) return fail(kInval, "rows of the key cache overlap");
+  if (!c.value) return 0;
+  const RowSet v(c.value, bytes,
+                 {c.value_block_stride_bytes, c.value_token_stride_bytes,
+                  c.value_head_stride_bytes},
+                 counts);
+  if (!rows_apart(v)) return fail(kInval, "rows of the value cache overlap");
+  if (rows_meet(k, v)) return fail(kInval, "the key and value caches overlap");
   return 0;
 }
 

@@ -596,7 +596,7 @@ int evict(const fkv_evict_args& c, fkv_stream_t stream) {
   if ((rc = check_evict(c)) || c.batch == 0) return rc;
   if (!c.kept || !c.weights || !c.seq_lens || ((!c.block_table || !c.new_table) && c.table_width > 0))
     return fail(kInval, "null pointer argument");
-  if ((rc = paged_check_layer(c.layer))) return rc;
+  if ((rc = paged_check_layer(c.layer)) || (rc = paged_check_written(c.layer))) return rc;
   const EvictPlan p(c);
   const int64_t heads = p.heads, most = p.most;
   const size_t need = p.bytes();
@@ -672,6 +672,7 @@ int write_tokens(const fkv_paged_layer& layer, int num_tokens, const void* key, 
       return fail(kInval, "%s's pointer and strides must be multiples of 16 bytes (token %lld, "
                   "head %lld)", k ? "value" : "key", (long long)a.row_stride[k],
                   (long long)a.head_stride[k]);
+  if ((rc = paged_check_written(layer))) return rc;
   a.to[0] = key_half(layer), a.to[1] = value_half(layer);
   a.slots = slots, a.slots64 = slots64;
   a.num_slots = layer.num_blocks * layer.tokens_per_block;

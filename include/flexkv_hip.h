@@ -502,7 +502,9 @@ int fkv_mx4_attention(const fkv_mx4_attention_args* args, fkv_stream_t stream);
  * h * head stride, head_size elements of `dtype`, and its V likewise: K and V may be halves of
  * one allocation (an engine's [2, N, T, H, D]), of each block, or two allocations, the heads before
  * the tokens or behind.  Pointers, strides and rows: multiples of 16 bytes; head_size at most
- * 1024, num_heads 1024, tokens_per_block 2^20.  Every block has to lie inside the allocation. */
+ * 1024, num_heads 1024, tokens_per_block 2^20.  Every block has to lie inside the allocation.  No
+ * two rows of a layer that is written to (all but attention) may share memory, K's and V's neither:
+ * such a layer is refused. */
 typedef struct fkv_paged_layer {
   void* key;
   void* value;                       /* null: a cache of one half (not for attention) */

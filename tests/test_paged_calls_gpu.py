@@ -1,0 +1,57 @@
+"""Calls on a paged cache that are refused, or that are allowed and easily got wrong."""
+import pytest
+import torch
+
+from flexkv_amd import c_ext
+
+from test_paged_gpu import BF16, DEV, Evict, _gen, _same
+
+pytestmark = pytest.mark.gpu
+
+
+# -- caches whose rows overlap -----------------------------------------------------------
+
+def _overlapping():
+    c = torch.zeros(4, 16, 2, 64, device=DEV, dtype=BF16)
+    other = torch.zeros_like(c)
+    flat = torch.zeros(8 * 16 * 2 * 64, device=DEV, dtype=BF16)
+    shape, step = (4, 16, 2, 64), 16 * 2 * 64
+    yield "key cache", c[:1].expand(shape), other
+    yield "key cache", c[:, :1].expand(shape), other
+    yield "value cache", other, c[:, :, :1].expand(shape)
+    yield "value cache", other, flat.as_strided(shape, (step - 8, 128, 64, 1))
+    yield "key and value", c, c
+    yield "key and value", flat.as_strided(shape, (step, 128, 64, 1)), \
+        flat.as_strided(shape, (step, 128, 64, 1), 3 * step + 128)
+
+
+def test_caches_whose_rows_overlap_are_not_written_to(per_call_path):
+    x = torch.ones(3, 2, 64, device=DEV, dtype=BF16)
+    slots = torch.arange(3, device=DEV)
+    e = Evict([40, 20], 16, T=16)
+    args = [t.to(DEV) for t in (e.w, e.table[:, :2], e.lens, e.new_table)]
+    for word, kc, vc in _overlapping():
+        with pytest.raises(RuntimeError, match=f"{word}.*overlap"):
+            c_ext.write_kv_tokens(x, x, kc, vc, slots)
+        with pytest.raises(RuntimeError, match=f"{word}.*overlap"):
+            c_ext.evict_kv_tokens(kc, vc, *args, 16, 3)
+        if word == "key cache":
+            with pytest.raises(RuntimeError, match="key cache overlap"):
+                c_ext.write_kv_tokens(x, None, kc, None, slots)
+        assert not kc.any() and not vc.any()
+        # attention only reads them
+        c_ext.paged_attention(x, kc, vc, args[1][:1], args[2][1:], None)
+
+
+def test_caches_side_by_side_are_written_to(per_call_path):
+    """K and V next to each other in each row, or in each token."""
+    g = _gen(1)
+    x = torch.randn(2, 5, 2, 64, generator=g).to(BF16)
+    slots = torch.randperm(64, generator=g)[:5]
+    for kc, vc in (torch.zeros(4, 16, 2, 2, 64, device=DEV, dtype=BF16).unbind(3),
+                   torch.zeros(4, 16, 2, 2, 64, device=DEV, dtype=BF16).unbind(2)):
+        c_ext.write_kv_tokens(x[0].to(DEV), x[1].to(DEV), kc, vc, slots.to(DEV))
+        for half, want in ((kc, x[0]), (vc, x[1])):
+            cache = torch.zeros(64, 2, 64, dtype=BF16)
+            cache[slots] = want
+            assert _same(half, cache.view(4, 16, 2, 64))
