@@ -585,7 +585,8 @@ def write_kv_tokens(key: torch.Tensor, value, key_cache: torch.Tensor, value_cac
     same type (bf16, fp16 or float32), of any block, token and head stride, such as the halves
     of an engine's [2, blocks, tokens, heads, head_size] (value and value_cache None: one
     latent half), no two rows of which may share memory; ``slots``: int64 or int32, block * tokens_per_block + offset, one below 0 or
-    past the cache being padding.  Slots have to differ.  Makes no gradients: inputs that
+    past the cache being padding.  Slots have to differ.  ``key`` and ``value`` may be views of
+    the cache, whose tokens then move: they are copied first.  Makes no gradients: inputs that
     require them are refused but under ``torch.no_grad()``.  Asynchronous on the current torch
     stream; may be captured into a graph."""
     fn = "write_kv_tokens"
@@ -611,6 +612,10 @@ def write_kv_tokens(key: torch.Tensor, value, key_cache: torch.Tensor, value_cac
             or not slots.is_contiguous():
         raise ValueError(f"{fn}: slots must be {n} contiguous int64 or int32 values, got "
                          f"{slots.dtype} {tuple(slots.shape)}")
+    # rows in the cache itself may be slots as well: all are read before any is written
+    caches = [c for c in (key_cache, value_cache) if c is not None]
+    key, value = (x.clone() if x is not None and any(_ranges_meet(x, c) for c in caches) else x
+                  for x in (key, value))
     rows = [key.data_ptr(), *_strides(key)]
     rows += [None, 0, 0] if value is None else [value.data_ptr(), *_strides(value)]
     with _on_device(device):

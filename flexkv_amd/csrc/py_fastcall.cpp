@@ -498,7 +498,7 @@ PyObject* write_kv_tokens_of(PyObject* const* a) {
   for (const at::Tensor* x : {key, value})
     if (x && (x->dim() != 3 || x->size(0) != n || x->size(1) != kc->size(2) ||
               x->size(2) != kc->size(3) || x->scalar_type() != kc->scalar_type() ||
-              x->stride(2) != 1))
+              x->stride(2) != 1 || ranges_meet(*x, *kc) || (vc && ranges_meet(*x, *vc))))
       Py_RETURN_FALSE;
   if (!index_vector(*slots, n)) Py_RETURN_FALSE;
   void* stream = c10::hip::getCurrentHIPStream().stream();

@@ -517,7 +517,8 @@ typedef struct fkv_paged_layer {
 /* Write new tokens into their slots: row n of key and value (elements of the cache's type, a
  * head's next to each other) becomes token slots[n] % T of block slots[n] / T.  slots: device
  * memory, int64 or int32 (slots_are_64bit); a slot below 0 or past the cache is padding and
- * writes nothing.  Slots of one call have to differ: one that comes twice leaves a mixture.
+ * writes nothing.  Slots of one call have to differ: one that comes twice leaves a mixture.  key and
+ * value may lie in the cache, but not in slots that are written.
  * `value` is null where the cache has one half.  Pointers and strides: multiples of 16 bytes.
  * Asynchronous on `stream`, and may be captured into a graph. */
 int fkv_write_kv_tokens(const fkv_paged_layer* layer, int num_tokens, const void* key,
@@ -591,7 +592,8 @@ int fkv_paged_attention(const fkv_paged_attention_args* args, fkv_stream_t strea
  *     new_weights[b][h][i]   its weight, 0 past the last (may be null; may be `weights` itself)
  * Each head keeps tokens of its own.  The blocks of new_table may not be among those that
  * block_table names for the tokens there are, nor come twice; block_table's are only read, and
- * may be shared.  Nothing outside the cache is read or written: a token of a block outside it, or
+ * may be shared.  kept and new_weights may overlap nothing else that the call uses.  Nothing outside
+ * the cache is read or written: a token of a block outside it, or
  * for one, is left out of the copy.  A sequence longer than its row of block_table keeps nothing:
  * kept is -1, and its new_weights stay.  A length below 0 is taken as 0.
  * Any dtype.  budget at least 1, recent at most budget, new_table's rows hold what may be kept.

@@ -55,3 +55,26 @@ def test_caches_side_by_side_are_written_to(per_call_path):
             cache = torch.zeros(64, 2, 64, dtype=BF16)
             cache[slots] = want
             assert _same(half, cache.view(4, 16, 2, 64))
+
+
+# -- tokens that come from the cache itself -------------------------------------------------
+
+@pytest.mark.parametrize("halves", [1, 2])
+def test_tokens_move_within_their_cache(per_call_path, halves):
+    """Each token to the next one's slot, all at once, from views of the cache."""
+    g = _gen(3)
+    blocks, T, H, D = 300, 16, 2, 64
+    cache = torch.randn(2, blocks, T, H, D, generator=g).to(BF16)
+    dev = cache.to(DEV)
+    flat = dev.view(2, blocks * T, H, D)
+    slots = torch.arange(blocks * T).roll(-1)
+    if halves == 2:
+        # and what was K becomes V
+        c_ext.write_kv_tokens(flat[1], flat[0], dev[0], dev[1], slots.to(DEV))
+        want = cache.flip(0)
+    else:
+        c_ext.write_kv_tokens(flat[0], None, dev[0], None, slots.to(DEV))
+        want = cache
+    want = want.reshape(2, blocks * T, H, D).roll(1, 1).view_as(cache)
+    assert _same(dev[0], want[0])
+    assert _same(dev[1], want[1] if halves == 2 else cache[1])
