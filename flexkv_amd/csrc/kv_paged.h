@@ -42,9 +42,10 @@ inline int paged_check_layer(const fkv_paged_layer& c) {
                            {c.value_block_stride_bytes, c.value_token_stride_bytes,
                             c.value_head_stride_bytes}};
   if (!p[0]) return fail(kInval, "null cache pointer");
-  PtrInfo info;
-  for (int k = 0; k < (p[1] ? 2 : 1); ++k) {
-    const char* const name = k ? "value" : "key";
+  const int halves = p[1] ? 2 : 1;
+  auto name_of = [](int k) { return k ? "value" : "key"; };
+  for (int k = 0; k < halves; ++k) {
+    const char* const name = name_of(k);
     for (int64_t v : s[k])
       if (v < 0 || v % 16)
         return fail(kInval, "the %s cache's strides must be non-negative multiples of 16 bytes "
@@ -52,6 +53,10 @@ inline int paged_check_layer(const fkv_paged_layer& c) {
                     (long long)s[k][1], (long long)s[k][2]);
     if (reinterpret_cast<uintptr_t>(p[k]) % 16)
       return fail(kInval, "the %s cache's pointer must be a multiple of 16 bytes", name);
+  }
+  PtrInfo info;
+  for (int k = 0; k < halves; ++k) {
+    const char* const name = name_of(k);
     const __int128 hi = static_cast<__int128>(c.num_blocks - 1) * s[k][0] +
                         static_cast<__int128>(c.tokens_per_block - 1) * s[k][1] +
                         static_cast<__int128>(c.num_heads - 1) * s[k][2] +

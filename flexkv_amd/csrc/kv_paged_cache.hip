@@ -659,6 +659,12 @@ int write_tokens(const fkv_paged_layer& layer, int num_tokens, const void* key, 
                  int slots64, fkv_stream_t stream) {
   int rc;
   if (num_tokens < 0) return fail(kInval, "negative count: num_tokens=%d", num_tokens);
+  if ((rc = paged_check_sizes(layer))) return rc;
+  const int64_t vecs = layer.head_size * paged_element_bytes(layer.dtype) / 16;
+  const int64_t units = vecs * layer.num_heads * num_tokens;
+  if (units > (int64_t(1) << 31) - kThreads)
+    return fail(kInval, "%d tokens of %d heads of %d are too many for one call", num_tokens,
+                layer.num_heads, layer.head_size);
   if ((rc = paged_check_layer(layer)) || num_tokens == 0) return rc;
   if (!key || !slots) return fail(kInval, "null pointer argument");
   if (!value != !layer.value)
@@ -677,11 +683,6 @@ int write_tokens(const fkv_paged_layer& layer, int num_tokens, const void* key, 
   a.slots = slots, a.slots64 = slots64;
   a.num_slots = layer.num_blocks * layer.tokens_per_block;
   a.tokens = layer.tokens_per_block;
-  const int64_t vecs = layer.head_size * paged_element_bytes(layer.dtype) / 16;
-  const int64_t units = vecs * layer.num_heads * num_tokens;
-  if (units > (int64_t(1) << 31) - kThreads)
-    return fail(kInval, "%d tokens of %d heads of %d are too many for one call", num_tokens,
-                layer.num_heads, layer.head_size);
   a.units = static_cast<uint32_t>(units);
   a.vecs = FastDiv(vecs), a.per_token = FastDiv(vecs * layer.num_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
