@@ -4,7 +4,7 @@ import torch
 
 from flexkv_amd import c_ext
 
-from test_paged_gpu import BF16, DEV, Evict, _gen, _same
+from test_paged_gpu import BF16, DEV, Case, Evict, _gen, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,56 @@ def test_tokens_move_within_their_cache(per_call_path, halves):
     want = want.reshape(2, blocks * T, H, D).roll(1, 1).view_as(cache)
     assert _same(dev[0], want[0])
     assert _same(dev[1], want[1] if halves == 2 else cache[1])
+
+
+# -- starts, and other streams ------------------------------------------------------------
+
+@pytest.mark.parametrize("first,last", [(0, 1 << 40), (-7, 0), (-(1 << 50), 1)])
+@pytest.mark.parametrize("queries", [3, 40])
+def test_starts_outside_the_rows_are_those_at_their_ends(first, last, queries):
+    """`last`: how far behind the rows."""
+    c = Case([100, 100], [queries, queries], index=torch.int64)
+    starts = torch.tensor([first, queries, 2 * queries + last], device=DEV)
+    out = torch.full((2 * queries, 8, 128), 3.0, device=DEV, dtype=BF16)
+    c.check(c.run(query_starts=starts, out=out))
+
+
+@pytest.mark.parametrize("queries", [1, 6, 50])
+def test_calls_on_two_streams_at_once(queries):
+    """Each with the weights and lse that it makes itself; so are those of replayed graphs."""
+    cases = [Case([900, 70], [queries, 1], H=1, seed=1), Case([9000], [queries], H=1, G=8, seed=2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    state = []
+    for c in cases:
+        d = c.device()
+        state.append((d, torch.zeros_like(d["query"]), torch.zeros(c.q.shape[:2], device=DEV),
+                      c.w.to(DEV)))
+    torch.cuda.synchronize()
+
+    def got():
+        torch.cuda.synchronize()
+        return [tuple(t.cpu() for t in s[1:]) for s in state]
+    for c, s, (d, out, lse, w) in zip(cases, streams, state):
+        with torch.cuda.stream(s):
+            c_ext.paged_attention(**d, out=out, lse=lse, weights=w)
+    eager = got()
+    for c, g in zip(cases, eager):
+        c.check(g)
+    graphs = []
+    for c, s, (d, out, lse, w) in zip(cases, streams, state):
+        before = c.w.to(DEV)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            w.copy_(before)
+            c_ext.paged_attention(**d, out=out, lse=lse, weights=w)
+        graphs.append((graph, before))
+    for _ in range(3):
+        for d, out, lse, w in state:
+            out.zero_(), lse.zero_(), w.zero_()
+        torch.cuda.synchronize()
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        for a, b in zip(got(), eager):
+            assert all(_same(x, y) for x, y in zip(a, b))
