@@ -594,7 +594,9 @@ struct EvictPlan {
 int evict(const fkv_evict_args& c, fkv_stream_t stream) {
   int rc;
   if ((rc = check_evict(c)) || c.batch == 0) return rc;
-  if (!c.kept || !c.weights || !c.seq_lens || ((!c.block_table || !c.new_table) && c.table_width > 0))
+  // a table of no blocks has neither entries nor weights
+  if (!c.kept || !c.seq_lens ||
+      ((!c.weights || !c.block_table || !c.new_table) && c.table_width > 0))
     return fail(kInval, "null pointer argument");
   if ((rc = paged_check_layer(c.layer)) || (rc = paged_check_written(c.layer))) return rc;
   const EvictPlan p(c);

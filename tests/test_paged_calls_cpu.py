@@ -131,3 +131,14 @@ def test_calls_of_more_threads_than_a_launch_has():
              "536869888 queries of 1 K/V heads are too many")
     _refused(_attend(pairs, False, **many), "536868864 queries of 1024 K/V heads are too many")
     _refused(_attend({}, False, **{**many, "group_size": 3}), "536868864 queries of 3 heads a K/V")
+
+
+def test_an_eviction_from_tables_of_no_blocks_needs_no_weights():
+    none = dict(table_width=0, new_table_width=0, weights_width=0)
+    assert _evict({}, False, **none) == 0
+    for kw in ({}, dict(weights=None), dict(weights=None, block_table=None, new_table=None)):
+        _refused(_evict({}, **none, **kw), "not device memory")
+    for kw in (dict(seq_lens=None), dict(kept=None)):
+        _refused(_evict({}, **none, **kw), "null pointer argument")
+    for kw in (dict(weights=None), dict(block_table=None), dict(new_table=None)):
+        _refused(_evict({}, **kw), "null pointer argument")

@@ -131,3 +131,22 @@ def test_calls_on_two_streams_at_once(queries):
                 graph.replay()
         for a, b in zip(got(), eager):
             assert all(_same(x, y) for x, y in zip(a, b))
+
+
+# -- tables of no blocks -------------------------------------------------------------------
+
+@pytest.mark.parametrize("wide", [0, 5])
+def test_sequences_whose_tables_have_no_blocks(per_call_path, wide):
+    """Nothing is seen, weighed or kept."""
+    cache = torch.ones(4, 16, 2, 64, device=DEV, dtype=BF16)
+    table = torch.zeros(3, 0, device=DEV, dtype=torch.int64)
+    lens = torch.tensor([0, -1, 1], device=DEV)          # the last: more than its row holds
+    w = torch.ones(3, 2, wide, device=DEV)
+    out = c_ext.paged_attention(torch.ones(3, 4, 64, device=DEV, dtype=BF16), cache, cache, table,
+                                lens, weights=w)
+    assert (out[:2] == 0).all() and out[2].isnan().all() and (w == 1).all()
+    new_weights = torch.full((3, 2, 7), 5.0, device=DEV)
+    kept = c_ext.evict_kv_tokens(cache, None, w, table, lens, table, 9, 2, new_weights)
+    assert kept.shape == (3, 2, 9) and (kept == -1).all()
+    assert (new_weights[:2] == 0).all() and (new_weights[2] == 5).all()
+    assert (cache == 1).all()
