@@ -1643,8 +1643,9 @@ LaunchPlan launch_plan(const fkv_paged_attention_args& c) {
     // workgroup where there are so many sequences that working the shares out takes long, or few keys.
     const int deal_steps =
         dim == 256 || p.tiles <= kComputeUnits / 2 ? kDealSteps / 2 : kDealSteps;
+    // the kernel adds the number of slots, a compute unit's each at most, to all steps in 32 bits
     const bool dealt = c.batch <= 4 * 64 && most_steps >= deal_steps &&
-                       tiles * std::max<int64_t>(1, most_steps) < int64_t(1) << 31;
+                       tiles * most_steps <= INT32_MAX - kComputeUnits;
     p.waves = (dealt || p.tiles <= kComputeUnits) && dim <= 128 ? 8 : 4;
     const int64_t places = kComputeUnits * 8 / p.waves / (dim == 256 ? 2 : 1);
     int64_t items = dealt ? std::max<int64_t>(1, places / heads) : tiles;

@@ -142,3 +142,20 @@ def test_an_eviction_from_tables_of_no_blocks_needs_no_weights():
         _refused(_evict({}, **none, **kw), "null pointer argument")
     for kw in (dict(weights=None), dict(block_table=None), dict(new_table=None)):
         _refused(_evict({}, **kw), "null pointer argument")
+
+
+def test_keys_are_dealt_out_while_their_steps_stay_in_32_bits():
+    """The steps of 32 tokens of all tiles, and with them up to 256 workgroups."""
+    lib, need = _lib.load(), ctypes.c_size_t()
+
+    def workspace(blocks):
+        # groups of 32 heads of 256 elements: two tiles a sequence
+        layer = _layer(dict(head_size=256, tokens_per_block=32))
+        a = _lib.PagedAttentionArgs(layer=layer, batch=231, num_queries=231, group_size=32,
+                                    table_width=blocks, scale=1.0)
+        assert lib.fkv_paged_attention_workspace(a, need) == 0
+        return need.value
+    most = (2 ** 31 - 1 - 256) // 462
+    assert workspace(2000) == workspace(most) > 0
+    for blocks in (most + 1, (2 ** 31 - 1) // 462, (2 ** 31 - 1) // 462 + 1):
+        assert workspace(blocks) == 0
