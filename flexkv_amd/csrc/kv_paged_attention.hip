@@ -1553,7 +1553,9 @@ int check_sizes(const fkv_paged_attention_args& c) {
     return fail(kInval, "attention takes a bf16 or fp16 cache, got dtype %d", layer.dtype);
   if (c.group_size < 1 || c.group_size > 1024)
     return fail(kInval, "group_size must be in [1, 1024], got %d", c.group_size);
-  if (!std::isfinite(c.scale)) return fail(kInval, "scale must be finite");
+  // an infinite one would make NaN of scores of 0
+  if (!std::isfinite(c.scale * kLog2e))
+    return fail(kInval, "scale must be finite, and in units of log 2 as well (up to 2^127)");
   const int64_t most = static_cast<int64_t>(c.table_width) * layer.tokens_per_block;
   if (c.table_width < 0 || most > int64_t(1) << 28)
     return fail(kInval, "table_width must be non-negative and hold at most 2^28 tokens, got %d "

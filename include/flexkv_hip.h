@@ -556,7 +556,7 @@ int fkv_write_kv_tokens(const fkv_paged_layer* layer, int num_tokens, const void
  * before they are divided by that of p, whose terms reach 2^8: values up to 2^119 over the
  * sequence's keys are safe, larger ones may give infinities or NaN; finite fp16 results past 65504,
  * which roundings make of values near it, are that value.  A row whose largest score, in
- * units of log 2, leaves what 32 bits hold gives NaN.
+ * units of log 2, leaves what 32 bits hold gives NaN; a scale that does in these units is refused.
  * Asynchronous on `stream`, and may be captured into a graph. */
 typedef struct fkv_paged_attention_args {
   fkv_paged_layer layer;

@@ -159,3 +159,11 @@ def test_keys_are_dealt_out_while_their_steps_stay_in_32_bits():
     assert workspace(2000) == workspace(most) > 0
     for blocks in (most + 1, (2 ** 31 - 1) // 462, (2 ** 31 - 1) // 462 + 1):
         assert workspace(blocks) == 0
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, float("inf"), float("nan")])
+def test_a_scale_that_is_infinite_in_units_of_log_2_is_refused(scale):
+    for call in (True, False):
+        _refused(_attend({}, call, scale=scale), "scale must be finite")
+    for finite in (2.0 ** 127, -(2.0 ** 127), 2.0 ** -149, 0.0):
+        assert _attend({}, False, scale=finite) == 0

@@ -92,3 +92,12 @@ def test_the_weights_a_row_gives_add_up_to_one(kw, scale):
         # two sums of up to 5000 terms, half of 2^-24 of it each time; quotient and exponentials 2^-20
         got = w[b].double().sum(1) / (n * c.G)
         assert ((got - 1).abs() <= 2.0 ** -10).all(), (b, got)
+
+
+@pytest.mark.parametrize("queries", [1, 50])
+@pytest.mark.parametrize("scale", [2.0 ** 127, -(2.0 ** 127), 2.0 ** -149])
+def test_the_largest_and_smallest_scales(queries, scale):
+    """With scores of 0 every key weighs alike."""
+    c = Case([200], [queries], H=1, G=2, D=64)
+    c.q = torch.zeros_like(c.q)
+    c.check(c.run(scale=scale), scale=scale)
