@@ -317,7 +317,7 @@ __device__ inline void keep(const float* w, int from, int to, int others, uint32
 }
 
 // One workgroup for a (sequence, head).  Bound by its compute unit's instructions and two dozen
-// barriers: 8192 tokens 13 us, 777 9.
+// barriers: 8192 tokens 13 us, 777 9 (without the copy).
 __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const EvictArgs a) {
   __shared__ Chooser chooser;
   const int b = a.heads_div.div(blockIdx.x), h = blockIdx.x - b * a.heads;
@@ -345,8 +345,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_choose_kernel(const Evic
 // The choice of long sequences, where there are few: a.parts workgroups for a (sequence, head), each
 // with a share of the tokens.  A launch for each digit, in which a workgroup first finds the digits
 // before from what all counted of them, then counts its own tokens', and one that keeps.  The
-// order that the counts are added up in does not change them.  Bound by the launches, 5 to 8 us each:
-// two sequences of 65536 tokens 27 us, 55 with a workgroup each.
+// order that the counts are added up in does not change them.  Bound by the launches, 5 to 9 us each:
+// two sequences of 65536 tokens 26 us, 58 with a workgroup each (without the copy).
 constexpr int kDigits = 1 << kRadixBits, kPasses = 3;
 struct Part {
   int b, h, part, n, from, to;
@@ -570,7 +570,8 @@ int copy_rows(int64_t rows) {
 
 // Workgroups that choose for one (sequence, head): one for each 2^13 tokens, of all no more than two a
 // compute unit; and one alone where it would not be four, since several take three launches more
-// (8192 tokens 16 us with one, 28 with two; 65536 60 with one, 30 with eight).
+// (a call with its copy, two sequences: 8192 tokens 17 us with one, 26 with two; 65536 62 with one, 30
+// with eight).
 int choice_parts(int64_t heads, int64_t tokens) {
   const int64_t parts = std::min<int64_t>({32, 512 / heads, tokens / Batch::kTokens});
   return parts < 4 ? 1 : static_cast<int>(parts);
